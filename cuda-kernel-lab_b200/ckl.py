@@ -69,6 +69,35 @@ class MoeWeights(C.Structure):
                 ("scales", C.c_void_p), ("zeros", C.c_void_p)]
 
 
+class Rope(C.Structure):
+    """ckl_rope: a rotary plan (rope_plan)."""
+    _fields_ = [("rot_dim", C.c_int), ("interleaved", C.c_int), ("scale", C.c_float),
+                ("reserved", C.c_int), ("turns", C.c_uint64 * (HEAD_DIM // 2))]
+
+
+class AppendParams(C.Structure):
+    """ckl_append_params (make_append_params)."""
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("q_stride", C.c_longlong), ("k_stride", C.c_longlong),
+                ("v_stride", C.c_longlong), ("q_out", C.c_void_p), ("k_cache", C.c_void_p),
+                ("v_cache", C.c_void_p), ("kv_indptr", C.c_void_p), ("kv_indices", C.c_void_p),
+                ("kv_last_page_len", C.c_void_p), ("q_indptr", C.c_void_p),
+                ("positions", C.c_void_p), ("B", C.c_int), ("N", C.c_int), ("Hq", C.c_int),
+                ("Hkv", C.c_int), ("num_pages", C.c_int)]
+
+
+class TreeParams(C.Structure):
+    """ckl_tree_params (make_tree_params)."""
+    _fields_ = [("q", C.c_void_p), ("k_cache", C.c_void_p), ("v_cache", C.c_void_p),
+                ("kv_indptr", C.c_void_p), ("kv_indices", C.c_void_p),
+                ("kv_last_page_len", C.c_void_p), ("q_indptr", C.c_void_p),
+                ("tree_mask", C.c_void_p), ("positions", C.c_void_p), ("slopes", C.c_void_p),
+                ("B", C.c_int), ("N", C.c_int), ("Hq", C.c_int), ("Hkv", C.c_int),
+                ("max_q", C.c_int), ("mask_words", C.c_int), ("num_chunks", C.c_int),
+                ("chunk_tokens", C.c_int), ("window", C.c_int), ("num_pages", C.c_int),
+                ("sm_scale", C.c_float), ("softcap", C.c_float)]
+
+
 EP_MAX_RANKS = 8
 IPC_HANDLE_BYTES = 64
 
@@ -131,6 +160,26 @@ _SIGS = {
                                           C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     "ckl_cascade_decode": (C.c_int, [C.POINTER(CascadePlan), C.c_void_p, C.c_void_p,
                                      C.c_void_p, C.c_size_t, C.c_void_p]),
+    "ckl_rope_plan": (C.c_int, [C.c_int, C.c_int, C.c_double, C.c_int, C.c_double, C.c_int,
+                                C.c_double, C.c_double, C.POINTER(Rope)]),
+    "ckl_rope_plan_freqs": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_double,
+                                      C.POINTER(Rope)]),
+    "ckl_rope_append": (C.c_int, [C.POINTER(AppendParams), C.POINTER(Rope), C.c_void_p]),
+    "ckl_tree_mask": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int,
+                                C.c_int, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "ckl_tree_plan": (C.c_int, [C.c_int] * 7 + [C.POINTER(C.c_int), C.POINTER(C.c_int)]),
+    "ckl_tree_workspace_size": (C.c_size_t, [C.POINTER(TreeParams)]),
+    "ckl_tree_attention": (C.c_int, [C.POINTER(TreeParams), C.c_void_p, C.c_void_p, C.c_void_p,
+                                     C.c_size_t, C.c_void_p]),
+    "ckl_cache_weights": (C.c_int, [C.POINTER(TreeParams), C.c_void_p, C.c_void_p, C.c_longlong,
+                                    C.c_float, C.c_void_p]),
+    "ckl_cache_select": (C.c_int, [C.c_void_p, C.c_longlong, C.c_void_p, C.c_void_p, C.c_int,
+                                   C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p,
+                                   C.c_void_p]),
+    "ckl_cache_compact": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                    C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_void_p,
+                                    C.c_void_p, C.c_void_p, C.c_longlong, C.c_void_p,
+                                    C.c_void_p]),
     "ckl_moe_packed_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
     "ckl_moe_scale_count": (C.c_size_t, [C.c_int, C.c_int, C.c_int, C.c_int]),
     "ckl_moe_zero_words": (C.c_size_t, [C.c_int, C.c_int, C.c_int, C.c_int]),
@@ -519,6 +568,290 @@ def cascade_tree_decode(tp: CascadeTreePlan, out=None, lse=None, workspace=None,
                                         _ptr(workspace), ws_bytes, _stream(stream)),
           "ckl_cascade_tree_decode")
     return out, lse
+
+
+# ------------------------------------------------------------------ writing and trimming the cache
+ROPE_SCALING = {"none": 0, "linear": 1, "ntk": 2, "by_parts": 3}
+
+
+def _here(name, *tensors):
+    """All tensors (None skipped) on the current device: the library launches there."""
+    dev = _torch().cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != dev:
+            raise CklError(1, name, f"a tensor is on {t.device}, the current device is cuda:{dev}")
+
+
+def _rows(t, dtype, n, name, who):
+    """A contiguous 1-D tensor of at least n elements, or None."""
+    if t is not None:
+        _need(t, dtype, name)
+        if t.numel() < n:
+            raise CklError(1, who, f"{name} has {t.numel()} elements, needs {n}")
+    return t
+
+
+def _cache_shape(k_cache, v_cache, who):
+    torch = _torch()
+    _need(k_cache, torch.float16, "k_cache")
+    _need(v_cache, torch.float16, "v_cache")
+    if (k_cache.dim() != 4 or k_cache.shape[1] != PAGE or k_cache.shape[3] != HEAD_DIM
+            or v_cache.shape != k_cache.shape):
+        raise CklError(2, who, f"caches {tuple(k_cache.shape)} / {tuple(v_cache.shape)}")
+    return k_cache.shape[0], k_cache.shape[2]
+
+
+def rope_plan(rot_dim=HEAD_DIM, *, base=10000.0, interleaved=False, scaling="none", factor=1.0,
+              original_len=0, beta_fast=32.0, beta_slow=1.0, inv_freq=None, scale=1.0):
+    """A rotary plan (ckl_rope_plan): scaling "none", "linear", "ntk" or "by_parts"; or the
+    caller's own angles per position inv_freq[rot_dim/2] and scale (ckl_rope_plan_freqs)."""
+    r = Rope()
+    if inv_freq is not None:
+        f = (C.c_double * (rot_dim // 2))(*[float(x) for x in inv_freq])
+        if len(inv_freq) != rot_dim // 2:
+            raise CklError(1, "rope_plan", f"{len(inv_freq)} frequencies for rot_dim {rot_dim}")
+        check(lib().ckl_rope_plan_freqs(f, rot_dim, int(interleaved), float(scale), C.byref(r)),
+              "ckl_rope_plan_freqs")
+        return r
+    if scaling not in ROPE_SCALING:
+        raise CklError(1, "rope_plan", f"unknown scaling {scaling!r}")
+    check(lib().ckl_rope_plan(rot_dim, int(interleaved), float(base), ROPE_SCALING[scaling],
+                              float(factor), int(original_len), float(beta_fast),
+                              float(beta_slow), C.byref(r)), "ckl_rope_plan")
+    return r
+
+
+def make_append_params(q, k, v, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, *,
+                       q_out=None, q_indptr=None, positions=None):
+    """ckl_append_params for new tokens q [N,Hq,128] (or None), k and v [N,Hkv,128] -- fp16,
+    tokens any multiple of 8 elements apart, e.g. slices of one fused projection. The params
+    keep every tensor alive; q_out (allocated when None) is p.q_rotated."""
+    torch = _torch()
+    who = "make_append_params"
+    P, Hkv = _cache_shape(k_cache, v_cache, who)
+    strides = []
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        if t is None and name == "q":
+            strides.append(0)
+            continue
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.float16:
+            raise CklError(1, who, f"{name}: expected a CUDA float16 tensor")
+        if t.dim() != 3 or t.shape[2] != HEAD_DIM or t.shape[0] != k.shape[0]:
+            raise CklError(2, who, f"{name} {tuple(t.shape)}")
+        if t.numel() and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != HEAD_DIM)):
+            raise CklError(1, who, f"{name}: a token's heads must be contiguous")
+        # the token stride of a single token means nothing: give it its row
+        strides.append(t.stride(0) if t.shape[0] > 1 else t.shape[1] * HEAD_DIM)
+    if k.shape[1] != Hkv or v.shape[1] != Hkv:
+        raise CklError(2, who, f"k {tuple(k.shape)} / v {tuple(v.shape)} for {Hkv} cached heads")
+    N = k.shape[0]
+    for t, n in ((kv_indptr, "kv_indptr"), (kv_indices, "kv_indices"),
+                 (kv_last_page_len, "kv_last_page_len")):
+        _need(t, torch.int32, n)
+    B = kv_indptr.numel() - 1
+    _rows(kv_last_page_len, torch.int32, B, "kv_last_page_len", who)
+    _rows(q_indptr, torch.int32, B + 1, "q_indptr", who)
+    _rows(positions, torch.int32, N, "positions", who)
+    if q is not None and q_out is None:
+        q_out = torch.empty((N, q.shape[1], HEAD_DIM), dtype=torch.float16, device=q.device)
+    if q is not None:
+        _need(q_out, torch.float16, "q_out")
+        if tuple(q_out.shape) != tuple(q.shape):
+            raise CklError(2, who, f"q_out {tuple(q_out.shape)} for q {tuple(q.shape)}")
+    else:
+        q_out = None
+    _here(who, q, k, v, q_out, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len,
+          q_indptr, positions)
+    ptr = lambda t: None if t is None else t.data_ptr()
+    p = AppendParams(ptr(q), ptr(k), ptr(v), *strides, ptr(q_out), ptr(k_cache), ptr(v_cache),
+                     ptr(kv_indptr), ptr(kv_indices), ptr(kv_last_page_len), ptr(q_indptr),
+                     ptr(positions), B, N, 0 if q is None else q.shape[1], Hkv, P)
+    p._keep = (q, k, v, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, q_indptr,
+               positions)
+    p.q_rotated = q_out
+    return p
+
+
+def rope_append(p: AppendParams, rope: Rope = None, stream=None):
+    """Rotates and appends (ckl_rope_append) -> the rotated q (p.q_rotated). rope None copies
+    q and k unturned."""
+    check(lib().ckl_rope_append(C.byref(p), None if rope is None else C.byref(rope),
+                                _stream(stream)), "ckl_rope_append")
+    return p.q_rotated
+
+
+def tree_mask(parents, q_indptr, kv_indptr, kv_last_page_len, max_q, *, mask=None,
+              positions=None, stream=None):
+    """Ancestor masks of draft trees (ckl_tree_mask) -> (mask int32 [N, ceil(max_q/32)] holding
+    the uint32 words, positions int32 [N])."""
+    torch = _torch()
+    _need(parents, torch.int32, "parents")
+    N, B, W = parents.numel(), kv_indptr.numel() - 1, (max_q + 31) // 32
+    _need(kv_indptr, torch.int32, "kv_indptr")
+    for t, n, name in ((q_indptr, B + 1, "q_indptr"), (kv_last_page_len, B, "kv_last_page_len")):
+        _need(t, torch.int32, name)
+        _rows(t, torch.int32, n, name, "tree_mask")
+    if mask is None:
+        mask = torch.empty((N, W), dtype=torch.int32, device=parents.device)
+    if positions is None:
+        positions = torch.empty(N, dtype=torch.int32, device=parents.device)
+    _rows(mask, torch.int32, N * W, "mask", "tree_mask")
+    _rows(positions, torch.int32, N, "positions", "tree_mask")
+    _here("tree_mask", parents, q_indptr, kv_indptr, kv_last_page_len, mask, positions)
+    check(lib().ckl_tree_mask(_ptr(parents), _ptr(q_indptr), _ptr(kv_indptr),
+                              _ptr(kv_last_page_len), B, N, W, _ptr(mask), _ptr(positions),
+                              _stream(stream)), "ckl_tree_mask")
+    return mask, positions
+
+
+def make_tree_params(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, *, max_len,
+                     q_indptr=None, max_q=1, tree_mask=None, positions=None, slopes=None,
+                     softcap=0.0, window=0, sm_scale=None, force_chunks=0):
+    """ckl_tree_params with its key split (ckl_tree_plan) for q [N,Hq,128] and sequences of up
+    to max_q drafted and max_len cached tokens. tree_mask: int32 [N, words], bit j = drafted
+    token j is seen (tree_mask()); None: a chain. The params keep every tensor alive."""
+    torch = _torch()
+    who = "make_tree_params"
+    _need(q, torch.float16, "q")
+    P, Hkv = _cache_shape(k_cache, v_cache, who)
+    if q.dim() != 3 or q.shape[2] != HEAD_DIM or q.shape[1] == 0 or q.shape[1] % Hkv:
+        raise CklError(2, who, f"q {tuple(q.shape)} for {Hkv} cached heads")
+    N, Hq = q.shape[0], q.shape[1]
+    for t, n in ((kv_indptr, "kv_indptr"), (kv_indices, "kv_indices"),
+                 (kv_last_page_len, "kv_last_page_len")):
+        _need(t, torch.int32, n)
+    B = kv_indptr.numel() - 1
+    _rows(kv_last_page_len, torch.int32, B, "kv_last_page_len", who)
+    _rows(q_indptr, torch.int32, B + 1, "q_indptr", who)
+    _rows(positions, torch.int32, N, "positions", who)
+    _rows(slopes, torch.float32, Hq, "slopes", who)
+    words = 0
+    if tree_mask is not None:
+        _need(tree_mask, torch.int32, "tree_mask")
+        if tree_mask.dim() != 2 or tree_mask.shape[0] < N:
+            raise CklError(2, who, f"tree_mask {tuple(tree_mask.shape)} for {N} tokens")
+        words = tree_mask.shape[1]
+    _here(who, q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, q_indptr, tree_mask,
+          positions, slopes)
+    nc, ct = C.c_int(1), C.c_int(PAGE)
+    if B > 0 and N > 0:
+        check(lib().ckl_tree_plan(Hq // Hkv, B, Hkv, max_q, max_len, window, force_chunks,
+                                  C.byref(nc), C.byref(ct)), "ckl_tree_plan")
+    ptr = lambda t: None if t is None else t.data_ptr()
+    p = TreeParams(ptr(q), ptr(k_cache), ptr(v_cache), ptr(kv_indptr), ptr(kv_indices),
+                   ptr(kv_last_page_len), ptr(q_indptr), ptr(tree_mask), ptr(positions),
+                   ptr(slopes), B, N, Hq, Hkv, max_q, words, nc.value, ct.value, window, P,
+                   1.0 / math.sqrt(HEAD_DIM) if sm_scale is None else sm_scale, softcap)
+    p._keep = (q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, q_indptr, tree_mask,
+               positions, slopes)
+    return p
+
+
+def tree_workspace_size(p: TreeParams):
+    return lib().ckl_tree_workspace_size(C.byref(p))
+
+
+def tree_attention(p: TreeParams, out=None, lse=None, workspace=None, stream=None):
+    """Attention of drafted tokens over the cache (ckl_tree_attention) -> (out fp16 [N,Hq,128],
+    lse fp32 [N,Hq])."""
+    torch = _torch()
+    dev = p._keep[0].device
+    if out is None:
+        out = torch.empty((p.N, p.Hq, HEAD_DIM), dtype=torch.float16, device=dev)
+    elif out.dtype != torch.float16 or out.numel() != p.N * p.Hq * HEAD_DIM or not out.is_contiguous():
+        raise CklError(1, "tree_attention", f"out {out.dtype} {tuple(out.shape)}")
+    if lse is None:
+        lse = torch.empty((p.N, p.Hq), dtype=torch.float32, device=dev)
+    elif lse.dtype != torch.float32 or lse.numel() != p.N * p.Hq or not lse.is_contiguous():
+        raise CklError(1, "tree_attention", f"lse {lse.dtype} {tuple(lse.shape)}")
+    need = tree_workspace_size(p)
+    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    if need and ws_bytes < need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        ws_bytes = need
+    check(lib().ckl_tree_attention(C.byref(p), _ptr(out), _ptr(lse), _ptr(workspace), ws_bytes,
+                                   _stream(stream)), "ckl_tree_attention")
+    return out, lse
+
+
+def cache_weights(p: TreeParams, lse, acc, *, decay=1.0, stream=None):
+    """acc[b, place] = decay * acc + the attention weight the place received from this call's
+    tokens (ckl_cache_weights), in place; lse from tree_attention, acc fp32 [B, >= max_len]
+    with contiguous rows."""
+    torch = _torch()
+    _need(lse, torch.float32, "lse")
+    if not acc.is_cuda or acc.dtype != torch.float32 or acc.dim() != 2 or acc.stride(1) != 1:
+        raise CklError(1, "cache_weights", "acc: expected CUDA float32 rows")
+    if acc.shape[0] < p.B or lse.numel() < p.N * p.Hq:
+        raise CklError(2, "cache_weights", f"acc {tuple(acc.shape)} / lse {tuple(lse.shape)}")
+    if acc.stride(0) < acc.shape[1] and acc.shape[0] > 1:
+        raise CklError(1, "cache_weights", "acc rows overlap")
+    _here("cache_weights", lse, acc)
+    stride = acc.stride(0) if acc.shape[0] > 1 else acc.shape[1]
+    check(lib().ckl_cache_weights(C.byref(p), _ptr(lse), _ptr(acc), stride, decay,
+                                  _stream(stream)), "ckl_cache_weights")
+    return acc
+
+
+def cache_select(acc, kv_indptr, kv_last_page_len, keep, *, sink=0, recent=0, keep_idx=None,
+                 keep_count=None, stream=None):
+    """The tokens to keep of every sequence by accumulated weight (ckl_cache_select) ->
+    (keep_idx int32 [B, keep] ascending, -1 behind the count; keep_count int32 [B])."""
+    torch = _torch()
+    if not acc.is_cuda or acc.dtype != torch.float32 or acc.dim() != 2 or acc.stride(1) != 1:
+        raise CklError(1, "cache_select", "acc: expected CUDA float32 rows")
+    _need(kv_indptr, torch.int32, "kv_indptr")
+    _need(kv_last_page_len, torch.int32, "kv_last_page_len")
+    B = kv_indptr.numel() - 1
+    if acc.shape[0] < B or kv_last_page_len.numel() < B:
+        raise CklError(2, "cache_select", f"acc {tuple(acc.shape)} for {B} sequences")
+    if keep_idx is None:
+        keep_idx = torch.empty((B, max(keep, 0)), dtype=torch.int32, device=acc.device)
+    if keep_count is None:
+        keep_count = torch.empty(B, dtype=torch.int32, device=acc.device)
+    _rows(keep_idx, torch.int32, B * keep, "keep_idx", "cache_select")
+    _rows(keep_count, torch.int32, B, "keep_count", "cache_select")
+    _here("cache_select", acc, kv_indptr, kv_last_page_len, keep_idx, keep_count)
+    stride = acc.stride(0) if acc.shape[0] > 1 else acc.shape[1]
+    check(lib().ckl_cache_select(_ptr(acc), stride, _ptr(kv_indptr), _ptr(kv_last_page_len), B,
+                                 keep, sink, recent, _ptr(keep_idx), _ptr(keep_count),
+                                 _stream(stream)), "ckl_cache_select")
+    return keep_idx, keep_count
+
+
+def cache_compact(k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, keep_idx, keep_count,
+                  *, dst_start=None, acc=None, new_len=None, stream=None):
+    """Moves the kept tokens of every sequence together, in place (ckl_cache_compact) -> the
+    new lengths int32 [B]. keep_idx int32 [B, n], keep_count int32 [B]; acc fp32 [B, >= L]."""
+    torch = _torch()
+    who = "cache_compact"
+    P, Hkv = _cache_shape(k_cache, v_cache, who)
+    for t, n in ((kv_indptr, "kv_indptr"), (kv_indices, "kv_indices"),
+                 (kv_last_page_len, "kv_last_page_len"), (keep_idx, "keep_idx"),
+                 (keep_count, "keep_count")):
+        _need(t, torch.int32, n)
+    B = kv_indptr.numel() - 1
+    if keep_idx.dim() != 2 or keep_idx.shape[0] < B:
+        raise CklError(2, who, f"keep_idx {tuple(keep_idx.shape)} for {B} sequences")
+    _rows(kv_last_page_len, torch.int32, B, "kv_last_page_len", who)
+    _rows(keep_count, torch.int32, B, "keep_count", who)
+    _rows(dst_start, torch.int32, B, "dst_start", who)
+    stride = 0
+    if acc is not None:
+        if (not acc.is_cuda or acc.dtype != torch.float32 or acc.dim() != 2 or acc.stride(1) != 1
+                or acc.shape[0] < B or (acc.shape[0] > 1 and acc.stride(0) < acc.shape[1])):
+            raise CklError(1, who, "acc: expected CUDA float32 rows, one per sequence")
+        stride = acc.stride(0) if acc.shape[0] > 1 else acc.shape[1]
+    if new_len is None:
+        new_len = torch.empty(B, dtype=torch.int32, device=k_cache.device)
+    _rows(new_len, torch.int32, B, "new_len", who)
+    _here(who, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, keep_idx, keep_count,
+          dst_start, acc, new_len)
+    check(lib().ckl_cache_compact(_ptr(k_cache), _ptr(v_cache), _ptr(kv_indptr), _ptr(kv_indices),
+                                  _ptr(kv_last_page_len), B, Hkv, P, _ptr(keep_idx),
+                                  keep_idx.shape[1], _ptr(keep_count), _ptr(dst_start), _ptr(acc),
+                                  stride, _ptr(new_len), _stream(stream)), "ckl_cache_compact")
+    return new_len
 
 
 # ------------------------------------------------------------------ MoE

@@ -1,0 +1,127 @@
+// tree_common.cuh -- what the draft-tree attention and the cache-weight kernels share: the
+// launch arguments, the geometry of a sequence and its new tokens, the scores and who sees what.
+#pragma once
+
+#include "attn_common.cuh"
+
+namespace ckl {
+namespace tree {
+
+using namespace attn;
+
+struct Args {
+    const __half* q;
+    const int* indptr;
+    const int* indices;
+    const int* last;
+    const int* q_indptr;      // NULL: one token per sequence
+    const uint32_t* mask;     // NULL: chain
+    const int* positions;     // NULL: cache places
+    const float* slopes;      // NULL: no bias
+    float* part_o;            // [N*Hq][num_chunks][128], NULL with one chunk
+    float* part_lse;          // [N*Hq][num_chunks]
+    __half* out;
+    float* lse;
+    unsigned* err;
+    unsigned long long timeout_ns;
+    int B, N, Hq, Hkv, G, max_q, mask_words, num_chunks, chunk_tokens, window, num_pages;
+    float scale_log2;         // sm_scale * log2(e)
+    float cap_log2;           // softcap * log2(e), 0: no cap
+    float cap_in;             // 2 log2(e) sm_scale / softcap
+};
+
+// Length of sequence b from the page table; a last page outside [0, 16] is taken as full/empty.
+__device__ __forceinline__ int seq_len(const int* indptr, const int* last, int b, int* page0) {
+    *page0 = __ldg(indptr + b);
+    const int np = __ldg(indptr + b + 1) - *page0;
+    return np > 0 ? (np - 1) * PAGE + min(max(__ldg(last + b), 0), PAGE) : 0;
+}
+
+struct Seq {
+    int page0;      // first entry of the page list
+    int len;        // cached tokens, new ones included
+    int q0, T;      // first row and count of the new tokens
+    int ctx;        // cache place of new token 0 (negative when the table is too short)
+    __device__ __forceinline__ Seq(const Args& a, int b) {
+        len = seq_len(a.indptr, a.last, b, &page0);
+        q0 = a.q_indptr ? __ldg(a.q_indptr + b) : b;
+        T = a.q_indptr ? __ldg(a.q_indptr + b + 1) - q0 : 1;
+        if (q0 < 0 || q0 + T > a.N || T < 0) T = 0;      // rows outside the tensors: none
+        ctx = len - T;
+    }
+    // Position of cached token p (p itself behind the sequence).
+    __device__ __forceinline__ int pos(const Args& a, int p) const {
+        return a.positions && p >= ctx && p < len ? __ldg(a.positions + q0 + (p - ctx)) : p;
+    }
+};
+
+// Least and greatest position of the sequence's tokens (one warp; all lanes get both).
+__device__ __forceinline__ void pos_range(const Args& a, const Seq& s, int lane, int* lo, int* hi) {
+    if (!a.positions) {
+        *lo = s.ctx;
+        *hi = s.len - 1;
+        return;
+    }
+    int l = 0x7fffffff, h = -0x7fffffff - 1;
+    for (int i = lane; i < s.T; i += 32) {
+        const int p = __ldg(a.positions + s.q0 + i);
+        l = min(l, p);
+        h = max(h, p);
+    }
+    *lo = __reduce_min_sync(0xffffffffu, l);
+    *hi = __reduce_max_sync(0xffffffffu, h);
+}
+
+// First cache place that any token of the sequence can see, rounded down to a page: context
+// keys at or below (least position - window) are out of every window. 64-bit: positions span
+// all of int32.
+__device__ __forceinline__ int first_key(const Args& a, const Seq& s, int pos_lo) {
+    if (a.window <= 0) return 0;
+    const long long f = (long long)pos_lo - a.window + 1;
+    const int lim = max(min(s.ctx, s.len), 0);           // drafted keys have their own positions
+    const int k = f <= 0 ? 0 : (f >= lim ? lim : (int)f);
+    return k & ~(PAGE - 1);
+}
+
+// One query row's view of the keys.
+struct Row {
+    int i = -1;           // new token (-1: padding)
+    int pos = 0;
+    float slope2 = 0.f;   // slope * log2(e)
+    __device__ __forceinline__ void set(const Args& a, const Seq& s, int row, int nrows, int kvh) {
+        if (row >= nrows) return;
+        i = row / a.G;
+        pos = a.positions ? __ldg(a.positions + s.q0 + i) : s.ctx + i;
+        if (a.slopes) slope2 = __ldg(a.slopes + kvh * a.G + row % a.G) * LOG2E;
+    }
+    // Is cached token p (at position kpos) seen?
+    __device__ __forceinline__ bool sees(const Args& a, const Seq& s, int p, int kpos) const {
+        if (i < 0 || p >= s.len) return false;
+        if (a.window > 0 && (long long)pos - kpos >= a.window) return false;
+        const int j = p - s.ctx;
+        if (j < 0) return true;
+        if (!a.mask) return j <= i;
+        if (j >= 32 * a.mask_words) return false;
+        return (__ldg(a.mask + (size_t)(s.q0 + i) * a.mask_words + (j >> 5)) >> (j & 31)) & 1u;
+    }
+};
+
+// Score in the log2 domain from the raw product q.k. The cap is tanh(x) = 1 - 2/(1 + e^2x):
+// its error is absolute, ~2^-23 of the cap, where tanh.approx would lose 2^-11 of the score.
+template <bool EXT>
+__device__ __forceinline__ float score(const Args& a, float qk) {
+    if (EXT && a.cap_log2 > 0.f)
+        return fmaf(-2.f * a.cap_log2, __fdividef(1.f, 1.f + ex2(qk * a.cap_in)), a.cap_log2);
+    return qk * a.scale_log2;
+}
+template <bool EXT>
+__device__ __forceinline__ float bias(const Args& a, float slope2, int pos, int kpos) {
+    return EXT ? slope2 * (float)(kpos - pos) : 0.f;
+}
+
+// tree_attention.cu: checks the parameters that the attention and the weights share.
+ckl_status check_params(const ckl_tree_params* p, const char* who);
+ckl_status fill_args(const ckl_tree_params* p, Args* a);
+
+}  // namespace tree
+}  // namespace ckl

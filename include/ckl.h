@@ -535,6 +535,167 @@ CKL_API ckl_status ckl_moe_ep_layer_ex(const ckl_moe_ep_comm* comm, int T_max, c
                                        size_t workspace_bytes, void* stream);
 
 /* ======================================================================================
+ * Writing, verifying and trimming the paged cache (no reference counterpart: the reference
+ * reads a cache that its main() fills). One step of a serving loop: ckl_rope_append writes
+ * the new tokens, ckl_decode_attention / ckl_tree_attention read the cache,
+ * ckl_cache_compact keeps the accepted path of a draft tree; ckl_cache_weights,
+ * ckl_cache_select and ckl_cache_compact trim a long cache to a budget.
+ *
+ * New (drafted) tokens of a batch are packed: token n of [q_indptr[b], q_indptr[b+1])
+ * belongs to sequence b; q_indptr NULL means one token per sequence (N == B). The page table
+ * covers them already: with L_b cached tokens and T_b new ones, new token i of sequence b has
+ * cache place L_b - T_b + i (below 0: the page table has no place for it). Rows of tokens at
+ * or behind q_indptr[B] are never written. A kv_last_page_len outside [0, 16] counts as the
+ * nearest of these.
+ * ==================================================================================== */
+
+/* Rotary plan, built on the host once and passed by address to each call (copied into the
+ * launch). Pair i of a head is (x[i], x[i + rot_dim/2]), or (x[2i], x[2i+1]) when
+ * interleaved; at position p it is turned by the angle p * f_i and multiplied by `scale`;
+ * dims from rot_dim on are copied. turns[i] = f_i / (2 pi) as a 64-bit binary fraction:
+ * p * turns[i] mod 2^64 is the turn at position p, wrapped exactly for every int32 p. */
+typedef struct ckl_rope {
+    int rot_dim;        /* rotated dims of a head: even, 2..128 */
+    int interleaved;
+    float scale;
+    int reserved;
+    uint64_t turns[CKL_HEAD_DIM / 2];
+} ckl_rope;
+
+/* f_i = base^(-2i/rot_dim), i < rot_dim/2, stretched to `factor` times the context:
+ *   CKL_ROPE_LINEAR    f_i / factor
+ *   CKL_ROPE_NTK       base * factor^(rot_dim/(rot_dim-2)) in place of base (rot_dim 2: unchanged)
+ *   CKL_ROPE_BY_PARTS  pairs that turn more than beta_fast times over original_len tokens are
+ *                      left, those that turn less than beta_slow times are divided by factor,
+ *                      and in between the two are blended linearly in i (between the pair
+ *                      index of beta_fast rounded down and that of beta_slow rounded up);
+ *                      scale = 0.1 ln(factor) + 1
+ * factor >= 1; original_len, beta_fast > beta_slow > 0 are read by CKL_ROPE_BY_PARTS only.
+ * Host only. */
+enum { CKL_ROPE_NONE = 0, CKL_ROPE_LINEAR = 1, CKL_ROPE_NTK = 2, CKL_ROPE_BY_PARTS = 3 };
+CKL_API ckl_status ckl_rope_plan(int rot_dim, int interleaved, double base, int scaling,
+                                 double factor, int original_len, double beta_fast,
+                                 double beta_slow, ckl_rope* rope);
+
+/* The same from the caller's own f_i (inv_freq[rot_dim/2], 0 <= f_i <= pi) and scale. Host
+ * only. */
+CKL_API ckl_status ckl_rope_plan_freqs(const double* inv_freq, int rot_dim, int interleaved,
+                                       double scale, ckl_rope* rope);
+
+typedef struct ckl_append_params {
+    const void* q;                 /* [N][Hq][128] fp16, tokens q_stride elements apart (e.g. a
+                                      slice of a fused projection); NULL: only the cache is
+                                      written */
+    const void* k;                 /* [N][Hkv][128], k_stride apart */
+    const void* v;                 /* [N][Hkv][128], v_stride apart */
+    long long q_stride, k_stride, v_stride;   /* elements, multiples of 8, at least a row's */
+    void* q_out;                   /* [N][Hq][128] contiguous (the q of the attention calls) */
+    void* k_cache;                 /* [num_pages][16][Hkv][128] */
+    void* v_cache;
+    const int* kv_indptr;          /* [B+1] page table, covering the new tokens */
+    const int* kv_indices;
+    const int* kv_last_page_len;   /* [B] */
+    const int* q_indptr;           /* [B+1], or NULL: one token per sequence */
+    const int* positions;          /* [N] rotary positions, or NULL: the tokens' cache places */
+    int B, N, Hq, Hkv, num_pages;
+} ckl_append_params;
+
+/* Rotates q into q_out and k into the cache, and copies v into the cache, rounding once from
+ * fp32 to fp16; rope NULL copies q and k unturned. All tensors 16-byte aligned; outputs must
+ * not overlap the inputs (CKL_INVALID_ARG). A page id outside [0, num_pages) is not written.
+ * Two tokens with the same place (a page listed twice) race. */
+CKL_API ckl_status ckl_rope_append(const ckl_append_params* p, const ckl_rope* rope, void* stream);
+
+/* Ancestor masks of draft trees, for ckl_tree_attention. parents[n] is the index, within its
+ * own sequence's tokens, of drafted token n's parent, lower than its own; anything else marks
+ * a root. Bit j of mask row n (word j/32, bit j%32 of [N][mask_words]) is set when token j of
+ * the same sequence is token n or an ancestor of it; tokens from 32*mask_words on have no bit.
+ * positions (optional, [N]): L_b - T_b + the token's depth. */
+CKL_API ckl_status ckl_tree_mask(const int* parents, const int* q_indptr, const int* kv_indptr,
+                                 const int* kv_last_page_len, int B, int N, int mask_words,
+                                 uint32_t* mask, int* positions, void* stream);
+
+/* Attention of drafted tokens over the cache that already holds their k and v. */
+typedef struct ckl_tree_params {
+    const void* q;                 /* [N, Hq, 128] fp16, 16-byte aligned */
+    const void* k_cache;           /* [num_pages, 16, Hkv, 128] fp16, 16-byte aligned */
+    const void* v_cache;
+    const int* kv_indptr;          /* [B+1] */
+    const int* kv_indices;
+    const int* kv_last_page_len;   /* [B] */
+    const int* q_indptr;           /* [B+1], or NULL: one token per sequence */
+    const uint32_t* tree_mask;     /* [N][mask_words]: bit j of row n = drafted token j of the
+                                      sequence is seen by token n; NULL: a chain (j <= i) */
+    const int* positions;          /* [N] token positions, or NULL: the cache places */
+    const float* slopes;           /* [Hq] distance bias, or NULL */
+    int B, N, Hq, Hkv;
+    int max_q;                     /* most drafted tokens of a sequence */
+    int mask_words;
+    int num_chunks, chunk_tokens;  /* ckl_tree_plan */
+    int window;                    /* 0: none */
+    int num_pages;
+    float sm_scale;
+    float softcap;                 /* 0: none */
+} ckl_tree_params;
+
+/* The split of the keys: chunks of about one wave of CTAs, multiples of 16 tokens.
+ * max_len: the longest sequence; a window bounds the keys read. Longer sequences than planned
+ * for are still attended whole (the last chunk takes what is left). Host only. */
+CKL_API ckl_status ckl_tree_plan(int G, int B, int Hkv, int max_q, int max_len, int window,
+                                 int force_chunks, int* num_chunks, int* chunk_tokens);
+
+CKL_API size_t ckl_tree_workspace_size(const ckl_tree_params* p);
+
+/* For drafted token i of sequence b (row n = q_indptr[b] + i), head h, over the cached tokens
+ * p < L_b:   s = sm_scale q.k_p;  s = softcap tanh(s / softcap);  s += slopes[h] (kpos - qpos)
+ * seen when  p < L_b - T_b, or the mask's bit of drafted token p - (L_b - T_b) is set; and
+ *            qpos - kpos < window.
+ * qpos = positions[n]; kpos = p for the context, the position of the drafted token for its
+ * key. out [N,Hq,128] = softmax(s) v in fp16, lse [N,Hq] fp32 natural log; a token that sees
+ * nothing gives out = 0, lse = -inf. Keys that a token does not see, and cache places behind
+ * the sequence, do not reach its result even where they hold infinities or NaN. With
+ * max_q = 1 and no options the results are ckl_decode_attention's up to the fp32 summation
+ * order. G = Hq/Hkv is any integer from 1 to 128. A sequence with more than max_q tokens has
+ * the tokens behind max_q left unwritten and records CKL_INVALID_ARG
+ * (ckl_check_device_error). Two calls in flight need two workspaces. */
+CKL_API ckl_status ckl_tree_attention(const ckl_tree_params* p, void* out, float* lse,
+                                      void* workspace, size_t workspace_bytes, void* stream);
+
+/* Accumulates the attention weight that every cached token received:
+ *   acc[b][p] = decay * acc[b][p] + sum over the sequence's tokens i and all heads of
+ *               exp(s - lse[n][h]), for p < L_b
+ * with s and the seen keys as in ckl_tree_attention and lse its output (a row with lse = -inf
+ * adds nothing). acc fp32, rows acc_stride elements apart; places p >= acc_stride are not
+ * kept, places from L_b on are left. Sums are taken in a fixed order. p->num_chunks and
+ * chunk_tokens are not read. */
+CKL_API ckl_status ckl_cache_weights(const ckl_tree_params* p, const float* lse, float* acc,
+                                     long long acc_stride, float decay, void* stream);
+
+/* Chooses the tokens to keep of every sequence: all when L_b <= keep, else `keep` of them --
+ * the first `sink`, the last `recent`, and of the rest those with the highest acc[b][p], ties
+ * to the lowest p (NaN ranks below every number; places p >= acc_stride rank as NaN). Writes
+ * keep_count[b] and keep_idx[b] ([B][keep], ascending, -1 behind the count).
+ * sink + recent <= keep. */
+CKL_API ckl_status ckl_cache_select(const float* acc, long long acc_stride, const int* kv_indptr,
+                                    const int* kv_last_page_len, int B, int keep, int sink,
+                                    int recent, int* keep_idx, int* keep_count, void* stream);
+
+/* Moves kept tokens together, in place: cached token keep_idx[b][i] of sequence b goes to
+ * place dst_start[b] + i, i < keep_count[b] (dst_start NULL: 0). The indices ascend strictly
+ * from at least dst_start[b] and are below L_b, so every token moves towards the front; a
+ * sequence whose list breaks this is left as it was and records CKL_INVALID_ARG
+ * (ckl_check_device_error). keep_idx rows are keep_stride apart; keep_count is capped at it.
+ * acc (optional, as in ckl_cache_weights): its entries move along, and those of places
+ * [new length, L_b) become 0. new_len (optional, [B]): dst_start[b] + keep_count[b] (L_b for
+ * a refused list). Pages that hold a moved token's new place must belong to that sequence
+ * alone. */
+CKL_API ckl_status ckl_cache_compact(void* k_cache, void* v_cache, const int* kv_indptr,
+                                     const int* kv_indices, const int* kv_last_page_len, int B,
+                                     int Hkv, int num_pages, const int* keep_idx, int keep_stride,
+                                     const int* keep_count, const int* dst_start, float* acc,
+                                     long long acc_stride, int* new_len, void* stream);
+
+/* ======================================================================================
  * Measurement
  * ==================================================================================== */
 
