@@ -217,80 +217,160 @@ __device__ __forceinline__ uint32_t rank_key(float x) {
 }
 
 constexpr int S_THREADS = 1024;
+constexpr int S_WARPS = S_THREADS / 32;
+constexpr int S_BINS = 2048;               // radix passes over 11, 11 and 10 bits
+constexpr int S_MAX_KEYS = 47 << 10;       // keys of a CTA's slice kept in shared memory, at most
+constexpr int S_SLICE = 4096;              // places per CTA that a cluster is sized for
 
-// One CTA per sequence: radix select of the threshold, 8 bits a pass, then an ordered pass that
-// writes the kept places.
-__global__ void __launch_bounds__(S_THREADS)
-select_kernel(const float* acc, long long stride, const int* indptr, const int* last, int keep, int sink,
-              int recent, int* keep_idx, int* keep_count) {
-    __shared__ int hist[256];
-    __shared__ int s_bin, s_left;
-    __shared__ int wgt[32], weq[32];
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// A 32-bit word of shared memory of CTA `rank` of the cluster, at this CTA's address `p`.
+__device__ __forceinline__ int cluster_load(const int* p, int rank) {
+    uint32_t at;
+    int v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+
+struct SArgs {
+    const float* acc;
+    const int* indptr;
+    const int* last;
+    int* keep_idx;
+    int* keep_count;
+    long long stride;
+    int keep, sink, recent, cluster, max_keys;
+};
+
+// Keeps the `want` greatest of a sequence's middle places. A cluster of CTAs (one for short
+// sequences) shares the sequence: each loads its slice once, as ordered integers in shared
+// memory; three radix passes narrow the threshold, each a histogram per CTA that all CTAs of the
+// cluster add up from one another's shared memory; then every warp counts and writes its part of
+// the list in order. Bound by latency: per pass one cluster barrier, two block barriers. A pass
+// whose bin is taken whole ends the search (the usual case after two passes unless values tie).
+// grid = (cluster, B).
+__global__ void __launch_bounds__(S_THREADS) select_kernel(const SArgs a) {
+    extern __shared__ uint32_t keys[];                       // [max_keys]
+    __shared__ int hist[3][S_BINS];
+    __shared__ int warp_sum[S_WARPS], warp_eq[S_WARPS];
+    __shared__ int s_bin, s_left, s_in;
+    __shared__ int total[2];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    for (int i = tid; i < 3 * S_BINS; i += S_THREADS) (&hist[0][0])[i] = 0;
     pdl_wait();
     pdl_trigger();
-    const int b = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int b = blockIdx.y, rank = blockIdx.x;
     int page0;
-    const int len = tree::seq_len(indptr, last, b, &page0);
-    int* out = keep_idx + (size_t)b * keep;
-    const int n = min(len, keep);
-    if (tid == 0) keep_count[b] = n;
-    if (len <= keep) {
-        for (int i = tid; i < keep; i += S_THREADS) out[i] = i < len ? i : -1;
+    const int len = tree::seq_len(a.indptr, a.last, b, &page0);
+    int* out = a.keep_idx + (size_t)b * a.keep;
+    const int step = a.cluster * S_THREADS, me = rank * S_THREADS + tid;
+    if (me == 0) a.keep_count[b] = min(len, a.keep);
+    if (len <= a.keep) {                                     // the same for the whole cluster
+        for (int i = me; i < a.keep; i += step) out[i] = i < len ? i : -1;
         return;
     }
-    const float* row = acc + b * stride;
-    auto key = [&](int p) { return p < stride ? rank_key(__ldg(row + p)) : 0u; };
-    const int lo = sink, hi = len - recent;
-    int want = keep - sink - recent;                 // of the places [lo, hi); hi - lo > want
-    for (int i = tid; i < sink; i += S_THREADS) out[i] = i;
-    for (int i = tid; i < recent; i += S_THREADS) out[keep - recent + i] = hi + i;
+    const int hi = len - a.recent, mid = hi - a.sink;
+    int want = a.keep - a.sink - a.recent;                   // of the places [sink, hi); mid > want
+    for (int i = me; i < a.sink; i += step) out[i] = i;
+    for (int i = me; i < a.recent; i += step) out[a.keep - a.recent + i] = hi + i;
     if (want == 0) return;
+    // this CTA's slice of the middle, a multiple of a warp's 32 places per warp
+    const int slice = ((mid + a.cluster - 1) / a.cluster + 31) & ~31;
+    const int beg = a.sink + min(mid, rank * slice), n = a.sink + min(mid, (rank + 1) * slice) - beg;
+    const float* row = a.acc + b * a.stride + beg;
+    const long long have = a.stride - beg;                   // places of the row that exist
+    auto load = [&](int i) { return i < have ? rank_key(__ldg(row + i)) : 0u; };
+    const bool held = n <= a.max_keys;                       // longer slices are read again from L2
+    if (held)
+        for (int i = tid; i < n; i += S_THREADS) keys[i] = load(i);
+    auto key = [&](int i) { return held ? keys[i] : load(i); };
+    __syncthreads();
+
     uint32_t prefix = 0, known = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
-        __syncthreads();
-        for (int p = lo + tid; p < hi; p += S_THREADS) {
-            const uint32_t k = key(p);
-            if ((k & known) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1);
+    for (int pass = 0; pass < 3; pass++) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        const uint32_t field = pass == 2 ? 1023u : 2047u;
+        int* h = hist[pass];
+        for (int i = tid; i < n; i += S_THREADS) {
+            const uint32_t k = key(i);
+            if ((k & known) == prefix) atomicAdd(&h[(k >> shift) & field], 1);
         }
-        __syncthreads();
-        if (tid == 0) {
-            int left = want, bin = 255;
-            while (bin > 0 && hist[bin] < left) left -= hist[bin--];
-            s_bin = bin;
-            s_left = left;
+        if (a.cluster > 1) cluster_sync();
+        else __syncthreads();
+        // bins from the greatest down, two per thread
+        const int bin = S_BINS - 1 - 2 * tid;
+        int c0 = 0, c1 = 0;
+        if (a.cluster > 1) {
+            for (int r = 0; r < a.cluster; r++) {
+                c0 += cluster_load(&h[bin], r);
+                c1 += cluster_load(&h[bin - 1], r);
+            }
+        } else {
+            c0 = h[bin];
+            c1 = h[bin - 1];
         }
+        int x = c0 + c1;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 31) warp_sum[warp] = x;
+        __syncthreads();
+        int before = lane < warp ? warp_sum[lane] : 0;
+        before = __reduce_add_sync(0xffffffffu, before);
+        const int up0 = before + x - c0 - c1, up1 = up0 + c0;     // keys above each bin
+        if (up0 < want && want <= up1) { s_bin = bin; s_left = want - up0; s_in = c0; }
+        if (up1 < want && want <= up1 + c1) { s_bin = bin - 1; s_left = want - up1; s_in = c1; }
         __syncthreads();
         prefix |= (uint32_t)s_bin << shift;
-        known |= 255u << shift;
+        known |= field << shift;
         want = s_left;
-        __syncthreads();
+        if (s_in == want) break;                             // the whole bin is kept
     }
-    // keys above `prefix` are kept, and the first `want` of those equal to it
-    int gt0 = 0, eq0 = 0;
-    for (int base = lo; base < hi; base += S_THREADS) {
-        const int p = base + tid;
-        const uint32_t k = p < hi ? key(p) : 0u;
-        const bool gt = p < hi && k > prefix, eq = p < hi && k == prefix;
-        const uint32_t bg = __ballot_sync(0xffffffffu, gt), be = __ballot_sync(0xffffffffu, eq);
-        if (lane == 0) {
-            wgt[warp] = __popc(bg);
-            weq[warp] = __popc(be);
+    // keys above `prefix` in the known bits are kept, and the first `want` of those equal to it
+    const int per = ((n + S_WARPS - 1) / S_WARPS + 31) & ~31;
+    const int w0 = min(n, warp * per), w1 = min(n, w0 + per);
+    int gt = 0, eq = 0;
+    for (int i = w0 + lane; i < w1; i += 32) {
+        const uint32_t k = key(i) & known;
+        gt += k > prefix;
+        eq += k == prefix;
+    }
+    gt = __reduce_add_sync(0xffffffffu, gt);
+    eq = __reduce_add_sync(0xffffffffu, eq);
+    if (lane == 0) {
+        warp_sum[warp] = gt;
+        warp_eq[warp] = eq;
+    }
+    __syncthreads();
+    int g = __reduce_add_sync(0xffffffffu, lane < warp ? warp_sum[lane] : 0);
+    int e = __reduce_add_sync(0xffffffffu, lane < warp ? warp_eq[lane] : 0);
+    if (a.cluster > 1) {
+        if (warp == S_WARPS - 1 && lane == 0) {
+            total[0] = g + gt;
+            total[1] = e + eq;
         }
-        __syncthreads();
-        int g = gt0, e = eq0, gs = 0, es = 0;
-        for (int i = 0; i < 32; i++) {
-            if (i == warp) { g += gs; e += es; }
-            gs += wgt[i];
-            es += weq[i];
+        cluster_sync();
+        for (int r = 0; r < rank; r++) {
+            g += cluster_load(&total[0], r);
+            e += cluster_load(&total[1], r);
         }
+        cluster_sync();                                      // nobody leaves while it is read
+    }
+    out += a.sink;
+    for (int base = w0; base < w1; base += 32) {
+        const int i = base + lane;
+        const uint32_t k = i < w1 ? key(i) & known : 0u;
+        const bool is_gt = i < w1 && k > prefix, is_eq = i < w1 && k == prefix;
+        const uint32_t bg = __ballot_sync(0xffffffffu, is_gt), be = __ballot_sync(0xffffffffu, is_eq);
         const uint32_t below = (1u << lane) - 1u;
-        g += __popc(bg & below);
-        e += __popc(be & below);
-        if (gt || (eq && e < want)) out[sink + g + min(e, want)] = p;
-        gt0 += gs;
-        eq0 += es;
-        __syncthreads();
+        const int ei = e + __popc(be & below);
+        if (is_gt || (is_eq && ei < want)) out[g + __popc(bg & below) + min(ei, want)] = beg + i;
+        g += __popc(bg);
+        e += __popc(be);
     }
 }
 
@@ -414,7 +494,9 @@ const Setup* setup(const DeviceInfo* di) {
         cudaError_t e = cudaFuncSetAttribute(weights_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, w_smem(Q_BIG));
         if (e == cudaSuccess)
             e = cudaFuncSetAttribute(weights_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, w_smem(Q_BIG));
-        if (e != cudaSuccess) ks[di->device].st = cuda_status(e, "cache weights setup");
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S_MAX_KEYS * 4);
+        if (e != cudaSuccess) ks[di->device].st = cuda_status(e, "cache kernels setup");
     });
     return &ks[di->device];
 }
@@ -472,9 +554,32 @@ ckl_status ckl_cache_select(const float* acc, long long acc_stride, const int* k
     if (B == 0) return CKL_OK;
     if (!acc || !kv_indptr || !kv_last_page_len || !keep_idx || !keep_count)
         return fail(CKL_INVALID_ARG, "cache_select: NULL tensor pointer");
-    if (!device_info()) return CKL_CUDA_ERROR;
-    void* args[] = {&acc, &acc_stride, &kv_indptr, &kv_last_page_len, &keep, &sink, &recent, &keep_idx, &keep_count};
-    CKL_CUDA_TRY(launch((const void*)select_kernel, dim3((unsigned)B), dim3(S_THREADS), 0, (cudaStream_t)stream, args, true));
+    if (B > 65535) return fail(CKL_UNSUPPORTED_SHAPE, "cache_select: B=%d (at most 65535)", B);
+    const DeviceInfo* di = device_info();
+    if (!di) return CKL_CUDA_ERROR;
+    const Setup* ks = setup(di);
+    if (ks->st != CKL_OK) return ks->st;
+    // a CTA per S_SLICE places, as long as the clusters of all sequences fit the GPU at once
+    int cluster = 1;
+    while (cluster < 8 && (long long)cluster * S_SLICE < acc_stride && (long long)B * cluster * 2 <= di->sms) cluster *= 2;
+    const long long slice = ((acc_stride + cluster - 1) / cluster + 31) & ~31LL;
+    SArgs a{acc, kv_indptr, kv_last_page_len, keep_idx, keep_count, acc_stride, keep, sink, recent, cluster,
+            (int)std::min(slice, (long long)S_MAX_KEYS)};
+    void* args[] = {&a};
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)cluster, (unsigned)B);
+    cfg.blockDim = dim3(S_THREADS);
+    cfg.dynamicSmemBytes = (size_t)a.max_keys * 4;
+    cfg.stream = (cudaStream_t)stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    CKL_CUDA_TRY(cudaLaunchKernelExC(&cfg, (const void*)select_kernel, args));
     return CKL_OK;
 }
 
