@@ -574,6 +574,16 @@ def cascade_tree_decode(tp: CascadeTreePlan, out=None, lse=None, workspace=None,
 ROPE_SCALING = {"none": 0, "linear": 1, "ntk": 2, "by_parts": 3}
 
 
+def _empty(shape, dtype, device, stream):
+    """A tensor that the call on `stream` writes: allocated on that stream, so that its memory is
+    reused only behind the call."""
+    torch = _torch()
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
 def _here(name, *tensors):
     """All tensors (None skipped) on the current device: the library launches there."""
     dev = _torch().cuda.current_device()
@@ -692,9 +702,9 @@ def tree_mask(parents, q_indptr, kv_indptr, kv_last_page_len, max_q, *, mask=Non
         _need(t, torch.int32, name)
         _rows(t, torch.int32, n, name, "tree_mask")
     if mask is None:
-        mask = torch.empty((N, W), dtype=torch.int32, device=parents.device)
+        mask = _empty((N, W), torch.int32, parents.device, stream)
     if positions is None:
-        positions = torch.empty(N, dtype=torch.int32, device=parents.device)
+        positions = _empty(N, torch.int32, parents.device, stream)
     _rows(mask, torch.int32, N * W, "mask", "tree_mask")
     _rows(positions, torch.int32, N, "positions", "tree_mask")
     _here("tree_mask", parents, q_indptr, kv_indptr, kv_last_page_len, mask, positions)
@@ -757,17 +767,17 @@ def tree_attention(p: TreeParams, out=None, lse=None, workspace=None, stream=Non
     torch = _torch()
     dev = p._keep[0].device
     if out is None:
-        out = torch.empty((p.N, p.Hq, HEAD_DIM), dtype=torch.float16, device=dev)
+        out = _empty((p.N, p.Hq, HEAD_DIM), torch.float16, dev, stream)
     elif out.dtype != torch.float16 or out.numel() != p.N * p.Hq * HEAD_DIM or not out.is_contiguous():
         raise CklError(1, "tree_attention", f"out {out.dtype} {tuple(out.shape)}")
     if lse is None:
-        lse = torch.empty((p.N, p.Hq), dtype=torch.float32, device=dev)
+        lse = _empty((p.N, p.Hq), torch.float32, dev, stream)
     elif lse.dtype != torch.float32 or lse.numel() != p.N * p.Hq or not lse.is_contiguous():
         raise CklError(1, "tree_attention", f"lse {lse.dtype} {tuple(lse.shape)}")
     need = tree_workspace_size(p)
     ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
     if need and ws_bytes < need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        workspace = _empty(need, torch.uint8, dev, stream)
         ws_bytes = need
     check(lib().ckl_tree_attention(C.byref(p), _ptr(out), _ptr(lse), _ptr(workspace), ws_bytes,
                                    _stream(stream)), "ckl_tree_attention")
@@ -806,9 +816,9 @@ def cache_select(acc, kv_indptr, kv_last_page_len, keep, *, sink=0, recent=0, ke
     if acc.shape[0] < B or kv_last_page_len.numel() < B:
         raise CklError(2, "cache_select", f"acc {tuple(acc.shape)} for {B} sequences")
     if keep_idx is None:
-        keep_idx = torch.empty((B, max(keep, 0)), dtype=torch.int32, device=acc.device)
+        keep_idx = _empty((B, max(keep, 0)), torch.int32, acc.device, stream)
     if keep_count is None:
-        keep_count = torch.empty(B, dtype=torch.int32, device=acc.device)
+        keep_count = _empty(B, torch.int32, acc.device, stream)
     _rows(keep_idx, torch.int32, B * keep, "keep_idx", "cache_select")
     _rows(keep_count, torch.int32, B, "keep_count", "cache_select")
     _here("cache_select", acc, kv_indptr, kv_last_page_len, keep_idx, keep_count)
@@ -843,7 +853,7 @@ def cache_compact(k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, kee
             raise CklError(1, who, "acc: expected CUDA float32 rows, one per sequence")
         stride = acc.stride(0) if acc.shape[0] > 1 else acc.shape[1]
     if new_len is None:
-        new_len = torch.empty(B, dtype=torch.int32, device=k_cache.device)
+        new_len = _empty(B, torch.int32, k_cache.device, stream)
     _rows(new_len, torch.int32, B, "new_len", who)
     _here(who, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, keep_idx, keep_count,
           dst_start, acc, new_len)

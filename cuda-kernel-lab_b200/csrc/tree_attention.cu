@@ -6,14 +6,15 @@
 // through a TMA ring, computes S = Q K^T, an online softmax in the log2 domain and O += P V;
 // split sequences are joined by their log-sum-exps in a second kernel.
 //
-//   rows of up to 32 (few drafts, single-token decode): mma.sync, four warps that take pages
-//   in turn (`rows_kernel`).
+//   up to 32 rows (few drafts, single-token decode): mma.sync, four warps that take pages in
+//   turn (`rows_kernel` here);
+//   more rows: tcgen05 on 128-row tiles (tree_tile.cu).
 
 #include <algorithm>
 #include <climits>
 #include <mutex>
 
-#include "tree_common.cuh"
+#include "tree_tile.cuh"
 
 namespace ckl {
 namespace tree {
@@ -218,7 +219,7 @@ struct State {
     }
 };
 
-// grid = (B * Hkv, num_chunks, row tiles of 16 * NT).
+// grid = (B * Hkv, num_chunks).
 template <int NT, bool EXT>
 __global__ void __launch_bounds__(THREADS, 2)
 rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const Args a) {
@@ -250,9 +251,9 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
     const uint64_t deadline = globaltimer() + a.timeout_ns;
 
     const Seq s(a, b);
-    if (s.T > a.max_q && chunk == 0 && blockIdx.z == 0 && threadIdx.x == 0) atomicOr(a.err, DEVERR_BOUND);
-    const int nrows = min(s.T, a.max_q) * a.G, row0 = blockIdx.z * R;
-    if (row0 >= nrows) return;                                          // the whole CTA
+    if (s.T > a.max_q && chunk == 0 && threadIdx.x == 0) atomicOr(a.err, DEVERR_BOUND);
+    const int nrows = min(s.T, a.max_q) * a.G;
+    if (nrows == 0) return;                                             // the whole CTA
     int pos_lo = 0, pos_hi = 0;
     if (a.window > 0) pos_range(a, s, lane, &pos_lo, &pos_hi);
     const Keys keys(a, s, first_key(a, s, pos_lo), chunk);
@@ -291,18 +292,18 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
     } else {
         // stage the Q rows (zeros behind the rows in use), 16 chunks of 16 bytes each
         for (int c = threadIdx.x; c < R * 16; c += CONSUMERS * 32) {
-            const int r = c >> 4, cd = c & 15, rr = row0 + r;
+            const int rr = c >> 4, cd = c & 15;
             uint4 v = make_uint4(0u, 0u, 0u, 0u);
             if (rr < nrows)
                 v = __ldg(reinterpret_cast<const uint4*>(
                         a.q + ((size_t)(s.q0 + rr / a.G) * a.Hq + kvh * a.G + rr % a.G) * D) + cd);
-            *reinterpret_cast<uint4*>(qs + (r >> 4) * KV_TILE + tile_off(r & 15, cd)) = v;
+            *reinterpret_cast<uint4*>(qs + (rr >> 4) * KV_TILE + tile_off(rr & 15, cd)) = v;
         }
         asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS * 32) : "memory");
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int r = 0; r < 2; r++) st.row[n][r].set(a, s, row0 + 16 * n + 8 * r + g, nrows, kvh);
+            for (int r = 0; r < 2; r++) st.row[n][r].set(a, s, 16 * n + 8 * r + g, nrows, kvh);
         st.reset();
         bool ok = true;
         for (int i = warp; i < npg; i += CONSUMERS) {
@@ -344,8 +345,8 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
     __syncthreads();
     const float* ost = reinterpret_cast<const float*>(ring);
     for (int idx = threadIdx.x; idx < R * (D / 2); idx += THREADS) {
-        const int r = idx / (D / 2), d = 2 * (idx - r * (D / 2)), rr = row0 + r;
-        if (rr >= nrows) break;
+        const int r = idx / (D / 2), d = 2 * (idx - r * (D / 2));
+        if (r >= nrows) break;
         float M = -INFINITY;
 #pragma unroll
         for (int w = 0; w < CONSUMERS; w++) M = fmaxf(M, m_red[w * R + r]);
@@ -361,7 +362,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
         }
         const float inv = L != 0.f ? 1.f / L : 0.f;
         const float lse_v = L != 0.f ? (M + lg2(L)) * LN2 : -INFINITY;
-        const size_t row = (size_t)(s.q0 + rr / a.G) * a.Hq + kvh * a.G + rr % a.G;
+        const size_t row = (size_t)(s.q0 + r / a.G) * a.Hq + kvh * a.G + r % a.G;
         if (a.num_chunks == 1) {
             *reinterpret_cast<uint32_t*>(a.out + row * D + d) = pack_half2(o0 * inv, o1 * inv);
             if (d == 0) a.lse[row] = lse_v;
@@ -533,6 +534,7 @@ ckl_status fill_args(const ckl_tree_params* p, Args* a) {
     if (!di) return CKL_CUDA_ERROR;
     *a = Args{};
     a->q = static_cast<const __half*>(p->q);
+    a->v = static_cast<const __half*>(p->v_cache);
     a->indptr = p->kv_indptr;
     a->indices = p->kv_indices;
     a->last = p->kv_last_page_len;
@@ -568,6 +570,17 @@ ckl_status check_split(const ckl_tree_params* p) {
     return CKL_OK;
 }
 
+// More rows than the mma.sync kernel takes: a 16-row tile there re-reads every page, which holds
+// up to 32 rows; the tcgen05 kernel spends a 128-row tile on any number.
+bool use_tiles(const ckl_tree_params* p) { return (long long)p->max_q * (p->Hq / p->Hkv) > 32; }
+
+// CTAs of the tcgen05 kernel: num_chunks for each unit (sequence, kv head, row group), one wave
+// at most.
+int tile_ctas(const ckl_tree_params* p, int sms) {
+    const long long rows = (long long)p->max_q * (p->Hq / p->Hkv), per = 128LL * tile_count(rows);
+    return (int)std::min((long long)sms, (long long)p->B * p->Hkv * ((rows + per - 1) / per) * p->num_chunks);
+}
+
 size_t part_o_size(const ckl_tree_params* p) {
     return align_up((size_t)p->N * p->Hq * p->num_chunks * D * sizeof(float), 256);
 }
@@ -595,9 +608,13 @@ ckl_status ckl_tree_plan(int G, int B, int Hkv, int max_q, int max_len, int wind
     } else {
         const DeviceInfo* di = device_info();
         if (!di) return CKL_CUDA_ERROR;
-        const long long rows = (long long)max_q * G, per = 16LL * row_tiles((int)std::min(rows, 64LL));
+        const long long rows = (long long)max_q * G;
+        const long long per = rows > 32 ? 128LL * tile_count(rows) : 16LL * row_tiles((int)rows);
         const long long units = (long long)B * Hkv * ((rows + per - 1) / per);
-        chunks = std::min(std::max(1LL, 2LL * di->sms / units), (len + 255) / 256);
+        // two resident CTAs per SM up to 32 rows; the tcgen05 kernel takes the SM, and divides
+        // the work of all units evenly over its CTAs whatever the chunks are
+        const long long want = rows > 32 ? (di->sms + units - 1) / units : 2LL * di->sms / units;
+        chunks = std::min(std::max(1LL, want), (len + 255) / 256);
     }
     chunks = std::min(chunks, 65535LL);
     const long long tok = (((len + chunks - 1) / chunks) + PAGE - 1) / PAGE * PAGE;
@@ -607,7 +624,13 @@ ckl_status ckl_tree_plan(int G, int B, int Hkv, int max_q, int max_len, int wind
 }
 
 size_t ckl_tree_workspace_size(const ckl_tree_params* p) {
-    if (!p || p->N <= 0 || p->B <= 0 || p->num_chunks == 1) return 0;
+    if (!p || p->N <= 0 || p->B <= 0) return 0;
+    if (p->Hq > 0 && p->Hkv > 0 && p->max_q > 0 && p->num_chunks > 0 && use_tiles(p)) {
+        const DeviceInfo* di = device_info();
+        if (!di) return SIZE_MAX;
+        return tile_workspace(tile_ctas(p, di->sms), (long long)p->max_q * (p->Hq / p->Hkv));
+    }
+    if (p->num_chunks == 1) return 0;
     // shapes the launch would reject: report a size no caller can provide
     if (p->Hq <= 0 || p->num_chunks <= 0 || p->num_chunks > 65535 || (long long)p->N * p->Hq > 0x7fffffffLL)
         return SIZE_MAX;
@@ -644,16 +667,14 @@ ckl_status ckl_tree_attention(const ckl_tree_params* p, void* out, float* lse, v
         a.part_lse = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + part_o_size(p));
     }
     const cudaStream_t s = (cudaStream_t)stream;
-    const long long rows = (long long)p->max_q * a.G;
-    const int NT = row_tiles((int)std::min(rows, 64LL));
-    const long long tiles = (rows + 16 * NT - 1) / (16 * NT);
-    if (tiles > 65535) return fail(CKL_UNSUPPORTED_SHAPE, "tree_attention: max_q=%d is too large", p->max_q);
+    if (use_tiles(p)) return launch_tiles(p, a, workspace, tile_ctas(p, di->sms), s);
+    const int NT = row_tiles(p->max_q * a.G);
     const bool ext = p->softcap > 0.f || p->slopes;
     CUtensorMap tmK, tmV;
     st = encode_page_maps(p->k_cache, p->v_cache, p->Hkv, p->num_pages, &tmK, &tmV);
     if (st != CKL_OK) return st;
     void* args[] = {&tmK, &tmV, &a};
-    CKL_CUDA_TRY(launch(rows_fn(NT, ext), dim3((unsigned)(p->B * p->Hkv), (unsigned)p->num_chunks, (unsigned)tiles),
+    CKL_CUDA_TRY(launch(rows_fn(NT, ext), dim3((unsigned)(p->B * p->Hkv), (unsigned)p->num_chunks),
                         dim3(THREADS), rows_bytes(NT), s, args, true));
     if (p->num_chunks == 1) return CKL_OK;
     void* margs[] = {&a};

@@ -11,6 +11,7 @@ using namespace attn;
 
 struct Args {
     const __half* q;
+    const __half* v;          // the V cache (the streamed reads go through tensor maps)
     const int* indptr;
     const int* indices;
     const int* last;

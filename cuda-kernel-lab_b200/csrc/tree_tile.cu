@@ -1,0 +1,756 @@
+// tree_tile.cu -- the draft-tree attention for more than 32 stacked rows (drafted tokens x query
+// heads of a kv head) on the 5th-generation tensor cores.
+//
+// A CTA holds 128 * MT rows of one (sequence, kv head) as MT tiles, the M of tcgen05.mma, and
+// streams keys in blocks of 8 pages:
+//   S = Q K^T   M=128, N=64, twice per block: Q and K (both K-major) in shared memory, S in
+//               tensor memory (128 columns a tile);
+//   softmax     one thread per row: the row of S from tensor memory, online max and sum in
+//               registers, P = exp2(S - m) as fp16 back into tensor memory, over S;
+//   O += P V    M=128, N=128, K=16 a page: P from tensor memory, V (MN-major) from shared
+//               memory, O in tensor memory for the whole run.
+// Both tiles use the same K and V block: with 256 rows the stream is read once where the tensor
+// cores still keep up with it (512 flops per byte of K and V against the card's ~256).
+//
+// A page arrives as one 4 KB box per K and V: [64-dim half][16 tokens][64 dims]. A block's eight
+// pages lie 4 KB apart, so the keys 0-7 of all pages (8-row groups, 4 KB stride) form one MMA
+// operand of N = 64 and the keys 8-15 another: S column u*64 + 8*page + k is key 16*page + 8*u + k.
+//
+// Work is divided exactly: the key blocks of all (sequence, row group, kv head) units, end to
+// end, over one wave of CTAs. A unit that lies within one CTA is written out directly; where a
+// CTA's run of blocks crosses a unit's border it leaves a partial (at most two per CTA) and a
+// second kernel joins them.
+
+#include <algorithm>
+#include <mutex>
+
+#include "tree_tile.cuh"
+
+namespace ckl {
+namespace tree {
+namespace tile {
+
+constexpr int BLK_PAGES = 8;
+constexpr int BLK = BLK_PAGES * PAGE;              // 128 keys
+constexpr int KV_BLK = BLK_PAGES * KV_TILE;        // 32 KB of K or V
+constexpr int Q_TILE = 128 * D * 2;                // 32 KB: dims 0-63 of 128 rows, then 64-127
+constexpr int VST = 2;                             // V blocks in flight
+template <int MT> struct Cfg {
+    static constexpr int KST = MT == 1 ? 4 : 3;    // K blocks in flight
+    static constexpr int THREADS = 64 + 128 * MT;
+    static constexpr int ROWS = 128 * MT;
+    static constexpr int OFF_K = MT * Q_TILE;
+    static constexpr int OFF_V = OFF_K + KST * KV_BLK;
+    static constexpr int OFF_BAR = OFF_V + VST * KV_BLK;
+    static constexpr int NBAR = 2 * KST + 2 * VST + 4 * MT + 1;
+    static constexpr int SMEM = 1024 + OFF_BAR + NBAR * 8 + 32;
+    static constexpr uint32_t TMEM_COLS = MT == 1 ? 256 : 512;   // per tile: S (and P) 128, O 128
+};
+static_assert(Cfg<1>::SMEM <= 232448 && Cfg<2>::SMEM <= 232448, "shared memory of a CTA");
+
+__device__ __forceinline__ uint32_t sw128(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
+
+// Blocks of keys of a unit of sequence s whose keys start at `first`: at least one, so that rows
+// that see nothing are written too.
+__device__ __forceinline__ int blocks_of(const Seq& s, int first) {
+    return s.len > first ? (s.len - first + BLK - 1) / BLK : 1;
+}
+struct Work {                                       // of one sequence
+    int first = 0, nblk = 0, nrows = 0, units = 0;
+    __device__ __forceinline__ long long blocks() const { return (long long)nblk * units; }
+};
+template <int ROWS>
+__device__ __forceinline__ Work work_of(const Args& a, const Seq& s, int pos_lo) {
+    Work w;
+    w.nrows = min(s.T, a.max_q) * a.G;
+    if (w.nrows == 0) return w;
+    w.first = first_key(a, s, pos_lo);
+    w.nblk = blocks_of(s, w.first);
+    w.units = (w.nrows + ROWS - 1) / ROWS * a.Hkv;
+    return w;
+}
+// The same by one lane alone.
+template <int ROWS>
+__device__ __forceinline__ long long blocks_lane(const Args& a, int b) {
+    if (b >= a.B) return 0;
+    const Seq s(a, b);
+    int lo = s.ctx;
+    if (a.window > 0 && a.positions) {
+        lo = 0x7fffffff;
+        for (int i = 0; i < s.T; i++) lo = min(lo, __ldg(a.positions + s.q0 + i));
+    }
+    return work_of<ROWS>(a, s, lo).blocks();
+}
+// Blocks of sequences [0, upto) (one warp, all lanes get the sum).
+template <int ROWS>
+__device__ __forceinline__ long long blocks_before(const Args& a, int upto, int lane) {
+    long long sum = 0;
+    for (int b0 = 0; b0 < upto; b0 += 32) sum += b0 + lane < upto ? blocks_lane<ROWS>(a, b0 + lane) : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return sum;
+}
+// First block of CTA c of n over W blocks.
+__device__ __forceinline__ long long share(long long W, int c, int n) { return W * c / n; }
+
+// A CTA's run of blocks, unit by unit. All lanes of a warp hold the same state.
+struct Seg {
+    int b, kvh, row0, rows;      // rows of this unit: [row0, row0 + rows) of the sequence's
+    int blk0, blk1, nblk;
+};
+template <int ROWS>
+struct Walk {
+    long long left;              // blocks of this CTA not handed out yet
+    long long off;               // next block within sequence b
+    int b;
+    __device__ __forceinline__ Walk(long long left_, long long off_, int b_) : left(left_), off(off_), b(b_) {}
+    // The next segment, its sequence and work; false at the end.
+    __device__ __forceinline__ bool next(const Args& a, Seg* g, Seq* s, Work* w, int* pos_hi, int lane) {
+        while (left > 0 && b < a.B) {
+            *s = Seq(a, b);
+            int lo = s->ctx;
+            *pos_hi = s->len - 1;
+            if (a.window > 0) pos_range(a, *s, lane, &lo, pos_hi);
+            *w = work_of<ROWS>(a, *s, lo);
+            if (off >= w->blocks()) {
+                off -= w->blocks();
+                b++;
+                continue;
+            }
+            const int unit = (int)(off / w->nblk), z = unit / a.Hkv;
+            g->b = b;
+            g->kvh = unit - z * a.Hkv;
+            g->row0 = z * ROWS;
+            g->rows = min(ROWS, w->nrows - g->row0);
+            g->nblk = w->nblk;
+            g->blk0 = (int)(off - (long long)unit * w->nblk);
+            g->blk1 = (int)min((long long)w->nblk, g->blk0 + left);
+            off += g->blk1 - g->blk0;
+            left -= g->blk1 - g->blk0;
+            return true;
+        }
+        return false;
+    }
+};
+
+// Which of the keys [p, p + 32) row r sees, as bits.
+__device__ __forceinline__ uint32_t seen32(const Args& a, const Seq& s, const Row& r, int p) {
+    if (r.i < 0) return 0u;
+    const int in = s.len - p;                                     // keys within the sequence
+    uint32_t v = in >= 32 ? 0xffffffffu : in <= 0 ? 0u : (1u << in) - 1u;
+    const int j0 = p - s.ctx;                                     // drafted index of the first key
+    if (j0 > -32) {
+        uint32_t d;                                               // bits of drafted keys j0 .. j0 + 31
+        if (a.mask) {
+            const uint32_t* m = a.mask + (size_t)(s.q0 + r.i) * a.mask_words;
+            auto word = [&](int w) { return w >= 0 && w < a.mask_words ? __ldg(m + w) : 0u; };
+            const int w = j0 >> 5;                                // floor
+            d = __funnelshift_r(word(w), word(w + 1), j0 & 31);
+        } else {
+            const int n = r.i - j0 + 1;                           // j <= i
+            d = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
+        }
+        if (j0 < 0) d |= (1u << -j0) - 1u;                        // context keys
+        v &= d;
+    }
+    if (a.window > 0) {
+        for (uint32_t m = v; m; m &= m - 1) {
+            const int k = __ffs(m) - 1;
+            if ((long long)r.pos - s.pos(a, p + k) >= a.window) v &= ~(1u << k);
+        }
+    }
+    return v;
+}
+
+template <int MT, bool EXT>
+__global__ void __launch_bounds__(Cfg<MT>::THREADS, 1)
+tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const Args a) {
+    using C = Cfg<MT>;
+    constexpr int KST = C::KST;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* sm = align_ptr<1024>(smem_raw);
+    uint8_t* qs = sm;
+    uint8_t* kring = sm + C::OFF_K;
+    uint8_t* vring = sm + C::OFF_V;
+    uint64_t* k_full = reinterpret_cast<uint64_t*>(sm + C::OFF_BAR);
+    uint64_t* k_empty = k_full + KST;
+    uint64_t* v_full = k_empty + KST;
+    uint64_t* v_empty = v_full + VST;
+    uint64_t* q_full = v_empty + VST;        // [MT] Q staged for a segment (softmax -> MMA)
+    uint64_t* s_full = q_full + MT;          // [MT] S written (MMA -> softmax); O holds the blocks before
+    uint64_t* p_full = s_full + MT;          // [MT] P written (softmax -> MMA)
+    uint64_t* o_done = p_full + MT;          // [MT] O holds the block (MMA -> softmax, MMA)
+    uint64_t* done = o_done + MT;            // every issued MMA finished
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+    volatile int* odd = reinterpret_cast<volatile int*>(tmem_slot + 1);   // unseen V held inf or NaN
+    long long* range = reinterpret_cast<long long*>(tmem_slot + 2);       // {left, offset}, sequence
+    int* range_b = reinterpret_cast<int*>(range + 2);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < KST; i++) {
+            mbar_init(&k_full[i], 1);
+            mbar_init(&k_empty[i], 1);
+        }
+        for (int i = 0; i < VST; i++) {
+            mbar_init(&v_full[i], 1);
+            mbar_init(&v_empty[i], 1);
+        }
+        for (int t = 0; t < MT; t++) {
+            mbar_init(&q_full[t], 128);
+            mbar_init(&s_full[t], 1);
+            mbar_init(&p_full[t], 128);
+            mbar_init(&o_done[t], 1);
+        }
+        mbar_init(done, 1);
+        fence_barrier_init();
+        *odd = 0;
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, C::TMEM_COLS);
+        tmem_relinquish();
+    }
+    if (warp == 0 && lane == 0) {
+        tma_prefetch_desc(&tmK);
+        tma_prefetch_desc(&tmV);
+    }
+    pdl_wait();
+    if (warp == 2) {
+        const long long W = blocks_before<C::ROWS>(a, a.B, lane);
+        const long long beg = share(W, blockIdx.x, gridDim.x), end = share(W, blockIdx.x + 1, gridDim.x);
+        long long before = 0;
+        int b = a.B;
+        for (int b0 = 0; b0 < a.B && b == a.B; b0 += 32) {
+            const long long mine = blocks_lane<C::ROWS>(a, b0 + lane);
+            long long x = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long y = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += y;
+            }
+            const unsigned over = __ballot_sync(0xffffffffu, before + x > beg);
+            if (over) {
+                const int l = __ffs(over) - 1;
+                b = b0 + l;
+                before += __shfl_sync(0xffffffffu, x - mine, l);
+            } else {
+                before += __shfl_sync(0xffffffffu, x, 31);
+            }
+        }
+        if (lane == 0) {
+            range[0] = end - beg;
+            range[1] = beg - before;
+            *range_b = b;
+        }
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    pdl_trigger();
+    const uint32_t tmem = *tmem_slot;
+    const uint64_t deadline = globaltimer() + a.timeout_ns;
+    Walk<C::ROWS> walk(range[0], range[1], *range_b);
+    Seg g;
+    Seq s(a, 0);
+    Work w;
+    int pos_hi;
+
+    if (warp == 0) {
+        // ---------------------------------------------------------------- TMA producer
+        const uint64_t pol = policy_evict_first();
+        int ok = 1, n = 0;                              // n: blocks issued
+        while (ok && walk.next(a, &g, &s, &w, &pos_hi, lane)) {
+            const int p0 = w.first / PAGE, npg = (s.len + PAGE - 1) / PAGE;
+            int ids_at = 0, my_id = 0;
+            for (int j = g.blk0; j < g.blk1 && ok; j++, n++) {
+                const int at = p0 + j * BLK_PAGES;
+                // page ids, 32 per load; a page behind the sequence reads as zeros (its
+                // coordinate is past the tensor map's extent)
+                if (j == g.blk0 || at >= ids_at + 32) {
+                    ids_at = at;
+                    my_id = at + lane < npg ? __ldg(a.indices + s.page0 + at + lane) : a.num_pages;
+                }
+                const int page = __shfl_sync(0xffffffffu, my_id, at - ids_at + (lane & (BLK_PAGES - 1)));
+                const int ks = n % KST, vs = n % VST;
+                if (lane == 0) {
+                    if (n >= KST) ok = mbar_wait(&k_empty[ks], ((n / KST) - 1) & 1, deadline, a.err);
+                    if (ok) mbar_arrive_expect_tx(&k_full[ks], KV_BLK);
+                }
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+                if (!ok) break;
+                if (lane < BLK_PAGES)
+                    tma_load_5d(kring + ks * KV_BLK + lane * KV_TILE, &tmK, 0, 0, 0, g.kvh, page, &k_full[ks], pol);
+                if (lane == 0) {
+                    if (n >= VST) ok = mbar_wait(&v_empty[vs], ((n / VST) - 1) & 1, deadline, a.err);
+                    if (ok) mbar_arrive_expect_tx(&v_full[vs], KV_BLK);
+                }
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+                if (!ok) { n++; break; }                // its K is in flight, its V is not
+                if (lane < BLK_PAGES)
+                    tma_load_5d(vring + vs * KV_BLK + lane * KV_TILE, &tmV, 0, 0, 0, g.kvh, page, &v_full[vs], pol);
+            }
+        }
+        // every issued copy must land before the CTA exits (a wait for a phase that was never
+        // armed, after a timeout, ends at the deadline)
+        if (lane == 0) {
+            for (int i = 0; i < KST && i < n; i++)
+                mbar_wait(&k_full[i], ((i + (n - 1 - i) / KST * KST) / KST) & 1, deadline, a.err);
+            for (int i = 0; i < VST && i < n; i++)
+                mbar_wait(&v_full[i], ((i + (n - 1 - i) / VST * VST) / VST) & 1, deadline, a.err);
+        }
+    } else if (warp == 1) {
+        // ---------------------------------------------------------------- MMA issuer
+        const uint32_t idesc_s = umma_idesc_f16(128, 64, false, false);
+        const uint32_t idesc_o = umma_idesc_f16(128, D, false, true);
+        const uint32_t qa = smem_u32(qs), ka = smem_u32(kring), va = smem_u32(vring);
+        int ok = 1, n = 0;                              // n: blocks before this segment
+        int cnt[MT];                                    // blocks done by each tile
+#pragma unroll
+        for (int t = 0; t < MT; t++) cnt[t] = 0;
+        int qph[MT];
+#pragma unroll
+        for (int t = 0; t < MT; t++) qph[t] = 0;
+        while (ok && walk.next(a, &g, &s, &w, &pos_hi, lane)) {
+            const int nt = (g.rows + 127) / 128, nb = g.blk1 - g.blk0;
+            if (lane == 0) {
+                // S of block j (of this segment), tile t
+                auto qk = [&](int j, int t) {
+                    const int ks = (n + j) % KST;
+                    const uint32_t kb = ka + ks * KV_BLK, qb = qa + t * Q_TILE, d = tmem + t * 256;
+#pragma unroll
+                    for (int u = 0; u < 2; u++)
+#pragma unroll
+                        for (int kk = 0; kk < 8; kk++)
+                            umma_f16(d + u * 64,
+                                     umma_desc_sw128(qb + (kk >> 2) * (Q_TILE / 2) + (kk & 3) * 32, 16, 1024),
+                                     umma_desc_sw128(kb + u * 1024 + (kk >> 2) * HALF_TILE + (kk & 3) * 32, 16, KV_TILE),
+                                     idesc_s, kk != 0);
+                    umma_commit(&s_full[t]);
+                    if (t == nt - 1) umma_commit(&k_empty[ks]);
+                };
+                ok = mbar_wait(&k_full[n % KST], (n / KST) & 1, deadline, a.err);
+                for (int t = 0; t < nt && ok; t++) {
+                    ok = mbar_wait(&q_full[t], qph[t] & 1, deadline, a.err);
+                    qph[t]++;
+                    if (!ok) break;
+                    tc_fence_after_sync();
+                    qk(0, t);
+                }
+                for (int j = 0; j < nb && ok; j++) {
+                    const int vs = (n + j) % VST;
+                    for (int t = 0; t < nt && ok; t++) {
+                        ok = mbar_wait(&p_full[t], cnt[t] & 1, deadline, a.err);
+                        if (ok && t == 0) ok = mbar_wait(&v_full[vs], ((n + j) / VST) & 1, deadline, a.err);
+                        if (!ok) break;
+                        tc_fence_after_sync();
+                        const uint32_t vb = va + vs * KV_BLK, d = tmem + t * 256;
+#pragma unroll
+                        for (int pg = 0; pg < BLK_PAGES; pg++)
+                            umma_f16_ts(d + 128, d + pg * 8, umma_desc_sw128(vb + pg * KV_TILE, HALF_TILE, 1024),
+                                        idesc_o, (j | pg) != 0);
+                        umma_commit(&o_done[t]);
+                        if (t == nt - 1) umma_commit(&v_empty[vs]);
+                        cnt[t]++;
+                        if (j + 1 < nb) {
+                            const int k1 = n + j + 1;
+                            if (t == 0) ok = mbar_wait(&k_full[k1 % KST], (k1 / KST) & 1, deadline, a.err);
+                            // P (over S) must have been read before S is written again
+                            if (ok) ok = mbar_wait(&o_done[t], (cnt[t] - 1) & 1, deadline, a.err);
+                            if (!ok) break;
+                            tc_fence_after_sync();
+                            qk(j + 1, t);
+                        }
+                    }
+                }
+            }
+            ok = __shfl_sync(0xffffffffu, ok, 0);
+            n += nb;
+        }
+        if (lane == 0) umma_commit(done);
+        __syncwarp();
+    } else {
+        // ---------------------------------------------------------------- softmax: a row per thread
+        const int t = (warp - 2) >> 2, quarter = warp & 3;
+        const int r = quarter * 32 + lane;              // row of the tile
+        const uint32_t trow = tmem + t * 256 + ((uint32_t)(quarter * 32) << 16);
+        bool ok = true;
+        int cnt = 0, n = 0;                             // blocks of this tile; blocks of the CTA
+        while (walk.next(a, &g, &s, &w, &pos_hi, lane)) {
+            const int nt = (g.rows + 127) / 128, nb = g.blk1 - g.blk0;
+            if (t < nt) {
+                const int rr = g.row0 + t * 128 + r;
+                Row row;
+                row.set(a, s, rr, g.row0 + g.rows, g.kvh);
+                const size_t orow = (size_t)(s.q0 + max(row.i, 0)) * a.Hq + g.kvh * a.G + (rr - max(row.i, 0) * a.G);
+                {
+                    // the tile's earlier S have been read by the tensor core: its last o_done
+                    // was waited for in the epilogue
+                    const uint4* src = reinterpret_cast<const uint4*>(a.q + orow * D);
+#pragma unroll
+                    for (int c = 0; c < 16; c++) {
+                        const uint4 v = row.i >= 0 ? __ldg(src + c) : make_uint4(0u, 0u, 0u, 0u);
+                        *reinterpret_cast<uint4*>(qs + t * Q_TILE + (c >> 3) * (Q_TILE / 2) + sw128(r, c & 7)) = v;
+                    }
+                }
+                fence_proxy_async_smem();
+                mbar_arrive(&q_full[t]);
+
+                const bool idle = t * 128 + quarter * 32 >= g.rows;   // only padding rows: no softmax
+                float m = -INFINITY, l = 0.f;
+                for (int j = 0; j < nb; j++) {
+                    const int kbase = w.first + (g.blk0 + j) * BLK;
+                    const bool whole = kbase + BLK <= s.ctx && (a.window <= 0 || (long long)pos_hi - kbase < a.window);
+                    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], cnt & 1, deadline, a.err));
+                    if (!whole) {
+                        // 0 * inf is NaN in the product: V rows behind the sequence and values
+                        // that are not finite are zeroed; the latter are made up for below
+                        const int vs = (n + j) % VST;
+                        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&v_full[vs], ((n + j) / VST) & 1, deadline, a.err));
+                        if (ok) {
+                            uint8_t* vb = vring + vs * KV_BLK;
+                            const int nthr = nt * 128;
+                            bool found = false;
+                            for (int c = threadIdx.x - 64; c < BLK * 16; c += nthr) {
+                                // chunk c: page c / 256, half, token, 16-byte piece (swizzled; all
+                                // pieces of a 128-byte row are treated alike)
+                                const int key = (c >> 8) * PAGE + ((c >> 3) & 15);
+                                uint4* at = reinterpret_cast<uint4*>(vb + c * 16);
+                                uint4 v = *at;
+                                if (kbase + key >= s.len) {
+                                    *at = make_uint4(0u, 0u, 0u, 0u);
+                                    continue;
+                                }
+                                auto fix = [&](uint32_t& x) {
+                                    uint32_t keep = 0xffffffffu;
+                                    if ((x & 0x7c00u) == 0x7c00u) keep &= 0xffff0000u;
+                                    if ((x & 0x7c000000u) == 0x7c000000u) keep &= 0x0000ffffu;
+                                    x &= keep;
+                                    return keep != 0xffffffffu;
+                                };
+                                const bool f = fix(v.x) | fix(v.y) | fix(v.z) | fix(v.w);
+                                if (f) *at = v;
+                                found |= f;
+                            }
+                            if (found) *odd = 1;
+                            fence_proxy_async_smem();
+                        }
+                        asm volatile("bar.sync 1, %0;" ::"r"(nt * 128) : "memory");
+                    }
+                    cnt++;
+                    if (!ok) continue;
+                    if (idle) {                         // their P is whatever S held: no other row reads it
+                        mbar_arrive(&p_full[t]);
+                        continue;
+                    }
+                    tc_fence_after_sync();
+                    // S is read twice, for the maximum and for the weights: 32 columns at a time in
+                    // registers. Columns 32 q ..: keys 8 (q/2) .. + 8 of pages 4 (q%2) .. + 4
+                    uint32_t see[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+                    if (!whole) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) see[i] = seen32(a, s, row, kbase + 32 * i);
+                    }
+                    // the scores of columns 32 q .., -inf where unseen
+                    auto scored = [&](int q, float (&x)[32]) {
+                        if (EXT) {
+#pragma unroll
+                            for (int c = 0; c < 32; c++) x[c] = score<true>(a, x[c]);
+                            if (a.slopes) {
+#pragma unroll
+                                for (int c = 0; c < 32; c++) {
+                                    const int p = kbase + ((q & 1) * 4 + (c >> 3)) * PAGE + (q >> 1) * 8 + (c & 7);
+                                    x[c] += bias<true>(a, row.slope2, row.pos, whole ? p : s.pos(a, p));
+                                }
+                            }
+                        } else {
+#pragma unroll
+                            for (int c = 0; c < 32; c++) x[c] *= a.scale_log2;
+                        }
+                        if (!whole) {
+#pragma unroll
+                            for (int c = 0; c < 32; c++) {
+                                const int pg = (q & 1) * 4 + (c >> 3);
+                                if (!((see[pg >> 1] >> ((pg & 1) * 16 + (q >> 1) * 8 + (c & 7))) & 1u)) x[c] = -INFINITY;
+                            }
+                        }
+                    };
+                    float mx = -INFINITY;
+                    const bool raw = whole && !(EXT && a.slopes);   // the score grows with q.k: one is enough
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        float x[32];
+                        tmem_ld32(trow + q * 32, reinterpret_cast<uint32_t(&)[32]>(x));
+                        tmem_ld_wait();
+                        if (!raw) scored(q, x);
+                        float m4[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+                        for (int c = 4; c < 32; c++) m4[c & 3] = fmaxf(m4[c & 3], x[c]);
+                        mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+                    }
+                    if (raw) mx = score<EXT>(a, mx);
+                    if (__any_sync(0xffffffffu, mx > m + RESCALE_THRESHOLD)) {
+                        const float mn = fmaxf(m, mx);
+                        const float cf = mn == -INFINITY ? 1.f : ex2(m - mn);
+                        if (j > 0) {                    // O holds the blocks before: S waited for them
+#pragma unroll
+                            for (int c0 = 0; c0 < D; c0 += 32) {
+                                uint32_t v[32];
+                                tmem_ld32(trow + 128 + c0, v);
+                                tmem_ld_wait();
+#pragma unroll
+                                for (int i = 0; i < 32; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) * cf);
+                                tmem_st32(trow + 128 + c0, v);
+                            }
+                        }
+                        l *= cf;
+                        m = mn;
+                    }
+                    const float ms = m == -INFINITY ? 0.f : m;   // a row that saw nothing yet
+                    // P in fp16 for the product (2^-11 of each weight, as V's own rounding); l sums
+                    // the unrounded weights
+                    float l4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {        // pages 4h .. 4h + 3: S columns of q = h and h + 2
+                        uint32_t pk[32];
+#pragma unroll
+                        for (int u = 0; u < 2; u++) {
+                            float x[32];
+                            tmem_ld32(trow + (2 * u + h) * 32, reinterpret_cast<uint32_t(&)[32]>(x));
+                            tmem_ld_wait();
+                            const bool plain = !EXT && whole;      // the scale is folded into the exponent
+                            if (!plain) scored(2 * u + h, x);
+#pragma unroll
+                            for (int c = 0; c < 32; c += 2) {
+                                const float p0 = ex2(plain ? fmaf(x[c], a.scale_log2, -ms) : x[c] - ms);
+                                const float p1 = ex2(plain ? fmaf(x[c + 1], a.scale_log2, -ms) : x[c + 1] - ms);
+                                l4[(c >> 1) & 3] += p0 + p1;
+                                pk[(c >> 3) * 8 + u * 4 + ((c & 7) >> 1)] = pack_half2(p0, p1);
+                            }
+                        }
+                        // P of pages 0-3 goes over S columns 0-31, pages 4-7 over 32-63: only once
+                        // those are in registers
+                        tmem_st32(trow + h * 32, pk);
+                    }
+                    l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+                    tmem_st_wait();
+                    tc_fence_before_sync();
+                    mbar_arrive(&p_full[t]);
+                }
+                // epilogue: the last P V has landed
+                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&o_done[t], (cnt - 1) & 1, deadline, a.err));
+                if (ok) {
+                    tc_fence_after_sync();
+                    const bool full = g.blk0 == 0 && g.blk1 == g.nblk;
+                    const float inv = l != 0.f ? 1.f / l : 0.f;
+                    const float lse_v = l != 0.f ? ((m == -INFINITY ? 0.f : m) + lg2(l)) * LN2 : -INFINITY;
+                    const size_t slot = ((size_t)blockIdx.x * 2 + (g.blk0 == 0)) * C::ROWS + t * 128 + r;
+#pragma unroll
+                    for (int c0 = 0; c0 < D; c0 += 32) {
+                        uint32_t v[32];
+                        tmem_ld32(trow + 128 + c0, v);
+                        tmem_ld_wait();
+                        float o[32];
+#pragma unroll
+                        for (int i = 0; i < 32; i++) o[i] = __uint_as_float(v[i]) * inv;
+                        if (*odd) {
+                            // values of seen keys that were zeroed above: an infinity or NaN that
+                            // meets a weight is the result
+                            const int e = min(s.len, w.first + g.blk1 * BLK);
+                            for (int p = w.first + g.blk0 * BLK; p < e; p++) {
+                                const int k0 = w.first + (p - w.first) / BLK * BLK;
+                                if (k0 + BLK <= s.ctx && (a.window <= 0 || (long long)pos_hi - k0 < a.window)) {
+                                    p = k0 + BLK - 1;             // a whole block: nothing was zeroed
+                                    continue;
+                                }
+                                if (!row.sees(a, s, p, s.pos(a, p))) continue;
+                                const int pg = __ldg(a.indices + s.page0 + p / PAGE);
+                                if (pg < 0 || pg >= a.num_pages) continue;
+                                const __half* vr = a.v + (((size_t)pg * PAGE + p % PAGE) * a.Hkv + g.kvh) * D + c0;
+#pragma unroll
+                                for (int i = 0; i < 32; i++) {
+                                    const float y = __half2float(vr[i]);
+                                    if (!(fabsf(y) <= 65504.f)) o[i] += y;
+                                }
+                            }
+                        }
+                        if (row.i >= 0) {
+                            if (full) {
+                                uint4* dst = reinterpret_cast<uint4*>(a.out + orow * D + c0);
+#pragma unroll
+                                for (int i = 0; i < 4; i++)
+                                    dst[i] = make_uint4(pack_half2(o[8 * i], o[8 * i + 1]), pack_half2(o[8 * i + 2], o[8 * i + 3]),
+                                                        pack_half2(o[8 * i + 4], o[8 * i + 5]), pack_half2(o[8 * i + 6], o[8 * i + 7]));
+                            } else {
+                                float4* dst = reinterpret_cast<float4*>(a.part_o + slot * D + c0);
+#pragma unroll
+                                for (int i = 0; i < 8; i++)
+                                    dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                            }
+                        }
+                    }
+                    if (row.i >= 0) {
+                        if (full) a.lse[orow] = lse_v;
+                        else a.part_lse[slot] = lse_v;
+                    }
+                    tc_fence_before_sync();
+                }
+            }
+            n += nb;
+        }
+    }
+    // every MMA must have finished before tensor memory is released
+    if (threadIdx.x == 0) mbar_wait(done, 0, deadline, a.err);
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    if (warp == 1) tmem_dealloc(tmem, C::TMEM_COLS);
+}
+
+// Joins the units that more than one CTA worked on; one warp per row. grid = (row parts, B).
+template <int MT>
+__global__ void __launch_bounds__(256) tile_merge_kernel(const Args a, int ctas) {
+    constexpr int ROWS = Cfg<MT>::ROWS;
+    __shared__ long long s_before, s_all;
+    pdl_wait();
+    pdl_trigger();
+    const int b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const Seq s(a, b);
+    if (warp == 0) {
+        const long long x = blocks_before<ROWS>(a, b, lane);
+        if (lane == 0) s_before = x;
+    } else if (warp == 1) {
+        const long long x = blocks_before<ROWS>(a, a.B, lane);
+        if (lane == 0) s_all = x;
+    }
+    int lo = 0, hi;
+    if (a.window > 0) pos_range(a, s, lane, &lo, &hi);
+    const Work w = work_of<ROWS>(a, s, lo);
+    if (s.T > a.max_q && blockIdx.x == 0 && threadIdx.x == 0) atomicOr(a.err, DEVERR_BOUND);
+    __syncthreads();
+    const long long W = s_all, total = (long long)w.nrows * a.Hkv;
+    for (long long x = (long long)blockIdx.x * 8 + warp; x < total; x += (long long)gridDim.x * 8) {
+        const int kvh = (int)(x / w.nrows), rr = (int)(x - (long long)kvh * w.nrows), z = rr / ROWS;
+        const long long u0 = s_before + (long long)(z * a.Hkv + kvh) * w.nblk, u1 = u0 + w.nblk - 1;
+        // CTA of a block: the last c with share(c) <= block
+        auto owner = [&](long long u) {
+            int c = (int)(u * ctas / W);
+            while (c + 1 < ctas && share(W, c + 1, ctas) <= u) c++;
+            while (c > 0 && share(W, c, ctas) > u) c--;
+            return c;
+        };
+        const int c0 = owner(u0), c1 = owner(u1);
+        if (c0 == c1) continue;                                   // written by the CTA itself
+        // CTAs between without blocks (more CTAs than blocks) left nothing
+        const int r = rr - z * ROWS;
+        auto slot = [&](int c) { return ((size_t)c * 2 + (c == c0)) * ROWS + r; };
+        float m = -INFINITY;
+        bool nan = false;
+        for (int c = c0 + lane; c <= c1; c += 32) {
+            if (share(W, c, ctas) == share(W, c + 1, ctas)) continue;
+            const float y = a.part_lse[slot(c)];
+            nan |= y != y;
+            m = fmaxf(m, y);
+        }
+        m = warp_max(m);
+        nan = __any_sync(0xffffffffu, nan);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        float ws = 0.f;
+        if (m != -INFINITY || nan) {
+#pragma unroll 4
+            for (int c = c0; c <= c1; c++) {
+                if (share(W, c, ctas) == share(W, c + 1, ctas)) continue;
+                const float y = a.part_lse[slot(c)];
+                if (y == -INFINITY) continue;
+                const float e = ex2((y - m) * LOG2E);
+                const float4 v = reinterpret_cast<const float4*>(a.part_o + slot(c) * D)[lane];
+                ws += e;
+                acc.x += e * v.x;
+                acc.y += e * v.y;
+                acc.z += e * v.z;
+                acc.w += e * v.w;
+            }
+        }
+        const float inv = ws != 0.f ? 1.f / ws : 0.f;
+        const int i = rr / a.G;
+        const size_t row = (size_t)(s.q0 + i) * a.Hq + kvh * a.G + (rr - i * a.G);
+        uint2 pk;
+        pk.x = pack_half2(acc.x * inv, acc.y * inv);
+        pk.y = pack_half2(acc.z * inv, acc.w * inv);
+        reinterpret_cast<uint2*>(a.out + row * D)[lane] = pk;
+        if (lane == 0) a.lse[row] = ws != 0.f ? m + logf(ws) : -INFINITY;
+    }
+}
+
+const void* tile_fn(int MT, bool ext) {
+    if (MT == 1) return ext ? (const void*)tile_kernel<1, true> : (const void*)tile_kernel<1, false>;
+    return ext ? (const void*)tile_kernel<2, true> : (const void*)tile_kernel<2, false>;
+}
+
+ckl_status setup_tiles(const DeviceInfo* di) {
+    static ckl_status st[64];
+    static std::once_flag once[64];
+    std::call_once(once[di->device], [di] {
+        cudaError_t e = cudaSuccess;
+        for (int MT = 1; MT <= 2 && e == cudaSuccess; MT++)
+            for (int ext = 0; ext < 2 && e == cudaSuccess; ext++)
+                e = cudaFuncSetAttribute(tile_fn(MT, ext), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         MT == 1 ? Cfg<1>::SMEM : Cfg<2>::SMEM);
+        st[di->device] = cuda_status(e, "tree attention setup");
+    });
+    return st[di->device];
+}
+
+// One page as one box [64-dim half][16 tokens][64 dims] of one head.
+ckl_status encode_tile_map(const void* cache, int Hkv, int num_pages, CUtensorMap* tm) {
+    const uint64_t dims[5] = {64, (uint64_t)PAGE, 2, (uint64_t)Hkv, (uint64_t)num_pages};
+    const uint64_t strides[4] = {(uint64_t)Hkv * D * 2, 128, (uint64_t)D * 2, (uint64_t)PAGE * Hkv * D * 2};
+    const uint32_t box[5] = {64, (uint32_t)PAGE, 2, 1, 1};
+    return encode_tiled(tm, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void*>(cache), dims, strides, box,
+                        CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+size_t part_bytes(int ctas, int rows, size_t* o_bytes) {
+    // at most two segments of a CTA are partial
+    *o_bytes = align_up((size_t)ctas * 2 * rows * D * sizeof(float), 256);
+    return *o_bytes + align_up((size_t)ctas * 2 * rows * sizeof(float), 256);
+}
+
+}  // namespace tile
+
+int tile_count(long long rows) { return rows <= 128 ? 1 : 2; }
+
+size_t tile_workspace(int ctas, long long rows) {
+    size_t o;
+    return tile::part_bytes(ctas, 128 * tile_count(rows), &o);
+}
+
+ckl_status launch_tiles(const ckl_tree_params* p, Args a, void* workspace, int ctas, cudaStream_t s) {
+    using namespace tile;
+    const DeviceInfo* di = device_info();
+    if (!di) return CKL_CUDA_ERROR;
+    ckl_status st = setup_tiles(di);
+    if (st != CKL_OK) return st;
+    const int MT = tile_count((long long)p->max_q * a.G);
+    size_t o;
+    part_bytes(ctas, 128 * MT, &o);
+    a.part_o = static_cast<float*>(workspace);
+    a.part_lse = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + o);
+    CUtensorMap tmK, tmV;
+    st = encode_tile_map(p->k_cache, p->Hkv, p->num_pages, &tmK);
+    if (st != CKL_OK) return st;
+    st = encode_tile_map(p->v_cache, p->Hkv, p->num_pages, &tmV);
+    if (st != CKL_OK) return st;
+    void* args[] = {&tmK, &tmV, &a};
+    const bool ext = p->softcap > 0.f || p->slopes;
+    CKL_CUDA_TRY(launch(tile_fn(MT, ext), dim3((unsigned)ctas), dim3(64 + 128 * MT), MT == 1 ? Cfg<1>::SMEM : Cfg<2>::SMEM,
+                        s, args, true));
+    void* margs[] = {&a, &ctas};
+    const long long rows = (long long)p->max_q * p->Hq;
+    const unsigned gx = (unsigned)std::max(1LL, std::min((rows + 7) / 8, (long long)(8 * di->sms + p->B - 1) / p->B));
+    CKL_CUDA_TRY(launch(MT == 1 ? (const void*)tile_merge_kernel<1> : (const void*)tile_merge_kernel<2>,
+                        dim3(gx, (unsigned)p->B), dim3(256), 0, s, margs, true));
+    return CKL_OK;
+}
+
+}  // namespace tree
+}  // namespace ckl
