@@ -133,6 +133,14 @@ __device__ __forceinline__ void tma_load_5d(void* dst, const void* tmap, int c0,
         "r"(smem_u32(bar)), "l"(policy)
         : "memory");
 }
+// Tiled 3-D tensor load global -> shared, completing on an mbarrier.
+__device__ __forceinline__ void tma_load_3d(void* dst, const void* tmap, int c0, int c1, int c2, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
+        : "memory");
+}
 // Tiled 2-D tensor load global -> shared (x coordinate first), completing on an mbarrier.
 __device__ __forceinline__ void tma_load_2d(void* dst, const void* tmap, int c0, int c1, uint64_t* bar,
                                             uint64_t policy) {
@@ -213,10 +221,22 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}"
-        ::"r"(d_tmem), "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u),
-        "r"(0u)
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0u)
         : "memory");
+}
+// True in one lane of a converged warp. A branch on it is known to hold a single thread, so the
+// operands of the tensor-core instructions in it can live in uniform registers: 32 cycles per
+// M=128 N=64 instruction (A in tensor memory) where a branch on lane == 0 takes 50, measured on
+// chains of 256.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(p));
+    return p != 0;
 }
 // Arrive once on an mbarrier when every tcgen05 operation this thread issued has completed.
 __device__ __forceinline__ void umma_commit(uint64_t* bar) {

@@ -29,6 +29,7 @@ struct Args {
     float scale_log2;         // sm_scale * log2(e)
     float cap_log2;           // softcap * log2(e), 0: no cap
     float cap_in;             // 2 log2(e) sm_scale / softcap
+    int q_tma;                // the tcgen05 kernel reads Q tiles through a tensor map
 };
 
 // Length of sequence b from the page table; a last page outside [0, 16] is taken as full/empty.

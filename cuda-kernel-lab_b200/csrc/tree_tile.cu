@@ -23,6 +23,7 @@
 
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 
 #include "tree_tile.cuh"
 
@@ -37,14 +38,16 @@ constexpr int Q_TILE = 128 * D * 2;                // 32 KB: dims 0-63 of 128 ro
 constexpr int VST = 2;                             // V blocks in flight
 template <int MT> struct Cfg {
     static constexpr int KST = MT == 1 ? 4 : 3;    // K blocks in flight
+    static constexpr int SB = MT == 1 ? 2 : 1;     // S buffers of a tile
+    static constexpr int TILE_COLS = SB * 128 + 128;   // tensor memory of a tile: S (and P), then O
     static constexpr int THREADS = 64 + 128 * MT;
     static constexpr int ROWS = 128 * MT;
     static constexpr int OFF_K = MT * Q_TILE;
     static constexpr int OFF_V = OFF_K + KST * KV_BLK;
     static constexpr int OFF_BAR = OFF_V + VST * KV_BLK;
-    static constexpr int NBAR = 2 * KST + 2 * VST + 4 * MT + 1;
+    static constexpr int NBAR = 2 * KST + 2 * VST + (2 + SB + 2) * MT + 2;
     static constexpr int SMEM = 1024 + OFF_BAR + NBAR * 8 + 32;
-    static constexpr uint32_t TMEM_COLS = MT == 1 ? 256 : 512;   // per tile: S (and P) 128, O 128
+    static constexpr uint32_t TMEM_COLS = 512;
 };
 static_assert(Cfg<1>::SMEM <= 232448 && Cfg<2>::SMEM <= 232448, "shared memory of a CTA");
 
@@ -90,8 +93,20 @@ __device__ __forceinline__ long long blocks_before(const Args& a, int upto, int 
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     return sum;
 }
-// First block of CTA c of n over W blocks.
-__device__ __forceinline__ long long share(long long W, int c, int n) { return W * c / n; }
+// W blocks over n CTAs: the first W % n take one more than the others.
+struct Share {
+    long long each;
+    int n, more;
+    __device__ __forceinline__ Share(long long W, int n_) : n(n_) {
+        each = W >> 31 ? W / n : (long long)((unsigned)W / (unsigned)n);
+        more = (int)(W - each * n);
+    }
+    __device__ __forceinline__ long long first(int c) const { return each * c + min(c, more); }   // block of CTA c
+    __device__ __forceinline__ int owner(long long u) const {                                      // CTA of block u
+        const long long big = (each + 1) * more, x = u < big ? u : u - big, d = u < big ? each + 1 : each;
+        return (u < big ? 0 : more) + (int)(x >> 31 ? x / d : (long long)((unsigned)x / (unsigned)d));
+    }
+};
 
 // A CTA's run of blocks, unit by unit. All lanes of a warp hold the same state.
 struct Seg {
@@ -117,7 +132,7 @@ struct Walk {
                 b++;
                 continue;
             }
-            const int unit = (int)(off / w->nblk), z = unit / a.Hkv;
+            const int unit = off >> 31 ? (int)(off / w->nblk) : (int)((unsigned)off / (unsigned)w->nblk), z = unit / a.Hkv;
             g->b = b;
             g->kvh = unit - z * a.Hkv;
             g->row0 = z * ROWS;
@@ -164,9 +179,10 @@ __device__ __forceinline__ uint32_t seen32(const Args& a, const Seq& s, const Ro
 
 template <int MT, bool EXT>
 __global__ void __launch_bounds__(Cfg<MT>::THREADS, 1)
-tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const Args a) {
+tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+            const __grid_constant__ CUtensorMap tmQ, const Args a) {
     using C = Cfg<MT>;
-    constexpr int KST = C::KST;
+    constexpr int KST = C::KST, SB = C::SB, COLS = C::TILE_COLS;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* sm = align_ptr<1024>(smem_raw);
     uint8_t* qs = sm;
@@ -176,10 +192,11 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
     uint64_t* k_empty = k_full + KST;
     uint64_t* v_full = k_empty + KST;
     uint64_t* v_empty = v_full + VST;
-    uint64_t* q_full = v_empty + VST;        // [MT] Q staged for a segment (softmax -> MMA)
-    uint64_t* s_full = q_full + MT;          // [MT] S written (MMA -> softmax); O holds the blocks before
-    uint64_t* p_full = s_full + MT;          // [MT] P written (softmax -> MMA)
-    uint64_t* o_done = p_full + MT;          // [MT] O holds the block (MMA -> softmax, MMA)
+    uint64_t* q_empty = v_empty + VST;       // every S of a segment done: Q may be replaced
+    uint64_t* q_full = q_empty + 1;          // [MT] Q of a segment is there
+    uint64_t* s_full = q_full + MT;          // [MT][SB] S written (MMA -> softmax)
+    uint64_t* p_full = s_full + MT * SB;     // [MT][2] P of pages 0-3 / 4-7 written (softmax -> MMA)
+    uint64_t* o_done = p_full + MT * 2;      // [MT] O holds the block, its P has been read (MMA -> all)
     uint64_t* done = o_done + MT;            // every issued MMA finished
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
     volatile int* odd = reinterpret_cast<volatile int*>(tmem_slot + 1);   // unseen V held inf or NaN
@@ -197,11 +214,12 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
             mbar_init(&v_empty[i], 1);
         }
         for (int t = 0; t < MT; t++) {
-            mbar_init(&q_full[t], 128);
-            mbar_init(&s_full[t], 1);
-            mbar_init(&p_full[t], 128);
+            mbar_init(&q_full[t], a.q_tma ? 1 : 128);
+            for (int i = 0; i < SB; i++) mbar_init(&s_full[t * SB + i], 1);
+            for (int i = 0; i < 2; i++) mbar_init(&p_full[t * 2 + i], 128);
             mbar_init(&o_done[t], 1);
         }
+        mbar_init(q_empty, 1);
         mbar_init(done, 1);
         fence_barrier_init();
         *odd = 0;
@@ -217,7 +235,8 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
     pdl_wait();
     if (warp == 2) {
         const long long W = blocks_before<C::ROWS>(a, a.B, lane);
-        const long long beg = share(W, blockIdx.x, gridDim.x), end = share(W, blockIdx.x + 1, gridDim.x);
+        const Share sh(W, gridDim.x);
+        const long long beg = sh.first(blockIdx.x), end = sh.first(blockIdx.x + 1);
         long long before = 0;
         int b = a.B;
         for (int b0 = 0; b0 < a.B && b == a.B; b0 += 32) {
@@ -258,7 +277,10 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
     if (warp == 0) {
         // ---------------------------------------------------------------- TMA producer
         const uint64_t pol = policy_evict_first();
-        int ok = 1, n = 0;                              // n: blocks issued
+        int qn[MT];                                     // Q loads issued into each tile
+#pragma unroll
+        for (int t = 0; t < MT; t++) qn[t] = 0;
+        int ok = 1, n = 0, seg = 0;                     // n: blocks issued
         while (ok && walk.next(a, &g, &s, &w, &pos_hi, lane)) {
             const int p0 = w.first / PAGE, npg = (s.len + PAGE - 1) / PAGE;
             int ids_at = 0, my_id = 0;
@@ -288,7 +310,26 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                 if (!ok) { n++; break; }                // its K is in flight, its V is not
                 if (lane < BLK_PAGES)
                     tma_load_5d(vring + vs * KV_BLK + lane * KV_TILE, &tmV, 0, 0, 0, g.kvh, page, &v_full[vs], pol);
+                if (j == g.blk0 && a.q_tma) {
+                    // the segment's Q, behind its first block: the earlier segment still reads its own
+                    if (lane == 0) {
+                        if (seg > 0) ok = mbar_wait(q_empty, (seg - 1) & 1, deadline, a.err);
+#pragma unroll
+                        for (int t = 0; t < MT; t++) {
+                            if (!ok || t * 128 >= g.rows) break;
+                            uint8_t* dst = qs + t * Q_TILE;
+                            const int tok = s.q0 + (g.row0 + t * 128) / a.G;
+                            mbar_arrive_expect_tx(&q_full[t], Q_TILE);
+                            tma_load_3d(dst, &tmQ, 0, g.kvh * a.G, tok, &q_full[t]);
+                            tma_load_3d(dst + Q_TILE / 2, &tmQ, 64, g.kvh * a.G, tok, &q_full[t]);
+                            qn[t]++;
+                        }
+                    }
+                    ok = __shfl_sync(0xffffffffu, ok, 0);
+                    if (!ok) { n++; break; }
+                }
             }
+            seg++;
         }
         // every issued copy must land before the CTA exits (a wait for a phase that was never
         // armed, after a timeout, ends at the deadline)
@@ -297,82 +338,121 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                 mbar_wait(&k_full[i], ((i + (n - 1 - i) / KST * KST) / KST) & 1, deadline, a.err);
             for (int i = 0; i < VST && i < n; i++)
                 mbar_wait(&v_full[i], ((i + (n - 1 - i) / VST * VST) / VST) & 1, deadline, a.err);
+#pragma unroll
+            for (int t = 0; t < MT; t++)
+                if (qn[t] > 0) mbar_wait(&q_full[t], (qn[t] - 1) & 1, deadline, a.err);
         }
     } else if (warp == 1) {
         // ---------------------------------------------------------------- MMA issuer
+        // With one S buffer a tile's next S waits for its P V (P lies over the first half of S: the
+        // other half is written meanwhile); with two it runs ahead of the softmax.
         const uint32_t idesc_s = umma_idesc_f16(128, 64, false, false);
         const uint32_t idesc_o = umma_idesc_f16(128, D, false, true);
-        const uint32_t qa = smem_u32(qs), ka = smem_u32(kring), va = smem_u32(vring);
-        int ok = 1, n = 0;                              // n: blocks before this segment
-        int cnt[MT];                                    // blocks done by each tile
+        const uint64_t qd = umma_desc_sw128(smem_u32(qs), 16, 1024);
+        const uint64_t kd = umma_desc_sw128(smem_u32(kring), 16, KV_TILE);
+        const uint64_t vd = umma_desc_sw128(smem_u32(vring), HALF_TILE, 1024);
+        bool ok = true;
+        int n = 0;                                      // blocks before this segment
+        int done_blocks[MT], q_seen[MT];                // of each tile, before this segment
 #pragma unroll
-        for (int t = 0; t < MT; t++) cnt[t] = 0;
-        int qph[MT];
-#pragma unroll
-        for (int t = 0; t < MT; t++) qph[t] = 0;
+        for (int t = 0; t < MT; t++) done_blocks[t] = q_seen[t] = 0;
         while (ok && walk.next(a, &g, &s, &w, &pos_hi, lane)) {
             const int nt = (g.rows + 127) / 128, nb = g.blk1 - g.blk0;
-            if (lane == 0) {
-                // S of block j (of this segment), tile t
-                auto qk = [&](int j, int t) {
-                    const int ks = (n + j) % KST;
-                    const uint32_t kb = ka + ks * KV_BLK, qb = qa + t * Q_TILE, d = tmem + t * 256;
+            if (elect_one()) {
+                auto wait = [&](uint64_t* bar, int phase) { return mbar_wait(bar, phase & 1, deadline, a.err); };
+                // half u of S of block j (of this segment), tile t (offsets in descriptors: 16 bytes)
+                auto qk = [&](int j, int t, int buf, int u) {
+                    const uint64_t kb = kd + (uint64_t)((n + j) % KST * (KV_BLK / 16) + u * (1024 / 16));
+                    const uint64_t qb = qd + (uint64_t)(t * (Q_TILE / 16));
+                    const uint32_t d = tmem + t * COLS + buf * 128 + u * 64;
 #pragma unroll
-                    for (int u = 0; u < 2; u++)
-#pragma unroll
-                        for (int kk = 0; kk < 8; kk++)
-                            umma_f16(d + u * 64,
-                                     umma_desc_sw128(qb + (kk >> 2) * (Q_TILE / 2) + (kk & 3) * 32, 16, 1024),
-                                     umma_desc_sw128(kb + u * 1024 + (kk >> 2) * HALF_TILE + (kk & 3) * 32, 16, KV_TILE),
-                                     idesc_s, kk != 0);
-                    umma_commit(&s_full[t]);
-                    if (t == nt - 1) umma_commit(&k_empty[ks]);
+                    for (int kk = 0; kk < 8; kk++)
+                        umma_f16(d, qb + ((kk >> 2) * (Q_TILE / 2) + (kk & 3) * 32) / 16,
+                                 kb + ((kk >> 2) * HALF_TILE + (kk & 3) * 32) / 16, idesc_s, kk != 0);
                 };
-                ok = mbar_wait(&k_full[n % KST], (n / KST) & 1, deadline, a.err);
-                for (int t = 0; t < nt && ok; t++) {
-                    ok = mbar_wait(&q_full[t], qph[t] & 1, deadline, a.err);
-                    qph[t]++;
+                auto qk_done = [&](int j, int t, int buf) {
+                    umma_commit(&s_full[t * SB + buf]);
+                    if (t == nt - 1) {
+                        umma_commit(&k_empty[(n + j) % KST]);
+                        if (j == nb - 1) umma_commit(q_empty);
+                    }
+                };
+                ok = wait(&k_full[n % KST], n / KST);
+#pragma unroll
+                for (int t = 0; t < MT; t++) {
+                    if (t >= nt || !ok) break;
+                    const int c = done_blocks[t];
+                    ok = wait(&q_full[t], q_seen[t]);
+                    // every P of the earlier segment has been read
+                    if (ok && c > 0) ok = wait(&o_done[t], c - 1);
                     if (!ok) break;
                     tc_fence_after_sync();
-                    qk(0, t);
+                    qk(0, t, c % SB, 0);
+                    qk(0, t, c % SB, 1);
+                    qk_done(0, t, c % SB);
                 }
                 for (int j = 0; j < nb && ok; j++) {
-                    const int vs = (n + j) % VST;
-                    for (int t = 0; t < nt && ok; t++) {
-                        ok = mbar_wait(&p_full[t], cnt[t] & 1, deadline, a.err);
-                        if (ok && t == 0) ok = mbar_wait(&v_full[vs], ((n + j) / VST) & 1, deadline, a.err);
-                        if (!ok) break;
-                        tc_fence_after_sync();
-                        const uint32_t vb = va + vs * KV_BLK, d = tmem + t * 256;
+                    const int vs = (n + j) % VST, k1 = n + j + 1;
+                    const uint64_t vb = vd + (uint64_t)(vs * (KV_BLK / 16));
 #pragma unroll
-                        for (int pg = 0; pg < BLK_PAGES; pg++)
-                            umma_f16_ts(d + 128, d + pg * 8, umma_desc_sw128(vb + pg * KV_TILE, HALF_TILE, 1024),
-                                        idesc_o, (j | pg) != 0);
-                        umma_commit(&o_done[t]);
-                        if (t == nt - 1) umma_commit(&v_empty[vs]);
-                        cnt[t]++;
-                        if (j + 1 < nb) {
-                            const int k1 = n + j + 1;
-                            if (t == 0) ok = mbar_wait(&k_full[k1 % KST], (k1 / KST) & 1, deadline, a.err);
-                            // P (over S) must have been read before S is written again
-                            if (ok) ok = mbar_wait(&o_done[t], (cnt[t] - 1) & 1, deadline, a.err);
+                    for (int t = 0; t < MT; t++) {
+                        if (t >= nt || !ok) break;
+                        const int c = done_blocks[t] + j, buf = c % SB;
+                        const uint32_t sb = tmem + t * COLS + buf * 128, o = tmem + t * COLS + SB * 128;
+                        if (SB == 2 && j + 1 < nb) {
+                            // S of the next block into the other buffer, whose P belongs to block j - 1
+                            ok = wait(&k_full[k1 % KST], k1 / KST);
+                            if (ok && j > 0) ok = wait(&o_done[t], c - 1);
                             if (!ok) break;
                             tc_fence_after_sync();
-                            qk(j + 1, t);
+                            qk(j + 1, t, buf ^ 1, 0);
+                            qk(j + 1, t, buf ^ 1, 1);
+                            qk_done(j + 1, t, buf ^ 1);
+                        }
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            if (ok) ok = wait(&p_full[t * 2 + h], c);
+                            if (ok && t == 0 && h == 0) ok = wait(&v_full[vs], (n + j) / VST);
+                            if (!ok) break;
+                            tc_fence_after_sync();
+#pragma unroll
+                            for (int pg = 4 * h; pg < 4 * h + 4; pg++)
+                                umma_f16_ts(o, sb + pg * 8, vb + pg * (KV_TILE / 16), idesc_o, pg != 0 || j != 0);
+                        }
+                        if (!ok) break;
+                        umma_commit(&o_done[t]);
+                        if (t == nt - 1) umma_commit(&v_empty[vs]);
+                        if (SB == 1 && j + 1 < nb) {
+                            if (t == 0) ok = wait(&k_full[k1 % KST], k1 / KST);
+                            if (!ok) break;
+                            tc_fence_after_sync();
+                            qk(j + 1, t, 0, 1);
+                            ok = wait(&o_done[t], c);
+                            if (!ok) break;
+                            tc_fence_after_sync();
+                            qk(j + 1, t, 0, 0);
+                            qk_done(j + 1, t, 0);
                         }
                     }
                 }
             }
-            ok = __shfl_sync(0xffffffffu, ok, 0);
+            ok = __all_sync(0xffffffffu, ok);
             n += nb;
+#pragma unroll
+            for (int t = 0; t < MT; t++)
+                if (t < nt) {
+                    done_blocks[t] += nb;
+                    q_seen[t]++;
+                }
         }
-        if (lane == 0) umma_commit(done);
+        if (elect_one()) umma_commit(done);
         __syncwarp();
     } else {
         // ---------------------------------------------------------------- softmax: a row per thread
         const int t = (warp - 2) >> 2, quarter = warp & 3;
         const int r = quarter * 32 + lane;              // row of the tile
-        const uint32_t trow = tmem + t * 256 + ((uint32_t)(quarter * 32) << 16);
+        const uint32_t trow = tmem + t * COLS + ((uint32_t)(quarter * 32) << 16);
+        const uint32_t orow_t = trow + SB * 128;        // this thread's row of O
         bool ok = true;
         int cnt = 0, n = 0;                             // blocks of this tile; blocks of the CTA
         while (walk.next(a, &g, &s, &w, &pos_hi, lane)) {
@@ -382,71 +462,28 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                 Row row;
                 row.set(a, s, rr, g.row0 + g.rows, g.kvh);
                 const size_t orow = (size_t)(s.q0 + max(row.i, 0)) * a.Hq + g.kvh * a.G + (rr - max(row.i, 0) * a.G);
-                {
-                    // the tile's earlier S have been read by the tensor core: its last o_done
-                    // was waited for in the epilogue
+                if (!a.q_tma) {
+                    // a group size that does not divide the tile: every thread brings its row. The
+                    // tile's earlier S are done: its last o_done was waited for in the epilogue
                     const uint4* src = reinterpret_cast<const uint4*>(a.q + orow * D);
 #pragma unroll
                     for (int c = 0; c < 16; c++) {
                         const uint4 v = row.i >= 0 ? __ldg(src + c) : make_uint4(0u, 0u, 0u, 0u);
                         *reinterpret_cast<uint4*>(qs + t * Q_TILE + (c >> 3) * (Q_TILE / 2) + sw128(r, c & 7)) = v;
                     }
+                    fence_proxy_async_smem();
+                    mbar_arrive(&q_full[t]);
                 }
-                fence_proxy_async_smem();
-                mbar_arrive(&q_full[t]);
 
                 const bool idle = t * 128 + quarter * 32 >= g.rows;   // only padding rows: no softmax
                 float m = -INFINITY, l = 0.f;
-                for (int j = 0; j < nb; j++) {
-                    const int kbase = w.first + (g.blk0 + j) * BLK;
-                    const bool whole = kbase + BLK <= s.ctx && (a.window <= 0 || (long long)pos_hi - kbase < a.window);
-                    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], cnt & 1, deadline, a.err));
-                    if (!whole) {
-                        // 0 * inf is NaN in the product: V rows behind the sequence and values
-                        // that are not finite are zeroed; the latter are made up for below
-                        const int vs = (n + j) % VST;
-                        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&v_full[vs], ((n + j) / VST) & 1, deadline, a.err));
-                        if (ok) {
-                            uint8_t* vb = vring + vs * KV_BLK;
-                            const int nthr = nt * 128;
-                            bool found = false;
-                            for (int c = threadIdx.x - 64; c < BLK * 16; c += nthr) {
-                                // chunk c: page c / 256, half, token, 16-byte piece (swizzled; all
-                                // pieces of a 128-byte row are treated alike)
-                                const int key = (c >> 8) * PAGE + ((c >> 3) & 15);
-                                uint4* at = reinterpret_cast<uint4*>(vb + c * 16);
-                                uint4 v = *at;
-                                if (kbase + key >= s.len) {
-                                    *at = make_uint4(0u, 0u, 0u, 0u);
-                                    continue;
-                                }
-                                auto fix = [&](uint32_t& x) {
-                                    uint32_t keep = 0xffffffffu;
-                                    if ((x & 0x7c00u) == 0x7c00u) keep &= 0xffff0000u;
-                                    if ((x & 0x7c000000u) == 0x7c000000u) keep &= 0x0000ffffu;
-                                    x &= keep;
-                                    return keep != 0xffffffffu;
-                                };
-                                const bool f = fix(v.x) | fix(v.y) | fix(v.z) | fix(v.w);
-                                if (f) *at = v;
-                                found |= f;
-                            }
-                            if (found) *odd = 1;
-                            fence_proxy_async_smem();
-                        }
-                        asm volatile("bar.sync 1, %0;" ::"r"(nt * 128) : "memory");
-                    }
-                    cnt++;
-                    if (!ok) continue;
-                    if (idle) {                         // their P is whatever S held: no other row reads it
-                        mbar_arrive(&p_full[t]);
-                        continue;
-                    }
-                    tc_fence_after_sync();
-                    // S is read twice, for the maximum and for the weights: 32 columns at a time in
-                    // registers. Columns 32 q ..: keys 8 (q/2) .. + 8 of pages 4 (q%2) .. + 4
-                    uint32_t see[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
-                    if (!whole) {
+                // One block of the row: S from tensor memory, P back. S is read twice, for the maximum
+                // and for the weights, so that 32 columns at a time are in registers. Columns 32 q ..:
+                // keys 8 (q/2) .. + 8 of pages 4 (q%2) .. + 4. `whole`: every row sees every key.
+                auto soft = [&](auto whole_, int j, int kbase, uint32_t srow) {
+                    constexpr bool WHOLE = decltype(whole_)::value;
+                    uint32_t see[4];
+                    if (!WHOLE) {
 #pragma unroll
                         for (int i = 0; i < 4; i++) see[i] = seen32(a, s, row, kbase + 32 * i);
                     }
@@ -459,27 +496,28 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
 #pragma unroll
                                 for (int c = 0; c < 32; c++) {
                                     const int p = kbase + ((q & 1) * 4 + (c >> 3)) * PAGE + (q >> 1) * 8 + (c & 7);
-                                    x[c] += bias<true>(a, row.slope2, row.pos, whole ? p : s.pos(a, p));
+                                    x[c] += bias<true>(a, row.slope2, row.pos, WHOLE ? p : s.pos(a, p));
                                 }
                             }
                         } else {
 #pragma unroll
                             for (int c = 0; c < 32; c++) x[c] *= a.scale_log2;
                         }
-                        if (!whole) {
+                        if (!WHOLE) {
 #pragma unroll
                             for (int c = 0; c < 32; c++) {
-                                const int pg = (q & 1) * 4 + (c >> 3);
-                                if (!((see[pg >> 1] >> ((pg & 1) * 16 + (q >> 1) * 8 + (c & 7))) & 1u)) x[c] = -INFINITY;
+                                const int pg = c >> 3;               // of this half's four
+                                const uint32_t w2 = (q & 1) ? see[2 + (pg >> 1)] : see[pg >> 1];
+                                if (!((w2 >> ((q >> 1) * 8 + (pg & 1) * 16 + (c & 7))) & 1u)) x[c] = -INFINITY;
                             }
                         }
                     };
                     float mx = -INFINITY;
-                    const bool raw = whole && !(EXT && a.slopes);   // the score grows with q.k: one is enough
-#pragma unroll
+                    const bool raw = WHOLE && !(EXT && a.slopes);   // the score grows with q.k: one is enough
+#pragma unroll(WHOLE ? 4 : 1)
                     for (int q = 0; q < 4; q++) {
                         float x[32];
-                        tmem_ld32(trow + q * 32, reinterpret_cast<uint32_t(&)[32]>(x));
+                        tmem_ld32(srow + q * 32, reinterpret_cast<uint32_t(&)[32]>(x));
                         tmem_ld_wait();
                         if (!raw) scored(q, x);
                         float m4[4] = {x[0], x[1], x[2], x[3]};
@@ -491,15 +529,18 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                     if (__any_sync(0xffffffffu, mx > m + RESCALE_THRESHOLD)) {
                         const float mn = fmaxf(m, mx);
                         const float cf = mn == -INFINITY ? 1.f : ex2(m - mn);
-                        if (j > 0) {                    // O holds the blocks before: S waited for them
+                        if (j > 0 && !(ok = __all_sync(0xffffffffu, mbar_wait(&o_done[t], (cnt - 1) & 1, deadline, a.err))))
+                            return;
+                        if (j > 0) {                    // O holds the blocks before this one now
+                            tc_fence_after_sync();
 #pragma unroll
                             for (int c0 = 0; c0 < D; c0 += 32) {
                                 uint32_t v[32];
-                                tmem_ld32(trow + 128 + c0, v);
+                                tmem_ld32(orow_t + c0, v);
                                 tmem_ld_wait();
 #pragma unroll
                                 for (int i = 0; i < 32; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) * cf);
-                                tmem_st32(trow + 128 + c0, v);
+                                tmem_st32(orow_t + c0, v);
                             }
                         }
                         l *= cf;
@@ -509,32 +550,89 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                     // P in fp16 for the product (2^-11 of each weight, as V's own rounding); l sums
                     // the unrounded weights
                     float l4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
+                    constexpr bool FOLD = !EXT && WHOLE;         // the scale goes into the exponent
+#pragma unroll(WHOLE ? 2 : 1)
                     for (int h = 0; h < 2; h++) {        // pages 4h .. 4h + 3: S columns of q = h and h + 2
                         uint32_t pk[32];
 #pragma unroll
                         for (int u = 0; u < 2; u++) {
                             float x[32];
-                            tmem_ld32(trow + (2 * u + h) * 32, reinterpret_cast<uint32_t(&)[32]>(x));
+                            tmem_ld32(srow + (2 * u + h) * 32, reinterpret_cast<uint32_t(&)[32]>(x));
                             tmem_ld_wait();
-                            const bool plain = !EXT && whole;      // the scale is folded into the exponent
-                            if (!plain) scored(2 * u + h, x);
+                            if (!FOLD) scored(2 * u + h, x);
 #pragma unroll
                             for (int c = 0; c < 32; c += 2) {
-                                const float p0 = ex2(plain ? fmaf(x[c], a.scale_log2, -ms) : x[c] - ms);
-                                const float p1 = ex2(plain ? fmaf(x[c + 1], a.scale_log2, -ms) : x[c + 1] - ms);
+                                const float p0 = ex2(FOLD ? fmaf(x[c], a.scale_log2, -ms) : x[c] - ms);
+                                const float p1 = ex2(FOLD ? fmaf(x[c + 1], a.scale_log2, -ms) : x[c + 1] - ms);
                                 l4[(c >> 1) & 3] += p0 + p1;
                                 pk[(c >> 3) * 8 + u * 4 + ((c & 7) >> 1)] = pack_half2(p0, p1);
                             }
                         }
                         // P of pages 0-3 goes over S columns 0-31, pages 4-7 over 32-63: only once
                         // those are in registers
-                        tmem_st32(trow + h * 32, pk);
+                        tmem_st32(srow + h * 32, pk);
+                        tmem_st_wait();
+                        tc_fence_before_sync();
+                        mbar_arrive(&p_full[t * 2 + h]);
                     }
                     l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
-                    tmem_st_wait();
-                    tc_fence_before_sync();
-                    mbar_arrive(&p_full[t]);
+                };
+                for (int j = 0; j < nb; j++) {
+                    const int kbase = w.first + (g.blk0 + j) * BLK;
+                    const bool whole = kbase + BLK <= s.ctx && (a.window <= 0 || (long long)pos_hi - kbase < a.window);
+                    const uint32_t srow = trow + cnt % SB * 128;
+                    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t * SB + cnt % SB], (cnt / SB) & 1, deadline, a.err));
+                    if (!whole) {
+                        // 0 * inf is NaN in the product: V rows behind the sequence and values
+                        // that are not finite are zeroed; the latter are made up for below
+                        const int vs = (n + j) % VST;
+                        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&v_full[vs], ((n + j) / VST) & 1, deadline, a.err));
+                        if (ok) {
+                            uint8_t* vb = vring + vs * KV_BLK;
+                            const int nthr = nt * 128;
+                            bool found = false;
+                            // pages that every row sees whole are left; a window reaches all of them
+                            const int pg0 = a.window > 0 ? 0 : max(0, min(BLK_PAGES, (s.ctx - kbase) / PAGE));
+#pragma unroll 4
+                            for (int c = pg0 * 256 + threadIdx.x - 64; c < BLK * 16; c += nthr) {
+                                // chunk c: page c / 256, half, token, 16-byte piece (swizzled; all
+                                // pieces of a 128-byte row are treated alike)
+                                const int key = (c >> 8) * PAGE + ((c >> 3) & 15);
+                                uint4* at = reinterpret_cast<uint4*>(vb + c * 16);
+                                uint4 v = *at;
+                                bool f = false;
+                                auto fix = [&](uint32_t& x) {
+                                    uint32_t keep = 0xffffffffu;
+                                    if ((x & 0x7c00u) == 0x7c00u) keep &= 0xffff0000u;
+                                    if ((x & 0x7c000000u) == 0x7c000000u) keep &= 0x0000ffffu;
+                                    x &= keep;
+                                    f |= keep != 0xffffffffu;
+                                };
+                                fix(v.x);
+                                fix(v.y);
+                                fix(v.z);
+                                fix(v.w);
+                                const bool out = kbase + key >= s.len;
+                                if (out) v = make_uint4(0u, 0u, 0u, 0u);
+                                if (f || out) *at = v;
+                                found |= f && !out;
+                            }
+                            if (found) *odd = 1;
+                            fence_proxy_async_smem();
+                        }
+                        asm volatile("bar.sync 1, %0;" ::"r"(nt * 128) : "memory");
+                    }
+                    if (!ok) continue;
+                    if (idle) {                         // their P is whatever S held: no other row reads it
+                        mbar_arrive(&p_full[t * 2]);
+                        mbar_arrive(&p_full[t * 2 + 1]);
+                        cnt++;
+                        continue;
+                    }
+                    tc_fence_after_sync();
+                    if (whole) soft(std::true_type{}, j, kbase, srow);
+                    else soft(std::false_type{}, j, kbase, srow);
+                    cnt++;
                 }
                 // epilogue: the last P V has landed
                 if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&o_done[t], (cnt - 1) & 1, deadline, a.err));
@@ -547,7 +645,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
 #pragma unroll
                     for (int c0 = 0; c0 < D; c0 += 32) {
                         uint32_t v[32];
-                        tmem_ld32(trow + 128 + c0, v);
+                        tmem_ld32(orow_t + c0, v);
                         tmem_ld_wait();
                         float o[32];
 #pragma unroll
@@ -627,26 +725,18 @@ __global__ void __launch_bounds__(256) tile_merge_kernel(const Args a, int ctas)
     const Work w = work_of<ROWS>(a, s, lo);
     if (s.T > a.max_q && blockIdx.x == 0 && threadIdx.x == 0) atomicOr(a.err, DEVERR_BOUND);
     __syncthreads();
-    const long long W = s_all, total = (long long)w.nrows * a.Hkv;
+    const Share sh(s_all, ctas);
+    const long long total = (long long)w.nrows * a.Hkv;
     for (long long x = (long long)blockIdx.x * 8 + warp; x < total; x += (long long)gridDim.x * 8) {
         const int kvh = (int)(x / w.nrows), rr = (int)(x - (long long)kvh * w.nrows), z = rr / ROWS;
         const long long u0 = s_before + (long long)(z * a.Hkv + kvh) * w.nblk, u1 = u0 + w.nblk - 1;
-        // CTA of a block: the last c with share(c) <= block
-        auto owner = [&](long long u) {
-            int c = (int)(u * ctas / W);
-            while (c + 1 < ctas && share(W, c + 1, ctas) <= u) c++;
-            while (c > 0 && share(W, c, ctas) > u) c--;
-            return c;
-        };
-        const int c0 = owner(u0), c1 = owner(u1);
+        const int c0 = sh.owner(u0), c1 = sh.owner(u1);
         if (c0 == c1) continue;                                   // written by the CTA itself
-        // CTAs between without blocks (more CTAs than blocks) left nothing
         const int r = rr - z * ROWS;
         auto slot = [&](int c) { return ((size_t)c * 2 + (c == c0)) * ROWS + r; };
         float m = -INFINITY;
         bool nan = false;
         for (int c = c0 + lane; c <= c1; c += 32) {
-            if (share(W, c, ctas) == share(W, c + 1, ctas)) continue;
             const float y = a.part_lse[slot(c)];
             nan |= y != y;
             m = fmaxf(m, y);
@@ -658,7 +748,6 @@ __global__ void __launch_bounds__(256) tile_merge_kernel(const Args a, int ctas)
         if (m != -INFINITY || nan) {
 #pragma unroll 4
             for (int c = c0; c <= c1; c++) {
-                if (share(W, c, ctas) == share(W, c + 1, ctas)) continue;
                 const float y = a.part_lse[slot(c)];
                 if (y == -INFINITY) continue;
                 const float e = ex2((y - m) * LOG2E);
@@ -740,7 +829,16 @@ ckl_status launch_tiles(const ckl_tree_params* p, Args a, void* workspace, int c
     if (st != CKL_OK) return st;
     st = encode_tile_map(p->v_cache, p->Hkv, p->num_pages, &tmV);
     if (st != CKL_OK) return st;
-    void* args[] = {&tmK, &tmV, &a};
+    // Q tiles by tensor map: [tokens][heads of the group][64 dims] are the stacked rows in order
+    a.q_tma = 128 % a.G == 0;
+    const uint64_t qdims[3] = {(uint64_t)D, (uint64_t)p->Hq, (uint64_t)p->N};
+    const uint64_t qstrides[2] = {(uint64_t)D * 2, (uint64_t)p->Hq * D * 2};
+    const uint32_t qbox[3] = {64, (uint32_t)(a.q_tma ? a.G : 1), (uint32_t)(a.q_tma ? 128 / a.G : 1)};
+    CUtensorMap tmQ;
+    st = encode_tiled(&tmQ, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(p->q), qdims, qstrides, qbox,
+                      CU_TENSOR_MAP_SWIZZLE_128B);
+    if (st != CKL_OK) return st;
+    void* args[] = {&tmK, &tmV, &tmQ, &a};
     const bool ext = p->softcap > 0.f || p->slopes;
     CKL_CUDA_TRY(launch(tile_fn(MT, ext), dim3((unsigned)ctas), dim3(64 + 128 * MT), MT == 1 ? Cfg<1>::SMEM : Cfg<2>::SMEM,
                         s, args, true));
