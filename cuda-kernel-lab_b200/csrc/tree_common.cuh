@@ -44,6 +44,7 @@ struct Seq {
     int len;        // cached tokens, new ones included
     int q0, T;      // first row and count of the new tokens
     int ctx;        // cache place of new token 0 (negative when the table is too short)
+    __device__ __forceinline__ Seq() : page0(0), len(0), q0(0), T(0), ctx(0) {}
     __device__ __forceinline__ Seq(const Args& a, int b) {
         len = seq_len(a.indptr, a.last, b, &page0);
         q0 = a.q_indptr ? __ldg(a.q_indptr + b) : b;

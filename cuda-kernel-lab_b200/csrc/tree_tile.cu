@@ -40,7 +40,7 @@ template <int MT> struct Cfg {
     static constexpr int KST = MT == 1 ? 4 : 3;    // K blocks in flight
     static constexpr int SB = MT == 1 ? 2 : 1;     // S buffers of a tile
     static constexpr int TILE_COLS = SB * 128 + 128;   // tensor memory of a tile: S (and P), then O
-    static constexpr int THREADS = 64 + 128 * MT;
+    static constexpr int THREADS = 128 + 128 * MT; // warps 0-3: TMA, MMA, schedule, none; then a thread per row
     static constexpr int ROWS = 128 * MT;
     static constexpr int OFF_K = MT * Q_TILE;
     static constexpr int OFF_V = OFF_K + KST * KV_BLK;
@@ -270,10 +270,14 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
     const uint64_t deadline = globaltimer() + a.timeout_ns;
     Walk<C::ROWS> walk(range[0], range[1], *range_b);
     Seg g;
-    Seq s(a, 0);
+    Seq s;
     Work w;
     int pos_hi;
 
+    if (warp < 4) {
+    // 384 threads are launched with 168 registers each, and a thread that holds a row of S needs
+    // more: 128 * 72 + 256 * 216 = 384 * 168
+    if (MT == 2) regs_down<72>();
     if (warp == 0) {
         // ---------------------------------------------------------------- TMA producer
         const uint64_t pol = policy_evict_first();
@@ -447,9 +451,11 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
         }
         if (elect_one()) umma_commit(done);
         __syncwarp();
+    }
     } else {
+        if (MT == 2) regs_up<216>();
         // ---------------------------------------------------------------- softmax: a row per thread
-        const int t = (warp - 2) >> 2, quarter = warp & 3;
+        const int t = (warp - 4) >> 2, quarter = warp & 3;
         const int r = quarter * 32 + lane;              // row of the tile
         const uint32_t trow = tmem + t * COLS + ((uint32_t)(quarter * 32) << 16);
         const uint32_t orow_t = trow + SB * 128;        // this thread's row of O
@@ -477,9 +483,10 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
 
                 const bool idle = t * 128 + quarter * 32 >= g.rows;   // only padding rows: no softmax
                 float m = -INFINITY, l = 0.f;
-                // One block of the row: S from tensor memory, P back. S is read twice, for the maximum
-                // and for the weights, so that 32 columns at a time are in registers. Columns 32 q ..:
-                // keys 8 (q/2) .. + 8 of pages 4 (q%2) .. + 4. `whole`: every row sees every key.
+                // One block of the row: S from tensor memory, P back. Columns 32 q ..: keys 8 (q/2) ..
+                // + 8 of pages 4 (q%2) .. + 4. `whole`: every row sees every key; S is then held in
+                // registers. Other blocks (the last one or two, or a window's border) read S twice,
+                // for the maximum and for the weights, in rolled loops: little code to fetch.
                 auto soft = [&](auto whole_, int j, int kbase, uint32_t srow) {
                     constexpr bool WHOLE = decltype(whole_)::value;
                     uint32_t see[4];
@@ -512,20 +519,28 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                             }
                         }
                     };
+                    float row_s[WHOLE ? 4 : 1][32];
                     float mx = -INFINITY;
-                    const bool raw = WHOLE && !(EXT && a.slopes);   // the score grows with q.k: one is enough
+                    if (WHOLE) {
+#pragma unroll
+                        for (int q = 0; q < 4; q++)
+                            tmem_ld32(srow + q * 32, reinterpret_cast<uint32_t(&)[32]>(row_s[WHOLE ? q : 0]));
+                        tmem_ld_wait();
+                    }
 #pragma unroll(WHOLE ? 4 : 1)
                     for (int q = 0; q < 4; q++) {
-                        float x[32];
-                        tmem_ld32(srow + q * 32, reinterpret_cast<uint32_t(&)[32]>(x));
-                        tmem_ld_wait();
-                        if (!raw) scored(q, x);
+                        float (&x)[32] = row_s[WHOLE ? q : 0];
+                        if (!WHOLE) {
+                            tmem_ld32(srow + q * 32, reinterpret_cast<uint32_t(&)[32]>(x));
+                            tmem_ld_wait();
+                        }
+                        if (EXT || !WHOLE) scored(q, x);
                         float m4[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
                         for (int c = 4; c < 32; c++) m4[c & 3] = fmaxf(m4[c & 3], x[c]);
                         mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
                     }
-                    if (raw) mx = score<EXT>(a, mx);
+                    if (!EXT && WHOLE) mx *= a.scale_log2;       // > 0: the greatest product is enough
                     if (__any_sync(0xffffffffu, mx > m + RESCALE_THRESHOLD)) {
                         const float mn = fmaxf(m, mx);
                         const float cf = mn == -INFINITY ? 1.f : ex2(m - mn);
@@ -556,10 +571,12 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                         uint32_t pk[32];
 #pragma unroll
                         for (int u = 0; u < 2; u++) {
-                            float x[32];
-                            tmem_ld32(srow + (2 * u + h) * 32, reinterpret_cast<uint32_t(&)[32]>(x));
-                            tmem_ld_wait();
-                            if (!FOLD) scored(2 * u + h, x);
+                            float (&x)[32] = row_s[WHOLE ? 2 * u + h : 0];
+                            if (!WHOLE) {
+                                tmem_ld32(srow + (2 * u + h) * 32, reinterpret_cast<uint32_t(&)[32]>(x));
+                                tmem_ld_wait();
+                                scored(2 * u + h, x);
+                            }
 #pragma unroll
                             for (int c = 0; c < 32; c += 2) {
                                 const float p0 = ex2(FOLD ? fmaf(x[c], a.scale_log2, -ms) : x[c] - ms);
@@ -594,7 +611,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                             // pages that every row sees whole are left; a window reaches all of them
                             const int pg0 = a.window > 0 ? 0 : max(0, min(BLK_PAGES, (s.ctx - kbase) / PAGE));
 #pragma unroll 4
-                            for (int c = pg0 * 256 + threadIdx.x - 64; c < BLK * 16; c += nthr) {
+                            for (int c = pg0 * 256 + threadIdx.x - 128; c < BLK * 16; c += nthr) {
                                 // chunk c: page c / 256, half, token, 16-byte piece (swizzled; all
                                 // pieces of a 128-byte row are treated alike)
                                 const int key = (c >> 8) * PAGE + ((c >> 3) & 15);
@@ -641,7 +658,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                     const bool full = g.blk0 == 0 && g.blk1 == g.nblk;
                     const float inv = l != 0.f ? 1.f / l : 0.f;
                     const float lse_v = l != 0.f ? ((m == -INFINITY ? 0.f : m) + lg2(l)) * LN2 : -INFINITY;
-                    const size_t slot = ((size_t)blockIdx.x * 2 + (g.blk0 == 0)) * C::ROWS + t * 128 + r;
+                    const size_t slot0 = ((size_t)blockIdx.x * 2 + (g.blk0 == 0)) * C::ROWS;
 #pragma unroll
                     for (int c0 = 0; c0 < D; c0 += 32) {
                         uint32_t v[32];
@@ -679,16 +696,17 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                                     dst[i] = make_uint4(pack_half2(o[8 * i], o[8 * i + 1]), pack_half2(o[8 * i + 2], o[8 * i + 3]),
                                                         pack_half2(o[8 * i + 4], o[8 * i + 5]), pack_half2(o[8 * i + 6], o[8 * i + 7]));
                             } else {
-                                float4* dst = reinterpret_cast<float4*>(a.part_o + slot * D + c0);
+                                // [dims / 4][rows]: the threads of a warp write side by side
+                                float4* dst = reinterpret_cast<float4*>(a.part_o) + (slot0 * (D / 4) + (c0 / 4) * C::ROWS) + t * 128 + r;
 #pragma unroll
                                 for (int i = 0; i < 8; i++)
-                                    dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                                    dst[i * C::ROWS] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                             }
                         }
                     }
                     if (row.i >= 0) {
                         if (full) a.lse[orow] = lse_v;
-                        else a.part_lse[slot] = lse_v;
+                        else a.part_lse[slot0 + t * 128 + r] = lse_v;
                     }
                     tc_fence_before_sync();
                 }
@@ -704,69 +722,83 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
     if (warp == 1) tmem_dealloc(tmem, C::TMEM_COLS);
 }
 
-// Joins the units that more than one CTA worked on; one warp per row. grid = (row parts, B).
+// Joins the units that more than one CTA worked on. A CTA takes 32 rows of a unit at a time: the
+// lanes are the rows (a partial's rows lie side by side), a warp has 16 of the dims, and the
+// result goes through shared memory so that whole rows are written. grid = (row parts, B).
 template <int MT>
 __global__ void __launch_bounds__(256) tile_merge_kernel(const Args a, int ctas) {
     constexpr int ROWS = Cfg<MT>::ROWS;
     __shared__ long long s_before, s_all;
+    __shared__ uint2 s_out[32][D / 4 + 1];
     pdl_wait();
     pdl_trigger();
     const int b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const Seq s(a, b);
-    if (warp == 0) {
-        const long long x = blocks_before<ROWS>(a, b, lane);
-        if (lane == 0) s_before = x;
-    } else if (warp == 1) {
-        const long long x = blocks_before<ROWS>(a, a.B, lane);
-        if (lane == 0) s_all = x;
+    if (warp < 2) {
+        const long long x = blocks_before<ROWS>(a, warp ? a.B : b, lane);
+        if (lane == 0) (warp ? s_all : s_before) = x;
     }
+    const Seq s(a, b);
     int lo = 0, hi;
     if (a.window > 0) pos_range(a, s, lane, &lo, &hi);
     const Work w = work_of<ROWS>(a, s, lo);
     if (s.T > a.max_q && blockIdx.x == 0 && threadIdx.x == 0) atomicOr(a.err, DEVERR_BOUND);
     __syncthreads();
     const Share sh(s_all, ctas);
-    const long long total = (long long)w.nrows * a.Hkv;
-    for (long long x = (long long)blockIdx.x * 8 + warp; x < total; x += (long long)gridDim.x * 8) {
-        const int kvh = (int)(x / w.nrows), rr = (int)(x - (long long)kvh * w.nrows), z = rr / ROWS;
-        const long long u0 = s_before + (long long)(z * a.Hkv + kvh) * w.nblk, u1 = u0 + w.nblk - 1;
-        const int c0 = sh.owner(u0), c1 = sh.owner(u1);
+    const int parts = (w.nrows + 31) / 32, total = parts * a.Hkv;         // 32 rows of one kv head
+    for (int x = blockIdx.x; x < total; x += gridDim.x) {
+        const int kvh = x / parts, row0 = (x - kvh * parts) * 32, z = row0 / ROWS;
+        const long long u0 = s_before + (long long)(z * a.Hkv + kvh) * w.nblk;
+        const int c0 = sh.owner(u0), c1 = sh.owner(u0 + w.nblk - 1);
         if (c0 == c1) continue;                                   // written by the CTA itself
-        const int r = rr - z * ROWS;
-        auto slot = [&](int c) { return ((size_t)c * 2 + (c == c0)) * ROWS + r; };
+        const int rr = row0 + lane, r = rr - z * ROWS;
+        auto slot = [&](int c) { return ((size_t)c * 2 + (c == c0)) * ROWS; };
         float m = -INFINITY;
         bool nan = false;
-        for (int c = c0 + lane; c <= c1; c += 32) {
-            const float y = a.part_lse[slot(c)];
+#pragma unroll 4
+        for (int c = c0; c <= c1; c++) {
+            const float y = rr < w.nrows ? a.part_lse[slot(c) + r] : -INFINITY;
             nan |= y != y;
             m = fmaxf(m, y);
         }
-        m = warp_max(m);
-        nan = __any_sync(0xffffffffu, nan);
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        const bool any = m != -INFINITY || nan;
+        float4 acc[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         float ws = 0.f;
-        if (m != -INFINITY || nan) {
-#pragma unroll 4
-            for (int c = c0; c <= c1; c++) {
-                const float y = a.part_lse[slot(c)];
-                if (y == -INFINITY) continue;
-                const float e = ex2((y - m) * LOG2E);
-                const float4 v = reinterpret_cast<const float4*>(a.part_o + slot(c) * D)[lane];
-                ws += e;
-                acc.x += e * v.x;
-                acc.y += e * v.y;
-                acc.z += e * v.z;
-                acc.w += e * v.w;
+#pragma unroll 2
+        for (int c = c0; c <= c1; c++) {
+            const float y = rr < w.nrows ? a.part_lse[slot(c) + r] : -INFINITY;
+            const float e = any && y != -INFINITY ? ex2((y - m) * LOG2E) : 0.f;
+            ws += e;
+            const float4* po = reinterpret_cast<const float4*>(a.part_o) + slot(c) * (D / 4) + (warp * 4) * ROWS + r;
+            if (e != 0.f) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float4 v = po[i * ROWS];
+                    acc[i].x += e * v.x;
+                    acc[i].y += e * v.y;
+                    acc[i].z += e * v.z;
+                    acc[i].w += e * v.w;
+                }
             }
         }
         const float inv = ws != 0.f ? 1.f / ws : 0.f;
-        const int i = rr / a.G;
-        const size_t row = (size_t)(s.q0 + i) * a.Hq + kvh * a.G + (rr - i * a.G);
-        uint2 pk;
-        pk.x = pack_half2(acc.x * inv, acc.y * inv);
-        pk.y = pack_half2(acc.z * inv, acc.w * inv);
-        reinterpret_cast<uint2*>(a.out + row * D)[lane] = pk;
-        if (lane == 0) a.lse[row] = ws != 0.f ? m + logf(ws) : -INFINITY;
+        __syncthreads();                                          // the rows before are written
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            s_out[lane][warp * 4 + i] = make_uint2(pack_half2(acc[i].x * inv, acc[i].y * inv),
+                                                   pack_half2(acc[i].z * inv, acc[i].w * inv));
+        auto orow = [&](int row) {
+            const int i = row / a.G;
+            return (size_t)(s.q0 + i) * a.Hq + kvh * a.G + (row - i * a.G);
+        };
+        if (warp == 0 && rr < w.nrows) a.lse[orow(rr)] = ws != 0.f ? m + logf(ws) : -INFINITY;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int q = warp * 4 + i;
+            if (row0 + q < w.nrows) reinterpret_cast<uint2*>(a.out + orow(row0 + q) * D)[lane] = s_out[q][lane];
+        }
     }
 }
 
@@ -840,11 +872,11 @@ ckl_status launch_tiles(const ckl_tree_params* p, Args a, void* workspace, int c
     if (st != CKL_OK) return st;
     void* args[] = {&tmK, &tmV, &tmQ, &a};
     const bool ext = p->softcap > 0.f || p->slopes;
-    CKL_CUDA_TRY(launch(tile_fn(MT, ext), dim3((unsigned)ctas), dim3(64 + 128 * MT), MT == 1 ? Cfg<1>::SMEM : Cfg<2>::SMEM,
+    CKL_CUDA_TRY(launch(tile_fn(MT, ext), dim3((unsigned)ctas), dim3(128 + 128 * MT), MT == 1 ? Cfg<1>::SMEM : Cfg<2>::SMEM,
                         s, args, true));
     void* margs[] = {&a, &ctas};
-    const long long rows = (long long)p->max_q * p->Hq;
-    const unsigned gx = (unsigned)std::max(1LL, std::min((rows + 7) / 8, (long long)(8 * di->sms + p->B - 1) / p->B));
+    const long long parts = ((long long)p->max_q * a.G + 31) / 32 * p->Hkv;
+    const unsigned gx = (unsigned)std::max(1LL, std::min(parts, (long long)(8 * di->sms + p->B - 1) / p->B));
     CKL_CUDA_TRY(launch(MT == 1 ? (const void*)tile_merge_kernel<1> : (const void*)tile_merge_kernel<2>,
                         dim3(gx, (unsigned)p->B), dim3(256), 0, s, margs, true));
     return CKL_OK;
