@@ -3,8 +3,8 @@
 //
 // A CTA holds 128 * MT rows of one (sequence, kv head) as MT tiles, the M of tcgen05.mma, and
 // streams keys in blocks of 8 pages:
-//   S = Q K^T   M=128, N=64, twice per block: Q and K (both K-major) in shared memory, S in
-//               tensor memory (128 columns a tile);
+//   S = Q K^T   M=128, N=128: Q and K (both K-major) in shared memory, S in tensor memory (128
+//               columns a tile);
 //   softmax     one thread per row: the row of S from tensor memory, online max and sum in
 //               registers, P = exp2(S - m) as fp16 back into tensor memory, over S;
 //   O += P V    M=128, N=128, K=16 a page: P from tensor memory, V (MN-major) from shared
@@ -12,9 +12,10 @@
 // Both tiles use the same K and V block: with 256 rows the stream is read once where the tensor
 // cores still keep up with it (512 flops per byte of K and V against the card's ~256).
 //
-// A page arrives as one 4 KB box per K and V: [64-dim half][16 tokens][64 dims]. A block's eight
-// pages lie 4 KB apart, so the keys 0-7 of all pages (8-row groups, 4 KB stride) form one MMA
-// operand of N = 64 and the keys 8-15 another: S column u*64 + 8*page + k is key 16*page + 8*u + k.
+// V pages arrive as one 4 KB box each, [64-dim half][16 tokens][64 dims]. K pages take a 2 KB box
+// per half, so that the block's 128 keys of a half lie together and S is one N = 128 product: with
+// 4 KB boxes the eight pages' 8-row groups form two operands of N = 64, and Q would be read from
+// shared memory twice as often (49 against 65 cycles per K = 16 step for half the keys).
 //
 // Work is divided exactly: the key blocks of all (sequence, row group, kv head) units, end to
 // end, over one wave of CTAs. A unit that lies within one CTA is written out directly; where a
@@ -304,8 +305,9 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                 }
                 ok = __shfl_sync(0xffffffffu, ok, 0);
                 if (!ok) break;
-                if (lane < BLK_PAGES)
-                    tma_load_5d(kring + ks * KV_BLK + lane * KV_TILE, &tmK, 0, 0, 0, g.kvh, page, &k_full[ks], pol);
+                if (lane < 2 * BLK_PAGES)               // half lane / 8 of page lane % 8
+                    tma_load_5d(kring + ks * KV_BLK + (lane >> 3) * (KV_BLK / 2) + (lane & 7) * HALF_TILE, &tmK, 0, 0,
+                                lane >> 3, g.kvh, page, &k_full[ks], pol);
                 if (lane == 0) {
                     if (n >= VST) ok = mbar_wait(&v_empty[vs], ((n / VST) - 1) & 1, deadline, a.err);
                     if (ok) mbar_arrive_expect_tx(&v_full[vs], KV_BLK);
@@ -350,10 +352,10 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
         // ---------------------------------------------------------------- MMA issuer
         // With one S buffer a tile's next S waits for its P V (P lies over the first half of S: the
         // other half is written meanwhile); with two it runs ahead of the softmax.
-        const uint32_t idesc_s = umma_idesc_f16(128, 64, false, false);
+        const uint32_t idesc_s = umma_idesc_f16(128, BLK, false, false);
         const uint32_t idesc_o = umma_idesc_f16(128, D, false, true);
         const uint64_t qd = umma_desc_sw128(smem_u32(qs), 16, 1024);
-        const uint64_t kd = umma_desc_sw128(smem_u32(kring), 16, KV_TILE);
+        const uint64_t kd = umma_desc_sw128(smem_u32(kring), 16, 1024);
         const uint64_t vd = umma_desc_sw128(smem_u32(vring), HALF_TILE, 1024);
         bool ok = true;
         int n = 0;                                      // blocks before this segment
@@ -364,15 +366,15 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
             const int nt = (g.rows + 127) / 128, nb = g.blk1 - g.blk0;
             if (elect_one()) {
                 auto wait = [&](uint64_t* bar, int phase) { return mbar_wait(bar, phase & 1, deadline, a.err); };
-                // half u of S of block j (of this segment), tile t (offsets in descriptors: 16 bytes)
-                auto qk = [&](int j, int t, int buf, int u) {
-                    const uint64_t kb = kd + (uint64_t)((n + j) % KST * (KV_BLK / 16) + u * (1024 / 16));
+                // S of block j (of this segment), tile t (offsets in descriptors: 16 bytes)
+                auto qk = [&](int j, int t, int buf) {
+                    const uint64_t kb = kd + (uint64_t)((n + j) % KST * (KV_BLK / 16));
                     const uint64_t qb = qd + (uint64_t)(t * (Q_TILE / 16));
-                    const uint32_t d = tmem + t * COLS + buf * 128 + u * 64;
+                    const uint32_t d = tmem + t * COLS + buf * 128;
 #pragma unroll
                     for (int kk = 0; kk < 8; kk++)
                         umma_f16(d, qb + ((kk >> 2) * (Q_TILE / 2) + (kk & 3) * 32) / 16,
-                                 kb + ((kk >> 2) * HALF_TILE + (kk & 3) * 32) / 16, idesc_s, kk != 0);
+                                 kb + ((kk >> 2) * (KV_BLK / 2) + (kk & 3) * 32) / 16, idesc_s, kk != 0);
                 };
                 auto qk_done = [&](int j, int t, int buf) {
                     umma_commit(&s_full[t * SB + buf]);
@@ -391,8 +393,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                     if (ok && c > 0) ok = wait(&o_done[t], c - 1);
                     if (!ok) break;
                     tc_fence_after_sync();
-                    qk(0, t, c % SB, 0);
-                    qk(0, t, c % SB, 1);
+                    qk(0, t, c % SB);
                     qk_done(0, t, c % SB);
                 }
                 for (int j = 0; j < nb && ok; j++) {
@@ -409,8 +410,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                             if (ok && j > 0) ok = wait(&o_done[t], c - 1);
                             if (!ok) break;
                             tc_fence_after_sync();
-                            qk(j + 1, t, buf ^ 1, 0);
-                            qk(j + 1, t, buf ^ 1, 1);
+                            qk(j + 1, t, buf ^ 1);
                             qk_done(j + 1, t, buf ^ 1);
                         }
 #pragma unroll
@@ -428,13 +428,11 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                         if (t == nt - 1) umma_commit(&v_empty[vs]);
                         if (SB == 1 && j + 1 < nb) {
                             if (t == 0) ok = wait(&k_full[k1 % KST], k1 / KST);
+                            // P, over S, must have been read
+                            if (ok) ok = wait(&o_done[t], c);
                             if (!ok) break;
                             tc_fence_after_sync();
-                            qk(j + 1, t, 0, 1);
-                            ok = wait(&o_done[t], c);
-                            if (!ok) break;
-                            tc_fence_after_sync();
-                            qk(j + 1, t, 0, 0);
+                            qk(j + 1, t, 0);
                             qk_done(j + 1, t, 0);
                         }
                     }
@@ -483,40 +481,30 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
 
                 const bool idle = t * 128 + quarter * 32 >= g.rows;   // only padding rows: no softmax
                 float m = -INFINITY, l = 0.f;
-                // One block of the row: S from tensor memory, P back. Columns 32 q ..: keys 8 (q/2) ..
-                // + 8 of pages 4 (q%2) .. + 4. `whole`: every row sees every key; S is then held in
-                // registers. Other blocks (the last one or two, or a window's border) read S twice,
+                // One block of the row: S from tensor memory, P back. `whole`: every row sees every
+                // key; S is then held in registers. Other blocks (the last one or two, or a window's border) read S twice,
                 // for the maximum and for the weights, in rolled loops: little code to fetch.
                 auto soft = [&](auto whole_, int j, int kbase, uint32_t srow) {
                     constexpr bool WHOLE = decltype(whole_)::value;
-                    uint32_t see[4];
-                    if (!WHOLE) {
-#pragma unroll
-                        for (int i = 0; i < 4; i++) see[i] = seen32(a, s, row, kbase + 32 * i);
-                    }
                     // the scores of columns 32 q .., -inf where unseen
                     auto scored = [&](int q, float (&x)[32]) {
-                        if (EXT) {
+                        score32<EXT>(a, x);
+                        if (EXT && a.slopes) {
+                            if (WHOLE) {
+                                // slope (kpos - qpos), key by key from the block's first
+                                const float b0 = row.slope2 * (float)(kbase + 32 * q - row.pos);
 #pragma unroll
-                            for (int c = 0; c < 32; c++) x[c] = score<true>(a, x[c]);
-                            if (a.slopes) {
+                                for (int c = 0; c < 32; c++) x[c] += fmaf(row.slope2, (float)c, b0);
+                            } else {
 #pragma unroll
-                                for (int c = 0; c < 32; c++) {
-                                    const int p = kbase + ((q & 1) * 4 + (c >> 3)) * PAGE + (q >> 1) * 8 + (c & 7);
-                                    x[c] += bias<true>(a, row.slope2, row.pos, WHOLE ? p : s.pos(a, p));
-                                }
+                                for (int c = 0; c < 32; c++) x[c] += bias<true>(a, row.slope2, row.pos, s.pos(a, kbase + 32 * q + c));
                             }
-                        } else {
-#pragma unroll
-                            for (int c = 0; c < 32; c++) x[c] *= a.scale_log2;
                         }
                         if (!WHOLE) {
+                            const uint32_t v = seen32(a, s, row, kbase + 32 * q);
 #pragma unroll
-                            for (int c = 0; c < 32; c++) {
-                                const int pg = c >> 3;               // of this half's four
-                                const uint32_t w2 = (q & 1) ? see[2 + (pg >> 1)] : see[pg >> 1];
-                                if (!((w2 >> ((q >> 1) * 8 + (pg & 1) * 16 + (c & 7))) & 1u)) x[c] = -INFINITY;
-                            }
+                            for (int c = 0; c < 32; c++)
+                                if (!((v >> c) & 1u)) x[c] = -INFINITY;
                         }
                     };
                     float row_s[WHOLE ? 4 : 1][32];
@@ -564,35 +552,40 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                     const float ms = m == -INFINITY ? 0.f : m;   // a row that saw nothing yet
                     // P in fp16 for the product (2^-11 of each weight, as V's own rounding); l sums
                     // the unrounded weights
-                    float l4[4] = {0.f, 0.f, 0.f, 0.f};
+                    float2 l4[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) l4[i] = make_float2(0.f, 0.f);
                     constexpr bool FOLD = !EXT && WHOLE;         // the scale goes into the exponent
 #pragma unroll(WHOLE ? 2 : 1)
-                    for (int h = 0; h < 2; h++) {        // pages 4h .. 4h + 3: S columns of q = h and h + 2
+                    for (int h = 0; h < 2; h++) {        // pages 4h .. 4h + 3
                         uint32_t pk[32];
 #pragma unroll
                         for (int u = 0; u < 2; u++) {
-                            float (&x)[32] = row_s[WHOLE ? 2 * u + h : 0];
+                            float (&x)[32] = row_s[WHOLE ? 2 * h + u : 0];
                             if (!WHOLE) {
-                                tmem_ld32(srow + (2 * u + h) * 32, reinterpret_cast<uint32_t(&)[32]>(x));
+                                tmem_ld32(srow + (2 * h + u) * 32, reinterpret_cast<uint32_t(&)[32]>(x));
                                 tmem_ld_wait();
-                                scored(2 * u + h, x);
+                                scored(2 * h + u, x);
                             }
 #pragma unroll
                             for (int c = 0; c < 32; c += 2) {
-                                const float p0 = ex2(FOLD ? fmaf(x[c], a.scale_log2, -ms) : x[c] - ms);
-                                const float p1 = ex2(FOLD ? fmaf(x[c + 1], a.scale_log2, -ms) : x[c + 1] - ms);
-                                l4[(c >> 1) & 3] += p0 + p1;
-                                pk[(c >> 3) * 8 + u * 4 + ((c & 7) >> 1)] = pack_half2(p0, p1);
+                                const float2 v = make_float2(x[c], x[c + 1]);
+                                const float2 e = FOLD ? fma2(v, make_float2(a.scale_log2, a.scale_log2), make_float2(-ms, -ms))
+                                                      : add2(v, make_float2(-ms, -ms));
+                                const float2 p = make_float2(ex2(e.x), ex2(e.y));
+                                l4[(c >> 1) & 3] = add2(l4[(c >> 1) & 3], p);
+                                pk[u * 16 + (c >> 1)] = pack_half2(p.x, p.y);
                             }
                         }
-                        // P of pages 0-3 goes over S columns 0-31, pages 4-7 over 32-63: only once
-                        // those are in registers
+                        // P of pages 0-3 goes over S columns 0-31, pages 4-7 over 32-63: those are in
+                        // registers by now
                         tmem_st32(srow + h * 32, pk);
                         tmem_st_wait();
                         tc_fence_before_sync();
                         mbar_arrive(&p_full[t * 2 + h]);
                     }
-                    l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+                    const float2 l2 = add2(add2(l4[0], l4[1]), add2(l4[2], l4[3]));
+                    l += l2.x + l2.y;
                 };
                 for (int j = 0; j < nb; j++) {
                     const int kbase = w.first + (g.blk0 + j) * BLK;
@@ -821,11 +814,11 @@ ckl_status setup_tiles(const DeviceInfo* di) {
     return st[di->device];
 }
 
-// One page as one box [64-dim half][16 tokens][64 dims] of one head.
-ckl_status encode_tile_map(const void* cache, int Hkv, int num_pages, CUtensorMap* tm) {
+// A page of one head as a box [halves][16 tokens][64 dims].
+ckl_status encode_tile_map(const void* cache, int Hkv, int num_pages, int halves, CUtensorMap* tm) {
     const uint64_t dims[5] = {64, (uint64_t)PAGE, 2, (uint64_t)Hkv, (uint64_t)num_pages};
     const uint64_t strides[4] = {(uint64_t)Hkv * D * 2, 128, (uint64_t)D * 2, (uint64_t)PAGE * Hkv * D * 2};
-    const uint32_t box[5] = {64, (uint32_t)PAGE, 2, 1, 1};
+    const uint32_t box[5] = {64, (uint32_t)PAGE, (uint32_t)halves, 1, 1};
     return encode_tiled(tm, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void*>(cache), dims, strides, box,
                         CU_TENSOR_MAP_SWIZZLE_128B);
 }
@@ -857,9 +850,9 @@ ckl_status launch_tiles(const ckl_tree_params* p, Args a, void* workspace, int c
     a.part_o = static_cast<float*>(workspace);
     a.part_lse = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + o);
     CUtensorMap tmK, tmV;
-    st = encode_tile_map(p->k_cache, p->Hkv, p->num_pages, &tmK);
+    st = encode_tile_map(p->k_cache, p->Hkv, p->num_pages, 1, &tmK);
     if (st != CKL_OK) return st;
-    st = encode_tile_map(p->v_cache, p->Hkv, p->num_pages, &tmV);
+    st = encode_tile_map(p->v_cache, p->Hkv, p->num_pages, 2, &tmV);
     if (st != CKL_OK) return st;
     // Q tiles by tensor map: [tokens][heads of the group][64 dims] are the stacked rows in order
     a.q_tma = 128 % a.G == 0;
