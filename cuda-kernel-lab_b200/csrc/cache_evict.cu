@@ -5,8 +5,9 @@
 #include <algorithm>
 #include <climits>
 #include <mutex>
+#include <type_traits>
 
-#include "tree_common.cuh"
+#include "tree_tile.cuh"
 
 namespace ckl {
 namespace evict {
@@ -17,15 +18,25 @@ using tree::Seq;
 
 // ------------------------------------------------------------------ weights
 // acc[b][p] += sum over rows r (tokens x heads) of exp(s_rp - lse_r): one pass over K (half the
-// bytes of an attention call), bound by HBM for few rows. A warp owns whole pages, all kv heads
-// of them, so a token's sum stays in its registers and is added in a fixed order: no atomics,
-// no second kernel. S = K Q^T tiles by mma.sync as in the attention; the softmax is already
-// normalised by the caller's lse, so there is no running maximum.
-constexpr int W_WARPS = 8;
-constexpr int W_THREADS = W_WARPS * 32;
-constexpr int W_STAGES = 3;                    // K tiles (one page, one head: 4 KB) in flight per warp
-constexpr int W_PAGES = 2 * W_WARPS;           // pages of a CTA's chunk, at most
-constexpr int W_RING = W_WARPS * W_STAGES * KV_TILE;
+// bytes of an attention call), bound by HBM for few rows and by the exponentials for many.
+//
+// S^T = K Q^T on tcgen05 with the keys as M: 128 keys are the lanes of tensor memory and the rows
+// of a kv head its columns, so a thread owns a key and its sum over rows and heads stays with it:
+// no atomics and no second kernel, the same order of additions whatever the batch. The lse of the
+// attention call already normalises, so there is no running maximum either.
+//
+// The pages of all sequences, end to end, are divided evenly over one wave of CTAs. A CTA's run of
+// a sequence is taken W_SEG blocks at a time: for each kv head (and each W_ROWS of its rows) Q is
+// staged once and the blocks' K tiles stream past it. Warp 0 loads K (TMA), warp 1 issues the MMAs,
+// warps 2-3 stage Q and the rows' lse, position and slope, eight warps turn S into weights (two
+// threads per key, half of the columns each).
+constexpr int W_THREADS = 384;
+constexpr int W_BLK = 128;                     // keys of a tile
+constexpr int W_BLK_PAGES = W_BLK / PAGE;
+constexpr int W_TILE = W_BLK * D * 2;          // 32 KB: dims 0-63 of 128 keys, then 64-127
+constexpr int W_ROWS = 256;                    // rows per staged Q, at most (N of the MMA)
+constexpr int W_SEG = 16;                      // blocks of a segment
+constexpr int W_MAX_STAGES = 6;
 
 struct WArgs {
     tree::Args t;
@@ -33,179 +44,393 @@ struct WArgs {
     float* acc;
     long long acc_stride;
     float decay;
-    int q_tiles;                               // row tiles of 16 that fit in the Q buffer
+    int rows;                                  // rows per staged Q: a multiple of 16, at most W_ROWS
+    int stages;                                // K tiles in flight
+};
+struct RowInfo {                               // of the columns of a staged Q
+    float lse2[W_ROWS], slope2[W_ROWS];        // lse in log2 (+inf: adds nothing)
+    int pos[W_ROWS], i[W_ROWS];
+};
+constexpr size_t W_FIXED = 1024 + 2 * sizeof(RowInfo) + 2 * W_SEG * W_BLK * 4 + (2 * W_MAX_STAGES + 11) * 8 + 16;
+constexpr size_t w_smem(int rows, int stages) { return W_FIXED + (size_t)2 * rows * D * 2 + (size_t)stages * W_TILE; }
+
+struct WSeg {
+    int b, pg0, pg1;                           // pages of the sequence
+};
+// A CTA's run of pages, a segment of at most W_SEG blocks at a time.
+struct WWalk {
+    long long left, off;
+    int b;
+    __device__ __forceinline__ bool next(const tree::Args& a, WSeg* g) {
+        while (left > 0 && b < a.B) {
+            int page0;
+            const int np = (tree::seq_len(a.indptr, a.last, b, &page0) + PAGE - 1) / PAGE;
+            if (off >= np) {
+                off -= np;
+                b++;
+                continue;
+            }
+            g->b = b;
+            g->pg0 = (int)off;
+            g->pg1 = (int)min(min((long long)np, off + left), off + W_SEG * W_BLK_PAGES);
+            left -= g->pg1 - g->pg0;
+            off = g->pg1;
+            return true;
+        }
+        return false;
+    }
 };
 
-constexpr int w_smem(int q_tiles) { return 1024 + W_RING + q_tiles * (KV_TILE + 16 * 4) + W_WARPS * W_STAGES * 8; }
+__device__ __forceinline__ uint32_t w_sw(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
 
-// grid = (CTAs per sequence, B): a CTA takes chunks of pages blockIdx.x, + gridDim.x, ...
 template <bool EXT>
-__global__ void __launch_bounds__(W_THREADS) weights_kernel(const __grid_constant__ CUtensorMap tmK, const WArgs w) {
+__global__ void __launch_bounds__(W_THREADS, 1)
+weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmQ, const WArgs w) {
     extern __shared__ uint8_t smem_raw[];
     const tree::Args& a = w.t;
-    uint8_t* ring = align_ptr<1024>(smem_raw);
-    uint8_t* qs = ring + W_RING;                                          // [q_tiles] swizzled like a page
-    float* ls = reinterpret_cast<float*>(qs + (size_t)w.q_tiles * KV_TILE);   // [q_tiles][16] lse, log2
-    uint64_t* full = reinterpret_cast<uint64_t*>(ls + w.q_tiles * 16);
+    const int N = w.rows, KST = w.stages, q_bytes = N * D * 2;
+    uint8_t* kring = align_ptr<1024>(smem_raw);
+    uint8_t* qs = kring + KST * W_TILE;                              // [2] staged Q: dims 0-63, then 64-127
+    RowInfo* info = reinterpret_cast<RowInfo*>(qs + 2 * q_bytes);    // [2]
+    float* sums = reinterpret_cast<float*>(info + 2);                // [2 column halves][W_SEG][128]
+    uint64_t* k_full = reinterpret_cast<uint64_t*>(sums + 2 * W_SEG * W_BLK);
+    uint64_t* k_empty = k_full + W_MAX_STAGES;
+    uint64_t* q_full = k_empty + W_MAX_STAGES;   // [2] staged
+    uint64_t* q_empty = q_full + 2;              // [2] its MMAs are done
+    uint64_t* i_empty = q_empty + 2;             // [2] the row infos have been used
+    uint64_t* d_full = i_empty + 2;              // [2] S written
+    uint64_t* d_empty = d_full + 2;              // [2] S read
+    uint64_t* done = d_empty + 2;                // every issued MMA finished
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+    __shared__ long long s_left, s_off;
+    __shared__ int s_b;
+
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < W_WARPS * W_STAGES; i++) mbar_init(&full[i], 1);
+        for (int i = 0; i < KST; i++) {
+            mbar_init(&k_full[i], 1);
+            mbar_init(&k_empty[i], 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&q_full[i], 65);
+            mbar_init(&q_empty[i], 1);
+            mbar_init(&i_empty[i], 256);
+            mbar_init(&d_full[i], 1);
+            mbar_init(&d_empty[i], 256);
+        }
+        mbar_init(done, 1);
         fence_barrier_init();
     }
-    __syncthreads();
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    if (warp == 0 && lane == 0) tma_prefetch_desc(&tmK);
     pdl_wait();
-    pdl_trigger();
-    const uint64_t deadline = globaltimer() + a.timeout_ns;
-    const Seq s(a, blockIdx.y);
-    const int npages = (s.len + PAGE - 1) / PAGE;
-    if (npages == 0) return;
-    if (s.T > a.max_q && blockIdx.x == 0 && threadIdx.x == 0) atomicOr(a.err, DEVERR_BOUND);
-    const int nrows = min(s.T, a.max_q) * a.G;
-    int pos_lo = 0, pos_hi = 0;
-    if (a.window > 0) pos_range(a, s, lane, &pos_lo, &pos_hi);
-    const int first = nrows > 0 ? tree::first_key(a, s, pos_lo) / PAGE : npages;   // pages before: nobody sees them
-    const int cp = min(W_PAGES, max(1, (npages + gridDim.x - 1) / gridDim.x));   // even chunks
-
-    const int tiles = (nrows + 15) / 16;
-    const int tb = min(max(tiles, 1), w.q_tiles);              // row tiles per block
-    const int hb = max(1, w.q_tiles / max(tiles, 1));          // heads per block (1 when rows are split)
-    uint8_t* myring = ring + warp * W_STAGES * KV_TILE;
-    uint64_t* myfull = full + warp * W_STAGES;
-    const uint64_t pol = policy_evict_first();
-    int nload = 0, nuse = 0;                                   // this warp's tiles, since the start
-    bool ok = true;
-
-    for (int chunk = blockIdx.x; (long long)chunk * cp < npages; chunk += gridDim.x) {
-        const int pg0 = chunk * cp, pg1 = min(npages, pg0 + cp);
-        float sum[2][2][2];                                    // [page of this warp][8-key half][key]
+    if (warp == 2) {
+        // this CTA's pages: two sweeps over the lengths
+        auto pages = [&](int b) {
+            int p;
+            return b < a.B ? (tree::seq_len(a.indptr, a.last, b, &p) + PAGE - 1) / PAGE : 0;
+        };
+        long long total = 0;
+        for (int b0 = 0; b0 < a.B; b0 += 32) total += pages(b0 + lane);
 #pragma unroll
-        for (int i = 0; i < 2; i++) sum[i][0][0] = sum[i][0][1] = sum[i][1][0] = sum[i][1][1] = 0.f;
-        // this warp's pages of the chunk that somebody can see: pg0 + warp + 8 i
-        int mine[2], ids[2], np = 0;
+        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        const tree::Share sh(total, gridDim.x);
+        const long long beg = sh.first(blockIdx.x);
+        long long before = 0;
+        int b = a.B;
+        for (int b0 = 0; b0 < a.B && b == a.B; b0 += 32) {
+            const int mine = pages(b0 + lane);
+            long long x = mine;
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const int pg = pg0 + warp + 8 * i;
-            mine[i] = pg;
-            ids[i] = pg < pg1 ? __ldg(a.indices + s.page0 + pg) : 0;
-            if (pg < pg1) np = i + 1;
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long y = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += y;
+            }
+            const unsigned over = __ballot_sync(0xffffffffu, before + x > beg);
+            const int l = over ? __ffs(over) - 1 : 31;
+            if (over) b = b0 + l;
+            before += __shfl_sync(0xffffffffu, over ? x - mine : x, l);
         }
-        for (int h0 = 0; h0 < a.Hkv; h0 += hb)
-            for (int t0 = 0; t0 < tiles; t0 += tb) {
-                const int nh = min(hb, a.Hkv - h0), nt = min(tb, tiles - t0);
-                // the units of this block: pages x heads, in order; issue the first ones now
-                const int units = np * nh;
-                auto issue = [&](int u) {
-                    const int i = u / nh, h = h0 + u - i * nh, sg = nload % W_STAGES;
-                    if (lane == 0) {
-                        mbar_arrive_expect_tx(&myfull[sg], KV_TILE);
-                        tma_load_5d(myring + sg * KV_TILE, &tmK, 0, 0, h, 0, ids[i], &myfull[sg], pol);
+        if (lane == 0) {
+            s_left = sh.first(blockIdx.x + 1) - beg;
+            s_off = beg - before;
+            s_b = b;
+        }
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    pdl_trigger();
+    const uint32_t tmem = *tmem_slot;
+    const uint64_t deadline = globaltimer() + a.timeout_ns;
+    WWalk walk{s_left, s_off, s_b};
+    WSeg g;
+    bool ok = true;
+    int chunk = 0, n = 0;                        // staged Qs and K tiles so far
+    // every role walks the same segments, chunks (kv head, rows) and blocks; pages before the
+    // first key in anyone's window are not loaded
+    auto plan = [&](const Seq& s, int* first, int* nrows, int* pos_hi) {
+        int lo = 0;
+        *pos_hi = s.len - 1;
+        *nrows = min(s.T, a.max_q) * a.G;
+        if (a.window > 0) tree::pos_range(a, s, lane, &lo, pos_hi);
+        *first = tree::first_key(a, s, lo) / PAGE;
+    };
+
+    if (warp == 0) {
+        // ---------------------------------------------------------------- K producer
+        const uint64_t pol = policy_evict_first();
+        while (ok && walk.next(a, &g)) {
+            const Seq s(a, g.b);
+            int first, nrows, pos_hi;
+            plan(s, &first, &nrows, &pos_hi);
+            const int pg0 = max(g.pg0, first);
+            int ids[W_SEG / 4];                              // the segment's page ids, 32 per register
+#pragma unroll
+            for (int i = 0; i < W_SEG / 4; i++) {
+                const int pg = pg0 + 32 * i + lane;
+                ids[i] = pg < g.pg1 ? __ldg(a.indices + s.page0 + pg) : 0;
+            }
+            for (int h = 0; h < a.Hkv && ok; h++)
+                for (int r0 = 0; r0 < nrows && ok; r0 += N)
+                    for (int pg = pg0; pg < g.pg1 && ok; pg += W_BLK_PAGES, n++) {
+                        const int np = min(W_BLK_PAGES, g.pg1 - pg), st = n % KST, j = (pg - pg0) / W_BLK_PAGES;
+                        int id = ids[0];
+#pragma unroll
+                        for (int i = 1; i < W_SEG / 4; i++) id = (j >> 2) == i ? ids[i] : id;
+                        int page[W_BLK_PAGES];
+#pragma unroll
+                        for (int i = 0; i < W_BLK_PAGES; i++) page[i] = __shfl_sync(0xffffffffu, id, (j & 3) * 8 + i);
+                        if (n >= KST) ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[st], (n / KST - 1) & 1, deadline, a.err));
+                        if (!ok) break;
+                        if (elect_one()) {
+                            mbar_arrive_expect_tx(&k_full[st], np * KV_TILE);
+                            uint8_t* dst = kring + st * W_TILE;
+#pragma unroll
+                            for (int i = 0; i < W_BLK_PAGES; i++)
+                                if (i < np) {
+                                    tma_load_5d(dst + i * HALF_TILE, &tmK, 0, 0, 0, h, page[i], &k_full[st], pol);
+                                    tma_load_5d(dst + W_TILE / 2 + i * HALF_TILE, &tmK, 0, 0, 1, h, page[i], &k_full[st], pol);
+                                }
+                        }
                     }
-                    nload++;
-                };
-                // pages that nobody sees keep a sum of 0
-                const int u0 = np > 0 && mine[0] < first ? (np > 1 && mine[1] < first ? units : nh) : 0;
-                int next = u0;
-                for (; ok && next < units && next < u0 + W_STAGES; next++) issue(next);
-                __syncthreads();                               // the previous block's Q is done with
-                for (int c = threadIdx.x; c < nh * nt * 256; c += W_THREADS) {
-                    const int tile = c >> 8, r = (c >> 4) & 15, cd = c & 15;
-                    const int h = tile / nt, rr = (t0 + tile - h * nt) * 16 + r;
-                    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                    const size_t row = (size_t)(s.q0 + rr / a.G) * a.Hq + (h0 + h) * a.G + rr % a.G;
-                    if (rr < nrows) v = __ldg(reinterpret_cast<const uint4*>(a.q + row * D) + cd);
-                    *reinterpret_cast<uint4*>(qs + tile * KV_TILE + tile_off(r, cd)) = v;
-                    if (cd == 0) {
-                        // padding rows and rows that saw nothing: exp2(s - inf) = 0
-                        const float l = rr < nrows ? w.lse_in[row] : -INFINITY;
-                        ls[tile * 16 + r] = l == -INFINITY ? INFINITY : l * LOG2E;
-                    }
-                }
-                __syncthreads();
-                for (int u = u0; u < units && ok; u++) {
-                    const int i = u / nh, hh = u - i * nh, sg = nuse % W_STAGES;
-                    ok = __all_sync(0xffffffffu, mbar_wait(&myfull[sg], (nuse / W_STAGES) & 1, deadline, a.err));
-                    if (ok) {
-                        nuse++;
-                        const uint32_t kb = smem_u32(myring + sg * KV_TILE);
-                        const int k_key = (lane & 7) + ((lane >> 4) << 3), k_hi = (lane >> 3) & 1;
-                        const int q_row = (lane & 7) + (((lane >> 3) & 1) << 3), q_hi = lane >> 4;
-                        uint32_t kf[8][4];
+        }
+        // every issued copy must land before the CTA exits
+        if (lane == 0)
+            for (int i = 0; i < KST && i < n; i++)
+                mbar_wait(&k_full[i], ((i + (n - 1 - i) / KST * KST) / KST) & 1, deadline, a.err);
+    } else if (warp == 1) {
+        // ---------------------------------------------------------------- MMA issuer
+        const uint32_t idesc = umma_idesc_f16(W_BLK, N, false, false);
+        const uint64_t kd = umma_desc_sw128(smem_u32(kring), 16, 1024), qd = umma_desc_sw128(smem_u32(qs), 16, 1024);
+        while (ok && walk.next(a, &g)) {
+            const Seq s(a, g.b);
+            int first, nrows, pos_hi;
+            plan(s, &first, &nrows, &pos_hi);
+            const int pg0 = max(g.pg0, first), nb = max(0, (g.pg1 - pg0 + W_BLK_PAGES - 1) / W_BLK_PAGES);
+            const int chunks = nb > 0 ? a.Hkv * ((nrows + N - 1) / N) : 0;
+            if (elect_one()) {
+                for (int c = 0; c < chunks && ok; c++) {
+                    const int qb = (chunk + c) & 1;
+                    ok = mbar_wait(&q_full[qb], ((chunk + c) >> 1) & 1, deadline, a.err);
+                    for (int j = 0; j < nb && ok; j++) {
+                        const int m = n + c * nb + j, st = m % KST, d = m & 1;
+                        ok = mbar_wait(&k_full[st], (m / KST) & 1, deadline, a.err);
+                        if (ok && m >= 2) ok = mbar_wait(&d_empty[d], ((m >> 1) - 1) & 1, deadline, a.err);
+                        if (!ok) break;
+                        tc_fence_after_sync();
 #pragma unroll
                         for (int kk = 0; kk < 8; kk++)
-                            ldmatrix_x4(kb + tile_off(k_key, 2 * kk + k_hi), kf[kk][0], kf[kk][1], kf[kk][2], kf[kk][3]);
-                        const int g = lane >> 2, t = lane & 3;
-                        const int kbase = mine[i] * PAGE;
-                        const bool whole = kbase + PAGE <= s.ctx &&
-                                           (a.window <= 0 || (long long)pos_hi - kbase < a.window);
-                        float add[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
-                        for (int n = 0; n < nt; n++) {
-                            const int tile = hh * nt + n;
-                            const uint32_t qb = smem_u32(qs + tile * KV_TILE);
-                            float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-                            for (int kk = 0; kk < 8; kk++) {
-                                uint32_t a0, a1, a2, a3;
-                                ldmatrix_x4(qb + tile_off(q_row, 2 * kk + q_hi), a0, a1, a2, a3);
-                                mma_16816(sc[0], a0, a1, a2, a3, kf[kk][0], kf[kk][1]);
-                                mma_16816(sc[1], a0, a1, a2, a3, kf[kk][2], kf[kk][3]);
+                            umma_f16(tmem + d * 256, kd + st * (W_TILE / 16) + ((kk >> 2) * (W_TILE / 2) + (kk & 3) * 32) / 16,
+                                     qd + (qb * q_bytes + (kk >> 2) * (q_bytes / 2) + (kk & 3) * 32) / 16, idesc, kk != 0);
+                        umma_commit(&d_full[d]);
+                        umma_commit(&k_empty[st]);
+                        if (j == nb - 1) umma_commit(&q_empty[qb]);
+                    }
+                }
+            }
+            ok = __all_sync(0xffffffffu, ok);
+            chunk += chunks;
+            n += chunks * nb;
+        }
+        if (elect_one()) umma_commit(done);
+        __syncwarp();
+    } else if (warp < 4) {
+        // ---------------------------------------------------------------- Q and the rows' infos
+        const int tid = threadIdx.x - 64;
+        while (ok && walk.next(a, &g)) {
+            const Seq s(a, g.b);
+            int first, nrows, pos_hi;
+            plan(s, &first, &nrows, &pos_hi);
+            if (s.T > a.max_q && g.pg0 == 0 && tid == 0) atomicOr(a.err, DEVERR_BOUND);
+            if (max(g.pg0, first) >= g.pg1) continue;
+            for (int h = 0; h < a.Hkv && ok; h++)
+                for (int r0 = 0; r0 < nrows && ok; r0 += N, chunk++) {
+                    const int qb = chunk & 1;
+                    if (chunk >= 2) {
+                        ok = mbar_wait(&q_empty[qb], ((chunk >> 1) - 1) & 1, deadline, a.err);
+                        if (ok) ok = mbar_wait(&i_empty[qb], ((chunk >> 1) - 1) & 1, deadline, a.err);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                    }
+                    uint8_t* dst = qs + qb * q_bytes;
+                    if (a.q_tma) {
+                        // rows are tokens x heads of the group: a box per 64-dim half; rows behind
+                        // the sequence's may be another's, and weigh nothing
+                        if (tid == 0) {
+                            const int i0 = s.q0 + r0 / a.G;
+                            mbar_arrive_expect_tx(&q_full[qb], q_bytes);
+                            tma_load_3d(dst, &tmQ, 0, h * a.G, i0, &q_full[qb]);
+                            tma_load_3d(dst + q_bytes / 2, &tmQ, 64, h * a.G, i0, &q_full[qb]);
+                        }
+                    } else {
+#pragma unroll 8
+                        for (int c = tid; c < N * 16; c += 64) {
+                            const int r = c >> 4, cd = c & 15, rr = r0 + r;
+                            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                            if (rr < nrows) {
+                                const int i = rr / a.G;
+                                v = __ldg(reinterpret_cast<const uint4*>(
+                                        a.q + ((size_t)(s.q0 + i) * a.Hq + h * a.G + (rr - i * a.G)) * D) + cd);
                             }
+                            *reinterpret_cast<uint4*>(dst + (cd >> 3) * (q_bytes / 2) + w_sw(r, cd & 7)) = v;
+                        }
+                        fence_proxy_async_smem();
+                        if (tid == 0) mbar_arrive(&q_full[qb]);
+                    }
+                    for (int r = tid; r < N; r += 64) {
+                        Row row;
+                        row.set(a, s, r0 + r, nrows, h);
+                        float l = -INFINITY;
+                        if (row.i >= 0) l = w.lse_in[(size_t)(s.q0 + row.i) * a.Hq + h * a.G + (r0 + r - row.i * a.G)];
+                        // padding rows and rows that saw nothing: exp2(s - inf) = 0
+                        info[qb].lse2[r] = l == -INFINITY ? INFINITY : l * LOG2E;
+                        info[qb].slope2[r] = row.slope2;
+                        info[qb].pos[r] = row.pos;
+                        info[qb].i[r] = row.i;
+                    }
+                    mbar_arrive(&q_full[qb]);
+                }
+        }
+        // a staged Q that nobody waited for (after a timeout) must still land
+        if (!ok && tid == 0)
+            for (int c = max(0, chunk - 2); c < chunk; c++) mbar_wait(&q_full[c & 1], (c >> 1) & 1, deadline, a.err);
+    } else {
+        // ---------------------------------------------------------------- weights
+        const int quarter = warp & 3, hf = (warp - 4) >> 2;
+        const int key = quarter * 32 + lane;
+        const uint32_t trow = tmem + ((uint32_t)(quarter * 32) << 16);
+        const int c0 = hf * (N / 2), c1 = c0 + N / 2;                // this thread's columns
+        while (walk.next(a, &g)) {
+            const Seq s(a, g.b);
+            int first, nrows, pos_hi;
+            plan(s, &first, &nrows, &pos_hi);
+            const int pg0 = max(g.pg0, first), nb = max(0, (g.pg1 - pg0 + W_BLK_PAGES - 1) / W_BLK_PAGES);
+            const int chunks = nb > 0 ? a.Hkv * ((nrows + N - 1) / N) : 0;
+            for (int j = 0; j < nb; j++) sums[(hf * W_SEG + j) * W_BLK + key] = 0.f;
+            for (int c = 0; c < chunks; c++, chunk++) {
+                const int qb = chunk & 1;
+                const RowInfo& in = info[qb];
+                // the infos are read directly: q_full also says that they are there
+                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&q_full[qb], (chunk >> 1) & 1, deadline, a.err));
+                for (int j = 0; j < nb; j++, n++) {
+                    const int d = n & 1;
+                    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&d_full[d], (n >> 1) & 1, deadline, a.err));
+                    if (!ok) continue;
+                    tc_fence_after_sync();
+                    const int kbase = (pg0 + j * W_BLK_PAGES) * PAGE, p = kbase + key;
+                    const bool whole = kbase + W_BLK <= s.ctx && (a.window <= 0 || (long long)pos_hi - kbase < a.window);
+                    const int kpos = whole ? p : s.pos(a, p);
+                    float add[4] = {0.f, 0.f, 0.f, 0.f};
+                    // M columns from `col` on; the common case first: every row sees every key, no bias
+                    auto weigh = [&](auto columns, int col, float* x) {
+                        constexpr int M = decltype(columns)::value;
+                        if (EXT && a.slopes) {
 #pragma unroll
-                            for (int r = 0; r < 2; r++) {
-                                const float l2 = ls[tile * 16 + 8 * r + g];
-                                Row row;
-                                if ((EXT && a.slopes) || !whole)
-                                    row.set(a, s, (t0 + n) * 16 + 8 * r + g, nrows, h0 + hh);
+                            for (int i = 0; i < M; i++) x[i] += tree::bias<EXT>(a, in.slope2[col + i], in.pos[col + i], kpos);
+                        }
+                        if (!whole) {
+                            const int k = p - s.ctx;                 // drafted index of the key
+                            const bool inside = p < s.len, drafted = k >= 0;
+                            const bool bit = a.mask && drafted && inside && k < 32 * a.mask_words;
 #pragma unroll
-                                for (int h = 0; h < 2; h++)
+                            for (int i0 = 0; i0 < M; i0 += 8) {
+                                uint32_t word[8];
 #pragma unroll
-                                    for (int c = 0; c < 2; c++) {
-                                        const int p = kbase + 8 * h + 2 * t + c;
-                                        float x = tree::score<EXT>(a, sc[h][2 * r + c]);
-                                        if (EXT && a.slopes)
-                                            x += tree::bias<EXT>(a, row.slope2, row.pos, whole ? p : s.pos(a, p));
-                                        if (!whole && (p >= s.len || !row.sees(a, s, p, s.pos(a, p)))) x = -INFINITY;
-                                        add[h][c] += ex2(x - l2);
-                                    }
+                                for (int i = 0; i < 8; i++) {
+                                    const int r = in.i[col + i0 + i];
+                                    word[i] = bit && r >= 0 ? __ldg(a.mask + (size_t)(s.q0 + r) * a.mask_words + (k >> 5)) : 0u;
+                                }
+#pragma unroll
+                                for (int i = 0; i < 8; i++) {
+                                    const int r = in.i[col + i0 + i];
+                                    bool see = r >= 0 && inside;
+                                    if (drafted) see &= a.mask ? (bool)((word[i] >> (k & 31)) & 1u) : k <= r;
+                                    if (a.window > 0) see &= (long long)in.pos[col + i0 + i] - kpos < a.window;
+                                    if (!see) x[i0 + i] = -INFINITY;
+                                }
                             }
                         }
 #pragma unroll
-                        for (int h = 0; h < 2; h++)
+                        for (int i = 0; i < M; i += 4) {
+                            const float4 l = *reinterpret_cast<const float4*>(&in.lse2[col + i]);
+                            add[0] += ex2(x[i] - l.x);
+                            add[1] += ex2(x[i + 1] - l.y);
+                            add[2] += ex2(x[i + 2] - l.z);
+                            add[3] += ex2(x[i + 3] - l.w);
+                        }
+                    };
+                    int col = c0;
+                    for (; col + 32 <= c1; col += 32) {
+                        float x[32];
+                        tmem_ld32(trow + d * 256 + col, reinterpret_cast<uint32_t(&)[32]>(x));
+                        tmem_ld_wait();
+                        tree::score32<EXT>(a, x);
+                        weigh(std::integral_constant<int, 32>{}, col, x);
+                    }
+                    for (; col < c1; col += 8) {
+                        float x[8];
+                        tmem_ld8(trow + d * 256 + col, reinterpret_cast<uint32_t(&)[8]>(x));
+                        tmem_ld_wait();
 #pragma unroll
-                            for (int c = 0; c < 2; c++) {
-                                if (i == 0) sum[0][h][c] += add[h][c];
-                                else sum[1][h][c] += add[h][c];
-                            }
+                        for (int i = 0; i < 8; i++) x[i] = tree::score<EXT>(a, x[i]);
+                        weigh(std::integral_constant<int, 8>{}, col, x);
                     }
-                    __syncwarp();                              // every lane has read the stage
-                    if (next < units && ok) {
-                        issue(next);
-                        next++;
-                    }
+                    tc_fence_before_sync();
+                    mbar_arrive(&d_empty[d]);
+                    sums[(hf * W_SEG + j) * W_BLK + key] += (add[0] + add[1]) + (add[2] + add[3]);
                 }
-                if (!ok) {
-                    // copies still in flight must land before the CTA exits
-                    for (; nuse < nload; nuse++)
-                        if (lane == 0) mbar_wait(&myfull[nuse % W_STAGES], (nuse / W_STAGES) & 1, deadline, a.err);
-                }
+                if (ok) mbar_arrive(&i_empty[qb]);
             }
-        // the eight lanes of a key hold its rows g, g+8 of every tile
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    float x = sum[i][h][c];
-                    x += __shfl_xor_sync(0xffffffffu, x, 4);
-                    x += __shfl_xor_sync(0xffffffffu, x, 8);
-                    x += __shfl_xor_sync(0xffffffffu, x, 16);
-                    const int p = mine[i] * PAGE + 8 * h + 2 * (lane & 3) + c;
-                    if (lane < 4 && mine[i] < pg1 && p < s.len && p < w.acc_stride) {
-                        float* dst = w.acc + blockIdx.y * w.acc_stride + p;
+            asm volatile("bar.sync 1, 256;" ::: "memory");           // both column halves are summed
+            if (hf == 0 && ok) {
+                // pages that nobody sees only decay
+                for (int p = g.pg0 * PAGE + key; p < min(s.len, pg0 * PAGE); p += W_BLK)
+                    if (p < w.acc_stride && p < g.pg1 * PAGE) {
+                        float* dst = w.acc + g.b * w.acc_stride + p;
+                        *dst = w.decay != 0.f ? w.decay * *dst : 0.f;
+                    }
+                for (int j = 0; j < nb; j++) {
+                    const int p = (pg0 + j * W_BLK_PAGES) * PAGE + key;
+                    if (p < s.len && p < g.pg1 * PAGE && p < w.acc_stride) {
+                        float* dst = w.acc + g.b * w.acc_stride + p;
+                        const float x = sums[j * W_BLK + key] + sums[(W_SEG + j) * W_BLK + key];
                         *dst = w.decay != 0.f ? fmaf(w.decay, *dst, x) : x;
                     }
                 }
+            }
+            asm volatile("bar.sync 1, 256;" ::: "memory");           // before the sums are cleared
+        }
     }
+    // every MMA must have finished before tensor memory is released
+    if (threadIdx.x == 0) mbar_wait(done, 0, deadline, a.err);
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    if (warp == 1) tmem_dealloc(tmem, 512);
 }
 
 // ------------------------------------------------------------------ select
@@ -486,14 +711,13 @@ __global__ void __launch_bounds__(C_THREADS) compact_kernel(const CArgs a) {
 struct Setup {
     ckl_status st = CKL_OK;
 };
-constexpr int Q_SMALL = 3, Q_BIG = 28;         // 16-row tiles of Q per block: two CTAs an SM, or one
 const Setup* setup(const DeviceInfo* di) {
     static Setup ks[64];
     static std::once_flag once[64];
     std::call_once(once[di->device], [di] {
-        cudaError_t e = cudaFuncSetAttribute(weights_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, w_smem(Q_BIG));
+        cudaError_t e = cudaFuncSetAttribute(weights_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, di->smem_optin - 1024);
         if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(weights_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, w_smem(Q_BIG));
+            e = cudaFuncSetAttribute(weights_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, di->smem_optin - 1024);
         if (e == cudaSuccess)
             e = cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S_MAX_KEYS * 4);
         if (e != cudaSuccess) ks[di->device].st = cuda_status(e, "cache kernels setup");
@@ -529,19 +753,23 @@ ckl_status ckl_cache_weights(const ckl_tree_params* p, const float* lse, float* 
     w.acc = acc;
     w.acc_stride = acc_stride;
     w.decay = decay;
-    // rows of one head in one small Q block: two CTAs per SM; more rows: one CTA with a large
-    // block, so that K is read again as seldom as can be
-    const bool small = (long long)p->max_q * w.t.G <= 16 * Q_SMALL;
-    w.q_tiles = small ? Q_SMALL : Q_BIG;
-    const long long chunks = (acc_stride + PAGE - 1) / PAGE;
-    const unsigned gx = (unsigned)std::max(1LL, std::min(chunks, (long long)di->sms * (small ? 2 : 1) / p->B));
-    CUtensorMap tmK, tmV;
-    st = encode_page_maps(p->k_cache, p->v_cache, p->Hkv, p->num_pages, &tmK, &tmV);
+    // the rows of a kv head in one staged Q where they fit; the rest of shared memory streams K
+    const long long rows = (long long)p->max_q * w.t.G;
+    w.rows = (int)std::min((rows + 15) / 16 * 16, (long long)W_ROWS);
+    w.stages = 2;
+    while (w.stages < W_MAX_STAGES && w_smem(w.rows, w.stages + 1) <= (size_t)di->smem_optin - 1024) w.stages++;
+    const long long blocks = (acc_stride + W_BLK - 1) / W_BLK;   // of a sequence, at most (longer ones take longer)
+    const unsigned grid = (unsigned)std::min((long long)di->sms, blocks * p->B);
+    CUtensorMap tmK, tmQ;
+    st = tree::encode_half_map(p->k_cache, p->Hkv, p->num_pages, 1, &tmK);
     if (st != CKL_OK) return st;
-    void* args[] = {&tmK, &w};
+    w.t.q_tma = w.rows % w.t.G == 0;
+    st = tree::encode_q_map(p->q, p->N, p->Hq, w.t.q_tma ? w.t.G : 1, w.t.q_tma ? w.rows / w.t.G : 1, &tmQ);
+    if (st != CKL_OK) return st;
+    void* args[] = {&tmK, &tmQ, &w};
     const bool ext = p->softcap > 0.f || p->slopes;
-    CKL_CUDA_TRY(launch(ext ? (const void*)weights_kernel<true> : (const void*)weights_kernel<false>,
-                        dim3(gx, (unsigned)p->B), dim3(W_THREADS), w_smem(w.q_tiles), (cudaStream_t)stream, args, true));
+    CKL_CUDA_TRY(launch(ext ? (const void*)weights_kernel<true> : (const void*)weights_kernel<false>, dim3(grid),
+                        dim3(W_THREADS), w_smem(w.rows, w.stages), (cudaStream_t)stream, args, true));
     return CKL_OK;
 }
 

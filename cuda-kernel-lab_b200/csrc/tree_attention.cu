@@ -270,17 +270,17 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
             const int my_page = lane < cnt ? __ldg(a.indices + s.page0 + p0 + base + lane) : 0;
             for (int j = 0; j < cnt; j++) {
                 const int page = __shfl_sync(0xffffffffu, my_page, j);
-                if (lane == 0) {
+                if (elect_one()) {
                     const int i = base + j, sg = i % STAGES;
                     if (i >= STAGES) ok = mbar_wait(&empty[sg], ((i / STAGES) - 1) & 1, deadline, a.err);
                     if (ok) {
                         mbar_arrive_expect_tx(&full[sg], STAGE_BYTES);
                         load_page(ring + sg * STAGE_BYTES, &tmK, &tmV, kvh, page, &full[sg], pol);
-                        issued = i + 1;
                     }
                 }
-                ok = __shfl_sync(0xffffffffu, ok, 0);
+                ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
+                issued = base + j + 1;
             }
         }
         // every issued copy must land before the CTA reuses the ring or exits

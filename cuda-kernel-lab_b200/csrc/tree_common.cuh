@@ -86,6 +86,21 @@ __device__ __forceinline__ int first_key(const Args& a, const Seq& s, int pos_lo
     return k & ~(PAGE - 1);
 }
 
+// W blocks over n CTAs: the first W % n take one more than the others.
+struct Share {
+    long long each;
+    int n, more;
+    __device__ __forceinline__ Share(long long W, int n_) : n(n_) {
+        each = W >> 31 ? W / n : (long long)((unsigned)W / (unsigned)n);
+        more = (int)(W - each * n);
+    }
+    __device__ __forceinline__ long long first(int c) const { return each * c + min(c, more); }   // block of CTA c
+    __device__ __forceinline__ int owner(long long u) const {                                      // CTA of block u
+        const long long big = (each + 1) * more, x = u < big ? u : u - big, d = u < big ? each + 1 : each;
+        return (u < big ? 0 : more) + (int)(x >> 31 ? x / d : (long long)((unsigned)x / (unsigned)d));
+    }
+};
+
 // One query row's view of the keys.
 struct Row {
     int i = -1;           // new token (-1: padding)

@@ -46,7 +46,7 @@ template <int MT> struct Cfg {
     static constexpr int OFF_K = MT * Q_TILE;
     static constexpr int OFF_V = OFF_K + KST * KV_BLK;
     static constexpr int OFF_BAR = OFF_V + VST * KV_BLK;
-    static constexpr int NBAR = 2 * KST + 2 * VST + (2 + SB + 2) * MT + 2;
+    static constexpr int NBAR = 2 * KST + 2 * VST + (2 + 3 * SB) * MT + 2;
     static constexpr int SMEM = 1024 + OFF_BAR + NBAR * 8 + 32;
     static constexpr uint32_t TMEM_COLS = 512;
 };
@@ -94,21 +94,6 @@ __device__ __forceinline__ long long blocks_before(const Args& a, int upto, int 
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     return sum;
 }
-// W blocks over n CTAs: the first W % n take one more than the others.
-struct Share {
-    long long each;
-    int n, more;
-    __device__ __forceinline__ Share(long long W, int n_) : n(n_) {
-        each = W >> 31 ? W / n : (long long)((unsigned)W / (unsigned)n);
-        more = (int)(W - each * n);
-    }
-    __device__ __forceinline__ long long first(int c) const { return each * c + min(c, more); }   // block of CTA c
-    __device__ __forceinline__ int owner(long long u) const {                                      // CTA of block u
-        const long long big = (each + 1) * more, x = u < big ? u : u - big, d = u < big ? each + 1 : each;
-        return (u < big ? 0 : more) + (int)(x >> 31 ? x / d : (long long)((unsigned)x / (unsigned)d));
-    }
-};
-
 // A CTA's run of blocks, unit by unit. All lanes of a warp hold the same state.
 struct Seg {
     int b, kvh, row0, rows;      // rows of this unit: [row0, row0 + rows) of the sequence's
@@ -196,8 +181,10 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
     uint64_t* q_empty = v_empty + VST;       // every S of a segment done: Q may be replaced
     uint64_t* q_full = q_empty + 1;          // [MT] Q of a segment is there
     uint64_t* s_full = q_full + MT;          // [MT][SB] S written (MMA -> softmax)
-    uint64_t* p_full = s_full + MT * SB;     // [MT][2] P of pages 0-3 / 4-7 written (softmax -> MMA)
-    uint64_t* o_done = p_full + MT * 2;      // [MT] O holds the block, its P has been read (MMA -> all)
+    // [MT][SB][2] P of pages 0-3 / 4-7 written (softmax -> MMA): one per S buffer, since with two the
+    // softmax may end the next block before the MMA warp has seen this one
+    uint64_t* p_full = s_full + MT * SB;
+    uint64_t* o_done = p_full + MT * SB * 2;      // [MT] O holds the block, its P has been read (MMA -> all)
     uint64_t* done = o_done + MT;            // every issued MMA finished
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
     volatile int* odd = reinterpret_cast<volatile int*>(tmem_slot + 1);   // unseen V held inf or NaN
@@ -217,7 +204,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
         for (int t = 0; t < MT; t++) {
             mbar_init(&q_full[t], a.q_tma ? 1 : 128);
             for (int i = 0; i < SB; i++) mbar_init(&s_full[t * SB + i], 1);
-            for (int i = 0; i < 2; i++) mbar_init(&p_full[t * 2 + i], 128);
+            for (int i = 0; i < 2 * SB; i++) mbar_init(&p_full[t * SB * 2 + i], 128);
             mbar_init(&o_done[t], 1);
         }
         mbar_init(q_empty, 1);
@@ -297,25 +284,37 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                     ids_at = at;
                     my_id = at + lane < npg ? __ldg(a.indices + s.page0 + at + lane) : a.num_pages;
                 }
-                const int page = __shfl_sync(0xffffffffu, my_id, at - ids_at + (lane & (BLK_PAGES - 1)));
+                int page[BLK_PAGES];
+#pragma unroll
+                for (int i = 0; i < BLK_PAGES; i++) page[i] = __shfl_sync(0xffffffffu, my_id, at - ids_at + i);
                 const int ks = n % KST, vs = n % VST;
-                if (lane == 0) {
+                // one elected lane issues: a box per lane would be serialised at ~50 ns each
+                if (elect_one()) {
                     if (n >= KST) ok = mbar_wait(&k_empty[ks], ((n / KST) - 1) & 1, deadline, a.err);
-                    if (ok) mbar_arrive_expect_tx(&k_full[ks], KV_BLK);
+                    if (ok) {
+                        uint8_t* dst = kring + ks * KV_BLK;
+                        mbar_arrive_expect_tx(&k_full[ks], KV_BLK);
+#pragma unroll
+                        for (int i = 0; i < BLK_PAGES; i++) {
+                            tma_load_5d(dst + i * HALF_TILE, &tmK, 0, 0, 0, g.kvh, page[i], &k_full[ks], pol);
+                            tma_load_5d(dst + KV_BLK / 2 + i * HALF_TILE, &tmK, 0, 0, 1, g.kvh, page[i], &k_full[ks], pol);
+                        }
+                    }
                 }
-                ok = __shfl_sync(0xffffffffu, ok, 0);
+                ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                if (lane < 2 * BLK_PAGES)               // half lane / 8 of page lane % 8
-                    tma_load_5d(kring + ks * KV_BLK + (lane >> 3) * (KV_BLK / 2) + (lane & 7) * HALF_TILE, &tmK, 0, 0,
-                                lane >> 3, g.kvh, page, &k_full[ks], pol);
-                if (lane == 0) {
+                if (elect_one()) {
                     if (n >= VST) ok = mbar_wait(&v_empty[vs], ((n / VST) - 1) & 1, deadline, a.err);
-                    if (ok) mbar_arrive_expect_tx(&v_full[vs], KV_BLK);
+                    if (ok) {
+                        uint8_t* dst = vring + vs * KV_BLK;
+                        mbar_arrive_expect_tx(&v_full[vs], KV_BLK);
+#pragma unroll
+                        for (int i = 0; i < BLK_PAGES; i++)
+                            tma_load_5d(dst + i * KV_TILE, &tmV, 0, 0, 0, g.kvh, page[i], &v_full[vs], pol);
+                    }
                 }
-                ok = __shfl_sync(0xffffffffu, ok, 0);
+                ok = __all_sync(0xffffffffu, ok);
                 if (!ok) { n++; break; }                // its K is in flight, its V is not
-                if (lane < BLK_PAGES)
-                    tma_load_5d(vring + vs * KV_BLK + lane * KV_TILE, &tmV, 0, 0, 0, g.kvh, page, &v_full[vs], pol);
                 if (j == g.blk0 && a.q_tma) {
                     // the segment's Q, behind its first block: the earlier segment still reads its own
                     if (lane == 0) {
@@ -415,7 +414,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                         }
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
-                            if (ok) ok = wait(&p_full[t * 2 + h], c);
+                            if (ok) ok = wait(&p_full[(t * SB + buf) * 2 + h], c / SB);
                             if (ok && t == 0 && h == 0) ok = wait(&v_full[vs], (n + j) / VST);
                             if (!ok) break;
                             tc_fence_after_sync();
@@ -582,7 +581,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                         tmem_st32(srow + h * 32, pk);
                         tmem_st_wait();
                         tc_fence_before_sync();
-                        mbar_arrive(&p_full[t * 2 + h]);
+                        mbar_arrive(&p_full[(t * SB + cnt % SB) * 2 + h]);
                     }
                     const float2 l2 = add2(add2(l4[0], l4[1]), add2(l4[2], l4[3]));
                     l += l2.x + l2.y;
@@ -634,8 +633,8 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                     }
                     if (!ok) continue;
                     if (idle) {                         // their P is whatever S held: no other row reads it
-                        mbar_arrive(&p_full[t * 2]);
-                        mbar_arrive(&p_full[t * 2 + 1]);
+                        mbar_arrive(&p_full[(t * SB + cnt % SB) * 2]);
+                        mbar_arrive(&p_full[(t * SB + cnt % SB) * 2 + 1]);
                         cnt++;
                         continue;
                     }
@@ -814,15 +813,6 @@ ckl_status setup_tiles(const DeviceInfo* di) {
     return st[di->device];
 }
 
-// A page of one head as a box [halves][16 tokens][64 dims].
-ckl_status encode_tile_map(const void* cache, int Hkv, int num_pages, int halves, CUtensorMap* tm) {
-    const uint64_t dims[5] = {64, (uint64_t)PAGE, 2, (uint64_t)Hkv, (uint64_t)num_pages};
-    const uint64_t strides[4] = {(uint64_t)Hkv * D * 2, 128, (uint64_t)D * 2, (uint64_t)PAGE * Hkv * D * 2};
-    const uint32_t box[5] = {64, (uint32_t)PAGE, (uint32_t)halves, 1, 1};
-    return encode_tiled(tm, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void*>(cache), dims, strides, box,
-                        CU_TENSOR_MAP_SWIZZLE_128B);
-}
-
 size_t part_bytes(int ctas, int rows, size_t* o_bytes) {
     // at most two segments of a CTA are partial
     *o_bytes = align_up((size_t)ctas * 2 * rows * D * sizeof(float), 256);
@@ -830,6 +820,22 @@ size_t part_bytes(int ctas, int rows, size_t* o_bytes) {
 }
 
 }  // namespace tile
+
+ckl_status encode_half_map(const void* cache, int Hkv, int num_pages, int halves, CUtensorMap* tm) {
+    const uint64_t dims[5] = {64, (uint64_t)PAGE, 2, (uint64_t)Hkv, (uint64_t)num_pages};
+    const uint64_t strides[4] = {(uint64_t)Hkv * D * 2, 128, (uint64_t)D * 2, (uint64_t)PAGE * Hkv * D * 2};
+    const uint32_t box[5] = {64, (uint32_t)PAGE, (uint32_t)halves, 1, 1};
+    return encode_tiled(tm, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void*>(cache), dims, strides, box,
+                        CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+ckl_status encode_q_map(const void* q, int N, int Hq, int heads, int tokens, CUtensorMap* tm) {
+    const uint64_t dims[3] = {(uint64_t)D, (uint64_t)Hq, (uint64_t)N};
+    const uint64_t strides[2] = {(uint64_t)D * 2, (uint64_t)Hq * D * 2};
+    const uint32_t box[3] = {64, (uint32_t)heads, (uint32_t)tokens};
+    return encode_tiled(tm, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(q), dims, strides, box,
+                        CU_TENSOR_MAP_SWIZZLE_128B);
+}
 
 int tile_count(long long rows) { return rows <= 128 ? 1 : 2; }
 
@@ -850,18 +856,14 @@ ckl_status launch_tiles(const ckl_tree_params* p, Args a, void* workspace, int c
     a.part_o = static_cast<float*>(workspace);
     a.part_lse = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + o);
     CUtensorMap tmK, tmV;
-    st = encode_tile_map(p->k_cache, p->Hkv, p->num_pages, 1, &tmK);
+    st = encode_half_map(p->k_cache, p->Hkv, p->num_pages, 1, &tmK);
     if (st != CKL_OK) return st;
-    st = encode_tile_map(p->v_cache, p->Hkv, p->num_pages, 2, &tmV);
+    st = encode_half_map(p->v_cache, p->Hkv, p->num_pages, 2, &tmV);
     if (st != CKL_OK) return st;
     // Q tiles by tensor map: [tokens][heads of the group][64 dims] are the stacked rows in order
     a.q_tma = 128 % a.G == 0;
-    const uint64_t qdims[3] = {(uint64_t)D, (uint64_t)p->Hq, (uint64_t)p->N};
-    const uint64_t qstrides[2] = {(uint64_t)D * 2, (uint64_t)p->Hq * D * 2};
-    const uint32_t qbox[3] = {64, (uint32_t)(a.q_tma ? a.G : 1), (uint32_t)(a.q_tma ? 128 / a.G : 1)};
     CUtensorMap tmQ;
-    st = encode_tiled(&tmQ, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(p->q), qdims, qstrides, qbox,
-                      CU_TENSOR_MAP_SWIZZLE_128B);
+    st = encode_q_map(p->q, p->N, p->Hq, a.q_tma ? a.G : 1, a.q_tma ? 128 / a.G : 1, &tmQ);
     if (st != CKL_OK) return st;
     void* args[] = {&tmK, &tmV, &tmQ, &a};
     const bool ext = p->softcap > 0.f || p->slopes;

@@ -6,6 +6,10 @@
 namespace ckl {
 namespace tree {
 
+// K or V cache as pages of one head, a box of [halves][16 tokens][64 dims].
+ckl_status encode_half_map(const void* cache, int Hkv, int num_pages, int halves, CUtensorMap* tm);
+// q [N][Hq][128] as boxes of [tokens][heads][64 dims]: stacked rows in order.
+ckl_status encode_q_map(const void* q, int N, int Hq, int heads, int tokens, CUtensorMap* tm);
 // Row tiles of 128 that a CTA holds for up to `rows` stacked rows.
 int tile_count(long long rows);
 // Bytes of partials of `ctas` CTAs.

@@ -325,6 +325,25 @@ def test_tree_repeats_streams_and_graphs(ckl, dev, toks, Hq):
     assert torch.equal(out, want) and not torch.equal(out, a)
 
 
+@pytest.mark.parametrize("toks,Hq", [(9, 8), (33, 16), (3, 8)])
+def test_tree_many_calls_in_a_row(ckl, dev, toks, Hq):
+    """Hundreds of calls without a wait between them: the same bits, and no barrier that gave up
+    (one that a fast warp could pass twice shows as a time-out here)."""
+    import torch
+    bt = ref.Batch([1800 + 130 * i for i in range(8)], [toks] * 8, Hq, 2, 41)
+    p = run_tree(ckl, dev, bt)
+    ws = torch.empty(max(ckl.tree_workspace_size(p), 256), dtype=torch.uint8, device=dev)
+    want, wl = ckl.tree_attention(p)
+    out, lse = torch.empty_like(want), torch.empty_like(wl)
+    acc = torch.zeros((8, 3000), device=dev)
+    one = ckl.cache_weights(p, wl, acc.clone())
+    for _ in range(300):
+        ckl.tree_attention(p, out=out, lse=lse, workspace=ws)
+        ckl.cache_weights(p, wl, acc, decay=0.0)
+    finish(ckl)
+    assert torch.equal(out, want) and torch.equal(lse, wl) and torch.equal(acc, one)
+
+
 def test_tree_mask_of_parents(ckl, dev):
     bt = ref.Batch([30, 90, 4, 50], [5, 70, 0, 33], 2, 1, 3, extra_rows=2)
     parents, mask, pos = bt.random_tree(8)
