@@ -22,14 +22,15 @@ using tree::Seq;
 //
 // S^T = K Q^T on tcgen05 with the keys as M: 128 keys are the lanes of tensor memory and the rows
 // of a kv head its columns, so a thread owns a key and its sum over rows and heads stays with it:
-// no atomics and no second kernel, the same order of additions whatever the batch. The lse of the
+// no atomics and no second kernel, and additions in the same order whatever the batch. The lse of the
 // attention call already normalises, so there is no running maximum either.
 //
 // The pages of all sequences, end to end, are divided evenly over one wave of CTAs. A CTA's run of
 // a sequence is taken W_SEG blocks at a time: for each kv head (and each W_ROWS of its rows) Q is
 // staged once and the blocks' K tiles stream past it. Warp 0 loads K (TMA), warp 1 issues the MMAs,
-// warps 2-3 stage Q and the rows' lse, position and slope, eight warps turn S into weights (two
-// threads per key, half of the columns each).
+// warps 2-3 stage Q and the rows' lse, position and slope, and two groups of four warps turn S into
+// weights: for many rows each takes half of the columns of every tile, for few rows, where a tile
+// is mostly waiting, the tiles of every other kv head.
 constexpr int W_THREADS = 384;
 constexpr int W_BLK = 128;                     // keys of a tile
 constexpr int W_BLK_PAGES = W_BLK / PAGE;
@@ -37,6 +38,9 @@ constexpr int W_TILE = W_BLK * D * 2;          // 32 KB: dims 0-63 of 128 keys, 
 constexpr int W_ROWS = 256;                    // rows per staged Q, at most (N of the MMA)
 constexpr int W_SEG = 16;                      // blocks of a segment
 constexpr int W_MAX_STAGES = 6;
+constexpr int W_NARROW = 32;                   // up to so many rows a tile is one group of warps' work
+constexpr int W_BUFS = 8;                      // S buffers of a group then: 2 * 8 * 32 columns
+constexpr int W_QS = 8;                        // staged Qs then (2 otherwise): short segments change Q often
 
 struct WArgs {
     tree::Args t;
@@ -47,12 +51,21 @@ struct WArgs {
     int rows;                                  // rows per staged Q: a multiple of 16, at most W_ROWS
     int stages;                                // K tiles in flight
 };
-struct RowInfo {                               // of the columns of a staged Q
-    float lse2[W_ROWS], slope2[W_ROWS];        // lse in log2 (+inf: adds nothing)
-    int pos[W_ROWS], i[W_ROWS];
+// Of the columns of a staged Q, rows words each: lse in log2 (+inf: adds nothing), slope, position,
+// the sequence's token (-1 behind the rows).
+struct RowInfo {
+    float* base;
+    int rows;
+    __device__ __forceinline__ float* lse2(int c) const { return base + c; }
+    __device__ __forceinline__ float* slope2(int c) const { return base + rows + c; }
+    __device__ __forceinline__ int* pos(int c) const { return reinterpret_cast<int*>(base + 2 * rows + c); }
+    __device__ __forceinline__ int* i(int c) const { return reinterpret_cast<int*>(base + 3 * rows + c); }
 };
-constexpr size_t W_FIXED = 1024 + 2 * sizeof(RowInfo) + 2 * W_SEG * W_BLK * 4 + (2 * W_MAX_STAGES + 11) * 8 + 16;
-constexpr size_t w_smem(int rows, int stages) { return W_FIXED + (size_t)2 * rows * D * 2 + (size_t)stages * W_TILE; }
+constexpr size_t W_FIXED = 1024 + 2 * W_SEG * W_BLK * 4 + (2 * W_MAX_STAGES + 3 * W_QS + 4 * W_BUFS + 1) * 8 + 16;
+constexpr int w_qbufs(int rows) { return rows <= W_NARROW ? W_QS : 2; }
+constexpr size_t w_smem(int rows, int stages) {
+    return W_FIXED + (size_t)w_qbufs(rows) * rows * (D * 2 + 16) + (size_t)stages * W_TILE;
+}
 
 struct WSeg {
     int b, pg0, pg1;                           // pages of the sequence
@@ -81,6 +94,49 @@ struct WWalk {
     }
 };
 
+// Bits [at, at + 32) of the 128-bit set v3 v2 v1 v0 (at >= 0). By value: a choice between
+// variables must not become one between addresses, which would put them in local memory.
+__device__ __forceinline__ uint32_t bits32(uint32_t v0, uint32_t v1, uint32_t v2, uint32_t v3, int at) {
+    const int w = at >> 5;
+    const uint32_t lo = w == 0 ? v0 : w == 1 ? v1 : w == 2 ? v2 : w == 3 ? v3 : 0u;
+    const uint32_t hi = w == 0 ? v1 : w == 1 ? v2 : w == 2 ? v3 : 0u;
+    return __funnelshift_r(lo, hi, at & 31);
+}
+
+// Sum of the weights of M <= 32 columns from `col` on; x holds their scores (bias excluded). Where
+// not every column is a row that sees the key (`whole`), bit i of `see` says whether the token i
+// behind the first column's does.
+template <bool EXT, int M>
+__device__ __forceinline__ float weigh(const tree::Args& a, const RowInfo& in, bool whole, int kpos, uint32_t see, int col,
+                                       float (&x)[M]) {
+    if (EXT && a.slopes) {
+#pragma unroll
+        for (int i = 0; i < M; i++) x[i] += tree::bias<EXT>(a, *in.slope2(col + i), *in.pos(col + i), kpos);
+    }
+    if (!whole) {
+        const int t0 = *in.i(col);
+#pragma unroll
+        for (int i = 0; i < M; i += 4) {
+            const int4 t = *reinterpret_cast<const int4*>(in.i(col + i));
+            auto keep = [&](int tok) { return ((see >> ((tok - t0) & 31)) & ~(uint32_t)(tok >> 31) & 1u) != 0u; };
+            x[i] = keep(t.x) ? x[i] : -INFINITY;
+            x[i + 1] = keep(t.y) ? x[i + 1] : -INFINITY;
+            x[i + 2] = keep(t.z) ? x[i + 2] : -INFINITY;
+            x[i + 3] = keep(t.w) ? x[i + 3] : -INFINITY;
+        }
+    }
+    float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+#pragma unroll
+    for (int i = 0; i < M; i += 4) {
+        const float4 l = *reinterpret_cast<const float4*>(in.lse2(col + i));
+        s0 += ex2(x[i] - l.x);
+        s1 += ex2(x[i + 1] - l.y);
+        s2 += ex2(x[i + 2] - l.z);
+        s3 += ex2(x[i + 3] - l.w);
+    }
+    return (s0 + s1) + (s2 + s3);
+}
+
 __device__ __forceinline__ uint32_t w_sw(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
 
 template <bool EXT>
@@ -89,18 +145,22 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     extern __shared__ uint8_t smem_raw[];
     const tree::Args& a = w.t;
     const int N = w.rows, KST = w.stages, q_bytes = N * D * 2;
+    // S buffers: two of 256 columns, or W_BUFS narrow ones for each group of warps
+    const bool narrow = N <= W_NARROW;
+    const int d_cols = narrow ? W_NARROW : 256, bufs = narrow ? W_BUFS : 2;
+    const int qbufs = w_qbufs(N);
     uint8_t* kring = align_ptr<1024>(smem_raw);
-    uint8_t* qs = kring + KST * W_TILE;                              // [2] staged Q: dims 0-63, then 64-127
-    RowInfo* info = reinterpret_cast<RowInfo*>(qs + 2 * q_bytes);    // [2]
-    float* sums = reinterpret_cast<float*>(info + 2);                // [2 column halves][W_SEG][128]
+    uint8_t* qs = kring + KST * W_TILE;                              // [qbufs] staged Q: dims 0-63, then 64-127
+    float* infos = reinterpret_cast<float*>(qs + qbufs * q_bytes);   // [qbufs] row infos, 4 N words each
+    float* sums = infos + qbufs * 4 * N;                             // [2 groups][W_SEG][128]
     uint64_t* k_full = reinterpret_cast<uint64_t*>(sums + 2 * W_SEG * W_BLK);
     uint64_t* k_empty = k_full + W_MAX_STAGES;
-    uint64_t* q_full = k_empty + W_MAX_STAGES;   // [2] staged
-    uint64_t* q_empty = q_full + 2;              // [2] its MMAs are done
-    uint64_t* i_empty = q_empty + 2;             // [2] the row infos have been used
-    uint64_t* d_full = i_empty + 2;              // [2] S written
-    uint64_t* d_empty = d_full + 2;              // [2] S read
-    uint64_t* done = d_empty + 2;                // every issued MMA finished
+    uint64_t* q_full = k_empty + W_MAX_STAGES;   // [qbufs] staged
+    uint64_t* q_empty = q_full + W_QS;           // [qbufs] its MMAs are done
+    uint64_t* i_empty = q_empty + W_QS;          // [qbufs] the row infos have been used
+    uint64_t* d_full = i_empty + W_QS;              // [2 groups][W_BUFS] S written
+    uint64_t* d_empty = d_full + 2 * W_BUFS;     // [2 groups][W_BUFS] S read
+    uint64_t* done = d_empty + 2 * W_BUFS;                // every issued MMA finished
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
     __shared__ long long s_left, s_off;
     __shared__ int s_b;
@@ -111,12 +171,14 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             mbar_init(&k_full[i], 1);
             mbar_init(&k_empty[i], 1);
         }
-        for (int i = 0; i < 2; i++) {
+        for (int i = 0; i < qbufs; i++) {
             mbar_init(&q_full[i], 65);
             mbar_init(&q_empty[i], 1);
             mbar_init(&i_empty[i], 256);
+        }
+        for (int i = 0; i < 2 * W_BUFS; i++) {
             mbar_init(&d_full[i], 1);
-            mbar_init(&d_empty[i], 256);
+            mbar_init(&d_empty[i], narrow ? 128 : 256);
         }
         mbar_init(done, 1);
         fence_barrier_init();
@@ -165,6 +227,7 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     tc_fence_after_sync();
     pdl_trigger();
     const uint32_t tmem = *tmem_slot;
+    auto d_col = [&](int d) { return (uint32_t)((d / W_BUFS * bufs + d % W_BUFS) * d_cols); };   // of S buffer d
     const uint64_t deadline = globaltimer() + a.timeout_ns;
     WWalk walk{s_left, s_off, s_b};
     WSeg g;
@@ -226,6 +289,7 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         // ---------------------------------------------------------------- MMA issuer
         const uint32_t idesc = umma_idesc_f16(W_BLK, N, false, false);
         const uint64_t kd = umma_desc_sw128(smem_u32(kring), 16, 1024), qd = umma_desc_sw128(smem_u32(qs), 16, 1024);
+        int tiles[2] = {0, 0};                       // of each group
         while (ok && walk.next(a, &g)) {
             const Seq s(a, g.b);
             int first, nrows, pos_hi;
@@ -233,18 +297,20 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             const int pg0 = max(g.pg0, first), nb = max(0, (g.pg1 - pg0 + W_BLK_PAGES - 1) / W_BLK_PAGES);
             const int chunks = nb > 0 ? a.Hkv * ((nrows + N - 1) / N) : 0;
             if (elect_one()) {
+                int t0 = tiles[0], t1 = tiles[1];
                 for (int c = 0; c < chunks && ok; c++) {
-                    const int qb = (chunk + c) & 1;
-                    ok = mbar_wait(&q_full[qb], ((chunk + c) >> 1) & 1, deadline, a.err);
+                    const int qb = (chunk + c) % qbufs;
+                    ok = mbar_wait(&q_full[qb], ((chunk + c) / qbufs) & 1, deadline, a.err);
                     for (int j = 0; j < nb && ok; j++) {
-                        const int m = n + c * nb + j, st = m % KST, d = m & 1;
+                        const int m = n + c * nb + j, st = m % KST, gr = narrow ? c & 1 : 0;
+                        const int t = gr ? t1++ : t0++, d = gr * W_BUFS + t % bufs;
                         ok = mbar_wait(&k_full[st], (m / KST) & 1, deadline, a.err);
-                        if (ok && m >= 2) ok = mbar_wait(&d_empty[d], ((m >> 1) - 1) & 1, deadline, a.err);
+                        if (ok && t >= bufs) ok = mbar_wait(&d_empty[d], (t / bufs - 1) & 1, deadline, a.err);
                         if (!ok) break;
                         tc_fence_after_sync();
 #pragma unroll
                         for (int kk = 0; kk < 8; kk++)
-                            umma_f16(tmem + d * 256, kd + st * (W_TILE / 16) + ((kk >> 2) * (W_TILE / 2) + (kk & 3) * 32) / 16,
+                            umma_f16(tmem + d_col(d), kd + st * (W_TILE / 16) + ((kk >> 2) * (W_TILE / 2) + (kk & 3) * 32) / 16,
                                      qd + (qb * q_bytes + (kk >> 2) * (q_bytes / 2) + (kk & 3) * 32) / 16, idesc, kk != 0);
                         umma_commit(&d_full[d]);
                         umma_commit(&k_empty[st]);
@@ -255,6 +321,8 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             ok = __all_sync(0xffffffffu, ok);
             chunk += chunks;
             n += chunks * nb;
+            tiles[0] += nb * (narrow ? (chunks + 1) / 2 : chunks);
+            tiles[1] += nb * (narrow ? chunks / 2 : 0);
         }
         if (elect_one()) umma_commit(done);
         __syncwarp();
@@ -269,10 +337,10 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             if (max(g.pg0, first) >= g.pg1) continue;
             for (int h = 0; h < a.Hkv && ok; h++)
                 for (int r0 = 0; r0 < nrows && ok; r0 += N, chunk++) {
-                    const int qb = chunk & 1;
-                    if (chunk >= 2) {
-                        ok = mbar_wait(&q_empty[qb], ((chunk >> 1) - 1) & 1, deadline, a.err);
-                        if (ok) ok = mbar_wait(&i_empty[qb], ((chunk >> 1) - 1) & 1, deadline, a.err);
+                    const int qb = chunk % qbufs;
+                    if (chunk >= qbufs) {
+                        ok = mbar_wait(&q_empty[qb], (chunk / qbufs - 1) & 1, deadline, a.err);
+                        if (ok) ok = mbar_wait(&i_empty[qb], (chunk / qbufs - 1) & 1, deadline, a.err);
                         ok = __all_sync(0xffffffffu, ok);
                         if (!ok) break;
                     }
@@ -301,107 +369,108 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                         fence_proxy_async_smem();
                         if (tid == 0) mbar_arrive(&q_full[qb]);
                     }
+                    const RowInfo in{infos + qb * 4 * N, N};
                     for (int r = tid; r < N; r += 64) {
                         Row row;
                         row.set(a, s, r0 + r, nrows, h);
                         float l = -INFINITY;
                         if (row.i >= 0) l = w.lse_in[(size_t)(s.q0 + row.i) * a.Hq + h * a.G + (r0 + r - row.i * a.G)];
                         // padding rows and rows that saw nothing: exp2(s - inf) = 0
-                        info[qb].lse2[r] = l == -INFINITY ? INFINITY : l * LOG2E;
-                        info[qb].slope2[r] = row.slope2;
-                        info[qb].pos[r] = row.pos;
-                        info[qb].i[r] = row.i;
+                        *in.lse2(r) = l == -INFINITY ? INFINITY : l * LOG2E;
+                        *in.slope2(r) = row.slope2;
+                        *in.pos(r) = row.pos;
+                        *in.i(r) = row.i;
                     }
                     mbar_arrive(&q_full[qb]);
                 }
         }
         // a staged Q that nobody waited for (after a timeout) must still land
         if (!ok && tid == 0)
-            for (int c = max(0, chunk - 2); c < chunk; c++) mbar_wait(&q_full[c & 1], (c >> 1) & 1, deadline, a.err);
+            for (int c = max(0, chunk - qbufs); c < chunk; c++)
+                mbar_wait(&q_full[c % qbufs], (c / qbufs) & 1, deadline, a.err);
     } else {
         // ---------------------------------------------------------------- weights
         const int quarter = warp & 3, hf = (warp - 4) >> 2;
         const int key = quarter * 32 + lane;
         const uint32_t trow = tmem + ((uint32_t)(quarter * 32) << 16);
-        const int c0 = hf * (N / 2), c1 = c0 + N / 2;                // this thread's columns
+        const int c0 = narrow ? 0 : hf * (N / 2), c1 = narrow ? N : c0 + N / 2;   // this thread's columns
+        const int gr = narrow ? hf : 0;                              // narrow: the heads of that parity
+        int tile = 0;                                                // of this group
         while (walk.next(a, &g)) {
             const Seq s(a, g.b);
             int first, nrows, pos_hi;
             plan(s, &first, &nrows, &pos_hi);
             const int pg0 = max(g.pg0, first), nb = max(0, (g.pg1 - pg0 + W_BLK_PAGES - 1) / W_BLK_PAGES);
-            const int chunks = nb > 0 ? a.Hkv * ((nrows + N - 1) / N) : 0;
+            const int rchunks = (nrows + N - 1) / N, chunks = nb > 0 ? a.Hkv * rchunks : 0;
             for (int j = 0; j < nb; j++) sums[(hf * W_SEG + j) * W_BLK + key] = 0.f;
             for (int c = 0; c < chunks; c++, chunk++) {
-                const int qb = chunk & 1;
-                const RowInfo& in = info[qb];
+                const int qb = chunk % qbufs;
+                const RowInfo in{infos + qb * 4 * N, N};
                 // the infos are read directly: q_full also says that they are there
-                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&q_full[qb], (chunk >> 1) & 1, deadline, a.err));
-                for (int j = 0; j < nb; j++, n++) {
-                    const int d = n & 1;
-                    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&d_full[d], (n >> 1) & 1, deadline, a.err));
+                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&q_full[qb], (chunk / qbufs) & 1, deadline, a.err));
+                const int r0 = c % rchunks * N;                      // first row of this chunk
+                const int t_lo = (r0 + c0) / a.G;                    // tokens of this thread's columns
+                const int nt = r0 + c0 < nrows ? (min(nrows, r0 + c1) - 1) / a.G - t_lo + 1 : 0;
+                const int valid = nrows - r0;                        // columns that are rows: the others may hold
+                                                                     // another sequence's, and are left out
+                const bool mine = !narrow || (c & 1) == gr;
+                for (int j = 0; mine && j < nb; j++, tile++) {
+                    const int d = gr * W_BUFS + tile % bufs;
+                    const uint32_t d_at = d_col(d);
+                    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&d_full[d], (tile / bufs) & 1, deadline, a.err));
                     if (!ok) continue;
                     tc_fence_after_sync();
                     const int kbase = (pg0 + j * W_BLK_PAGES) * PAGE, p = kbase + key;
                     const bool whole = kbase + W_BLK <= s.ctx && (a.window <= 0 || (long long)pos_hi - kbase < a.window);
                     const int kpos = whole ? p : s.pos(a, p);
-                    float add[4] = {0.f, 0.f, 0.f, 0.f};
-                    // M columns from `col` on; the common case first: every row sees every key, no bias
-                    auto weigh = [&](auto columns, int col, float* x) {
-                        constexpr int M = decltype(columns)::value;
-                        if (EXT && a.slopes) {
-#pragma unroll
-                            for (int i = 0; i < M; i++) x[i] += tree::bias<EXT>(a, in.slope2[col + i], in.pos[col + i], kpos);
-                        }
-                        if (!whole) {
-                            const int k = p - s.ctx;                 // drafted index of the key
-                            const bool inside = p < s.len, drafted = k >= 0;
-                            const bool bit = a.mask && drafted && inside && k < 32 * a.mask_words;
-#pragma unroll
-                            for (int i0 = 0; i0 < M; i0 += 8) {
-                                uint32_t word[8];
-#pragma unroll
-                                for (int i = 0; i < 8; i++) {
-                                    const int r = in.i[col + i0 + i];
-                                    word[i] = bit && r >= 0 ? __ldg(a.mask + (size_t)(s.q0 + r) * a.mask_words + (k >> 5)) : 0u;
+                    uint32_t v0 = 0u, v1 = 0u, v2 = 0u, v3 = 0u;     // tokens t_lo .. + 127 that see the key
+                    if (!whole && p < s.len) {
+                        const int k = p - s.ctx;                     // drafted index of the key
+                        const bool bits = a.mask && k >= 0 && k < 32 * a.mask_words;
+                        const uint32_t* mw = a.mask + (size_t)(s.q0 + t_lo) * a.mask_words + (k >> 5);
+                        // tokens t_lo + 32 q .. that see the key
+                        auto seen = [&](int q) {
+                            uint32_t v = 0u;
+                            const int n32 = min(nt - 32 * q, 32);
+#pragma unroll 8
+                            for (int i = 0; i < n32; i++) {
+                                const int t = 32 * q + i;
+                                uint32_t see = 1u;
+                                if (k >= 0) see = !a.mask ? k <= t_lo + t : bits ? __ldg(mw + (size_t)t * a.mask_words) >> (k & 31) : 0u;
+                                if (a.window > 0) {
+                                    const int tp = a.positions ? __ldg(a.positions + s.q0 + t_lo + t) : s.ctx + t_lo + t;
+                                    if ((long long)tp - kpos >= a.window) see = 0u;
                                 }
-#pragma unroll
-                                for (int i = 0; i < 8; i++) {
-                                    const int r = in.i[col + i0 + i];
-                                    bool see = r >= 0 && inside;
-                                    if (drafted) see &= a.mask ? (bool)((word[i] >> (k & 31)) & 1u) : k <= r;
-                                    if (a.window > 0) see &= (long long)in.pos[col + i0 + i] - kpos < a.window;
-                                    if (!see) x[i0 + i] = -INFINITY;
-                                }
+                                v |= (see & 1u) << i;
                             }
-                        }
-#pragma unroll
-                        for (int i = 0; i < M; i += 4) {
-                            const float4 l = *reinterpret_cast<const float4*>(&in.lse2[col + i]);
-                            add[0] += ex2(x[i] - l.x);
-                            add[1] += ex2(x[i + 1] - l.y);
-                            add[2] += ex2(x[i + 2] - l.z);
-                            add[3] += ex2(x[i + 3] - l.w);
-                        }
-                    };
+                            return v;
+                        };
+                        v0 = seen(0);
+                        v1 = seen(1);
+                        v2 = seen(2);
+                        v3 = seen(3);
+                    }
+                    float add = 0.f;
+                    auto see_of = [&](int c) { return whole ? 0xffffffffu : bits32(v0, v1, v2, v3, max(*in.i(c), t_lo) - t_lo); };
                     int col = c0;
-                    for (; col + 32 <= c1; col += 32) {
+                    for (; col + 32 <= c1 && col < valid; col += 32) {
                         float x[32];
-                        tmem_ld32(trow + d * 256 + col, reinterpret_cast<uint32_t(&)[32]>(x));
+                        tmem_ld32(trow + d_at + col, reinterpret_cast<uint32_t(&)[32]>(x));
                         tmem_ld_wait();
                         tree::score32<EXT>(a, x);
-                        weigh(std::integral_constant<int, 32>{}, col, x);
+                        add += weigh<EXT, 32>(a, in, whole && col + 32 <= valid, kpos, see_of(col), col, x);
                     }
-                    for (; col < c1; col += 8) {
+                    for (; col < min(c1, valid); col += 8) {
                         float x[8];
-                        tmem_ld8(trow + d * 256 + col, reinterpret_cast<uint32_t(&)[8]>(x));
+                        tmem_ld8(trow + d_at + col, reinterpret_cast<uint32_t(&)[8]>(x));
                         tmem_ld_wait();
 #pragma unroll
                         for (int i = 0; i < 8; i++) x[i] = tree::score<EXT>(a, x[i]);
-                        weigh(std::integral_constant<int, 8>{}, col, x);
+                        add += weigh<EXT, 8>(a, in, whole && col + 8 <= valid, kpos, see_of(col), col, x);
                     }
                     tc_fence_before_sync();
                     mbar_arrive(&d_empty[d]);
-                    sums[(hf * W_SEG + j) * W_BLK + key] += (add[0] + add[1]) + (add[2] + add[3]);
+                    sums[(hf * W_SEG + j) * W_BLK + key] += add;
                 }
                 if (ok) mbar_arrive(&i_empty[qb]);
             }
