@@ -61,10 +61,11 @@ struct RowInfo {
     __device__ __forceinline__ int* pos(int c) const { return reinterpret_cast<int*>(base + 2 * rows + c); }
     __device__ __forceinline__ int* i(int c) const { return reinterpret_cast<int*>(base + 3 * rows + c); }
 };
-constexpr size_t W_FIXED = 1024 + 2 * W_SEG * W_BLK * 4 + (2 * W_MAX_STAGES + 3 * W_QS + 4 * W_BUFS + 1) * 8 + 16;
+constexpr size_t W_FIXED = 1024 + 2 * W_SEG * W_BLK * 4 + (2 * W_MAX_STAGES + 4 * W_QS + 4 * W_BUFS + 1) * 8 + 16;
 constexpr int w_qbufs(int rows) { return rows <= W_NARROW ? W_QS : 2; }
+constexpr int w_ibufs(int rows) { return rows <= W_NARROW ? W_QS : 4; }   // row infos: staged further ahead
 constexpr size_t w_smem(int rows, int stages) {
-    return W_FIXED + (size_t)w_qbufs(rows) * rows * (D * 2 + 16) + (size_t)stages * W_TILE;
+    return W_FIXED + (size_t)rows * (w_qbufs(rows) * D * 2 + w_ibufs(rows) * 16) + (size_t)stages * W_TILE;
 }
 
 struct WSeg {
@@ -148,16 +149,17 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     // S buffers: two of 256 columns, or W_BUFS narrow ones for each group of warps
     const bool narrow = N <= W_NARROW;
     const int d_cols = narrow ? W_NARROW : 256, bufs = narrow ? W_BUFS : 2;
-    const int qbufs = w_qbufs(N);
+    const int qbufs = w_qbufs(N), ibufs = w_ibufs(N);
     uint8_t* kring = align_ptr<1024>(smem_raw);
     uint8_t* qs = kring + KST * W_TILE;                              // [qbufs] staged Q: dims 0-63, then 64-127
-    float* infos = reinterpret_cast<float*>(qs + qbufs * q_bytes);   // [qbufs] row infos, 4 N words each
-    float* sums = infos + qbufs * 4 * N;                             // [2 groups][W_SEG][128]
+    float* infos = reinterpret_cast<float*>(qs + qbufs * q_bytes);   // [ibufs] row infos, 4 N words each
+    float* sums = infos + ibufs * 4 * N;                             // [2 groups][W_SEG][128]
     uint64_t* k_full = reinterpret_cast<uint64_t*>(sums + 2 * W_SEG * W_BLK);
     uint64_t* k_empty = k_full + W_MAX_STAGES;
     uint64_t* q_full = k_empty + W_MAX_STAGES;   // [qbufs] staged
     uint64_t* q_empty = q_full + W_QS;           // [qbufs] its MMAs are done
-    uint64_t* i_empty = q_empty + W_QS;          // [qbufs] the row infos have been used
+    uint64_t* i_full = q_empty + W_QS;           // [ibufs] row infos are there
+    uint64_t* i_empty = i_full + W_QS;           // [ibufs] the row infos have been used
     uint64_t* d_full = i_empty + W_QS;              // [2 groups][W_BUFS] S written
     uint64_t* d_empty = d_full + 2 * W_BUFS;     // [2 groups][W_BUFS] S read
     uint64_t* done = d_empty + 2 * W_BUFS;                // every issued MMA finished
@@ -172,8 +174,11 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             mbar_init(&k_empty[i], 1);
         }
         for (int i = 0; i < qbufs; i++) {
-            mbar_init(&q_full[i], 65);
+            mbar_init(&q_full[i], a.q_tma ? 1 : 64);
             mbar_init(&q_empty[i], 1);
+        }
+        for (int i = 0; i < ibufs; i++) {
+            mbar_init(&i_full[i], 64);
             mbar_init(&i_empty[i], 256);
         }
         for (int i = 0; i < 2 * W_BUFS; i++) {
@@ -337,13 +342,10 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             if (max(g.pg0, first) >= g.pg1) continue;
             for (int h = 0; h < a.Hkv && ok; h++)
                 for (int r0 = 0; r0 < nrows && ok; r0 += N, chunk++) {
-                    const int qb = chunk % qbufs;
-                    if (chunk >= qbufs) {
-                        ok = mbar_wait(&q_empty[qb], (chunk / qbufs - 1) & 1, deadline, a.err);
-                        if (ok) ok = mbar_wait(&i_empty[qb], (chunk / qbufs - 1) & 1, deadline, a.err);
-                        ok = __all_sync(0xffffffffu, ok);
-                        if (!ok) break;
-                    }
+                    const int qb = chunk % qbufs, ib = chunk % ibufs;
+                    if (chunk >= qbufs)
+                        ok = __all_sync(0xffffffffu, mbar_wait(&q_empty[qb], (chunk / qbufs - 1) & 1, deadline, a.err));
+                    if (!ok) break;
                     uint8_t* dst = qs + qb * q_bytes;
                     if (a.q_tma) {
                         // rows are tokens x heads of the group: a box per 64-dim half; rows behind
@@ -367,9 +369,12 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                             *reinterpret_cast<uint4*>(dst + (cd >> 3) * (q_bytes / 2) + w_sw(r, cd & 7)) = v;
                         }
                         fence_proxy_async_smem();
-                        if (tid == 0) mbar_arrive(&q_full[qb]);
+                        mbar_arrive(&q_full[qb]);
                     }
-                    const RowInfo in{infos + qb * 4 * N, N};
+                    if (chunk >= ibufs)
+                        ok = __all_sync(0xffffffffu, mbar_wait(&i_empty[ib], (chunk / ibufs - 1) & 1, deadline, a.err));
+                    if (!ok) { chunk++; break; }
+                    const RowInfo in{infos + ib * 4 * N, N};
                     for (int r = tid; r < N; r += 64) {
                         Row row;
                         row.set(a, s, r0 + r, nrows, h);
@@ -381,7 +386,7 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                         *in.pos(r) = row.pos;
                         *in.i(r) = row.i;
                     }
-                    mbar_arrive(&q_full[qb]);
+                    mbar_arrive(&i_full[ib]);
                 }
         }
         // a staged Q that nobody waited for (after a timeout) must still land
@@ -404,10 +409,9 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             const int rchunks = (nrows + N - 1) / N, chunks = nb > 0 ? a.Hkv * rchunks : 0;
             for (int j = 0; j < nb; j++) sums[(hf * W_SEG + j) * W_BLK + key] = 0.f;
             for (int c = 0; c < chunks; c++, chunk++) {
-                const int qb = chunk % qbufs;
-                const RowInfo in{infos + qb * 4 * N, N};
-                // the infos are read directly: q_full also says that they are there
-                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&q_full[qb], (chunk / qbufs) & 1, deadline, a.err));
+                const int ib = chunk % ibufs;
+                const RowInfo in{infos + ib * 4 * N, N};
+                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&i_full[ib], (chunk / ibufs) & 1, deadline, a.err));
                 const int r0 = c % rchunks * N;                      // first row of this chunk
                 const int t_lo = (r0 + c0) / a.G;                    // tokens of this thread's columns
                 const int nt = r0 + c0 < nrows ? (min(nrows, r0 + c1) - 1) / a.G - t_lo + 1 : 0;
@@ -426,22 +430,30 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                     uint32_t v0 = 0u, v1 = 0u, v2 = 0u, v3 = 0u;     // tokens t_lo .. + 127 that see the key
                     if (!whole && p < s.len) {
                         const int k = p - s.ctx;                     // drafted index of the key
-                        const bool bits = a.mask && k >= 0 && k < 32 * a.mask_words;
+                        const bool bits = k >= 0 && k < 32 * a.mask_words;
                         const uint32_t* mw = a.mask + (size_t)(s.q0 + t_lo) * a.mask_words + (k >> 5);
                         // tokens t_lo + 32 q .. that see the key
                         auto seen = [&](int q) {
-                            uint32_t v = 0u;
                             const int n32 = min(nt - 32 * q, 32);
+                            if (n32 <= 0) return 0u;
+                            uint32_t v = 0xffffffffu;
+                            if (a.mask) {
+                                if (k >= 0) v = 0u;
+                                if (bits) {
 #pragma unroll 8
-                            for (int i = 0; i < n32; i++) {
-                                const int t = 32 * q + i;
-                                uint32_t see = 1u;
-                                if (k >= 0) see = !a.mask ? k <= t_lo + t : bits ? __ldg(mw + (size_t)t * a.mask_words) >> (k & 31) : 0u;
-                                if (a.window > 0) {
-                                    const int tp = a.positions ? __ldg(a.positions + s.q0 + t_lo + t) : s.ctx + t_lo + t;
-                                    if ((long long)tp - kpos >= a.window) see = 0u;
+                                    for (int i = 0; i < n32; i++)
+                                        v |= ((__ldg(mw + (size_t)(32 * q + i) * a.mask_words) >> (k & 31)) & 1u) << i;
                                 }
-                                v |= (see & 1u) << i;
+                            } else {
+                                const int f = k - t_lo - 32 * q;      // a chain: tokens from k on
+                                v = f <= 0 ? 0xffffffffu : f >= 32 ? 0u : 0xffffffffu << f;
+                            }
+                            if (a.window > 0) {
+                                for (int i = 0; i < n32; i++) {
+                                    const int t = t_lo + 32 * q + i;
+                                    const int tp = a.positions ? __ldg(a.positions + s.q0 + t) : s.ctx + t;
+                                    if ((long long)tp - kpos >= a.window) v &= ~(1u << i);
+                                }
                             }
                             return v;
                         };
@@ -472,7 +484,7 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                     mbar_arrive(&d_empty[d]);
                     sums[(hf * W_SEG + j) * W_BLK + key] += add;
                 }
-                if (ok) mbar_arrive(&i_empty[qb]);
+                if (ok) mbar_arrive(&i_empty[ib]);
             }
             asm volatile("bar.sync 1, 256;" ::: "memory");           // both column halves are summed
             if (hf == 0 && ok) {
