@@ -571,44 +571,86 @@ def cascade_tree_decode(tp: CascadeTreePlan, out=None, lse=None, workspace=None,
 
 
 # ------------------------------------------------------------------ writing and trimming the cache
+# A decode step calls these once a layer, where the host's time shows: the checks below read few
+# attributes, and tensors cross as plain integers.
 ROPE_SCALING = {"none": 0, "linear": 1, "ntk": 2, "by_parts": 3}
+_T = None                  # torch and its dtypes, bound by the first call
+_I32 = _F16 = _F32 = _U8 = None
+_raw_device = _raw_stream = None
+
+
+def _bind():
+    global _T, _I32, _F16, _F32, _U8, _raw_device, _raw_stream
+    torch = _torch()
+    _I32, _F16, _F32, _U8 = torch.int32, torch.float16, torch.float32, torch.uint8
+    # the current device and stream without building objects for them, where torch has that
+    _raw_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                          lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+    _T = torch
+
+
+def _stream_of(stream):
+    """The raw handle of `stream`, or of the current device's current stream."""
+    return stream.cuda_stream if stream is not None else _raw_stream(_raw_device())
+
+
+def _device():
+    return _raw_device()
 
 
 def _empty(shape, dtype, device, stream):
     """A tensor that the call on `stream` writes: allocated on that stream, so that its memory is
     reused only behind the call."""
-    torch = _torch()
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
+        return _T.empty(shape, dtype=dtype, device=device)
+    with _T.cuda.stream(stream):
+        return _T.empty(shape, dtype=dtype, device=device)
 
 
-def _here(name, *tensors):
-    """All tensors (None skipped) on the current device: the library launches there."""
-    dev = _torch().cuda.current_device()
-    for t in tensors:
-        if t is not None and t.device.index != dev:
-            raise CklError(1, name, f"a tensor is on {t.device}, the current device is cuda:{dev}")
+def _bad(t, dtype, n, name, who, dev):
+    """Why t is refused (the checks of _at, one by one)."""
+    if not isinstance(t, _T.Tensor) or not t.is_cuda:
+        raise CklError(1, who, f"{name}: expected a CUDA tensor")
+    if t.dtype is not dtype or not t.is_contiguous():
+        raise CklError(1, who, f"{name}: expected contiguous {dtype}, got {t.dtype}")
+    if t.get_device() != dev:
+        raise CklError(1, who, f"{name} is on {t.device}, the current device is cuda:{dev}")
+    raise CklError(2, who, f"{name} has {t.numel()} elements, needs {n}")
 
 
-def _rows(t, dtype, n, name, who):
-    """A contiguous 1-D tensor of at least n elements, or None."""
-    if t is not None:
-        _need(t, dtype, name)
-        if t.numel() < n:
-            raise CklError(1, who, f"{name} has {t.numel()} elements, needs {n}")
-    return t
+def _at(t, dtype, n, name, who, dev):
+    """Address of a contiguous tensor of at least n elements on device dev."""
+    try:
+        if t.dtype is dtype and t.get_device() == dev and t.is_contiguous() and t.numel() >= n:
+            return t.data_ptr()
+    except AttributeError:
+        pass
+    _bad(t, dtype, n, name, who, dev)
 
 
-def _cache_shape(k_cache, v_cache, who):
-    torch = _torch()
-    _need(k_cache, torch.float16, "k_cache")
-    _need(v_cache, torch.float16, "v_cache")
-    if (k_cache.dim() != 4 or k_cache.shape[1] != PAGE or k_cache.shape[3] != HEAD_DIM
-            or v_cache.shape != k_cache.shape):
+def _opt(t, dtype, n, name, who, dev):
+    return None if t is None else _at(t, dtype, n, name, who, dev)
+
+
+def _acc_rows(acc, B, who, dev):
+    """(address, row stride) of fp32 rows, one per sequence at least."""
+    if acc.dtype is not _F32 or acc.get_device() != dev or acc.dim() != 2 or acc.stride(1) != 1:
+        raise CklError(1, who, "acc: expected float32 rows on the current device")
+    rows, cols = acc.shape
+    stride = acc.stride(0) if rows > 1 else cols
+    if rows < B or stride < cols:
+        raise CklError(2, who, f"acc: {rows} rows of {cols}, {stride} apart, for {B} sequences")
+    return acc.data_ptr(), stride
+
+
+def _cache_shape(k_cache, v_cache, who, dev):
+    """(pages, kv heads, addresses) of K and V caches [pages, 16, heads, 128]."""
+    shape = k_cache.shape
+    if len(shape) != 4 or shape[1] != PAGE or shape[3] != HEAD_DIM or v_cache.shape != shape:
         raise CklError(2, who, f"caches {tuple(k_cache.shape)} / {tuple(v_cache.shape)}")
-    return k_cache.shape[0], k_cache.shape[2]
+    return (shape[0], shape[2], _at(k_cache, _F16, 0, "k_cache", who, dev),
+            _at(v_cache, _F16, 0, "v_cache", who, dev))
 
 
 def rope_plan(rot_dim=HEAD_DIM, *, base=10000.0, interleaved=False, scaling="none", factor=1.0,
@@ -617,7 +659,7 @@ def rope_plan(rot_dim=HEAD_DIM, *, base=10000.0, interleaved=False, scaling="non
     caller's own angles per position inv_freq[rot_dim/2] and scale (ckl_rope_plan_freqs)."""
     r = Rope()
     if inv_freq is not None:
-        f = (C.c_double * (rot_dim // 2))(*[float(x) for x in inv_freq])
+        f = (C.c_double * (rot_dim // 2))(*[float(x) for x in inv_freq][:rot_dim // 2])
         if len(inv_freq) != rot_dim // 2:
             raise CklError(1, "rope_plan", f"{len(inv_freq)} frequencies for rot_dim {rot_dim}")
         check(lib().ckl_rope_plan_freqs(f, rot_dim, int(interleaved), float(scale), C.byref(r)),
@@ -636,46 +678,42 @@ def make_append_params(q, k, v, k_cache, v_cache, kv_indptr, kv_indices, kv_last
     """ckl_append_params for new tokens q [N,Hq,128] (or None), k and v [N,Hkv,128] -- fp16,
     tokens any multiple of 8 elements apart, e.g. slices of one fused projection. The params
     keep every tensor alive; q_out (allocated when None) is p.q_rotated."""
-    torch = _torch()
-    who = "make_append_params"
-    P, Hkv = _cache_shape(k_cache, v_cache, who)
-    strides = []
+    if _T is None:
+        _bind()
+    who, dev = "make_append_params", _device()
+    P, Hkv, kc, vc = _cache_shape(k_cache, v_cache, who, dev)
+    N = k.shape[0]
+    addr, strides = [], []
     for t, name in ((q, "q"), (k, "k"), (v, "v")):
         if t is None and name == "q":
+            addr.append(None)
             strides.append(0)
             continue
-        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.float16:
-            raise CklError(1, who, f"{name}: expected a CUDA float16 tensor")
-        if t.dim() != 3 or t.shape[2] != HEAD_DIM or t.shape[0] != k.shape[0]:
+        if not isinstance(t, _T.Tensor) or t.dtype is not _F16 or t.get_device() != dev:
+            raise CklError(1, who, f"{name}: expected a float16 tensor on cuda:{dev}")
+        if t.dim() != 3 or t.shape[2] != HEAD_DIM or t.shape[0] != N:
             raise CklError(2, who, f"{name} {tuple(t.shape)}")
         if t.numel() and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != HEAD_DIM)):
             raise CklError(1, who, f"{name}: a token's heads must be contiguous")
         # the token stride of a single token means nothing: give it its row
-        strides.append(t.stride(0) if t.shape[0] > 1 else t.shape[1] * HEAD_DIM)
+        strides.append(t.stride(0) if N > 1 else t.shape[1] * HEAD_DIM)
+        addr.append(t.data_ptr())
     if k.shape[1] != Hkv or v.shape[1] != Hkv:
         raise CklError(2, who, f"k {tuple(k.shape)} / v {tuple(v.shape)} for {Hkv} cached heads")
-    N = k.shape[0]
-    for t, n in ((kv_indptr, "kv_indptr"), (kv_indices, "kv_indices"),
-                 (kv_last_page_len, "kv_last_page_len")):
-        _need(t, torch.int32, n)
+    ip = _at(kv_indptr, _I32, 1, "kv_indptr", who, dev)
     B = kv_indptr.numel() - 1
-    _rows(kv_last_page_len, torch.int32, B, "kv_last_page_len", who)
-    _rows(q_indptr, torch.int32, B + 1, "q_indptr", who)
-    _rows(positions, torch.int32, N, "positions", who)
-    if q is not None and q_out is None:
-        q_out = torch.empty((N, q.shape[1], HEAD_DIM), dtype=torch.float16, device=q.device)
-    if q is not None:
-        _need(q_out, torch.float16, "q_out")
-        if tuple(q_out.shape) != tuple(q.shape):
-            raise CklError(2, who, f"q_out {tuple(q_out.shape)} for q {tuple(q.shape)}")
-    else:
+    if q is None:
         q_out = None
-    _here(who, q, k, v, q_out, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len,
-          q_indptr, positions)
-    ptr = lambda t: None if t is None else t.data_ptr()
-    p = AppendParams(ptr(q), ptr(k), ptr(v), *strides, ptr(q_out), ptr(k_cache), ptr(v_cache),
-                     ptr(kv_indptr), ptr(kv_indices), ptr(kv_last_page_len), ptr(q_indptr),
-                     ptr(positions), B, N, 0 if q is None else q.shape[1], Hkv, P)
+    elif q_out is None:
+        q_out = _T.empty((N, q.shape[1], HEAD_DIM), dtype=_F16, device=q.device)
+    elif tuple(q_out.shape) != tuple(q.shape):
+        raise CklError(2, who, f"q_out {tuple(q_out.shape)} for q {tuple(q.shape)}")
+    p = AppendParams(*addr, *strides, _opt(q_out, _F16, 0, "q_out", who, dev), kc, vc, ip,
+                     _at(kv_indices, _I32, 0, "kv_indices", who, dev),
+                     _at(kv_last_page_len, _I32, B, "kv_last_page_len", who, dev),
+                     _opt(q_indptr, _I32, B + 1, "q_indptr", who, dev),
+                     _opt(positions, _I32, N, "positions", who, dev), B, N,
+                     0 if q is None else q.shape[1], Hkv, P)
     p._keep = (q, k, v, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, q_indptr,
                positions)
     p.q_rotated = q_out
@@ -685,8 +723,9 @@ def make_append_params(q, k, v, k_cache, v_cache, kv_indptr, kv_indices, kv_last
 def rope_append(p: AppendParams, rope: Rope = None, stream=None):
     """Rotates and appends (ckl_rope_append) -> the rotated q (p.q_rotated). rope None copies
     q and k unturned."""
-    check(lib().ckl_rope_append(C.byref(p), None if rope is None else C.byref(rope),
-                                _stream(stream)), "ckl_rope_append")
+    st = lib().ckl_rope_append(p, rope, _stream_of(stream))
+    if st:
+        check(st, "ckl_rope_append")
     return p.q_rotated
 
 
@@ -694,23 +733,21 @@ def tree_mask(parents, q_indptr, kv_indptr, kv_last_page_len, max_q, *, mask=Non
               positions=None, stream=None):
     """Ancestor masks of draft trees (ckl_tree_mask) -> (mask int32 [N, ceil(max_q/32)] holding
     the uint32 words, positions int32 [N])."""
-    torch = _torch()
-    _need(parents, torch.int32, "parents")
+    if _T is None:
+        _bind()
+    who, dev = "tree_mask", _device()
+    a = _at(parents, _I32, 0, "parents", who, dev)
+    ip = _at(kv_indptr, _I32, 1, "kv_indptr", who, dev)
     N, B, W = parents.numel(), kv_indptr.numel() - 1, (max_q + 31) // 32
-    _need(kv_indptr, torch.int32, "kv_indptr")
-    for t, n, name in ((q_indptr, B + 1, "q_indptr"), (kv_last_page_len, B, "kv_last_page_len")):
-        _need(t, torch.int32, name)
-        _rows(t, torch.int32, n, name, "tree_mask")
     if mask is None:
-        mask = _empty((N, W), torch.int32, parents.device, stream)
+        mask = _empty((N, W), _I32, parents.device, stream)
     if positions is None:
-        positions = _empty(N, torch.int32, parents.device, stream)
-    _rows(mask, torch.int32, N * W, "mask", "tree_mask")
-    _rows(positions, torch.int32, N, "positions", "tree_mask")
-    _here("tree_mask", parents, q_indptr, kv_indptr, kv_last_page_len, mask, positions)
-    check(lib().ckl_tree_mask(_ptr(parents), _ptr(q_indptr), _ptr(kv_indptr),
-                              _ptr(kv_last_page_len), B, N, W, _ptr(mask), _ptr(positions),
-                              _stream(stream)), "ckl_tree_mask")
+        positions = _empty(N, _I32, parents.device, stream)
+    check(lib().ckl_tree_mask(a, _at(q_indptr, _I32, B + 1, "q_indptr", who, dev), ip,
+                              _at(kv_last_page_len, _I32, B, "kv_last_page_len", who, dev), B, N, W,
+                              _at(mask, _I32, N * W, "mask", who, dev),
+                              _at(positions, _I32, N, "positions", who, dev), _stream_of(stream)),
+          "ckl_tree_mask")
     return mask, positions
 
 
@@ -720,37 +757,33 @@ def make_tree_params(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_le
     """ckl_tree_params with its key split (ckl_tree_plan) for q [N,Hq,128] and sequences of up
     to max_q drafted and max_len cached tokens. tree_mask: int32 [N, words], bit j = drafted
     token j is seen (tree_mask()); None: a chain. The params keep every tensor alive."""
-    torch = _torch()
-    who = "make_tree_params"
-    _need(q, torch.float16, "q")
-    P, Hkv = _cache_shape(k_cache, v_cache, who)
-    if q.dim() != 3 or q.shape[2] != HEAD_DIM or q.shape[1] == 0 or q.shape[1] % Hkv:
+    if _T is None:
+        _bind()
+    who, dev = "make_tree_params", _device()
+    P, Hkv, kc, vc = _cache_shape(k_cache, v_cache, who, dev)
+    qa = _at(q, _F16, 0, "q", who, dev)
+    if q.dim() != 3 or q.shape[2] != HEAD_DIM or Hkv == 0 or q.shape[1] == 0 or q.shape[1] % Hkv:
         raise CklError(2, who, f"q {tuple(q.shape)} for {Hkv} cached heads")
     N, Hq = q.shape[0], q.shape[1]
-    for t, n in ((kv_indptr, "kv_indptr"), (kv_indices, "kv_indices"),
-                 (kv_last_page_len, "kv_last_page_len")):
-        _need(t, torch.int32, n)
+    ip = _at(kv_indptr, _I32, 1, "kv_indptr", who, dev)
     B = kv_indptr.numel() - 1
-    _rows(kv_last_page_len, torch.int32, B, "kv_last_page_len", who)
-    _rows(q_indptr, torch.int32, B + 1, "q_indptr", who)
-    _rows(positions, torch.int32, N, "positions", who)
-    _rows(slopes, torch.float32, Hq, "slopes", who)
     words = 0
     if tree_mask is not None:
-        _need(tree_mask, torch.int32, "tree_mask")
+        _at(tree_mask, _I32, 0, "tree_mask", who, dev)
         if tree_mask.dim() != 2 or tree_mask.shape[0] < N:
             raise CklError(2, who, f"tree_mask {tuple(tree_mask.shape)} for {N} tokens")
         words = tree_mask.shape[1]
-    _here(who, q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, q_indptr, tree_mask,
-          positions, slopes)
     nc, ct = C.c_int(1), C.c_int(PAGE)
     if B > 0 and N > 0:
         check(lib().ckl_tree_plan(Hq // Hkv, B, Hkv, max_q, max_len, window, force_chunks,
                                   C.byref(nc), C.byref(ct)), "ckl_tree_plan")
-    ptr = lambda t: None if t is None else t.data_ptr()
-    p = TreeParams(ptr(q), ptr(k_cache), ptr(v_cache), ptr(kv_indptr), ptr(kv_indices),
-                   ptr(kv_last_page_len), ptr(q_indptr), ptr(tree_mask), ptr(positions),
-                   ptr(slopes), B, N, Hq, Hkv, max_q, words, nc.value, ct.value, window, P,
+    p = TreeParams(qa, kc, vc, ip, _at(kv_indices, _I32, 0, "kv_indices", who, dev),
+                   _at(kv_last_page_len, _I32, B, "kv_last_page_len", who, dev),
+                   _opt(q_indptr, _I32, B + 1, "q_indptr", who, dev),
+                   None if tree_mask is None else tree_mask.data_ptr(),
+                   _opt(positions, _I32, N, "positions", who, dev),
+                   _opt(slopes, _F32, Hq, "slopes", who, dev), B, N, Hq, Hkv, max_q, words,
+                   nc.value, ct.value, window, P,
                    1.0 / math.sqrt(HEAD_DIM) if sm_scale is None else sm_scale, softcap)
     p._keep = (q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, q_indptr, tree_mask,
                positions, slopes)
@@ -758,29 +791,31 @@ def make_tree_params(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_le
 
 
 def tree_workspace_size(p: TreeParams):
-    return lib().ckl_tree_workspace_size(C.byref(p))
+    return lib().ckl_tree_workspace_size(p)
 
 
 def tree_attention(p: TreeParams, out=None, lse=None, workspace=None, stream=None):
     """Attention of drafted tokens over the cache (ckl_tree_attention) -> (out fp16 [N,Hq,128],
     lse fp32 [N,Hq])."""
-    torch = _torch()
+    who, L = "tree_attention", lib()
     dev = p._keep[0].device
+    rows = p.N * p.Hq
     if out is None:
-        out = _empty((p.N, p.Hq, HEAD_DIM), torch.float16, dev, stream)
-    elif out.dtype != torch.float16 or out.numel() != p.N * p.Hq * HEAD_DIM or not out.is_contiguous():
-        raise CklError(1, "tree_attention", f"out {out.dtype} {tuple(out.shape)}")
+        out = _empty((p.N, p.Hq, HEAD_DIM), _F16, dev, stream)
     if lse is None:
-        lse = _empty((p.N, p.Hq), torch.float32, dev, stream)
-    elif lse.dtype != torch.float32 or lse.numel() != p.N * p.Hq or not lse.is_contiguous():
-        raise CklError(1, "tree_attention", f"lse {lse.dtype} {tuple(lse.shape)}")
-    need = tree_workspace_size(p)
-    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    if need and ws_bytes < need:
-        workspace = _empty(need, torch.uint8, dev, stream)
-        ws_bytes = need
-    check(lib().ckl_tree_attention(C.byref(p), _ptr(out), _ptr(lse), _ptr(workspace), ws_bytes,
-                                   _stream(stream)), "ckl_tree_attention")
+        lse = _empty((p.N, p.Hq), _F32, dev, stream)
+    d = dev.index
+    oa, la = _at(out, _F16, rows * HEAD_DIM, "out", who, d), _at(lse, _F32, rows, "lse", who, d)
+    need = L.ckl_tree_workspace_size(p)
+    wa, have = None, 0
+    if workspace is not None:
+        wa, have = _at(workspace, workspace.dtype, 0, "workspace", who, d), workspace.nbytes
+    if have < need:
+        workspace = _empty(need, _U8, dev, stream)
+        wa, have = workspace.data_ptr(), need
+    st = L.ckl_tree_attention(p, oa, la, wa, have, _stream_of(stream))
+    if st:
+        check(st, "ckl_tree_attention")
     return out, lse
 
 
@@ -788,18 +823,12 @@ def cache_weights(p: TreeParams, lse, acc, *, decay=1.0, stream=None):
     """acc[b, place] = decay * acc + the attention weight the place received from this call's
     tokens (ckl_cache_weights), in place; lse from tree_attention, acc fp32 [B, >= max_len]
     with contiguous rows."""
-    torch = _torch()
-    _need(lse, torch.float32, "lse")
-    if not acc.is_cuda or acc.dtype != torch.float32 or acc.dim() != 2 or acc.stride(1) != 1:
-        raise CklError(1, "cache_weights", "acc: expected CUDA float32 rows")
-    if acc.shape[0] < p.B or lse.numel() < p.N * p.Hq:
-        raise CklError(2, "cache_weights", f"acc {tuple(acc.shape)} / lse {tuple(lse.shape)}")
-    if acc.stride(0) < acc.shape[1] and acc.shape[0] > 1:
-        raise CklError(1, "cache_weights", "acc rows overlap")
-    _here("cache_weights", lse, acc)
-    stride = acc.stride(0) if acc.shape[0] > 1 else acc.shape[1]
-    check(lib().ckl_cache_weights(C.byref(p), _ptr(lse), _ptr(acc), stride, decay,
-                                  _stream(stream)), "ckl_cache_weights")
+    who, dev = "cache_weights", p._keep[0].get_device()
+    aa, stride = _acc_rows(acc, p.B, who, dev)
+    st = lib().ckl_cache_weights(p, _at(lse, _F32, p.N * p.Hq, "lse", who, dev), aa, stride, decay,
+                                 _stream_of(stream))
+    if st:
+        check(st, "ckl_cache_weights")
     return acc
 
 
@@ -807,25 +836,21 @@ def cache_select(acc, kv_indptr, kv_last_page_len, keep, *, sink=0, recent=0, ke
                  keep_count=None, stream=None):
     """The tokens to keep of every sequence by accumulated weight (ckl_cache_select) ->
     (keep_idx int32 [B, keep] ascending, -1 behind the count; keep_count int32 [B])."""
-    torch = _torch()
-    if not acc.is_cuda or acc.dtype != torch.float32 or acc.dim() != 2 or acc.stride(1) != 1:
-        raise CklError(1, "cache_select", "acc: expected CUDA float32 rows")
-    _need(kv_indptr, torch.int32, "kv_indptr")
-    _need(kv_last_page_len, torch.int32, "kv_last_page_len")
+    if _T is None:
+        _bind()
+    who, dev = "cache_select", _device()
+    ip = _at(kv_indptr, _I32, 1, "kv_indptr", who, dev)
     B = kv_indptr.numel() - 1
-    if acc.shape[0] < B or kv_last_page_len.numel() < B:
-        raise CklError(2, "cache_select", f"acc {tuple(acc.shape)} for {B} sequences")
+    aa, stride = _acc_rows(acc, B, who, dev)
     if keep_idx is None:
-        keep_idx = _empty((B, max(keep, 0)), torch.int32, acc.device, stream)
+        keep_idx = _empty((B, max(keep, 0)), _I32, acc.device, stream)
     if keep_count is None:
-        keep_count = _empty(B, torch.int32, acc.device, stream)
-    _rows(keep_idx, torch.int32, B * keep, "keep_idx", "cache_select")
-    _rows(keep_count, torch.int32, B, "keep_count", "cache_select")
-    _here("cache_select", acc, kv_indptr, kv_last_page_len, keep_idx, keep_count)
-    stride = acc.stride(0) if acc.shape[0] > 1 else acc.shape[1]
-    check(lib().ckl_cache_select(_ptr(acc), stride, _ptr(kv_indptr), _ptr(kv_last_page_len), B,
-                                 keep, sink, recent, _ptr(keep_idx), _ptr(keep_count),
-                                 _stream(stream)), "ckl_cache_select")
+        keep_count = _empty(B, _I32, acc.device, stream)
+    st = lib().ckl_cache_select(aa, stride, ip, _at(kv_last_page_len, _I32, B, "kv_last_page_len", who, dev),
+                                B, keep, sink, recent, _at(keep_idx, _I32, B * keep, "keep_idx", who, dev),
+                                _at(keep_count, _I32, B, "keep_count", who, dev), _stream_of(stream))
+    if st:
+        check(st, "ckl_cache_select")
     return keep_idx, keep_count
 
 
@@ -833,34 +858,26 @@ def cache_compact(k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, kee
                   *, dst_start=None, acc=None, new_len=None, stream=None):
     """Moves the kept tokens of every sequence together, in place (ckl_cache_compact) -> the
     new lengths int32 [B]. keep_idx int32 [B, n], keep_count int32 [B]; acc fp32 [B, >= L]."""
-    torch = _torch()
-    who = "cache_compact"
-    P, Hkv = _cache_shape(k_cache, v_cache, who)
-    for t, n in ((kv_indptr, "kv_indptr"), (kv_indices, "kv_indices"),
-                 (kv_last_page_len, "kv_last_page_len"), (keep_idx, "keep_idx"),
-                 (keep_count, "keep_count")):
-        _need(t, torch.int32, n)
+    if _T is None:
+        _bind()
+    who, dev = "cache_compact", _device()
+    P, Hkv, kc, vc = _cache_shape(k_cache, v_cache, who, dev)
+    ip = _at(kv_indptr, _I32, 1, "kv_indptr", who, dev)
     B = kv_indptr.numel() - 1
-    if keep_idx.dim() != 2 or keep_idx.shape[0] < B:
-        raise CklError(2, who, f"keep_idx {tuple(keep_idx.shape)} for {B} sequences")
-    _rows(kv_last_page_len, torch.int32, B, "kv_last_page_len", who)
-    _rows(keep_count, torch.int32, B, "keep_count", who)
-    _rows(dst_start, torch.int32, B, "dst_start", who)
-    stride = 0
-    if acc is not None:
-        if (not acc.is_cuda or acc.dtype != torch.float32 or acc.dim() != 2 or acc.stride(1) != 1
-                or acc.shape[0] < B or (acc.shape[0] > 1 and acc.stride(0) < acc.shape[1])):
-            raise CklError(1, who, "acc: expected CUDA float32 rows, one per sequence")
-        stride = acc.stride(0) if acc.shape[0] > 1 else acc.shape[1]
+    ia = _at(keep_idx, _I32, 0, "keep_idx", who, dev)
+    shape = keep_idx.shape
+    if len(shape) != 2 or shape[0] < B:
+        raise CklError(2, who, f"keep_idx {tuple(shape)} for {B} sequences")
+    aa, stride = (None, 0) if acc is None else _acc_rows(acc, B, who, dev)
     if new_len is None:
-        new_len = _empty(B, torch.int32, k_cache.device, stream)
-    _rows(new_len, torch.int32, B, "new_len", who)
-    _here(who, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, keep_idx, keep_count,
-          dst_start, acc, new_len)
-    check(lib().ckl_cache_compact(_ptr(k_cache), _ptr(v_cache), _ptr(kv_indptr), _ptr(kv_indices),
-                                  _ptr(kv_last_page_len), B, Hkv, P, _ptr(keep_idx),
-                                  keep_idx.shape[1], _ptr(keep_count), _ptr(dst_start), _ptr(acc),
-                                  stride, _ptr(new_len), _stream(stream)), "ckl_cache_compact")
+        new_len = _empty(B, _I32, k_cache.device, stream)
+    st = lib().ckl_cache_compact(kc, vc, ip, _at(kv_indices, _I32, 0, "kv_indices", who, dev),
+                                 _at(kv_last_page_len, _I32, B, "kv_last_page_len", who, dev), B, Hkv, P, ia,
+                                 shape[1], _at(keep_count, _I32, B, "keep_count", who, dev),
+                                 _opt(dst_start, _I32, B, "dst_start", who, dev), aa, stride,
+                                 _at(new_len, _I32, B, "new_len", who, dev), _stream_of(stream))
+    if st:
+        check(st, "ckl_cache_compact")
     return new_len
 
 
