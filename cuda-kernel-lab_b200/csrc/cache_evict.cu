@@ -524,9 +524,10 @@ __device__ __forceinline__ uint32_t rank_key(float x) {
 
 constexpr int S_THREADS = 1024;
 constexpr int S_WARPS = S_THREADS / 32;
-constexpr int S_BINS = 2048;               // radix passes over 11, 11 and 10 bits
-constexpr int S_MAX_KEYS = 47 << 10;       // keys of a CTA's slice kept in shared memory, at most
-constexpr int S_SLICE = 4096;              // places per CTA that a cluster is sized for
+constexpr int S_BINS = 2048;               // words of a pass's histogram
+constexpr int S_KEYS = 16;                 // keys a thread holds in registers
+constexpr int S_CLUSTER = 8;               // CTAs of a sequence, at most
+constexpr int S_SLICE = 8192;              // places per CTA that a cluster is sized for
 
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -547,73 +548,77 @@ struct SArgs {
     int* keep_idx;
     int* keep_count;
     long long stride;
-    int keep, sink, recent, cluster, max_keys;
+    int keep, sink, recent, cluster;
+};
+struct SShared {
+    int hist[3][S_BINS];                   // three passes of 2048 bins, or four of 256
+    int warp_gt[S_WARPS], warp_eq[S_WARPS];
+    int part[4][256];
+    int bin, left, in;
+    int total[2];
 };
 
-// Keeps the `want` greatest of a sequence's middle places. A cluster of CTAs (one for short
-// sequences) shares the sequence: each loads its slice once, as ordered integers in shared
-// memory; three radix passes narrow the threshold, each a histogram per CTA that all CTAs of the
-// cluster add up from one another's shared memory; then every warp counts and writes its part of
-// the list in order. Bound by latency: per pass one cluster barrier, two block barriers. A pass
-// whose bin is taken whole ends the search (the usual case after two passes unless values tie).
-// grid = (cluster, B).
-__global__ void __launch_bounds__(S_THREADS) select_kernel(const SArgs a) {
-    extern __shared__ uint32_t keys[];                       // [max_keys]
-    __shared__ int hist[3][S_BINS];
-    __shared__ int warp_sum[S_WARPS], warp_eq[S_WARPS];
-    __shared__ int s_bin, s_left, s_in;
-    __shared__ int total[2];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    for (int i = tid; i < 3 * S_BINS; i += S_THREADS) (&hist[0][0])[i] = 0;
-    pdl_wait();
-    pdl_trigger();
-    const int b = blockIdx.y, rank = blockIdx.x;
-    int page0;
-    const int len = tree::seq_len(a.indptr, a.last, b, &page0);
-    int* out = a.keep_idx + (size_t)b * a.keep;
-    const int step = a.cluster * S_THREADS, me = rank * S_THREADS + tid;
-    if (me == 0) a.keep_count[b] = min(len, a.keep);
-    if (len <= a.keep) {                                     // the same for the whole cluster
-        for (int i = me; i < a.keep; i += step) out[i] = i < len ? i : -1;
-        return;
-    }
-    const int hi = len - a.recent, mid = hi - a.sink;
-    int want = a.keep - a.sink - a.recent;                   // of the places [sink, hi); mid > want
-    for (int i = me; i < a.sink; i += step) out[i] = i;
-    for (int i = me; i < a.recent; i += step) out[a.keep - a.recent + i] = hi + i;
-    if (want == 0) return;
-    // this CTA's slice of the middle, a multiple of a warp's 32 places per warp
-    const int slice = ((mid + a.cluster - 1) / a.cluster + 31) & ~31;
+// Keeps the `want` greatest of the places [a.sink, a.sink + mid): radix passes over the ordered
+// keys narrow the threshold, then every warp counts and writes its part of the list in order. A
+// warp owns a run of 32-place rows of the CTA's slice; HELD: a thread has its keys in registers,
+// otherwise (slices beyond 16K places) they are read again each time.
+// CLUSTERED: the CTAs of a cluster share the sequence and add up one another's histograms, in 8-bit
+// digits (one remote pair of words per thread and pass; 11-bit digits would move 64 KB per CTA);
+// a single CTA takes 11 bits a pass. A pass whose bin is taken whole ends the search.
+template <bool CLUSTERED, bool HELD>
+__device__ __forceinline__ void select_part(const SArgs& a, SShared& sh, const float* acc_row, int mid, int want,
+                                            int* out, int tid, int rank) {
+    constexpr int PASSES = CLUSTERED ? 4 : 3;
+    const int warp = tid >> 5, lane = tid & 31;
+    // this CTA's slice of the middle, a warp's rows of it
+    const int slice = CLUSTERED ? ((mid + a.cluster - 1) / a.cluster + 31) & ~31 : mid;
     const int beg = a.sink + min(mid, rank * slice), n = a.sink + min(mid, (rank + 1) * slice) - beg;
-    const float* row = a.acc + b * a.stride + beg;
+    const int per = ((n + S_WARPS - 1) / S_WARPS + 31) & ~31;
+    const int w0 = min(n, warp * per), w1 = min(n, w0 + per);
+    const float* row = acc_row + beg;
     const long long have = a.stride - beg;                   // places of the row that exist
     auto load = [&](int i) { return i < have ? rank_key(__ldg(row + i)) : 0u; };
-    const bool held = n <= a.max_keys;                       // longer slices are read again from L2
-    if (held)
-        for (int i = tid; i < n; i += S_THREADS) keys[i] = load(i);
-    auto key = [&](int i) { return held ? keys[i] : load(i); };
-    __syncthreads();
+    uint32_t held[HELD ? S_KEYS : 1];
+    if (HELD) {
+#pragma unroll
+        for (int r = 0; r < S_KEYS; r++) {
+            const int i = w0 + r * 32 + lane;
+            held[HELD ? r : 0] = i < w1 ? load(i) : 0u;
+        }
+    }
+    // f(first place of the row, this lane's key, whether it has one) for every row of the warp
+    auto rows = [&](auto f) {
+        if (HELD) {
+#pragma unroll
+            for (int r = 0; r < S_KEYS; r++)
+                if (w0 + r * 32 < w1) f(w0 + r * 32, held[HELD ? r : 0], w0 + r * 32 + lane < w1);
+        } else {
+            for (int i = w0; i < w1; i += 32) f(i, i + lane < w1 ? load(i + lane) : 0u, i + lane < w1);
+        }
+    };
 
     uint32_t prefix = 0, known = 0;
-    for (int pass = 0; pass < 3; pass++) {
-        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-        const uint32_t field = pass == 2 ? 1023u : 2047u;
-        int* h = hist[pass];
-        for (int i = tid; i < n; i += S_THREADS) {
-            const uint32_t k = key(i);
-            if ((k & known) == prefix) atomicAdd(&h[(k >> shift) & field], 1);
-        }
-        if (a.cluster > 1) cluster_sync();
-        else __syncthreads();
-        // bins from the greatest down, two per thread
-        const int bin = S_BINS - 1 - 2 * tid;
-        int c0 = 0, c1 = 0;
-        if (a.cluster > 1) {
-            for (int r = 0; r < a.cluster; r++) {
-                c0 += cluster_load(&h[bin], r);
-                c1 += cluster_load(&h[bin - 1], r);
-            }
+    for (int pass = 0; pass < PASSES; pass++) {
+        const int shift = CLUSTERED ? 24 - 8 * pass : pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        const uint32_t field = CLUSTERED ? 255u : pass == 2 ? 1023u : 2047u;
+        int* h = CLUSTERED ? sh.hist[0] + pass * 256 : sh.hist[pass];
+        rows([&](int, uint32_t k, bool in) {
+            if (in && (k & known) == prefix) atomicAdd(&h[(k >> shift) & field], 1);
+        });
+        // bins from the greatest down: two per thread, or one each in the first 256
+        int bin, c0 = 0, c1 = 0;
+        if (CLUSTERED) {
+            cluster_sync();
+            const int r = (tid >> 8) * 2;
+            bin = 255 - (tid & 255);
+            if (r < a.cluster) c0 = cluster_load(&h[bin], r);
+            if (r + 1 < a.cluster) c0 += cluster_load(&h[bin], r + 1);
+            sh.part[tid >> 8][bin] = c0;
+            __syncthreads();
+            c0 = tid < 256 ? sh.part[0][bin] + sh.part[1][bin] + sh.part[2][bin] + sh.part[3][bin] : 0;
         } else {
+            __syncthreads();
+            bin = S_BINS - 1 - 2 * tid;
             c0 = h[bin];
             c1 = h[bin - 1];
         }
@@ -623,61 +628,85 @@ __global__ void __launch_bounds__(S_THREADS) select_kernel(const SArgs a) {
             const int y = __shfl_up_sync(0xffffffffu, x, o);
             if (lane >= o) x += y;
         }
-        if (lane == 31) warp_sum[warp] = x;
+        if (lane == 31) sh.warp_gt[warp] = x;
         __syncthreads();
-        int before = lane < warp ? warp_sum[lane] : 0;
-        before = __reduce_add_sync(0xffffffffu, before);
+        const int before = __reduce_add_sync(0xffffffffu, lane < warp ? sh.warp_gt[lane] : 0);
         const int up0 = before + x - c0 - c1, up1 = up0 + c0;     // keys above each bin
-        if (up0 < want && want <= up1) { s_bin = bin; s_left = want - up0; s_in = c0; }
-        if (up1 < want && want <= up1 + c1) { s_bin = bin - 1; s_left = want - up1; s_in = c1; }
+        if (up0 < want && want <= up1) { sh.bin = bin; sh.left = want - up0; sh.in = c0; }
+        if (up1 < want && want <= up1 + c1) { sh.bin = bin - 1; sh.left = want - up1; sh.in = c1; }
         __syncthreads();
-        prefix |= (uint32_t)s_bin << shift;
+        prefix |= (uint32_t)sh.bin << shift;
         known |= field << shift;
-        want = s_left;
-        if (s_in == want) break;                             // the whole bin is kept
+        want = sh.left;
+        if (sh.in == want) break;                            // the whole bin is kept
     }
     // keys above `prefix` in the known bits are kept, and the first `want` of those equal to it
-    const int per = ((n + S_WARPS - 1) / S_WARPS + 31) & ~31;
-    const int w0 = min(n, warp * per), w1 = min(n, w0 + per);
     int gt = 0, eq = 0;
-    for (int i = w0 + lane; i < w1; i += 32) {
-        const uint32_t k = key(i) & known;
-        gt += k > prefix;
-        eq += k == prefix;
-    }
+    rows([&](int, uint32_t k, bool in) {
+        gt += in && (k & known) > prefix;
+        eq += in && (k & known) == prefix;
+    });
     gt = __reduce_add_sync(0xffffffffu, gt);
     eq = __reduce_add_sync(0xffffffffu, eq);
     if (lane == 0) {
-        warp_sum[warp] = gt;
-        warp_eq[warp] = eq;
+        sh.warp_gt[warp] = gt;
+        sh.warp_eq[warp] = eq;
     }
     __syncthreads();
-    int g = __reduce_add_sync(0xffffffffu, lane < warp ? warp_sum[lane] : 0);
-    int e = __reduce_add_sync(0xffffffffu, lane < warp ? warp_eq[lane] : 0);
-    if (a.cluster > 1) {
+    int g = __reduce_add_sync(0xffffffffu, lane < warp ? sh.warp_gt[lane] : 0);
+    int e = __reduce_add_sync(0xffffffffu, lane < warp ? sh.warp_eq[lane] : 0);
+    if (CLUSTERED) {
         if (warp == S_WARPS - 1 && lane == 0) {
-            total[0] = g + gt;
-            total[1] = e + eq;
+            sh.total[0] = g + gt;
+            sh.total[1] = e + eq;
         }
         cluster_sync();
-        for (int r = 0; r < rank; r++) {
-            g += cluster_load(&total[0], r);
-            e += cluster_load(&total[1], r);
-        }
+        g += __reduce_add_sync(0xffffffffu, lane < rank ? cluster_load(&sh.total[0], lane) : 0);
+        e += __reduce_add_sync(0xffffffffu, lane < rank ? cluster_load(&sh.total[1], lane) : 0);
         cluster_sync();                                      // nobody leaves while it is read
     }
-    out += a.sink;
-    for (int base = w0; base < w1; base += 32) {
-        const int i = base + lane;
-        const uint32_t k = i < w1 ? key(i) & known : 0u;
-        const bool is_gt = i < w1 && k > prefix, is_eq = i < w1 && k == prefix;
+    const uint32_t below = (1u << lane) - 1u;
+    rows([&](int i0, uint32_t k, bool in) {
+        const bool is_gt = in && (k & known) > prefix, is_eq = in && (k & known) == prefix;
         const uint32_t bg = __ballot_sync(0xffffffffu, is_gt), be = __ballot_sync(0xffffffffu, is_eq);
-        const uint32_t below = (1u << lane) - 1u;
         const int ei = e + __popc(be & below);
-        if (is_gt || (is_eq && ei < want)) out[g + __popc(bg & below) + min(ei, want)] = beg + i;
+        if (is_gt || (is_eq && ei < want)) out[g + __popc(bg & below) + min(ei, want)] = beg + i0 + lane;
         g += __popc(bg);
         e += __popc(be);
+    });
+}
+
+// grid = (cluster, B): bound by latency. 1 x 131072 places: 18.7 us, against 34 with the keys in
+// shared memory and 11-bit digits across the cluster.
+template <bool CLUSTERED>
+__global__ void __launch_bounds__(S_THREADS) select_kernel(const SArgs a) {
+    __shared__ SShared sh;
+    const int tid = threadIdx.x;
+    for (int i = tid; i < (CLUSTERED ? 4 * 256 : 3 * S_BINS); i += S_THREADS) (&sh.hist[0][0])[i] = 0;
+    pdl_wait();
+    pdl_trigger();
+    const int b = blockIdx.y, rank = CLUSTERED ? blockIdx.x : 0;
+    int page0;
+    const int len = tree::seq_len(a.indptr, a.last, b, &page0);
+    int* out = a.keep_idx + (size_t)b * a.keep;
+    const int step = gridDim.x * S_THREADS, me = rank * S_THREADS + tid;
+    if (me == 0) a.keep_count[b] = min(len, a.keep);
+    if (len <= a.keep) {                                     // the same for the whole cluster
+        for (int i = me; i < a.keep; i += step) out[i] = i < len ? i : -1;
+        return;
     }
+    const int hi = len - a.recent, mid = hi - a.sink;
+    const int want = a.keep - a.sink - a.recent;             // of the places [sink, hi); mid > want
+    for (int i = me; i < a.sink; i += step) out[i] = i;
+    for (int i = me; i < a.recent; i += step) out[a.keep - a.recent + i] = hi + i;
+    if (want == 0) return;
+    __syncthreads();                                         // the histograms are zero
+    const float* row = a.acc + b * a.stride;
+    const int slice = CLUSTERED ? (mid + a.cluster - 1) / a.cluster : mid;
+    if (slice <= S_KEYS * S_THREADS - 31)                    // a slice is rounded up to a warp's 32 places
+        select_part<CLUSTERED, true>(a, sh, row, mid, want, out + a.sink, tid, rank);
+    else
+        select_part<CLUSTERED, false>(a, sh, row, mid, want, out + a.sink, tid, rank);
 }
 
 // ------------------------------------------------------------------ compact
@@ -824,8 +853,6 @@ const Setup* setup(const DeviceInfo* di) {
         cudaError_t e = cudaFuncSetAttribute(weights_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, di->smem_optin - 1024);
         if (e == cudaSuccess)
             e = cudaFuncSetAttribute(weights_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, di->smem_optin - 1024);
-        if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S_MAX_KEYS * 4);
         if (e != cudaSuccess) ks[di->device].st = cuda_status(e, "cache kernels setup");
     });
     return &ks[di->device];
@@ -895,15 +922,17 @@ ckl_status ckl_cache_select(const float* acc, long long acc_stride, const int* k
     if (ks->st != CKL_OK) return ks->st;
     // a CTA per S_SLICE places, as long as the clusters of all sequences fit the GPU at once
     int cluster = 1;
-    while (cluster < 8 && (long long)cluster * S_SLICE < acc_stride && (long long)B * cluster * 2 <= di->sms) cluster *= 2;
-    const long long slice = ((acc_stride + cluster - 1) / cluster + 31) & ~31LL;
-    SArgs a{acc, kv_indptr, kv_last_page_len, keep_idx, keep_count, acc_stride, keep, sink, recent, cluster,
-            (int)std::min(slice, (long long)S_MAX_KEYS)};
+    while (cluster < S_CLUSTER && (long long)cluster * S_SLICE < acc_stride && (long long)B * cluster * 2 <= di->sms) cluster *= 2;
+    SArgs a{acc, kv_indptr, kv_last_page_len, keep_idx, keep_count, acc_stride, keep, sink, recent, cluster};
     void* args[] = {&a};
+    if (cluster == 1) {
+        CKL_CUDA_TRY(launch((const void*)select_kernel<false>, dim3(1, (unsigned)B), dim3(S_THREADS), 0,
+                            (cudaStream_t)stream, args, true));
+        return CKL_OK;
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)cluster, (unsigned)B);
     cfg.blockDim = dim3(S_THREADS);
-    cfg.dynamicSmemBytes = (size_t)a.max_keys * 4;
     cfg.stream = (cudaStream_t)stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -913,7 +942,7 @@ ckl_status ckl_cache_select(const float* acc, long long acc_stride, const int* k
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    CKL_CUDA_TRY(cudaLaunchKernelExC(&cfg, (const void*)select_kernel, args));
+    CKL_CUDA_TRY(cudaLaunchKernelExC(&cfg, (const void*)select_kernel<true>, args));
     return CKL_OK;
 }
 
