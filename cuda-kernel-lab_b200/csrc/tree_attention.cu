@@ -72,37 +72,69 @@ struct State {
         const int q_row = (lane & 7) + (((lane >> 3) & 1) << 3), q_hi = lane >> 4;
         const uint32_t vb = kb + KV_TILE;
 
-        float sc[NT][2][4];
+        float sc[NT][2][4], sd[NT][2][4];        // two chains of additions, joined below
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int h = 0; h < 2; h++) sc[n][h][0] = sc[n][h][1] = sc[n][h][2] = sc[n][h][3] = 0.f;
+            for (int c = 0; c < 8; c++) sc[n][c >> 2][c & 3] = sd[n][c >> 2][c & 3] = 0.f;
+        // fragments are loaded a batch ahead of the products that use them: a warp has its page to
+        // itself, and waiting for every ldmatrix in turn took most of a page's 1.5 us
+        constexpr int KB = NT == 1 ? 8 : 4;
 #pragma unroll
-        for (int kk = 0; kk < 8; kk++) {
-            uint32_t b00, b01, b10, b11;
-            ldmatrix_x4(kb + tile_off(k_key, 2 * kk + k_hi), b00, b01, b10, b11);
+        for (int k0 = 0; k0 < 8; k0 += KB) {
+            uint32_t kf[KB][4], qf[NT][KB][4];
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
-                uint32_t a0, a1, a2, a3;
-                ldmatrix_x4(qb + n * KV_TILE + tile_off(q_row, 2 * kk + q_hi), a0, a1, a2, a3);
-                mma_16816(sc[n][0], a0, a1, a2, a3, b00, b01);
-                mma_16816(sc[n][1], a0, a1, a2, a3, b10, b11);
-            }
+            for (int i = 0; i < KB; i++)
+                ldmatrix_x4(kb + tile_off(k_key, 2 * (k0 + i) + k_hi), kf[i][0], kf[i][1], kf[i][2], kf[i][3]);
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int i = 0; i < KB; i++)
+                    ldmatrix_x4(qb + n * KV_TILE + tile_off(q_row, 2 * (k0 + i) + q_hi), qf[n][i][0], qf[n][i][1],
+                                qf[n][i][2], qf[n][i][3]);
+#pragma unroll
+            for (int i = 0; i < KB; i++)
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    float (&s0)[4] = (i & 1) ? sd[n][0] : sc[n][0], (&s1)[4] = (i & 1) ? sd[n][1] : sc[n][1];
+                    mma_16816(s0, qf[n][i][0], qf[n][i][1], qf[n][i][2], qf[n][i][3], kf[i][0], kf[i][1]);
+                    mma_16816(s1, qf[n][i][0], qf[n][i][1], qf[n][i][2], qf[n][i][3], kf[i][2], kf[i][3]);
+                }
         }
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int h = 0; h < 2; h++)
+            for (int c = 0; c < 8; c++) sc[n][c >> 2][c & 3] += sd[n][c >> 2][c & 3];
+        constexpr int VB = NT == 1 ? 8 : 4;
+        uint32_t vf[VB][4];
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    float& x = sc[n][h][c];
-                    const int p = kbase + 8 * h + 2 * t + (c & 1);
-                    x = score<EXT>(a, x);
-                    if (EXT && a.slopes) {
-                        const Row& r = row[n][c >> 1];
-                        x += bias<EXT>(a, r.slope2, r.pos, whole ? p : s.pos(a, p));
-                    }
-                }
+        for (int i = 0; i < VB; i++)
+            ldmatrix_x4_trans(vb + tile_off(v_key, 2 * i + v_hi), vf[i][0], vf[i][1], vf[i][2], vf[i][3]);
+        if (EXT && a.cap_log2 > 0.f) {
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int c = 0; c < 8; c++) sc[n][c >> 2][c & 3] = score<true>(a, sc[n][c >> 2][c & 3]);
+        } else {
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int c = 0; c < 8; c++) sc[n][c >> 2][c & 3] *= a.scale_log2;
+        }
+        if (EXT && a.slopes) {
+            int kp[4] = {kbase + 2 * t, kbase + 2 * t + 1, kbase + 8 + 2 * t, kbase + 9 + 2 * t};
+            if (!whole) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) kp[i] = s.pos(a, kp[i]);
+            }
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int r = 0; r < 2; r++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        sc[n][i >> 1][2 * r + (i & 1)] += bias<true>(a, row[n][r].slope2, row[n][r].pos, kp[i]);
+        }
         uint32_t vm0 = 0xffffffffu, vm1 = 0xffffffffu;   // V rows 2t, 2t+1 / 8+2t, +1 in range
         bool odd = false;                                // masked V rows hold inf or NaN
         if (!whole) {
@@ -131,16 +163,29 @@ struct State {
             odd = __any_sync(0xffffffffu, bad != 0);
         }
         uint32_t pa[NT][4];
+        float mx[NT][2];
+        bool need = false;
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int r = 0; r < 2; r++) {
-                float mx = fmaxf(fmaxf(sc[n][0][2 * r], sc[n][0][2 * r + 1]),
-                                 fmaxf(sc[n][1][2 * r], sc[n][1][2 * r + 1]));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                if (__any_sync(0xffffffffu, mx > m[n][r] + RESCALE_THRESHOLD)) {
-                    const float mn = fmaxf(m[n][r], mx);
+            for (int r = 0; r < 2; r++)
+                mx[n][r] = fmaxf(fmaxf(sc[n][0][2 * r], sc[n][0][2 * r + 1]), fmaxf(sc[n][1][2 * r], sc[n][1][2 * r + 1]));
+#pragma unroll
+        for (int w = 1; w <= 2; w <<= 1)
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int r = 0; r < 2; r++) mx[n][r] = fmaxf(mx[n][r], __shfl_xor_sync(0xffffffffu, mx[n][r], w));
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int r = 0; r < 2; r++) need |= mx[n][r] > m[n][r] + RESCALE_THRESHOLD;
+        if (__any_sync(0xffffffffu, need)) {
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int r = 0; r < 2; r++) {
+                    const float mn = fmaxf(m[n][r], mx[n][r]);
                     const float cf = mn == -INFINITY ? 1.f : ex2(m[n][r] - mn);
                     m[n][r] = mn;
                     l[n][r] *= cf;
@@ -150,36 +195,47 @@ struct State {
                         o[n][j][2 * r + 1] *= cf;
                     }
                 }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
                 const float ms = m[n][r] == -INFINITY ? 0.f : m[n][r];   // a row that saw nothing yet
                 float p[2][2];
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     p[h][0] = ex2(sc[n][h][2 * r] - ms);
                     p[h][1] = ex2(sc[n][h][2 * r + 1] - ms);
-                    l[n][r] += p[h][0] + p[h][1];
                 }
+                l[n][r] += (p[0][0] + p[0][1]) + (p[1][0] + p[1][1]);
                 // P in fp16 for the product (2^-11 of each weight, as V's own rounding); l sums
                 // the unrounded weights
                 pa[n][r] = pack_half2(p[0][0], p[0][1]);
                 pa[n][2 + r] = pack_half2(p[1][0], p[1][1]);
             }
-        }
         if (odd) {
             by_row(s, sc, kb, kbase, lane);
             return;
         }
 #pragma unroll
-        for (int jj = 0; jj < 8; jj++) {
-            uint32_t v0, v1, v2, v3;
-            ldmatrix_x4_trans(vb + tile_off(v_key, 2 * jj + v_hi), v0, v1, v2, v3);
-            v0 &= vm0;
-            v1 &= vm1;
-            v2 &= vm0;
-            v3 &= vm1;
+        for (int j0 = 0; j0 < 8; j0 += VB) {
+            if (j0 > 0) {
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
-                mma_16816(o[n][2 * jj], pa[n][0], pa[n][1], pa[n][2], pa[n][3], v0, v1);
-                mma_16816(o[n][2 * jj + 1], pa[n][0], pa[n][1], pa[n][2], pa[n][3], v2, v3);
+                for (int i = 0; i < VB; i++)
+                    ldmatrix_x4_trans(vb + tile_off(v_key, 2 * (j0 + i) + v_hi), vf[i][0], vf[i][1], vf[i][2], vf[i][3]);
+            }
+#pragma unroll
+            for (int i = 0; i < VB; i++) {
+                const int jj = j0 + i;
+                vf[i][0] &= vm0;
+                vf[i][1] &= vm1;
+                vf[i][2] &= vm0;
+                vf[i][3] &= vm1;
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    mma_16816(o[n][2 * jj], pa[n][0], pa[n][1], pa[n][2], pa[n][3], vf[i][0], vf[i][1]);
+                    mma_16816(o[n][2 * jj + 1], pa[n][0], pa[n][1], pa[n][2], pa[n][3], vf[i][2], vf[i][3]);
+                }
             }
         }
     }
@@ -343,34 +399,51 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                         make_float2(st.o[n][j][2 * r], st.o[n][j][2 * r + 1]);
     }
     __syncthreads();
+    // join the four warps: 16 threads a row, 8 dims each
     const float* ost = reinterpret_cast<const float*>(ring);
-    for (int idx = threadIdx.x; idx < R * (D / 2); idx += THREADS) {
-        const int r = idx / (D / 2), d = 2 * (idx - r * (D / 2));
+    if (warp == CONSUMERS) return;
+#pragma unroll
+    for (int i = 0; i < NT * 2; i++) {
+        const int r = i * 8 + (threadIdx.x >> 4), d = (threadIdx.x & 15) * 4;
         if (r >= nrows) break;
-        float M = -INFINITY;
+        float M = -INFINITY, L = 0.f, sw[CONSUMERS];
 #pragma unroll
         for (int w = 0; w < CONSUMERS; w++) M = fmaxf(M, m_red[w * R + r]);
         if (M == -INFINITY) M = 0.f;             // no key seen (or only NaN scores, which stay NaN)
-        float L = 0.f, o0 = 0.f, o1 = 0.f;
+        float4 o[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
 #pragma unroll
         for (int w = 0; w < CONSUMERS; w++) {
-            const float sw = ex2(m_red[w * R + r] - M);
-            const float2 o = *reinterpret_cast<const float2*>(ost + ((size_t)w * R + r) * D + d);
-            L += l_red[w * R + r] * sw;
-            o0 += o.x * sw;
-            o1 += o.y * sw;
+            sw[w] = ex2(m_red[w * R + r] - M);
+            L += l_red[w * R + r] * sw[w];
         }
+#pragma unroll
+        for (int w = 0; w < CONSUMERS; w++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const float4 v = *reinterpret_cast<const float4*>(ost + ((size_t)w * R + r) * D + 64 * h + d);
+                o[h].x += v.x * sw[w];
+                o[h].y += v.y * sw[w];
+                o[h].z += v.z * sw[w];
+                o[h].w += v.w * sw[w];
+            }
         const float inv = L != 0.f ? 1.f / L : 0.f;
         const float lse_v = L != 0.f ? (M + lg2(L)) * LN2 : -INFINITY;
         const size_t row = (size_t)(s.q0 + r / a.G) * a.Hq + kvh * a.G + r % a.G;
-        if (a.num_chunks == 1) {
-            *reinterpret_cast<uint32_t*>(a.out + row * D + d) = pack_half2(o0 * inv, o1 * inv);
-            if (d == 0) a.lse[row] = lse_v;
-        } else {
-            const size_t slot = row * a.num_chunks + chunk;
-            // a chunk without keys for this row leaves only its lse: the merge skips it
-            if (L != 0.f) *reinterpret_cast<float2*>(a.part_o + slot * D + d) = make_float2(o0 * inv, o1 * inv);
-            if (d == 0) a.part_lse[slot] = lse_v;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            o[h].x *= inv;
+            o[h].y *= inv;
+            o[h].z *= inv;
+            o[h].w *= inv;
+            if (a.num_chunks == 1)
+                *reinterpret_cast<uint2*>(a.out + row * D + 64 * h + d) = make_uint2(pack_half2(o[h].x, o[h].y), pack_half2(o[h].z, o[h].w));
+            else if (L != 0.f)                   // a chunk without keys for this row leaves only its
+                                                 // lse: the merge skips it
+                *reinterpret_cast<float4*>(a.part_o + (row * a.num_chunks + chunk) * D + 64 * h + d) = o[h];
+        }
+        if (d == 0) {
+            if (a.num_chunks == 1) a.lse[row] = lse_v;
+            else a.part_lse[row * a.num_chunks + chunk] = lse_v;
         }
     }
 }
