@@ -6,7 +6,7 @@
 // through a TMA ring, computes S = Q K^T, an online softmax in the log2 domain and O += P V;
 // split sequences are joined by their log-sum-exps in a second kernel.
 //
-//   up to 32 rows (few drafts, single-token decode): mma.sync, four warps that take pages in
+//   up to 16 rows (few drafts, single-token decode): mma.sync, four warps that take pages in
 //   turn (`rows_kernel` here);
 //   more rows: tcgen05 on 128-row tiles (tree_tile.cu).
 
@@ -25,10 +25,8 @@ constexpr int STAGES = 8;
 static_assert(STAGES % CONSUMERS == 0, "every stage must belong to one consumer warp");
 constexpr int RING_BYTES = STAGES * STAGE_BYTES;
 
-template <int NT>
-constexpr int rows_smem() {
-    return 1024 + RING_BYTES + NT * 16 * D * 2 + 2 * STAGES * 8 + 2 * CONSUMERS * NT * 16 * 4;
-}
+constexpr int R = 16;                              // rows of the MMA tile
+constexpr int ROWS_SMEM = 1024 + RING_BYTES + KV_TILE + 2 * STAGES * 8 + 2 * CONSUMERS * R * 4;
 
 // The keys of this CTA: [beg, end), beg a multiple of 16.
 struct Keys {
@@ -41,85 +39,66 @@ struct Keys {
     }
 };
 
-// ------------------------------------------------------------------ up to 32 rows: mma.sync
-// Online-softmax state of one warp for NT tiles of 16 rows. Lane (g = lane/4, t = lane%4)
-// holds rows g and g+8 of each tile, dims 8j + 2t + {0,1} of o[j]. Q fragments come from
-// shared memory per page (for one tile they stay in registers).
-template <int NT, bool EXT>
+// ------------------------------------------------------------------ up to 16 rows: mma.sync
+// Online-softmax state of one warp for a tile of 16 rows. Lane (g = lane/4, t = lane%4) holds rows
+// g and g+8, dims 8j + 2t + {0,1} of o[j], and the fragments of Q.
+template <bool EXT>
 struct State {
-    float o[NT][16][4];
-    float m[NT][2], l[NT][2];
-    Row row[NT][2];
+    float o[16][4];
+    float m[2], l[2];
+    Row row[2];
+    uint32_t q[8][4];
 
-    __device__ __forceinline__ void reset() {
+    __device__ __forceinline__ void reset(uint32_t qb, int lane) {
+        // A fragments of Q: matrices rows 0-7 / 8-15 x dims 16kk.. / +8
+        const int q_row = (lane & 7) + (((lane >> 3) & 1) << 3), q_hi = lane >> 4;
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
+        for (int kk = 0; kk < 8; kk++)
+            ldmatrix_x4(qb + tile_off(q_row, 2 * kk + q_hi), q[kk][0], q[kk][1], q[kk][2], q[kk][3]);
 #pragma unroll
-            for (int j = 0; j < 16; j++) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
-            m[n][0] = m[n][1] = -INFINITY;
-            l[n][0] = l[n][1] = 0.f;
-        }
+        for (int j = 0; j < 16; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+        m[0] = m[1] = -INFINITY;
+        l[0] = l[1] = 0.f;
     }
 
     // Attend the page at shared address kb (K; V at kb + KV_TILE) that holds cached tokens
-    // [kbase, kbase + 16). `whole`: every row sees every key of it.
-    __device__ __forceinline__ void page(const Args& a, const Seq& s, uint32_t kb, uint32_t qb,
-                                         int kbase, bool whole, int lane) {
+    // [kbase, kbase + 16). `whole`: every row sees every key of it. A warp has its page to itself
+    // and nothing to overlap it with but its own instructions: fragments are loaded well ahead of
+    // the products, S is summed in two chains, one vote covers both rows' maxima, and branches stay
+    // out of the loops over scores (a page took 1.45 us with the loops written plainly).
+    __device__ __forceinline__ void page(const Args& a, const Seq& s, uint32_t kb, int kbase, bool whole, int lane) {
         const int t = lane & 3;
         const int k_key = (lane & 7) + ((lane >> 4) << 3), k_hi = (lane >> 3) & 1;
         const int v_key = (lane & 7) + (((lane >> 3) & 1) << 3), v_hi = lane >> 4;
-        // A fragments of Q: matrices rows 0-7 / 8-15 x dims 16kk.. / +8
-        const int q_row = (lane & 7) + (((lane >> 3) & 1) << 3), q_hi = lane >> 4;
         const uint32_t vb = kb + KV_TILE;
-
-        float sc[NT][2][4], sd[NT][2][4];        // two chains of additions, joined below
+        float sc[2][4], sd[2][4];
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+        for (int c = 0; c < 8; c++) sc[c >> 2][c & 3] = sd[c >> 2][c & 3] = 0.f;
+        {
+            uint32_t kf[8][4];
 #pragma unroll
-            for (int c = 0; c < 8; c++) sc[n][c >> 2][c & 3] = sd[n][c >> 2][c & 3] = 0.f;
-        // fragments are loaded a batch ahead of the products that use them: a warp has its page to
-        // itself, and waiting for every ldmatrix in turn took most of a page's 1.5 us
-        constexpr int KB = NT == 1 ? 8 : 4;
+            for (int i = 0; i < 8; i++)
+                ldmatrix_x4(kb + tile_off(k_key, 2 * i + k_hi), kf[i][0], kf[i][1], kf[i][2], kf[i][3]);
 #pragma unroll
-        for (int k0 = 0; k0 < 8; k0 += KB) {
-            uint32_t kf[KB][4], qf[NT][KB][4];
-#pragma unroll
-            for (int i = 0; i < KB; i++)
-                ldmatrix_x4(kb + tile_off(k_key, 2 * (k0 + i) + k_hi), kf[i][0], kf[i][1], kf[i][2], kf[i][3]);
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int i = 0; i < KB; i++)
-                    ldmatrix_x4(qb + n * KV_TILE + tile_off(q_row, 2 * (k0 + i) + q_hi), qf[n][i][0], qf[n][i][1],
-                                qf[n][i][2], qf[n][i][3]);
-#pragma unroll
-            for (int i = 0; i < KB; i++)
-#pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    float (&s0)[4] = (i & 1) ? sd[n][0] : sc[n][0], (&s1)[4] = (i & 1) ? sd[n][1] : sc[n][1];
-                    mma_16816(s0, qf[n][i][0], qf[n][i][1], qf[n][i][2], qf[n][i][3], kf[i][0], kf[i][1]);
-                    mma_16816(s1, qf[n][i][0], qf[n][i][1], qf[n][i][2], qf[n][i][3], kf[i][2], kf[i][3]);
-                }
+            for (int i = 0; i < 8; i += 2) {
+                mma_16816(sc[0], q[i][0], q[i][1], q[i][2], q[i][3], kf[i][0], kf[i][1]);
+                mma_16816(sc[1], q[i][0], q[i][1], q[i][2], q[i][3], kf[i][2], kf[i][3]);
+                mma_16816(sd[0], q[i + 1][0], q[i + 1][1], q[i + 1][2], q[i + 1][3], kf[i + 1][0], kf[i + 1][1]);
+                mma_16816(sd[1], q[i + 1][0], q[i + 1][1], q[i + 1][2], q[i + 1][3], kf[i + 1][2], kf[i + 1][3]);
+            }
         }
+        uint32_t vf[8][4];
 #pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int c = 0; c < 8; c++) sc[n][c >> 2][c & 3] += sd[n][c >> 2][c & 3];
-        constexpr int VB = NT == 1 ? 8 : 4;
-        uint32_t vf[VB][4];
-#pragma unroll
-        for (int i = 0; i < VB; i++)
+        for (int i = 0; i < 8; i++)
             ldmatrix_x4_trans(vb + tile_off(v_key, 2 * i + v_hi), vf[i][0], vf[i][1], vf[i][2], vf[i][3]);
+#pragma unroll
+        for (int c = 0; c < 8; c++) sc[c >> 2][c & 3] += sd[c >> 2][c & 3];
         if (EXT && a.cap_log2 > 0.f) {
 #pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int c = 0; c < 8; c++) sc[n][c >> 2][c & 3] = score<true>(a, sc[n][c >> 2][c & 3]);
+            for (int c = 0; c < 8; c++) sc[c >> 2][c & 3] = score<true>(a, sc[c >> 2][c & 3]);
         } else {
 #pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int c = 0; c < 8; c++) sc[n][c >> 2][c & 3] *= a.scale_log2;
+            for (int c = 0; c < 8; c++) sc[c >> 2][c & 3] *= a.scale_log2;
         }
         if (EXT && a.slopes) {
             int kp[4] = {kbase + 2 * t, kbase + 2 * t + 1, kbase + 8 + 2 * t, kbase + 9 + 2 * t};
@@ -128,145 +107,107 @@ struct State {
                 for (int i = 0; i < 4; i++) kp[i] = s.pos(a, kp[i]);
             }
 #pragma unroll
-            for (int n = 0; n < NT; n++)
+            for (int r = 0; r < 2; r++)
 #pragma unroll
-                for (int r = 0; r < 2; r++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        sc[n][i >> 1][2 * r + (i & 1)] += bias<true>(a, row[n][r].slope2, row[n][r].pos, kp[i]);
+                for (int i = 0; i < 4; i++) sc[i >> 1][2 * r + (i & 1)] += bias<true>(a, row[r].slope2, row[r].pos, kp[i]);
         }
-        uint32_t vm0 = 0xffffffffu, vm1 = 0xffffffffu;   // V rows 2t, 2t+1 / 8+2t, +1 in range
         bool odd = false;                                // masked V rows hold inf or NaN
         if (!whole) {
 #pragma unroll
-            for (int n = 0; n < NT; n++)
+            for (int h = 0; h < 2; h++)
 #pragma unroll
-                for (int h = 0; h < 2; h++)
-#pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        const int p = kbase + 8 * h + 2 * t + (c & 1);
-                        if (p >= s.len || !row[n][c >> 1].sees(a, s, p, s.pos(a, p))) sc[n][h][c] = -INFINITY;
-                    }
-            // 0 * inf is NaN in the product: rows behind the sequence are zeroed, and where
-            // another row is not finite the page is summed row by row below
+                for (int c = 0; c < 4; c++) {
+                    const int p = kbase + 8 * h + 2 * t + (c & 1);
+                    if (p >= s.len || !row[c >> 1].sees(a, s, p, s.pos(a, p))) sc[h][c] = -INFINITY;
+                }
+            // 0 * inf is NaN in the product: rows behind the sequence are zeroed, and where another
+            // row is not finite the page is summed row by row below
             const int left = s.len - kbase;
             auto keep = [&](int k) { return (k < left ? 0xffffu : 0u) | (k + 1 < left ? 0xffff0000u : 0u); };
-            vm0 = keep(2 * t);
-            vm1 = keep(8 + 2 * t);
+            const uint32_t vm0 = keep(2 * t), vm1 = keep(8 + 2 * t);
             uint32_t bad = 0;
 #pragma unroll
-            for (int jj = 0; jj < 8; jj++) {
-                uint32_t v0, v1, v2, v3;
-                ldmatrix_x4_trans(vb + tile_off(v_key, 2 * jj + v_hi), v0, v1, v2, v3);
-                bad |= not_finite(v0 & vm0) | not_finite(v1 & vm1) | not_finite(v2 & vm0) | not_finite(v3 & vm1);
+            for (int i = 0; i < 8; i++) {
+                vf[i][0] &= vm0;
+                vf[i][1] &= vm1;
+                vf[i][2] &= vm0;
+                vf[i][3] &= vm1;
+                bad |= not_finite(vf[i][0]) | not_finite(vf[i][1]) | not_finite(vf[i][2]) | not_finite(vf[i][3]);
             }
             odd = __any_sync(0xffffffffu, bad != 0);
         }
-        uint32_t pa[NT][4];
-        float mx[NT][2];
-        bool need = false;
+        float mx[2];
 #pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int r = 0; r < 2; r++)
-                mx[n][r] = fmaxf(fmaxf(sc[n][0][2 * r], sc[n][0][2 * r + 1]), fmaxf(sc[n][1][2 * r], sc[n][1][2 * r + 1]));
+        for (int r = 0; r < 2; r++)
+            mx[r] = fmaxf(fmaxf(sc[0][2 * r], sc[0][2 * r + 1]), fmaxf(sc[1][2 * r], sc[1][2 * r + 1]));
 #pragma unroll
         for (int w = 1; w <= 2; w <<= 1)
 #pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int r = 0; r < 2; r++) mx[n][r] = fmaxf(mx[n][r], __shfl_xor_sync(0xffffffffu, mx[n][r], w));
-#pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int r = 0; r < 2; r++) need |= mx[n][r] > m[n][r] + RESCALE_THRESHOLD;
-        if (__any_sync(0xffffffffu, need)) {
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int r = 0; r < 2; r++) {
-                    const float mn = fmaxf(m[n][r], mx[n][r]);
-                    const float cf = mn == -INFINITY ? 1.f : ex2(m[n][r] - mn);
-                    m[n][r] = mn;
-                    l[n][r] *= cf;
-#pragma unroll
-                    for (int j = 0; j < 16; j++) {
-                        o[n][j][2 * r] *= cf;
-                        o[n][j][2 * r + 1] *= cf;
-                    }
-                }
-        }
-#pragma unroll
-        for (int n = 0; n < NT; n++)
+            for (int r = 0; r < 2; r++) mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], w));
+        if (__any_sync(0xffffffffu, mx[0] > m[0] + RESCALE_THRESHOLD || mx[1] > m[1] + RESCALE_THRESHOLD)) {
 #pragma unroll
             for (int r = 0; r < 2; r++) {
-                const float ms = m[n][r] == -INFINITY ? 0.f : m[n][r];   // a row that saw nothing yet
-                float p[2][2];
+                const float mn = fmaxf(m[r], mx[r]);
+                const float cf = mn == -INFINITY ? 1.f : ex2(m[r] - mn);
+                m[r] = mn;
+                l[r] *= cf;
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    p[h][0] = ex2(sc[n][h][2 * r] - ms);
-                    p[h][1] = ex2(sc[n][h][2 * r + 1] - ms);
+                for (int j = 0; j < 16; j++) {
+                    o[j][2 * r] *= cf;
+                    o[j][2 * r + 1] *= cf;
                 }
-                l[n][r] += (p[0][0] + p[0][1]) + (p[1][0] + p[1][1]);
-                // P in fp16 for the product (2^-11 of each weight, as V's own rounding); l sums
-                // the unrounded weights
-                pa[n][r] = pack_half2(p[0][0], p[0][1]);
-                pa[n][2 + r] = pack_half2(p[1][0], p[1][1]);
             }
+        }
+        uint32_t pa[4];
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+            const float ms = m[r] == -INFINITY ? 0.f : m[r];     // a row that saw nothing yet
+            float p[2][2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                p[h][0] = ex2(sc[h][2 * r] - ms);
+                p[h][1] = ex2(sc[h][2 * r + 1] - ms);
+            }
+            l[r] += (p[0][0] + p[0][1]) + (p[1][0] + p[1][1]);
+            // P in fp16 for the product (2^-11 of each weight, as V's own rounding); l sums the
+            // unrounded weights
+            pa[r] = pack_half2(p[0][0], p[0][1]);
+            pa[2 + r] = pack_half2(p[1][0], p[1][1]);
+        }
         if (odd) {
             by_row(s, sc, kb, kbase, lane);
             return;
         }
 #pragma unroll
-        for (int j0 = 0; j0 < 8; j0 += VB) {
-            if (j0 > 0) {
-#pragma unroll
-                for (int i = 0; i < VB; i++)
-                    ldmatrix_x4_trans(vb + tile_off(v_key, 2 * (j0 + i) + v_hi), vf[i][0], vf[i][1], vf[i][2], vf[i][3]);
-            }
-#pragma unroll
-            for (int i = 0; i < VB; i++) {
-                const int jj = j0 + i;
-                vf[i][0] &= vm0;
-                vf[i][1] &= vm1;
-                vf[i][2] &= vm0;
-                vf[i][3] &= vm1;
-#pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    mma_16816(o[n][2 * jj], pa[n][0], pa[n][1], pa[n][2], pa[n][3], vf[i][0], vf[i][1]);
-                    mma_16816(o[n][2 * jj + 1], pa[n][0], pa[n][1], pa[n][2], pa[n][3], vf[i][2], vf[i][3]);
-                }
-            }
+        for (int i = 0; i < 8; i++) {
+            mma_16816(o[2 * i], pa[0], pa[1], pa[2], pa[3], vf[i][0], vf[i][1]);
+            mma_16816(o[2 * i + 1], pa[0], pa[1], pa[2], pa[3], vf[i][2], vf[i][3]);
         }
     }
 
     // O += P V of a masked page whose V is not finite everywhere, key by key: a key that a row
     // does not see (score -inf) is skipped for it.
-    __device__ __forceinline__ void by_row(const Seq& s, const float (&sc)[NT][2][4], uint32_t kb,
-                                        int kbase, int lane) {
+    __device__ __forceinline__ void by_row(const Seq& s, const float (&sc)[2][4], uint32_t kb, int kbase, int lane) {
         const int t = lane & 3;
 #pragma unroll 1
         for (int k = 0; k < PAGE && kbase + k < s.len; k++) {
             const int src = (lane & ~3) | ((k & 7) >> 1);
 #pragma unroll
-            for (int n = 0; n < NT; n++)
+            for (int r = 0; r < 2; r++) {
+                const int c = 2 * r;
+                const float mine = k < 8 ? ((k & 1) ? sc[0][c + 1] : sc[0][c]) : ((k & 1) ? sc[1][c + 1] : sc[1][c]);
+                const float x = __shfl_sync(0xffffffffu, mine, src);
+                if (x == -INFINITY) continue;
+                const float p = ex2(x - m[r]);
 #pragma unroll
-                for (int r = 0; r < 2; r++) {
-                    const int c = 2 * r;
-                    const float mine = k < 8 ? ((k & 1) ? sc[n][0][c + 1] : sc[n][0][c])
-                                             : ((k & 1) ? sc[n][1][c + 1] : sc[n][1][c]);
-                    const float x = __shfl_sync(0xffffffffu, mine, src);
-                    if (x == -INFINITY) continue;
-                    const float p = ex2(x - m[n][r]);
-#pragma unroll
-                    for (int j = 0; j < 16; j++) {
-                        uint32_t v;
-                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(kb + KV_TILE + tile_off(k, j) + 4 * t));
-                        const __half2 hv = *reinterpret_cast<__half2*>(&v);
-                        o[n][j][c] = fmaf(p, __low2float(hv), o[n][j][c]);
-                        o[n][j][c + 1] = fmaf(p, __high2float(hv), o[n][j][c + 1]);
-                    }
+                for (int j = 0; j < 16; j++) {
+                    uint32_t v;
+                    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(kb + KV_TILE + tile_off(k, j) + 4 * t));
+                    const __half2 hv = *reinterpret_cast<__half2*>(&v);
+                    o[j][c] = fmaf(p, __low2float(hv), o[j][c]);
+                    o[j][c + 1] = fmaf(p, __high2float(hv), o[j][c + 1]);
                 }
+            }
         }
     }
 
@@ -276,14 +217,13 @@ struct State {
 };
 
 // grid = (B * Hkv, num_chunks).
-template <int NT, bool EXT>
+template <bool EXT>
 __global__ void __launch_bounds__(THREADS, 2)
 rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const Args a) {
-    constexpr int R = 16 * NT;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* ring = align_ptr<1024>(smem_raw);
-    uint8_t* qs = ring + RING_BYTES;                                    // NT tiles, swizzled like a page
-    uint64_t* full = reinterpret_cast<uint64_t*>(qs + NT * KV_TILE);
+    uint8_t* qs = ring + RING_BYTES;                                    // swizzled like a page
+    uint64_t* full = reinterpret_cast<uint64_t*>(qs + KV_TILE);
     uint64_t* empty = full + STAGES;
     float* m_red = reinterpret_cast<float*>(empty + STAGES);            // [CONSUMERS][R]
     float* l_red = m_red + CONSUMERS * R;
@@ -316,7 +256,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
     const int p0 = keys.beg / PAGE;
     const int npg = keys.end > keys.beg ? (keys.end - keys.beg + PAGE - 1) / PAGE : 0;
 
-    State<NT, EXT> st;
+    State<EXT> st;
     const int g = lane >> 2, t = lane & 3;
     if (warp == CONSUMERS) {
         const uint64_t pol = policy_evict_first();
@@ -353,14 +293,12 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
             if (rr < nrows)
                 v = __ldg(reinterpret_cast<const uint4*>(
                         a.q + ((size_t)(s.q0 + rr / a.G) * a.Hq + kvh * a.G + rr % a.G) * D) + cd);
-            *reinterpret_cast<uint4*>(qs + (rr >> 4) * KV_TILE + tile_off(rr & 15, cd)) = v;
+            *reinterpret_cast<uint4*>(qs + tile_off(rr, cd)) = v;
         }
         asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS * 32) : "memory");
 #pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int r = 0; r < 2; r++) st.row[n][r].set(a, s, 16 * n + 8 * r + g, nrows, kvh);
-        st.reset();
+        for (int r = 0; r < 2; r++) st.row[r].set(a, s, 8 * r + g, nrows, kvh);
+        st.reset(smem_u32(qs), lane);
         bool ok = true;
         for (int i = warp; i < npg; i += CONSUMERS) {
             const int sg = i % STAGES;
@@ -368,42 +306,38 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
             if (!__all_sync(0xffffffffu, got)) { ok = false; break; }
             const int kbase = (p0 + i) * PAGE;
             const bool whole = kbase + PAGE <= s.ctx && (a.window <= 0 || (long long)pos_hi - kbase < a.window);
-            st.page(a, s, smem_u32(ring + sg * STAGE_BYTES), smem_u32(qs), kbase, whole, lane);
+            st.page(a, s, smem_u32(ring + sg * STAGE_BYTES), kbase, whole, lane);
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty[sg]);
         }
 #pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int r = 0; r < 2; r++) {
-                float l = st.l[n][r];
-                l += __shfl_xor_sync(0xffffffffu, l, 1);
-                l += __shfl_xor_sync(0xffffffffu, l, 2);
-                if (t == 0) {
-                    m_red[warp * R + 16 * n + 8 * r + g] = ok ? st.m[n][r] : -INFINITY;
-                    l_red[warp * R + 16 * n + 8 * r + g] = ok ? l : 0.f;
-                }
+        for (int r = 0; r < 2; r++) {
+            float l = st.l[r];
+            l += __shfl_xor_sync(0xffffffffu, l, 1);
+            l += __shfl_xor_sync(0xffffffffu, l, 2);
+            if (t == 0) {
+                m_red[warp * R + 8 * r + g] = ok ? st.m[r] : -INFINITY;
+                l_red[warp * R + 8 * r + g] = ok ? l : 0.f;
             }
+        }
     }
     // all consumers are done with the ring and every copy has landed: it holds the warps' O now
     __syncthreads();
     if (warp < CONSUMERS) {
         float* ost = reinterpret_cast<float*>(ring);   // [CONSUMERS][R][128]
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+        for (int r = 0; r < 2; r++)
 #pragma unroll
-            for (int r = 0; r < 2; r++)
-#pragma unroll
-                for (int j = 0; j < 16; j++)
-                    *reinterpret_cast<float2*>(ost + ((size_t)warp * R + 16 * n + 8 * r + g) * D + 8 * j + 2 * t) =
-                        make_float2(st.o[n][j][2 * r], st.o[n][j][2 * r + 1]);
+            for (int j = 0; j < 16; j++)
+                *reinterpret_cast<float2*>(ost + ((size_t)warp * R + 8 * r + g) * D + 8 * j + 2 * t) =
+                    make_float2(st.o[j][2 * r], st.o[j][2 * r + 1]);
     }
     __syncthreads();
     // join the four warps: 16 threads a row, 8 dims each
     const float* ost = reinterpret_cast<const float*>(ring);
     if (warp == CONSUMERS) return;
 #pragma unroll
-    for (int i = 0; i < NT * 2; i++) {
+    for (int i = 0; i < R / 8; i++) {
         const int r = i * 8 + (threadIdx.x >> 4), d = (threadIdx.x & 15) * 4;
         if (r >= nrows) break;
         float M = -INFINITY, L = 0.f, sw[CONSUMERS];
@@ -546,11 +480,7 @@ mask_kernel(const int* parents, const int* q_indptr, const int* indptr, const in
 }
 
 // ------------------------------------------------------------------ host
-const void* rows_fn(int NT, bool ext) {
-    if (NT == 1) return ext ? (const void*)rows_kernel<1, true> : (const void*)rows_kernel<1, false>;
-    return ext ? (const void*)rows_kernel<2, true> : (const void*)rows_kernel<2, false>;
-}
-size_t rows_bytes(int NT) { return NT == 1 ? rows_smem<1>() : rows_smem<2>(); }
+const void* rows_fn(bool ext) { return ext ? (const void*)rows_kernel<true> : (const void*)rows_kernel<false>; }
 
 struct Setup {
     ckl_status st = CKL_OK;
@@ -561,17 +491,12 @@ const Setup* setup(const DeviceInfo* di) {
     std::call_once(once[di->device], [di] {
         Setup& k = ks[di->device];
         cudaError_t e = cudaSuccess;
-        for (int NT = 1; NT <= 2 && e == cudaSuccess; NT++)
-            for (int ext = 0; ext < 2 && e == cudaSuccess; ext++)
-                e = cudaFuncSetAttribute(rows_fn(NT, ext), cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)rows_bytes(NT));
+        for (int ext = 0; ext < 2 && e == cudaSuccess; ext++)
+            e = cudaFuncSetAttribute(rows_fn(ext), cudaFuncAttributeMaxDynamicSharedMemorySize, ROWS_SMEM);
         if (e != cudaSuccess) k.st = cuda_status(e, "tree attention setup");
     });
     return &ks[di->device];
 }
-
-// Row tiles per CTA of the mma.sync kernel.
-int row_tiles(int rows) { return rows <= 16 ? 1 : 2; }
 
 ckl_status check_params(const ckl_tree_params* p, const char* who) {
     if (!p) return fail(CKL_INVALID_ARG, "%s: params is NULL", who);
@@ -643,9 +568,10 @@ ckl_status check_split(const ckl_tree_params* p) {
     return CKL_OK;
 }
 
-// More rows than the mma.sync kernel takes: a 16-row tile there re-reads every page, which holds
-// up to 32 rows; the tcgen05 kernel spends a 128-row tile on any number.
-bool use_tiles(const ckl_tree_params* p) { return (long long)p->max_q * (p->Hq / p->Hkv) > 32; }
+// More rows than an m16 tile holds go to the tcgen05 kernel, which spends a 128-row tile on any
+// number. At 24 rows a second m16 tile per warp (32 rows) against it, in us: 1 x 1000 keys 17.9 / 15.9,
+// 1 x 4000 17.2 / 21.1, 1 x 30000 45.6 / 40.3, 8 x 4000 54.6 / 39.5, 8 x 16384 167 / 100.
+bool use_tiles(long long rows) { return rows > R; }
 
 // CTAs of the tcgen05 kernel: num_chunks for each unit (sequence, kv head, row group), one wave
 // at most.
@@ -682,11 +608,12 @@ ckl_status ckl_tree_plan(int G, int B, int Hkv, int max_q, int max_len, int wind
         const DeviceInfo* di = device_info();
         if (!di) return CKL_CUDA_ERROR;
         const long long rows = (long long)max_q * G;
-        const long long per = rows > 32 ? 128LL * tile_count(rows) : 16LL * row_tiles((int)rows);
+        const bool tiles = use_tiles(rows);
+        const long long per = tiles ? 128LL * tile_count(rows) : R;
         const long long units = (long long)B * Hkv * ((rows + per - 1) / per);
-        // two resident CTAs per SM up to 32 rows; the tcgen05 kernel takes the SM, and divides
+        // two resident CTAs per SM up to 16 rows; the tcgen05 kernel takes the SM, and divides
         // the work of all units evenly over its CTAs whatever the chunks are
-        const long long want = rows > 32 ? (di->sms + units - 1) / units : 2LL * di->sms / units;
+        const long long want = tiles ? (di->sms + units - 1) / units : 2LL * di->sms / units;
         chunks = std::min(std::max(1LL, want), (len + 255) / 256);
     }
     chunks = std::min(chunks, 65535LL);
@@ -698,7 +625,7 @@ ckl_status ckl_tree_plan(int G, int B, int Hkv, int max_q, int max_len, int wind
 
 size_t ckl_tree_workspace_size(const ckl_tree_params* p) {
     if (!p || p->N <= 0 || p->B <= 0) return 0;
-    if (p->Hq > 0 && p->Hkv > 0 && p->max_q > 0 && p->num_chunks > 0 && use_tiles(p)) {
+    if (p->Hq > 0 && p->Hkv > 0 && p->max_q > 0 && p->num_chunks > 0 && use_tiles((long long)p->max_q * (p->Hq / p->Hkv))) {
         const DeviceInfo* di = device_info();
         if (!di) return SIZE_MAX;
         return tile_workspace(tile_ctas(p, di->sms), (long long)p->max_q * (p->Hq / p->Hkv));
@@ -740,15 +667,14 @@ ckl_status ckl_tree_attention(const ckl_tree_params* p, void* out, float* lse, v
         a.part_lse = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + part_o_size(p));
     }
     const cudaStream_t s = (cudaStream_t)stream;
-    if (use_tiles(p)) return launch_tiles(p, a, workspace, tile_ctas(p, di->sms), s);
-    const int NT = row_tiles(p->max_q * a.G);
+    if (use_tiles((long long)p->max_q * (p->Hq / p->Hkv))) return launch_tiles(p, a, workspace, tile_ctas(p, di->sms), s);
     const bool ext = p->softcap > 0.f || p->slopes;
     CUtensorMap tmK, tmV;
     st = encode_page_maps(p->k_cache, p->v_cache, p->Hkv, p->num_pages, &tmK, &tmV);
     if (st != CKL_OK) return st;
     void* args[] = {&tmK, &tmV, &a};
-    CKL_CUDA_TRY(launch(rows_fn(NT, ext), dim3((unsigned)(p->B * p->Hkv), (unsigned)p->num_chunks),
-                        dim3(THREADS), rows_bytes(NT), s, args, true));
+    CKL_CUDA_TRY(launch(rows_fn(ext), dim3((unsigned)(p->B * p->Hkv), (unsigned)p->num_chunks),
+                        dim3(THREADS), ROWS_SMEM, s, args, true));
     if (p->num_chunks == 1) return CKL_OK;
     void* margs[] = {&a};
     const long long mrows = (long long)p->max_q * p->Hq;

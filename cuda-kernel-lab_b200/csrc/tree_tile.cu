@@ -715,13 +715,17 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
 }
 
 // Joins the units that more than one CTA worked on. A CTA takes 32 rows of a unit at a time: the
-// lanes are the rows (a partial's rows lie side by side), a warp has 16 of the dims, and the
-// result goes through shared memory so that whole rows are written. grid = (row parts, B).
-template <int MT>
+// lanes are the rows (a partial's rows lie side by side), and the result goes through shared memory
+// so that whole rows are written. Its eight warps have 16 of the dims each; with SPLIT (few rows,
+// each in many pieces) they share the pieces of one such 16 between them, and a row's dims are
+// eight CTAs' work. grid = (row parts (* 8), B).
+template <int MT, bool SPLIT>
 __global__ void __launch_bounds__(256) tile_merge_kernel(const Args a, int ctas) {
     constexpr int ROWS = Cfg<MT>::ROWS;
     __shared__ long long s_before, s_all;
-    __shared__ uint2 s_out[32][D / 4 + 1];
+    __shared__ uint2 s_out[SPLIT ? 1 : 32][D / 4 + 1];
+    __shared__ float4 s_acc[SPLIT ? 8 : 1][4][32];
+    __shared__ float s_w[8][32];
     pdl_wait();
     pdl_trigger();
     const int b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -736,8 +740,10 @@ __global__ void __launch_bounds__(256) tile_merge_kernel(const Args a, int ctas)
     if (s.T > a.max_q && blockIdx.x == 0 && threadIdx.x == 0) atomicOr(a.err, DEVERR_BOUND);
     __syncthreads();
     const Share sh(s_all, ctas);
-    const int parts = (w.nrows + 31) / 32, total = parts * a.Hkv;         // 32 rows of one kv head
-    for (int x = blockIdx.x; x < total; x += gridDim.x) {
+    const int parts = (w.nrows + 31) / 32, total = parts * a.Hkv * (SPLIT ? 8 : 1);   // 32 rows of one kv head
+    const int c_first = SPLIT ? warp : 0, c_step = SPLIT ? 8 : 1;
+    for (int y = blockIdx.x; y < total; y += gridDim.x) {
+        const int x = SPLIT ? y >> 3 : y, dims = SPLIT ? y & 7 : warp;
         const int kvh = x / parts, row0 = (x - kvh * parts) * 32, z = row0 / ROWS;
         const long long u0 = s_before + (long long)(z * a.Hkv + kvh) * w.nblk;
         const int c0 = sh.owner(u0), c1 = sh.owner(u0 + w.nblk - 1);
@@ -746,50 +752,76 @@ __global__ void __launch_bounds__(256) tile_merge_kernel(const Args a, int ctas)
         auto slot = [&](int c) { return ((size_t)c * 2 + (c == c0)) * ROWS; };
         float m = -INFINITY;
         bool nan = false;
-#pragma unroll 4
+#pragma unroll 8
         for (int c = c0; c <= c1; c++) {
-            const float y = rr < w.nrows ? a.part_lse[slot(c) + r] : -INFINITY;
-            nan |= y != y;
-            m = fmaxf(m, y);
+            const float v = rr < w.nrows ? a.part_lse[slot(c) + r] : -INFINITY;
+            nan |= v != v;
+            m = fmaxf(m, v);
         }
         const bool any = m != -INFINITY || nan;
         float4 acc[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         float ws = 0.f;
-#pragma unroll 2
-        for (int c = c0; c <= c1; c++) {
-            const float y = rr < w.nrows ? a.part_lse[slot(c) + r] : -INFINITY;
-            const float e = any && y != -INFINITY ? ex2((y - m) * LOG2E) : 0.f;
+#pragma unroll 4
+        for (int c = c0 + c_first; c <= c1; c += c_step) {
+            const float v = rr < w.nrows ? a.part_lse[slot(c) + r] : -INFINITY;
+            const float e = any && v != -INFINITY ? ex2((v - m) * LOG2E) : 0.f;
             ws += e;
-            const float4* po = reinterpret_cast<const float4*>(a.part_o) + slot(c) * (D / 4) + (warp * 4) * ROWS + r;
-            if (e != 0.f) {
+            const float4* po = reinterpret_cast<const float4*>(a.part_o) + slot(c) * (D / 4) + (dims * 4) * ROWS + r;
+            if (e != 0.f) {                                       // nothing to add, and maybe nothing written
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const float4 v = po[i * ROWS];
-                    acc[i].x += e * v.x;
-                    acc[i].y += e * v.y;
-                    acc[i].z += e * v.z;
-                    acc[i].w += e * v.w;
+                    const float4 o = po[i * ROWS];
+                    acc[i].x += e * o.x;
+                    acc[i].y += e * o.y;
+                    acc[i].z += e * o.z;
+                    acc[i].w += e * o.w;
                 }
             }
         }
-        const float inv = ws != 0.f ? 1.f / ws : 0.f;
-        __syncthreads();                                          // the rows before are written
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            s_out[lane][warp * 4 + i] = make_uint2(pack_half2(acc[i].x * inv, acc[i].y * inv),
-                                                   pack_half2(acc[i].z * inv, acc[i].w * inv));
         auto orow = [&](int row) {
             const int i = row / a.G;
             return (size_t)(s.q0 + i) * a.Hq + kvh * a.G + (row - i * a.G);
         };
+        __syncthreads();                                          // the rows before are written
+        if (SPLIT) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) s_acc[SPLIT ? warp : 0][i][lane] = acc[i];
+            s_w[warp][lane] = ws;
+            __syncthreads();
+            if (warp < 4) {                                       // four of the dims each, warps in order
+                float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+                ws = 0.f;
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const float4 o = s_acc[SPLIT ? k : 0][warp][lane];
+                    t.x += o.x;
+                    t.y += o.y;
+                    t.z += o.z;
+                    t.w += o.w;
+                    ws += s_w[k][lane];
+                }
+                const float inv = ws != 0.f ? 1.f / ws : 0.f;
+                if (rr < w.nrows) {
+                    reinterpret_cast<uint2*>(a.out + orow(rr) * D)[dims * 4 + warp] =
+                        make_uint2(pack_half2(t.x * inv, t.y * inv), pack_half2(t.z * inv, t.w * inv));
+                    if (dims == 0 && warp == 0) a.lse[orow(rr)] = ws != 0.f ? m + logf(ws) : -INFINITY;
+                }
+            }
+            continue;
+        }
+        const float inv = ws != 0.f ? 1.f / ws : 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            s_out[SPLIT ? 0 : lane][warp * 4 + i] = make_uint2(pack_half2(acc[i].x * inv, acc[i].y * inv),
+                                                               pack_half2(acc[i].z * inv, acc[i].w * inv));
         if (warp == 0 && rr < w.nrows) a.lse[orow(rr)] = ws != 0.f ? m + logf(ws) : -INFINITY;
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int q = warp * 4 + i;
-            if (row0 + q < w.nrows) reinterpret_cast<uint2*>(a.out + orow(row0 + q) * D)[lane] = s_out[q][lane];
+            if (row0 + q < w.nrows) reinterpret_cast<uint2*>(a.out + orow(row0 + q) * D)[lane] = s_out[SPLIT ? 0 : q][lane];
         }
     }
 }
@@ -871,9 +903,13 @@ ckl_status launch_tiles(const ckl_tree_params* p, Args a, void* workspace, int c
                         s, args, true));
     void* margs[] = {&a, &ctas};
     const long long parts = ((long long)p->max_q * a.G + 31) / 32 * p->Hkv;
-    const unsigned gx = (unsigned)std::max(1LL, std::min(parts, (long long)(8 * di->sms + p->B - 1) / p->B));
-    CKL_CUDA_TRY(launch(MT == 1 ? (const void*)tile_merge_kernel<1> : (const void*)tile_merge_kernel<2>,
-                        dim3(gx, (unsigned)p->B), dim3(256), 0, s, margs, true));
+    // few rows in many pieces each: split the pieces too
+    const bool split = parts * p->B < di->sms;
+    const long long want = split ? parts * 8 : parts;
+    const unsigned gx = (unsigned)std::max(1LL, std::min(want, (long long)(8 * di->sms + p->B - 1) / p->B));
+    const void* fn = MT == 1 ? (split ? (const void*)tile_merge_kernel<1, true> : (const void*)tile_merge_kernel<1, false>)
+                             : (split ? (const void*)tile_merge_kernel<2, true> : (const void*)tile_merge_kernel<2, false>);
+    CKL_CUDA_TRY(launch(fn, dim3(gx, (unsigned)p->B), dim3(256), 0, s, margs, true));
     return CKL_OK;
 }
 
