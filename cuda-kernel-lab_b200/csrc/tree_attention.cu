@@ -601,7 +601,7 @@ ckl_status ckl_tree_plan(int G, int B, int Hkv, int max_q, int max_len, int wind
     long long len = max_len;
     if (window > 0) len = std::min(len, (long long)window + max_q + 2 * PAGE);
     len = std::max(len, 1LL);
-    long long chunks;
+    long long chunks, unit_keys = PAGE;
     if (force_chunks > 0) {
         chunks = force_chunks;
     } else {
@@ -611,13 +611,30 @@ ckl_status ckl_tree_plan(int G, int B, int Hkv, int max_q, int max_len, int wind
         const bool tiles = use_tiles(rows);
         const long long per = tiles ? 128LL * tile_count(rows) : R;
         const long long units = (long long)B * Hkv * ((rows + per - 1) / per);
-        // two resident CTAs per SM up to 16 rows; the tcgen05 kernel takes the SM, and divides
-        // the work of all units evenly over its CTAs whatever the chunks are
-        const long long want = tiles ? (di->sms + units - 1) / units : 2LL * di->sms / units;
-        chunks = std::min(std::max(1LL, want), (len + 255) / 256);
+        if (tiles) {
+            // One CTA per SM. In blocks of 128 keys: the CTA's share, 2 more for a join, 2 more
+            // where the shares do not end with the units (a second segment's start and end). All
+            // SMs are taken when the work is long; short work is cut where units divide evenly (at
+            // 24 rows, 1 x 1000 keys: 8 x 1 blocks 14.4 us, 4 x 2 16.5 us; 4 x 600 keys: 1 x 5
+            // blocks 17.8 us, 3 pieces 21 us; 8 x 8000 keys: 2 pieces 61 us, 148 shares 58.8 us).
+            const long long blocks = (len + 127) / 128, most = std::min(di->sms / units, blocks);
+            double best = (double)blocks * units / di->sms + 4.0;
+            chunks = (di->sms + units - 1) / units;
+            for (long long n = 1; n <= std::max(most, 1LL); n++) {
+                const double cost = (double)((blocks + n - 1) / n) + (blocks % n ? 2.0 : 0.0) + (n > 1 ? 2.0 : 0.0);
+                if (units * n <= di->sms && cost < best) {
+                    best = cost;
+                    chunks = n;
+                }
+            }
+        } else {
+            // two resident CTAs per SM, about one wave; a page per warp at least
+            chunks = std::min(std::max(1LL, 2LL * di->sms / units), (len + 4 * PAGE - 1) / (4 * PAGE));
+            unit_keys = 4 * PAGE;
+        }
     }
     chunks = std::min(chunks, 65535LL);
-    const long long tok = (((len + chunks - 1) / chunks) + PAGE - 1) / PAGE * PAGE;
+    const long long tok = (((len + chunks - 1) / chunks) + unit_keys - 1) / unit_keys * unit_keys;
     *chunk_tokens = (int)std::min(tok, (long long)(INT_MAX / PAGE) * PAGE);
     *num_chunks = (int)((len + *chunk_tokens - 1) / *chunk_tokens);
     return CKL_OK;
