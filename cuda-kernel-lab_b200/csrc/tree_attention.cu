@@ -557,6 +557,7 @@ ckl_status fill_args(const ckl_tree_params* p, Args* a) {
     if (p->softcap > 0.f) {
         a->cap_log2 = p->softcap * LOG2E;
         a->cap_in = 2.f * LOG2E * p->sm_scale / p->softcap;
+        a->cap_k = p->sm_scale / p->softcap;
     }
     return CKL_OK;
 }

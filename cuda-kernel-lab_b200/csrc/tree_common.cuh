@@ -29,6 +29,7 @@ struct Args {
     float scale_log2;         // sm_scale * log2(e)
     float cap_log2;           // softcap * log2(e), 0: no cap
     float cap_in;             // 2 log2(e) sm_scale / softcap
+    float cap_k;              // sm_scale / softcap
     int q_tma;                // the tcgen05 kernel reads Q tiles through a tensor map
 };
 
@@ -133,43 +134,43 @@ __device__ __forceinline__ float score(const Args& a, float qk) {
     return qk * a.scale_log2;
 }
 constexpr float C0 = 0.999999642f, C1 = -0.333312094f, C2 = 0.132992104f, C3 = -0.0516967401f, C4 = 0.014976955f;   // tanh(y)/y in y^2
-// The scores of 32 products that one thread holds. Capped scores are nearly always far below the
-// cap: up to 0.6 of it tanh(y) = y P(y^2) with P of degree 4 (fitted here to tanh(y)/y by weighted
-// least squares; off by at most 2^-25 of the cap), eight operations on two values each in place
-// of two of the special-function unit, which the exponentials already fill.
+// Capped scores are nearly always far below the cap: up to CAP_SMALL of it tanh(y) = y P(y^2) with
+// P of degree 4 (fitted here to tanh(y)/y by weighted least squares; off by at most 2^-25 of the
+// cap), seven operations on two values each in place of two of the special-function unit, which
+// the exponentials already fill.
+constexpr float CAP_SMALL = 0.6f;
+// P for two products q.k.
+__device__ __forceinline__ float2 cap_factor2(const Args& a, float2 qk) {
+    const float2 y = mul2(qk, make_float2(a.cap_k, a.cap_k)), t = mul2(y, y);
+    float2 p = fma2(make_float2(C4, C4), t, make_float2(C3, C3));
+    p = fma2(p, t, make_float2(C2, C2));
+    p = fma2(p, t, make_float2(C1, C1));
+    return fma2(p, t, make_float2(C0, C0));
+}
+// The scores of 32 products that one thread holds.
 template <bool EXT>
 __device__ __forceinline__ void score32(const Args& a, float (&x)[32]) {
     const float2 sc = make_float2(a.scale_log2, a.scale_log2);
+    bool capped = false;
     if (EXT && a.cap_log2 > 0.f) {
-        const float k = a.cap_in * (0.5f * LN2);                  // sm_scale / softcap
         float m4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < 32; c++) m4[c & 3] = fmaxf(m4[c & 3], fabsf(x[c]));
-        const float top = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * k;
-        if (!__any_sync(0xffffffffu, !(top <= 0.6f))) {
-            const float2 k2 = make_float2(k, k);
-#pragma unroll
-            for (int c = 0; c < 32; c += 2) {
-                const float2 v = make_float2(x[c], x[c + 1]), y = mul2(v, k2), t = mul2(y, y);
-                float2 p = fma2(make_float2(C4, C4), t, make_float2(C3, C3));
-                p = fma2(p, t, make_float2(C2, C2));
-                p = fma2(p, t, make_float2(C1, C1));
-                p = fma2(p, t, make_float2(C0, C0));
-                const float2 r = mul2(mul2(v, sc), p);
-                x[c] = r.x;
-                x[c + 1] = r.y;
-            }
-        } else {
+        const float top = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * a.cap_k;
+        if (__any_sync(0xffffffffu, !(top <= CAP_SMALL))) {
 #pragma unroll
             for (int c = 0; c < 32; c++) x[c] = score<true>(a, x[c]);
+            return;
         }
-        return;
+        capped = true;
     }
 #pragma unroll
     for (int c = 0; c < 32; c += 2) {
-        const float2 r = mul2(make_float2(x[c], x[c + 1]), sc);
-        x[c] = r.x;
-        x[c + 1] = r.y;
+        float2 v = make_float2(x[c], x[c + 1]);
+        if (EXT && capped) v = mul2(v, cap_factor2(a, v));
+        v = mul2(v, sc);
+        x[c] = v.x;
+        x[c + 1] = v.y;
     }
 }
 template <bool EXT>

@@ -480,59 +480,82 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
 
                 const bool idle = t * 128 + quarter * 32 >= g.rows;   // only padding rows: no softmax
                 float m = -INFINITY, l = 0.f;
-                // One block of the row: S from tensor memory, P back. `whole`: every row sees every
-                // key; S is then held in registers. Other blocks (the last one or two, or a window's border) read S twice,
-                // for the maximum and for the weights, in rolled loops: little code to fetch.
-                auto soft = [&](auto whole_, int j, int kbase, uint32_t srow) {
-                    constexpr bool WHOLE = decltype(whole_)::value;
+                // One block of the row: S from tensor memory, P back. Where every row sees every key S is
+                // held in registers, with a version each for plain scores (1), capped ones (2), a
+                // distance bias (3) and both (4). Other blocks -- the last one or two, a window's
+                // border, scores beyond the polynomial of the cap -- read S twice (0), for the maximum
+                // and for the weights, in rolled loops: little code to fetch.
+                auto soft = [&](auto kind_, int j, int kbase, uint32_t srow) {
+                    constexpr int KIND = decltype(kind_)::value;
+                    constexpr bool HELD = KIND != 0, CAP = KIND == 2 || KIND == 4, BIAS = KIND >= 3;
+                    const float2 sc2 = make_float2(a.scale_log2, a.scale_log2);
                     // the scores of columns 32 q .., -inf where unseen
                     auto scored = [&](int q, float (&x)[32]) {
                         score32<EXT>(a, x);
                         if (EXT && a.slopes) {
-                            if (WHOLE) {
-                                // slope (kpos - qpos), key by key from the block's first
-                                const float b0 = row.slope2 * (float)(kbase + 32 * q - row.pos);
 #pragma unroll
-                                for (int c = 0; c < 32; c++) x[c] += fmaf(row.slope2, (float)c, b0);
-                            } else {
-#pragma unroll
-                                for (int c = 0; c < 32; c++) x[c] += bias<true>(a, row.slope2, row.pos, s.pos(a, kbase + 32 * q + c));
-                            }
+                            for (int c = 0; c < 32; c++) x[c] += bias<true>(a, row.slope2, row.pos, s.pos(a, kbase + 32 * q + c));
                         }
-                        if (!WHOLE) {
-                            const uint32_t v = seen32(a, s, row, kbase + 32 * q);
+                        const uint32_t v = seen32(a, s, row, kbase + 32 * q);
 #pragma unroll
-                            for (int c = 0; c < 32; c++)
-                                if (!((v >> c) & 1u)) x[c] = -INFINITY;
-                        }
+                        for (int c = 0; c < 32; c++)
+                            if (!((v >> c) & 1u)) x[c] = -INFINITY;
                     };
-                    float row_s[WHOLE ? 4 : 1][32];
+                    float row_s[HELD ? 4 : 1][32];
                     float mx = -INFINITY;
-                    if (WHOLE) {
+                    if (HELD) {
 #pragma unroll
                         for (int q = 0; q < 4; q++)
-                            tmem_ld32(srow + q * 32, reinterpret_cast<uint32_t(&)[32]>(row_s[WHOLE ? q : 0]));
+                            tmem_ld32(srow + q * 32, reinterpret_cast<uint32_t(&)[32]>(row_s[HELD ? q : 0]));
                         tmem_ld_wait();
                     }
-#pragma unroll(WHOLE ? 4 : 1)
+                    if (CAP) {
+                        float lo = INFINITY;
+#pragma unroll
+                        for (int q = 0; q < 4; q++)
+#pragma unroll
+                            for (int c = 0; c < 32; c += 2) {
+                                const float x0 = row_s[HELD ? q : 0][c], x1 = row_s[HELD ? q : 0][c + 1];
+                                mx = fmaxf(mx, fmaxf(x0, x1));
+                                lo = fminf(lo, fminf(x0, x1));
+                            }
+                        if (__any_sync(0xffffffffu, !(fmaxf(mx, -lo) * a.cap_k <= CAP_SMALL))) return false;
+                    }
+#pragma unroll(HELD ? 4 : 1)
                     for (int q = 0; q < 4; q++) {
-                        float (&x)[32] = row_s[WHOLE ? q : 0];
-                        if (!WHOLE) {
+                        float (&x)[32] = row_s[HELD ? q : 0];
+                        if (!HELD) {
                             tmem_ld32(srow + q * 32, reinterpret_cast<uint32_t(&)[32]>(x));
                             tmem_ld_wait();
+                            scored(q, x);
                         }
-                        if (EXT || !WHOLE) scored(q, x);
-                        float m4[4] = {x[0], x[1], x[2], x[3]};
+                        if (BIAS) {
+                            // slope (kpos - qpos), key by key from the first
+                            const float b0 = row.slope2 * (float)(kbase + 32 * q - row.pos);
+                            const float2 s2 = make_float2(row.slope2, row.slope2), b2 = make_float2(b0, b0);
 #pragma unroll
-                        for (int c = 4; c < 32; c++) m4[c & 3] = fmaxf(m4[c & 3], x[c]);
-                        mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+                            for (int c = 0; c < 32; c += 2) {
+                                const float2 v = make_float2(x[c], x[c + 1]);
+                                const float2 e = fma2(CAP ? mul2(v, cap_factor2(a, v)) : v, sc2, fma2(s2, make_float2(c, c + 1), b2));
+                                x[c] = e.x;
+                                x[c + 1] = e.y;
+                            }
+                        }
+                        if (KIND != 2) {
+                            float m4[4] = {x[0], x[1], x[2], x[3]};
+                            if (q == 0 && KIND == 4) mx = -INFINITY;
+#pragma unroll
+                            for (int c = 4; c < 32; c++) m4[c & 3] = fmaxf(m4[c & 3], x[c]);
+                            mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+                        }
                     }
-                    if (!EXT && WHOLE) mx *= a.scale_log2;       // > 0: the greatest product is enough
+                    // plain and capped scores grow with the product: the greatest is enough
+                    if (KIND == 1 || KIND == 2) mx = score<CAP>(a, mx);
                     if (__any_sync(0xffffffffu, mx > m + RESCALE_THRESHOLD)) {
                         const float mn = fmaxf(m, mx);
                         const float cf = mn == -INFINITY ? 1.f : ex2(m - mn);
                         if (j > 0 && !(ok = __all_sync(0xffffffffu, mbar_wait(&o_done[t], (cnt - 1) & 1, deadline, a.err))))
-                            return;
+                            return true;
                         if (j > 0) {                    // O holds the blocks before this one now
                             tc_fence_after_sync();
 #pragma unroll
@@ -549,19 +572,19 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                         m = mn;
                     }
                     const float ms = m == -INFINITY ? 0.f : m;   // a row that saw nothing yet
+                    const float2 ms2 = make_float2(-ms, -ms);
                     // P in fp16 for the product (2^-11 of each weight, as V's own rounding); l sums
                     // the unrounded weights
                     float2 l4[4];
 #pragma unroll
                     for (int i = 0; i < 4; i++) l4[i] = make_float2(0.f, 0.f);
-                    constexpr bool FOLD = !EXT && WHOLE;         // the scale goes into the exponent
-#pragma unroll(WHOLE ? 2 : 1)
+#pragma unroll(HELD ? 2 : 1)
                     for (int h = 0; h < 2; h++) {        // pages 4h .. 4h + 3
                         uint32_t pk[32];
 #pragma unroll
                         for (int u = 0; u < 2; u++) {
-                            float (&x)[32] = row_s[WHOLE ? 2 * h + u : 0];
-                            if (!WHOLE) {
+                            float (&x)[32] = row_s[HELD ? 2 * h + u : 0];
+                            if (!HELD) {
                                 tmem_ld32(srow + (2 * h + u) * 32, reinterpret_cast<uint32_t(&)[32]>(x));
                                 tmem_ld_wait();
                                 scored(2 * h + u, x);
@@ -569,8 +592,9 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
 #pragma unroll
                             for (int c = 0; c < 32; c += 2) {
                                 const float2 v = make_float2(x[c], x[c + 1]);
-                                const float2 e = FOLD ? fma2(v, make_float2(a.scale_log2, a.scale_log2), make_float2(-ms, -ms))
-                                                      : add2(v, make_float2(-ms, -ms));
+                                // plain and capped: the scale goes into the exponent
+                                const float2 e = KIND == 1 ? fma2(v, sc2, ms2)
+                                               : KIND == 2 ? fma2(mul2(v, cap_factor2(a, v)), sc2, ms2) : add2(v, ms2);
                                 const float2 p = make_float2(ex2(e.x), ex2(e.y));
                                 l4[(c >> 1) & 3] = add2(l4[(c >> 1) & 3], p);
                                 pk[u * 16 + (c >> 1)] = pack_half2(p.x, p.y);
@@ -585,7 +609,9 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                     }
                     const float2 l2 = add2(add2(l4[0], l4[1]), add2(l4[2], l4[3]));
                     l += l2.x + l2.y;
+                    return true;
                 };
+                const bool capped = EXT && a.cap_log2 > 0.f, biased = EXT && a.slopes;
                 for (int j = 0; j < nb; j++) {
                     const int kbase = w.first + (g.blk0 + j) * BLK;
                     const bool whole = kbase + BLK <= s.ctx && (a.window <= 0 || (long long)pos_hi - kbase < a.window);
@@ -639,8 +665,12 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                         continue;
                     }
                     tc_fence_after_sync();
-                    if (whole) soft(std::true_type{}, j, kbase, srow);
-                    else soft(std::false_type{}, j, kbase, srow);
+                    bool did = false;
+                    if (whole && !EXT) did = soft(std::integral_constant<int, 1>{}, j, kbase, srow);
+                    if (EXT && whole && capped && !biased) did = soft(std::integral_constant<int, EXT ? 2 : 1>{}, j, kbase, srow);
+                    if (EXT && whole && !capped && biased) did = soft(std::integral_constant<int, EXT ? 3 : 1>{}, j, kbase, srow);
+                    if (EXT && whole && capped && biased) did = soft(std::integral_constant<int, EXT ? 4 : 1>{}, j, kbase, srow);
+                    if (!did) soft(std::integral_constant<int, 0>{}, j, kbase, srow);
                     cnt++;
                 }
                 // epilogue: the last P V has landed
