@@ -41,12 +41,12 @@ template <int MT> struct Cfg {
     static constexpr int KST = MT == 1 ? 4 : 3;    // K blocks in flight
     static constexpr int SB = MT == 1 ? 2 : 1;     // S buffers of a tile
     static constexpr int TILE_COLS = SB * 128 + 128;   // tensor memory of a tile: S (and P), then O
-    static constexpr int THREADS = 128 + 128 * MT; // warps 0-3: TMA, MMA, schedule, none; then a thread per row
+    static constexpr int THREADS = 128 + 128 * MT; // warps 0-3: TMA, MMA, two that look V over; then a thread per row
     static constexpr int ROWS = 128 * MT;
     static constexpr int OFF_K = MT * Q_TILE;
     static constexpr int OFF_V = OFF_K + KST * KV_BLK;
     static constexpr int OFF_BAR = OFF_V + VST * KV_BLK;
-    static constexpr int NBAR = 2 * KST + 2 * VST + (2 + 3 * SB) * MT + 2;
+    static constexpr int NBAR = 2 * KST + 3 * VST + (2 + 3 * SB) * MT + 2;
     static constexpr int SMEM = 1024 + OFF_BAR + NBAR * 8 + 32;
     static constexpr uint32_t TMEM_COLS = 512;
 };
@@ -178,7 +178,8 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
     uint64_t* k_empty = k_full + KST;
     uint64_t* v_full = k_empty + KST;
     uint64_t* v_empty = v_full + VST;
-    uint64_t* q_empty = v_empty + VST;       // every S of a segment done: Q may be replaced
+    uint64_t* v_ready = v_empty + VST;       // V looked over, where some row does not see it all
+    uint64_t* q_empty = v_ready + VST;       // every S of a segment done: Q may be replaced
     uint64_t* q_full = q_empty + 1;          // [MT] Q of a segment is there
     uint64_t* s_full = q_full + MT;          // [MT][SB] S written (MMA -> softmax)
     // [MT][SB][2] P of pages 0-3 / 4-7 written (softmax -> MMA): one per S buffer, since with two the
@@ -200,6 +201,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
         for (int i = 0; i < VST; i++) {
             mbar_init(&v_full[i], 1);
             mbar_init(&v_empty[i], 1);
+            mbar_init(&v_ready[i], 64);
         }
         for (int t = 0; t < MT; t++) {
             mbar_init(&q_full[t], a.q_tma ? 1 : 128);
@@ -222,13 +224,17 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
     }
     pdl_wait();
     if (warp == 2) {
-        const long long W = blocks_before<C::ROWS>(a, a.B, lane);
+        const long long first = blocks_lane<C::ROWS>(a, lane);         // of sequences 0 .. 31
+        long long W = first;
+        for (int b0 = 32; b0 < a.B; b0 += 32) W += blocks_lane<C::ROWS>(a, b0 + lane);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) W += __shfl_xor_sync(0xffffffffu, W, o);
         const Share sh(W, gridDim.x);
         const long long beg = sh.first(blockIdx.x), end = sh.first(blockIdx.x + 1);
         long long before = 0;
         int b = a.B;
         for (int b0 = 0; b0 < a.B && b == a.B; b0 += 32) {
-            const long long mine = blocks_lane<C::ROWS>(a, b0 + lane);
+            const long long mine = b0 ? blocks_lane<C::ROWS>(a, b0 + lane) : first;
             long long x = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -415,7 +421,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
                             if (ok) ok = wait(&p_full[(t * SB + buf) * 2 + h], c / SB);
-                            if (ok && t == 0 && h == 0) ok = wait(&v_full[vs], (n + j) / VST);
+                            if (ok && t == 0 && h == 0) ok = wait(&v_full[vs], (n + j) / VST) && wait(&v_ready[vs], (n + j) / VST);
                             if (!ok) break;
                             tc_fence_after_sync();
 #pragma unroll
@@ -448,6 +454,53 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
         }
         if (elect_one()) umma_commit(done);
         __syncwarp();
+    } else {
+        // ---------------------------------------------------------------- V of masked blocks
+        // 0 * inf is NaN in the product: V rows behind the sequence and values that are not finite
+        // are zeroed before P V; the latter are made up for where they are seen (epilogue). Every
+        // block passes here, in order, so that no phase of v_ready can be mistaken for another.
+        bool ok = true;
+        int n = 0;
+        while (ok && walk.next(a, &g, &s, &w, &pos_hi, lane)) {
+            for (int j = g.blk0; j < g.blk1 && ok; j++, n++) {
+                const int vs = n % VST, kbase = w.first + j * BLK;
+                ok = __all_sync(0xffffffffu, mbar_wait(&v_full[vs], (n / VST) & 1, deadline, a.err));
+                if (!ok) break;
+                if (!(kbase + BLK <= s.ctx && (a.window <= 0 || (long long)pos_hi - kbase < a.window))) {
+                    uint8_t* vb = vring + vs * KV_BLK;
+                    bool found = false;
+                    // pages that every row sees whole are left; a window reaches all of them
+                    const int pg0 = a.window > 0 ? 0 : max(0, min(BLK_PAGES, (s.ctx - kbase) / PAGE));
+#pragma unroll 4
+                    for (int c = pg0 * 256 + threadIdx.x - 64; c < BLK * 16; c += 64) {
+                        // chunk c: page c / 256, half, token, 16-byte piece (swizzled; all pieces of
+                        // a 128-byte row are treated alike)
+                        const int key = (c >> 8) * PAGE + ((c >> 3) & 15);
+                        uint4* at = reinterpret_cast<uint4*>(vb + c * 16);
+                        uint4 v = *at;
+                        bool f = false;
+                        auto fix = [&](uint32_t& x) {
+                            uint32_t keep = 0xffffffffu;
+                            if ((x & 0x7c00u) == 0x7c00u) keep &= 0xffff0000u;
+                            if ((x & 0x7c000000u) == 0x7c000000u) keep &= 0x0000ffffu;
+                            x &= keep;
+                            f |= keep != 0xffffffffu;
+                        };
+                        fix(v.x);
+                        fix(v.y);
+                        fix(v.z);
+                        fix(v.w);
+                        const bool out = kbase + key >= s.len;
+                        if (out) v = make_uint4(0u, 0u, 0u, 0u);
+                        if (f || out) *at = v;
+                        found |= f && !out;
+                    }
+                    if (found) *odd = 1;
+                    fence_proxy_async_smem();
+                }
+                mbar_arrive(&v_ready[vs]);
+            }
+        }
     }
     } else {
         if (MT == 2) regs_up<216>();
@@ -483,23 +536,33 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                 // One block of the row: S from tensor memory, P back. Where every row sees every key S is
                 // held in registers, with a version each for plain scores (1), capped ones (2), a
                 // distance bias (3) and both (4). Other blocks -- the last one or two, a window's
-                // border, scores beyond the polynomial of the cap -- read S twice (0), for the maximum
-                // and for the weights, in rolled loops: little code to fetch.
+                // border, scores beyond the polynomial of the cap -- go through rolled loops (0), scores
+                // back into tensor memory in between: little code to fetch.
                 auto soft = [&](auto kind_, int j, int kbase, uint32_t srow) {
                     constexpr int KIND = decltype(kind_)::value;
                     constexpr bool HELD = KIND != 0, CAP = KIND == 2 || KIND == 4, BIAS = KIND >= 3;
                     const float2 sc2 = make_float2(a.scale_log2, a.scale_log2);
                     // the scores of columns 32 q .., -inf where unseen
+                    uint32_t see0 = ~0u, see1 = ~0u, see2 = ~0u, see3 = ~0u;
+                    if (!HELD) {
+                        auto seen = [&](int q) {
+                            const int p = kbase + 32 * q;
+                            return p + 32 <= s.ctx && a.window <= 0 ? ~0u : seen32(a, s, row, p);
+                        };
+                        see0 = seen(0);
+                        see1 = seen(1);
+                        see2 = seen(2);
+                        see3 = seen(3);
+                    }
                     auto scored = [&](int q, float (&x)[32]) {
                         score32<EXT>(a, x);
                         if (EXT && a.slopes) {
 #pragma unroll
                             for (int c = 0; c < 32; c++) x[c] += bias<true>(a, row.slope2, row.pos, s.pos(a, kbase + 32 * q + c));
                         }
-                        const uint32_t v = seen32(a, s, row, kbase + 32 * q);
+                        const uint32_t v = q == 0 ? see0 : q == 1 ? see1 : q == 2 ? see2 : see3;
 #pragma unroll
-                        for (int c = 0; c < 32; c++)
-                            if (!((v >> c) & 1u)) x[c] = -INFINITY;
+                        for (int c = 0; c < 32; c++) x[c] = (v >> c) & 1u ? x[c] : -INFINITY;
                     };
                     float row_s[HELD ? 4 : 1][32];
                     float mx = -INFINITY;
@@ -528,6 +591,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                             tmem_ld32(srow + q * 32, reinterpret_cast<uint32_t(&)[32]>(x));
                             tmem_ld_wait();
                             scored(q, x);
+                            tmem_st32(srow + q * 32, reinterpret_cast<uint32_t(&)[32]>(x));
                         }
                         if (BIAS) {
                             // slope (kpos - qpos), key by key from the first
@@ -549,6 +613,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                             mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
                         }
                     }
+                    if (!HELD) tmem_st_wait();
                     // plain and capped scores grow with the product: the greatest is enough
                     if (KIND == 1 || KIND == 2) mx = score<CAP>(a, mx);
                     if (__any_sync(0xffffffffu, mx > m + RESCALE_THRESHOLD)) {
@@ -587,7 +652,6 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                             if (!HELD) {
                                 tmem_ld32(srow + (2 * h + u) * 32, reinterpret_cast<uint32_t(&)[32]>(x));
                                 tmem_ld_wait();
-                                scored(2 * h + u, x);
                             }
 #pragma unroll
                             for (int c = 0; c < 32; c += 2) {
@@ -617,46 +681,6 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                     const bool whole = kbase + BLK <= s.ctx && (a.window <= 0 || (long long)pos_hi - kbase < a.window);
                     const uint32_t srow = trow + cnt % SB * 128;
                     if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t * SB + cnt % SB], (cnt / SB) & 1, deadline, a.err));
-                    if (!whole) {
-                        // 0 * inf is NaN in the product: V rows behind the sequence and values
-                        // that are not finite are zeroed; the latter are made up for below
-                        const int vs = (n + j) % VST;
-                        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&v_full[vs], ((n + j) / VST) & 1, deadline, a.err));
-                        if (ok) {
-                            uint8_t* vb = vring + vs * KV_BLK;
-                            const int nthr = nt * 128;
-                            bool found = false;
-                            // pages that every row sees whole are left; a window reaches all of them
-                            const int pg0 = a.window > 0 ? 0 : max(0, min(BLK_PAGES, (s.ctx - kbase) / PAGE));
-#pragma unroll 4
-                            for (int c = pg0 * 256 + threadIdx.x - 128; c < BLK * 16; c += nthr) {
-                                // chunk c: page c / 256, half, token, 16-byte piece (swizzled; all
-                                // pieces of a 128-byte row are treated alike)
-                                const int key = (c >> 8) * PAGE + ((c >> 3) & 15);
-                                uint4* at = reinterpret_cast<uint4*>(vb + c * 16);
-                                uint4 v = *at;
-                                bool f = false;
-                                auto fix = [&](uint32_t& x) {
-                                    uint32_t keep = 0xffffffffu;
-                                    if ((x & 0x7c00u) == 0x7c00u) keep &= 0xffff0000u;
-                                    if ((x & 0x7c000000u) == 0x7c000000u) keep &= 0x0000ffffu;
-                                    x &= keep;
-                                    f |= keep != 0xffffffffu;
-                                };
-                                fix(v.x);
-                                fix(v.y);
-                                fix(v.z);
-                                fix(v.w);
-                                const bool out = kbase + key >= s.len;
-                                if (out) v = make_uint4(0u, 0u, 0u, 0u);
-                                if (f || out) *at = v;
-                                found |= f && !out;
-                            }
-                            if (found) *odd = 1;
-                            fence_proxy_async_smem();
-                        }
-                        asm volatile("bar.sync 1, %0;" ::"r"(nt * 128) : "memory");
-                    }
                     if (!ok) continue;
                     if (idle) {                         // their P is whatever S held: no other row reads it
                         mbar_arrive(&p_full[(t * SB + cnt % SB) * 2]);
