@@ -30,6 +30,7 @@ struct Args {
     float cap_log2;           // softcap * log2(e), 0: no cap
     float cap_in;             // 2 log2(e) sm_scale / softcap
     float cap_k;              // sm_scale / softcap
+    float cap_poly[5];        // of a capped score / q.k in (q.k)^2, see cap_factor2
     int q_tma;                // the tcgen05 kernel reads Q tiles through a tensor map
 };
 
@@ -133,19 +134,19 @@ __device__ __forceinline__ float score(const Args& a, float qk) {
         return fmaf(-2.f * a.cap_log2, rcp(1.f + ex2(qk * a.cap_in)), a.cap_log2);
     return qk * a.scale_log2;
 }
-constexpr float C0 = 0.999999642f, C1 = -0.333312094f, C2 = 0.132992104f, C3 = -0.0516967401f, C4 = 0.014976955f;   // tanh(y)/y in y^2
-// Capped scores are nearly always far below the cap: up to CAP_SMALL of it tanh(y) = y P(y^2) with
-// P of degree 4 (fitted here to tanh(y)/y by weighted least squares; off by at most 2^-25 of the
-// cap), seven operations on two values each in place of two of the special-function unit, which
-// the exponentials already fill.
+// tanh(y)/y in y^2 for y <= CAP_SMALL: fitted to it by weighted least squares, off by at most 2^-25.
+// The launch scales the terms, so that the polynomial is one in (q.k)^2.
+constexpr float TANH_POLY[5] = {0.999999642f, -0.333312094f, 0.132992104f, -0.0516967401f, 0.014976955f};
 constexpr float CAP_SMALL = 0.6f;
-// P for two products q.k.
+// Capped scores are nearly always far below the cap: up to CAP_SMALL of it a score is q.k times a
+// polynomial of degree 4 in (q.k)^2, six operations on two values each where the exact form takes
+// two of the special-function unit, which the exponentials already fill. -> score / q.k, log2 domain
 __device__ __forceinline__ float2 cap_factor2(const Args& a, float2 qk) {
-    const float2 y = mul2(qk, make_float2(a.cap_k, a.cap_k)), t = mul2(y, y);
-    float2 p = fma2(make_float2(C4, C4), t, make_float2(C3, C3));
-    p = fma2(p, t, make_float2(C2, C2));
-    p = fma2(p, t, make_float2(C1, C1));
-    return fma2(p, t, make_float2(C0, C0));
+    const float2 t = mul2(qk, qk);
+    float2 p = fma2(make_float2(a.cap_poly[4], a.cap_poly[4]), t, make_float2(a.cap_poly[3], a.cap_poly[3]));
+    p = fma2(p, t, make_float2(a.cap_poly[2], a.cap_poly[2]));
+    p = fma2(p, t, make_float2(a.cap_poly[1], a.cap_poly[1]));
+    return fma2(p, t, make_float2(a.cap_poly[0], a.cap_poly[0]));
 }
 // The scores of 32 products that one thread holds.
 template <bool EXT>
@@ -167,8 +168,7 @@ __device__ __forceinline__ void score32(const Args& a, float (&x)[32]) {
 #pragma unroll
     for (int c = 0; c < 32; c += 2) {
         float2 v = make_float2(x[c], x[c + 1]);
-        if (EXT && capped) v = mul2(v, cap_factor2(a, v));
-        v = mul2(v, sc);
+        v = mul2(v, EXT && capped ? cap_factor2(a, v) : sc);
         x[c] = v.x;
         x[c + 1] = v.y;
     }

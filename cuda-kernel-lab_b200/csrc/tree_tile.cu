@@ -600,7 +600,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
 #pragma unroll
                             for (int c = 0; c < 32; c += 2) {
                                 const float2 v = make_float2(x[c], x[c + 1]);
-                                const float2 e = fma2(CAP ? mul2(v, cap_factor2(a, v)) : v, sc2, fma2(s2, make_float2(c, c + 1), b2));
+                                const float2 e = fma2(v, CAP ? cap_factor2(a, v) : sc2, fma2(s2, make_float2(c, c + 1), b2));
                                 x[c] = e.x;
                                 x[c + 1] = e.y;
                             }
@@ -656,9 +656,9 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
 #pragma unroll
                             for (int c = 0; c < 32; c += 2) {
                                 const float2 v = make_float2(x[c], x[c + 1]);
-                                // plain and capped: the scale goes into the exponent
+                                // plain and capped: the score is a factor in the exponent
                                 const float2 e = KIND == 1 ? fma2(v, sc2, ms2)
-                                               : KIND == 2 ? fma2(mul2(v, cap_factor2(a, v)), sc2, ms2) : add2(v, ms2);
+                                               : KIND == 2 ? fma2(v, cap_factor2(a, v), ms2) : add2(v, ms2);
                                 const float2 p = make_float2(ex2(e.x), ex2(e.y));
                                 l4[(c >> 1) & 3] = add2(l4[(c >> 1) & 3], p);
                                 pk[u * 16 + (c >> 1)] = pack_half2(p.x, p.y);
