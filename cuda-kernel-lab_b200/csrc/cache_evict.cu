@@ -25,7 +25,8 @@ using tree::Seq;
 // no atomics and no second kernel, and additions in the same order whatever the batch. The lse of the
 // attention call already normalises, so there is no running maximum either.
 //
-// The pages of all sequences, end to end, are divided evenly over one wave of CTAs. A CTA's run of
+// The blocks of all sequences, end to end, are divided evenly over one wave of CTAs (by whole
+// blocks: the ring turns over a part of a block no faster than a whole one). A CTA's run of
 // a sequence is taken W_SEG blocks at a time: for each kv head (and each W_ROWS of its rows) Q is
 // staged once and the blocks' K tiles stream past it. Warp 0 loads K (TMA), warp 1 issues the MMAs,
 // warps 2-3 stage Q and the rows' lse, position and slope, and two groups of four warps turn S into
@@ -69,9 +70,9 @@ constexpr size_t w_smem(int rows, int stages) {
 }
 
 struct WSeg {
-    int b, pg0, pg1;                           // pages of the sequence
+    int b, pg0, pg1;                           // pages of the sequence, whole blocks but for its end
 };
-// A CTA's run of pages, a segment of at most W_SEG blocks at a time.
+// A CTA's run of blocks, a segment of at most W_SEG at a time.
 struct WWalk {
     long long left, off;
     int b;
@@ -79,16 +80,18 @@ struct WWalk {
         while (left > 0 && b < a.B) {
             int page0;
             const int np = (tree::seq_len(a.indptr, a.last, b, &page0) + PAGE - 1) / PAGE;
-            if (off >= np) {
-                off -= np;
+            const int blocks = (np + W_BLK_PAGES - 1) / W_BLK_PAGES;
+            if (off >= blocks) {
+                off -= blocks;
                 b++;
                 continue;
             }
+            const int b1 = (int)min(min((long long)blocks, off + left), off + W_SEG);
             g->b = b;
-            g->pg0 = (int)off;
-            g->pg1 = (int)min(min((long long)np, off + left), off + W_SEG * W_BLK_PAGES);
-            left -= g->pg1 - g->pg0;
-            off = g->pg1;
+            g->pg0 = (int)off * W_BLK_PAGES;
+            g->pg1 = min(np, b1 * W_BLK_PAGES);
+            left -= b1 - off;
+            off = b1;
             return true;
         }
         return false;
@@ -195,13 +198,14 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     if (warp == 0 && lane == 0) tma_prefetch_desc(&tmK);
     pdl_wait();
     if (warp == 2) {
-        // this CTA's pages: two sweeps over the lengths
-        auto pages = [&](int b) {
+        // this CTA's blocks: two sweeps over the lengths
+        auto blocks = [&](int b) {
             int p;
-            return b < a.B ? (tree::seq_len(a.indptr, a.last, b, &p) + PAGE - 1) / PAGE : 0;
+            return b < a.B ? (tree::seq_len(a.indptr, a.last, b, &p) + W_BLK - 1) / W_BLK : 0;
         };
-        long long total = 0;
-        for (int b0 = 0; b0 < a.B; b0 += 32) total += pages(b0 + lane);
+        const int first = blocks(lane);                              // of sequences 0 .. 31
+        long long total = first;
+        for (int b0 = 32; b0 < a.B; b0 += 32) total += blocks(b0 + lane);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
         const tree::Share sh(total, gridDim.x);
@@ -209,7 +213,7 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         long long before = 0;
         int b = a.B;
         for (int b0 = 0; b0 < a.B && b == a.B; b0 += 32) {
-            const int mine = pages(b0 + lane);
+            const int mine = b0 ? blocks(b0 + lane) : first;
             long long x = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
