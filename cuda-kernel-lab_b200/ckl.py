@@ -635,7 +635,7 @@ def _opt(t, dtype, n, name, who, dev):
 
 def _acc_rows(acc, B, who, dev):
     """(address, row stride) of fp32 rows, one per sequence at least."""
-    if acc.dtype is not _F32 or acc.get_device() != dev or acc.dim() != 2 or acc.stride(1) != 1:
+    if not isinstance(acc, _T.Tensor) or acc.dtype is not _F32 or acc.get_device() != dev or acc.dim() != 2 or acc.stride(1) != 1:
         raise CklError(1, who, "acc: expected float32 rows on the current device")
     rows, cols = acc.shape
     stride = acc.stride(0) if rows > 1 else cols
@@ -646,6 +646,9 @@ def _acc_rows(acc, B, who, dev):
 
 def _cache_shape(k_cache, v_cache, who, dev):
     """(pages, kv heads, addresses) of K and V caches [pages, 16, heads, 128]."""
+    for t in (k_cache, v_cache):
+        if not isinstance(t, _T.Tensor):
+            _bad(t, _F16, 0, "cache", who, dev)
     shape = k_cache.shape
     if len(shape) != 4 or shape[1] != PAGE or shape[3] != HEAD_DIM or v_cache.shape != shape:
         raise CklError(2, who, f"caches {tuple(k_cache.shape)} / {tuple(v_cache.shape)}")
@@ -682,7 +685,7 @@ def make_append_params(q, k, v, k_cache, v_cache, kv_indptr, kv_indices, kv_last
         _bind()
     who, dev = "make_append_params", _device()
     P, Hkv, kc, vc = _cache_shape(k_cache, v_cache, who, dev)
-    N = k.shape[0]
+    N = k.shape[0] if isinstance(k, _T.Tensor) and k.dim() else 0
     addr, strides = [], []
     for t, name in ((q, "q"), (k, "k"), (v, "v")):
         if t is None and name == "q":

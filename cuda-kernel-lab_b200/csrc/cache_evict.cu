@@ -76,6 +76,11 @@ struct WSeg {
 struct WWalk {
     long long left, off;
     int b;
+    uint64_t deadline;                         // of the waits for eight staged Qs: a call has no limit,
+                                               // however many it takes
+    __device__ __forceinline__ void renew(const tree::Args& a, int chunk) {
+        if (chunk % 8 == 0) deadline = globaltimer() + a.timeout_ns;
+    }
     __device__ __forceinline__ bool next(const tree::Args& a, WSeg* g) {
         while (left > 0 && b < a.B) {
             int page0;
@@ -237,8 +242,7 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     pdl_trigger();
     const uint32_t tmem = *tmem_slot;
     auto d_col = [&](int d) { return (uint32_t)((d / W_BUFS * bufs + d % W_BUFS) * d_cols); };   // of S buffer d
-    const uint64_t deadline = globaltimer() + a.timeout_ns;
-    WWalk walk{s_left, s_off, s_b};
+    WWalk walk{s_left, s_off, s_b, globaltimer() + a.timeout_ns};
     WSeg g;
     bool ok = true;
     int chunk = 0, n = 0;                        // staged Qs and K tiles so far
@@ -267,7 +271,8 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                 ids[i] = pg < g.pg1 ? __ldg(a.indices + s.page0 + pg) : 0;
             }
             for (int h = 0; h < a.Hkv && ok; h++)
-                for (int r0 = 0; r0 < nrows && ok; r0 += N)
+                for (int r0 = 0; r0 < nrows && ok; r0 += N, chunk++) {
+                    walk.renew(a, chunk);
                     for (int pg = pg0; pg < g.pg1 && ok; pg += W_BLK_PAGES, n++) {
                         const int np = min(W_BLK_PAGES, g.pg1 - pg), st = n % KST, j = (pg - pg0) / W_BLK_PAGES;
                         int id = ids[0];
@@ -276,7 +281,7 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                         int page[W_BLK_PAGES];
 #pragma unroll
                         for (int i = 0; i < W_BLK_PAGES; i++) page[i] = __shfl_sync(0xffffffffu, id, (j & 3) * 8 + i);
-                        if (n >= KST) ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[st], (n / KST - 1) & 1, deadline, a.err));
+                        if (n >= KST) ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[st], (n / KST - 1) & 1, walk.deadline, a.err));
                         if (!ok) break;
                         if (elect_one()) {
                             mbar_arrive_expect_tx(&k_full[st], np * KV_TILE);
@@ -289,11 +294,12 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                                 }
                         }
                     }
+                }
         }
         // every issued copy must land before the CTA exits
         if (lane == 0)
             for (int i = 0; i < KST && i < n; i++)
-                mbar_wait(&k_full[i], ((i + (n - 1 - i) / KST * KST) / KST) & 1, deadline, a.err);
+                mbar_wait(&k_full[i], ((i + (n - 1 - i) / KST * KST) / KST) & 1, walk.deadline, a.err);
     } else if (warp == 1) {
         // ---------------------------------------------------------------- MMA issuer
         const uint32_t idesc = umma_idesc_f16(W_BLK, N, false, false);
@@ -309,12 +315,13 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                 int t0 = tiles[0], t1 = tiles[1];
                 for (int c = 0; c < chunks && ok; c++) {
                     const int qb = (chunk + c) % qbufs;
-                    ok = mbar_wait(&q_full[qb], ((chunk + c) / qbufs) & 1, deadline, a.err);
+                    walk.renew(a, chunk + c);
+                    ok = mbar_wait(&q_full[qb], ((chunk + c) / qbufs) & 1, walk.deadline, a.err);
                     for (int j = 0; j < nb && ok; j++) {
                         const int m = n + c * nb + j, st = m % KST, gr = narrow ? c & 1 : 0;
                         const int t = gr ? t1++ : t0++, d = gr * W_BUFS + t % bufs;
-                        ok = mbar_wait(&k_full[st], (m / KST) & 1, deadline, a.err);
-                        if (ok && t >= bufs) ok = mbar_wait(&d_empty[d], (t / bufs - 1) & 1, deadline, a.err);
+                        ok = mbar_wait(&k_full[st], (m / KST) & 1, walk.deadline, a.err);
+                        if (ok && t >= bufs) ok = mbar_wait(&d_empty[d], (t / bufs - 1) & 1, walk.deadline, a.err);
                         if (!ok) break;
                         tc_fence_after_sync();
 #pragma unroll
@@ -347,8 +354,9 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             for (int h = 0; h < a.Hkv && ok; h++)
                 for (int r0 = 0; r0 < nrows && ok; r0 += N, chunk++) {
                     const int qb = chunk % qbufs, ib = chunk % ibufs;
+                    walk.renew(a, chunk);
                     if (chunk >= qbufs)
-                        ok = __all_sync(0xffffffffu, mbar_wait(&q_empty[qb], (chunk / qbufs - 1) & 1, deadline, a.err));
+                        ok = __all_sync(0xffffffffu, mbar_wait(&q_empty[qb], (chunk / qbufs - 1) & 1, walk.deadline, a.err));
                     if (!ok) break;
                     uint8_t* dst = qs + qb * q_bytes;
                     if (a.q_tma) {
@@ -376,7 +384,7 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                         mbar_arrive(&q_full[qb]);
                     }
                     if (chunk >= ibufs)
-                        ok = __all_sync(0xffffffffu, mbar_wait(&i_empty[ib], (chunk / ibufs - 1) & 1, deadline, a.err));
+                        ok = __all_sync(0xffffffffu, mbar_wait(&i_empty[ib], (chunk / ibufs - 1) & 1, walk.deadline, a.err));
                     if (!ok) { chunk++; break; }
                     const RowInfo in{infos + ib * 4 * N, N};
                     for (int r = tid; r < N; r += 64) {
@@ -396,7 +404,7 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         // a staged Q that nobody waited for (after a timeout) must still land
         if (!ok && tid == 0)
             for (int c = max(0, chunk - qbufs); c < chunk; c++)
-                mbar_wait(&q_full[c % qbufs], (c / qbufs) & 1, deadline, a.err);
+                mbar_wait(&q_full[c % qbufs], (c / qbufs) & 1, walk.deadline, a.err);
     } else {
         // ---------------------------------------------------------------- weights
         const int quarter = warp & 3, hf = (warp - 4) >> 2;
@@ -414,8 +422,9 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             for (int j = 0; j < nb; j++) sums[(hf * W_SEG + j) * W_BLK + key] = 0.f;
             for (int c = 0; c < chunks; c++, chunk++) {
                 const int ib = chunk % ibufs;
+                walk.renew(a, chunk);
                 const RowInfo in{infos + ib * 4 * N, N};
-                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&i_full[ib], (chunk / ibufs) & 1, deadline, a.err));
+                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&i_full[ib], (chunk / ibufs) & 1, walk.deadline, a.err));
                 const int r0 = c % rchunks * N;                      // first row of this chunk
                 const int t_lo = (r0 + c0) / a.G;                    // tokens of this thread's columns
                 const int nt = r0 + c0 < nrows ? (min(nrows, r0 + c1) - 1) / a.G - t_lo + 1 : 0;
@@ -425,7 +434,7 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                 for (int j = 0; mine && j < nb; j++, tile++) {
                     const int d = gr * W_BUFS + tile % bufs;
                     const uint32_t d_at = d_col(d);
-                    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&d_full[d], (tile / bufs) & 1, deadline, a.err));
+                    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&d_full[d], (tile / bufs) & 1, walk.deadline, a.err));
                     if (!ok) continue;
                     tc_fence_after_sync();
                     const int kbase = (pg0 + j * W_BLK_PAGES) * PAGE, p = kbase + key;
@@ -511,7 +520,7 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         }
     }
     // every MMA must have finished before tensor memory is released
-    if (threadIdx.x == 0) mbar_wait(done, 0, deadline, a.err);
+    if (threadIdx.x == 0) mbar_wait(done, 0, walk.deadline, a.err);
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
@@ -964,8 +973,15 @@ ckl_status ckl_cache_compact(void* k_cache, void* v_cache, const int* kv_indptr,
         return fail(CKL_INVALID_ARG, "cache_compact: NULL tensor pointer");
     if (((uintptr_t)k_cache | (uintptr_t)v_cache) & 15)
         return fail(CKL_INVALID_ARG, "cache_compact: k_cache and v_cache must be 16-byte aligned");
-    if (k_cache == v_cache) return fail(CKL_INVALID_ARG, "cache_compact: k_cache and v_cache are the same");
     if (num_pages > INT_MAX / PAGE) return fail(CKL_UNSUPPORTED_SHAPE, "cache_compact: num_pages=%d", num_pages);
+    // what a CTA writes, others still read: the caches and the lengths stand alone
+    auto overlap = [](const void* p, size_t pn, const void* q, size_t qn) {
+        return p && q && (uintptr_t)p < (uintptr_t)q + qn && (uintptr_t)q < (uintptr_t)p + pn;
+    };
+    const size_t cache = (size_t)num_pages * PAGE * Hkv * D * sizeof(__half), ints = (size_t)B * sizeof(int);
+    if (overlap(k_cache, cache, v_cache, cache)) return fail(CKL_INVALID_ARG, "cache_compact: k_cache and v_cache overlap");
+    for (const int* in : {keep_count, dst_start, kv_last_page_len, kv_indptr, kv_indptr + 1})
+        if (overlap(new_len, ints, in, ints)) return fail(CKL_INVALID_ARG, "cache_compact: new_len overlaps an input");
     const DeviceInfo* di = device_info();
     if (!di) return CKL_CUDA_ERROR;
     CArgs a{};

@@ -1,4 +1,4 @@
-// tree_tile.cu -- the draft-tree attention for more than 32 stacked rows (drafted tokens x query
+// tree_tile.cu -- the draft-tree attention for more than 16 stacked rows (drafted tokens x query
 // heads of a kv head) on the 5th-generation tensor cores.
 //
 // A CTA holds 128 * MT rows of one (sequence, kv head) as MT tiles, the M of tcgen05.mma, and
@@ -104,7 +104,9 @@ struct Walk {
     long long left;              // blocks of this CTA not handed out yet
     long long off;               // next block within sequence b
     int b;
-    __device__ __forceinline__ Walk(long long left_, long long off_, int b_) : left(left_), off(off_), b(b_) {}
+    uint64_t deadline;           // of a segment's waits: a call has no limit, however many there are
+    __device__ __forceinline__ Walk(const Args& a, long long left_, long long off_, int b_)
+        : left(left_), off(off_), b(b_), deadline(globaltimer() + a.timeout_ns) {}
     // The next segment, its sequence and work; false at the end.
     __device__ __forceinline__ bool next(const Args& a, Seg* g, Seq* s, Work* w, int* pos_hi, int lane) {
         while (left > 0 && b < a.B) {
@@ -128,6 +130,7 @@ struct Walk {
             g->blk1 = (int)min((long long)w->nblk, g->blk0 + left);
             off += g->blk1 - g->blk0;
             left -= g->blk1 - g->blk0;
+            deadline = globaltimer() + a.timeout_ns;
             return true;
         }
         return false;
@@ -261,8 +264,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
     tc_fence_after_sync();
     pdl_trigger();
     const uint32_t tmem = *tmem_slot;
-    const uint64_t deadline = globaltimer() + a.timeout_ns;
-    Walk<C::ROWS> walk(range[0], range[1], *range_b);
+    Walk<C::ROWS> walk(a, range[0], range[1], *range_b);
     Seg g;
     Seq s;
     Work w;
@@ -296,7 +298,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                 const int ks = n % KST, vs = n % VST;
                 // one elected lane issues: a box per lane would be serialised at ~50 ns each
                 if (elect_one()) {
-                    if (n >= KST) ok = mbar_wait(&k_empty[ks], ((n / KST) - 1) & 1, deadline, a.err);
+                    if (n >= KST) ok = mbar_wait(&k_empty[ks], ((n / KST) - 1) & 1, walk.deadline, a.err);
                     if (ok) {
                         uint8_t* dst = kring + ks * KV_BLK;
                         mbar_arrive_expect_tx(&k_full[ks], KV_BLK);
@@ -310,7 +312,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 if (elect_one()) {
-                    if (n >= VST) ok = mbar_wait(&v_empty[vs], ((n / VST) - 1) & 1, deadline, a.err);
+                    if (n >= VST) ok = mbar_wait(&v_empty[vs], ((n / VST) - 1) & 1, walk.deadline, a.err);
                     if (ok) {
                         uint8_t* dst = vring + vs * KV_BLK;
                         mbar_arrive_expect_tx(&v_full[vs], KV_BLK);
@@ -324,7 +326,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                 if (j == g.blk0 && a.q_tma) {
                     // the segment's Q, behind its first block: the earlier segment still reads its own
                     if (lane == 0) {
-                        if (seg > 0) ok = mbar_wait(q_empty, (seg - 1) & 1, deadline, a.err);
+                        if (seg > 0) ok = mbar_wait(q_empty, (seg - 1) & 1, walk.deadline, a.err);
 #pragma unroll
                         for (int t = 0; t < MT; t++) {
                             if (!ok || t * 128 >= g.rows) break;
@@ -346,12 +348,12 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
         // armed, after a timeout, ends at the deadline)
         if (lane == 0) {
             for (int i = 0; i < KST && i < n; i++)
-                mbar_wait(&k_full[i], ((i + (n - 1 - i) / KST * KST) / KST) & 1, deadline, a.err);
+                mbar_wait(&k_full[i], ((i + (n - 1 - i) / KST * KST) / KST) & 1, walk.deadline, a.err);
             for (int i = 0; i < VST && i < n; i++)
-                mbar_wait(&v_full[i], ((i + (n - 1 - i) / VST * VST) / VST) & 1, deadline, a.err);
+                mbar_wait(&v_full[i], ((i + (n - 1 - i) / VST * VST) / VST) & 1, walk.deadline, a.err);
 #pragma unroll
             for (int t = 0; t < MT; t++)
-                if (qn[t] > 0) mbar_wait(&q_full[t], (qn[t] - 1) & 1, deadline, a.err);
+                if (qn[t] > 0) mbar_wait(&q_full[t], (qn[t] - 1) & 1, walk.deadline, a.err);
         }
     } else if (warp == 1) {
         // ---------------------------------------------------------------- MMA issuer
@@ -370,7 +372,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
         while (ok && walk.next(a, &g, &s, &w, &pos_hi, lane)) {
             const int nt = (g.rows + 127) / 128, nb = g.blk1 - g.blk0;
             if (elect_one()) {
-                auto wait = [&](uint64_t* bar, int phase) { return mbar_wait(bar, phase & 1, deadline, a.err); };
+                auto wait = [&](uint64_t* bar, int phase) { return mbar_wait(bar, phase & 1, walk.deadline, a.err); };
                 // S of block j (of this segment), tile t (offsets in descriptors: 16 bytes)
                 auto qk = [&](int j, int t, int buf) {
                     const uint64_t kb = kd + (uint64_t)((n + j) % KST * (KV_BLK / 16));
@@ -464,7 +466,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
         while (ok && walk.next(a, &g, &s, &w, &pos_hi, lane)) {
             for (int j = g.blk0; j < g.blk1 && ok; j++, n++) {
                 const int vs = n % VST, kbase = w.first + j * BLK;
-                ok = __all_sync(0xffffffffu, mbar_wait(&v_full[vs], (n / VST) & 1, deadline, a.err));
+                ok = __all_sync(0xffffffffu, mbar_wait(&v_full[vs], (n / VST) & 1, walk.deadline, a.err));
                 if (!ok) break;
                 if (!(kbase + BLK <= s.ctx && (a.window <= 0 || (long long)pos_hi - kbase < a.window))) {
                     uint8_t* vb = vring + vs * KV_BLK;
@@ -619,7 +621,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                     if (__any_sync(0xffffffffu, mx > m + RESCALE_THRESHOLD)) {
                         const float mn = fmaxf(m, mx);
                         const float cf = mn == -INFINITY ? 1.f : ex2(m - mn);
-                        if (j > 0 && !(ok = __all_sync(0xffffffffu, mbar_wait(&o_done[t], (cnt - 1) & 1, deadline, a.err))))
+                        if (j > 0 && !(ok = __all_sync(0xffffffffu, mbar_wait(&o_done[t], (cnt - 1) & 1, walk.deadline, a.err))))
                             return true;
                         if (j > 0) {                    // O holds the blocks before this one now
                             tc_fence_after_sync();
@@ -680,7 +682,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                     const int kbase = w.first + (g.blk0 + j) * BLK;
                     const bool whole = kbase + BLK <= s.ctx && (a.window <= 0 || (long long)pos_hi - kbase < a.window);
                     const uint32_t srow = trow + cnt % SB * 128;
-                    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t * SB + cnt % SB], (cnt / SB) & 1, deadline, a.err));
+                    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t * SB + cnt % SB], (cnt / SB) & 1, walk.deadline, a.err));
                     if (!ok) continue;
                     if (idle) {                         // their P is whatever S held: no other row reads it
                         mbar_arrive(&p_full[(t * SB + cnt % SB) * 2]);
@@ -698,7 +700,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                     cnt++;
                 }
                 // epilogue: the last P V has landed
-                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&o_done[t], (cnt - 1) & 1, deadline, a.err));
+                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&o_done[t], (cnt - 1) & 1, walk.deadline, a.err));
                 if (ok) {
                     tc_fence_after_sync();
                     const bool full = g.blk0 == 0 && g.blk1 == g.nblk;
@@ -761,7 +763,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
         }
     }
     // every MMA must have finished before tensor memory is released
-    if (threadIdx.x == 0) mbar_wait(done, 0, deadline, a.err);
+    if (threadIdx.x == 0) mbar_wait(done, 0, walk.deadline, a.err);
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();

@@ -651,12 +651,13 @@ CKL_API size_t ckl_tree_workspace_size(const ckl_tree_params* p);
  * seen when  p < L_b - T_b, or the mask's bit of drafted token p - (L_b - T_b) is set; and
  *            qpos - kpos < window.
  * qpos = positions[n]; kpos = p for the context, the position of the drafted token for its
- * key. out [N,Hq,128] = softmax(s) v in fp16, lse [N,Hq] fp32 natural log; a token that sees
- * nothing gives out = 0, lse = -inf. Keys that a token does not see, and cache places behind
- * the sequence, do not reach its result even where they hold infinities or NaN. With
- * max_q = 1 and no options the results are ckl_decode_attention's up to the fp32 summation
- * order. G = Hq/Hkv is any integer from 1 to 128. A sequence with more than max_q tokens has
- * the tokens behind max_q left unwritten and records CKL_INVALID_ARG
+ * key (with slopes, kpos - qpos must fit an int). out [N,Hq,128] = softmax(s) v in fp16, lse
+ * [N,Hq] fp32 natural log; a token that sees nothing gives out = 0, lse = -inf. Keys that a
+ * token does not see, and cache places behind the sequence, do not reach its result even where
+ * they hold infinities or NaN. With max_q = 1 and no options the results are
+ * ckl_decode_attention's up to the fp32 summation order. G = Hq/Hkv is any integer from 1 to
+ * 128. A sequence with more than max_q tokens has the tokens behind max_q left unwritten and
+ * records CKL_INVALID_ARG
  * (ckl_check_device_error). Two calls in flight need two workspaces. */
 CKL_API ckl_status ckl_tree_attention(const ckl_tree_params* p, void* out, float* lse,
                                       void* workspace, size_t workspace_bytes, void* stream);
@@ -665,9 +666,9 @@ CKL_API ckl_status ckl_tree_attention(const ckl_tree_params* p, void* out, float
  *   acc[b][p] = decay * acc[b][p] + sum over the sequence's tokens i and all heads of
  *               exp(s - lse[n][h]), for p < L_b
  * with s and the seen keys as in ckl_tree_attention and lse its output (a row with lse = -inf
- * adds nothing). acc fp32, rows acc_stride elements apart; places p >= acc_stride are not
- * kept, places from L_b on are left. Sums are taken in a fixed order. p->num_chunks and
- * chunk_tokens are not read. */
+ * adds nothing). decay in [0, 1]; 0 does not read acc. acc fp32, rows acc_stride elements apart;
+ * places p >= acc_stride are not kept, places from L_b on are left. Sums are taken in a fixed
+ * order. p->num_chunks and chunk_tokens are not read. */
 CKL_API ckl_status ckl_cache_weights(const ckl_tree_params* p, const float* lse, float* acc,
                                      long long acc_stride, float decay, void* stream);
 
@@ -687,8 +688,9 @@ CKL_API ckl_status ckl_cache_select(const float* acc, long long acc_stride, cons
  * (ckl_check_device_error). keep_idx rows are keep_stride apart; keep_count is capped at it.
  * acc (optional, as in ckl_cache_weights): its entries move along, and those of places
  * [new length, L_b) become 0. new_len (optional, [B]): dst_start[b] + keep_count[b] (L_b for
- * a refused list). Pages that hold a moved token's new place must belong to that sequence
- * alone. */
+ * a refused list), apart from every input. Pages that hold a moved token's new place must belong
+ * to that sequence alone; a token whose page id is outside [0, num_pages) moves as zeros, and
+ * none moves to such a page. */
 CKL_API ckl_status ckl_cache_compact(void* k_cache, void* v_cache, const int* kv_indptr,
                                      const int* kv_indices, const int* kv_last_page_len, int B,
                                      int Hkv, int num_pages, const int* keep_idx, int keep_stride,

@@ -151,3 +151,18 @@ def test_rope_plan_refuses(ckl, kw):
     with pytest.raises(ckl.CklError) as e:
         ckl.rope_plan(**kw)
     assert e.value.status == INVALID
+
+
+def test_compact_refuses_outputs_that_overlap(ckl):
+    """What one part of the call writes, other parts still read."""
+    L = ckl.lib()
+    # caches of 4 pages x 16 x 2 heads x 256 bytes = 32 KB; five sequences
+    com = lambda k, v, cnt=P, start=None, new=None: L.ckl_cache_compact(
+        k, v, P + 0x400, P, P + 0x800, 5, 2, 4, P, 8, cnt, start, None, 0, new, None)
+    assert com(0x100000, 0x100000 + 32768 - 16) == INVALID
+    assert com(0x100000 + 16, 0x100000) == INVALID
+    for new in (P - 16, P, P + 16):
+        assert com(0x100000, 0x200000, new=new) == INVALID                 # keep_count
+    assert com(0x100000, 0x200000, start=P + 0x100, new=P + 0x100) == INVALID
+    assert com(0x100000, 0x200000, new=P + 0x414) == INVALID               # the end of kv_indptr
+    assert com(0x100000, 0x200000, new=P + 0x800) == INVALID               # kv_last_page_len

@@ -633,3 +633,51 @@ def test_python_refusals(ckl, dev):
                                                q_indptr=up(bt.q_indptr, dev)), ckl.rope_plan(128))
     with pytest.raises(ckl.CklError):
         ckl.cache_weights(p, torch.empty((5, 4), device=dev), torch.empty((1, 30), device=dev))
+
+
+def test_python_refuses_what_is_no_tensor(ckl, dev):
+    import torch
+    bt = ref.Batch([20, 30], [2, 3], 4, 2, 1)
+    t = table(bt, dev)
+    q, k, v = up(bt.q, dev), up(bt.k, dev), up(bt.v, dev)
+    for bad in (None, bt.k, 3):
+        with pytest.raises(ckl.CklError):
+            ckl.make_tree_params(q, bad, v, **t, max_len=30)
+        with pytest.raises(ckl.CklError):
+            ckl.make_append_params(q, bad, q[:, 2:], k, v, **t)
+        with pytest.raises(ckl.CklError):
+            ckl.make_append_params(q, q[:, :2], q[:, 2:], k, bad, **t)
+        with pytest.raises(ckl.CklError):
+            ckl.cache_select(bad, t["kv_indptr"], t["kv_last_page_len"], 4)
+    idx = torch.zeros((2, 4), dtype=torch.int32, device=dev)
+    cnt = torch.zeros(2, dtype=torch.int32, device=dev)
+    with pytest.raises(ckl.CklError):                          # the lengths over the counts
+        ckl.cache_compact(k, v, **t, keep_idx=idx, keep_count=cnt, new_len=cnt)
+
+
+def test_tree_and_weights_calls_longer_than_the_wait_limit(ckl, dev):
+    """The limit on a wait bounds a wait, not a call: 6144 units of 64 key blocks (about 42 a CTA,
+    over 2 ms) with a limit of 1 ms give what they give without one."""
+    import torch
+    T, G, Hkv, B, L = 6144, 1, 32, 8, 8192
+    g = torch.Generator(device=dev).manual_seed(3)
+    q = torch.randn((B * T, Hkv * G, 128), device=dev, dtype=torch.float16, generator=g)
+    k = torch.randn((64, 16, Hkv, 128), device=dev, dtype=torch.float16, generator=g)
+    v = torch.randn((64, 16, Hkv, 128), device=dev, dtype=torch.float16, generator=g)
+    i32 = lambda x: torch.as_tensor(x, dtype=torch.int32, device=dev)
+    pages = L // 16
+    indptr = i32([b * pages for b in range(B + 1)])
+    indices = torch.randint(0, 64, (B * pages,), device=dev, dtype=torch.int32, generator=g)
+    p = ckl.make_tree_params(q, k, v, indptr, indices, i32([16] * B), max_len=L, max_q=T,
+                             q_indptr=i32([b * T for b in range(B + 1)]))
+    out, lse = ckl.tree_attention(p)
+    acc = ckl.cache_weights(p, lse, torch.zeros((B, L), device=dev))
+    finish(ckl)
+    ckl.lib().ckl_set_spin_timeout_ns(1000000)
+    try:
+        o2, l2 = ckl.tree_attention(p)
+        a2 = ckl.cache_weights(p, lse, torch.zeros((B, L), device=dev))
+        finish(ckl)
+    finally:
+        ckl.lib().ckl_set_spin_timeout_ns(1000000000)
+    assert torch.equal(out, o2) and torch.equal(lse, l2) and torch.equal(acc, a2)
