@@ -559,7 +559,7 @@ ckl_status fill_args(const ckl_tree_params* p, Args* a) {
         a->cap_in = 2.f * LOG2E * p->sm_scale / p->softcap;
         a->cap_k = p->sm_scale / p->softcap;
         double k = a->scale_log2;
-        for (int i = 0; i < 5; i++, k *= (double)a->cap_k * a->cap_k) a->cap_poly[i] = (float)(TANH_POLY[i] * k);
+        for (int i = 0; i < 4; i++, k *= (double)a->cap_k * a->cap_k) a->cap_poly[i] = (float)(TANH_POLY[i] * k);
     }
     return CKL_OK;
 }
