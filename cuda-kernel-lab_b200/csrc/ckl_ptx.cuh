@@ -225,12 +225,6 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
         ::"r"(d_tmem), "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0u)
         : "memory");
 }
-// Moves registers between the warpgroups of a CTA (every warp of a warpgroup executes it): the
-// shares must add up to what the CTA was launched with.
-template <int N>
-__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N>
-__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 // True in one lane of a converged warp. A branch on it is known to hold a single thread, so the
 // operands of the tensor-core instructions in it can live in uniform registers: 32 cycles per
 // M=128 N=64 instruction (A in tensor memory) where a branch on lane == 0 takes 50, measured on

@@ -2,9 +2,9 @@
 // heads of a kv head) on the 5th-generation tensor cores.
 //
 // A CTA holds 128 * MT rows of one (sequence, kv head) as MT tiles, the M of tcgen05.mma, and
-// streams keys in blocks of 8 pages:
-//   S = Q K^T   M=128, N=128: Q and K (both K-major) in shared memory, S in tensor memory (128
-//               columns a tile);
+// streams keys in blocks of 8 pages, taken in parts of 128 keys (one tile) or 64 (two):
+//   S = Q K^T   M=128, N=a part: Q and K (both K-major) in shared memory, S in tensor memory, two
+//               buffers a tile;
 //   softmax     one thread per row: the row of S from tensor memory, online max and sum in
 //               registers, P = exp2(S - m) as fp16 back into tensor memory, over S;
 //   O += P V    M=128, N=128, K=16 a page: P from tensor memory, V (MN-major) from shared
@@ -12,10 +12,14 @@
 // Both tiles use the same K and V block: with 256 rows the stream is read once where the tensor
 // cores still keep up with it (512 flops per byte of K and V against the card's ~256).
 //
+// Tensor memory is what the parts are cut to: 512 columns hold two tiles' O and twice 64 columns of S
+// each. With one buffer of 128 the softmax waited for P V and the next S in turn (16 x 24 drafts,
+// capped: 118 us, now 109; 8 x 64 drafts, where the SM clock falls to 1.5 GHz under the products:
+// 147 us, now 149, as a product of N = 64 reads Q twice as often: 49 cycles per K = 16 step, of N =
+// 128 65).
+//
 // V pages arrive as one 4 KB box each, [64-dim half][16 tokens][64 dims]. K pages take a 2 KB box
-// per half, so that the block's 128 keys of a half lie together and S is one N = 128 product: with
-// 4 KB boxes the eight pages' 8-row groups form two operands of N = 64, and Q would be read from
-// shared memory twice as often (49 against 65 cycles per K = 16 step for half the keys).
+// per half, so that a part's keys of a half lie together and S is one product.
 //
 // Work is divided exactly: the key blocks of all (sequence, row group, kv head) units, end to
 // end, over one wave of CTAs. A unit that lies within one CTA is written out directly; where a
@@ -39,14 +43,16 @@ constexpr int Q_TILE = 128 * D * 2;                // 32 KB: dims 0-63 of 128 ro
 constexpr int VST = 2;                             // V blocks in flight
 template <int MT> struct Cfg {
     static constexpr int KST = MT == 1 ? 4 : 3;    // K blocks in flight
-    static constexpr int SB = MT == 1 ? 2 : 1;     // S buffers of a tile
-    static constexpr int TILE_COLS = SB * 128 + 128;   // tensor memory of a tile: S (and P), then O
+    static constexpr int SW = MT == 1 ? 128 : 64;  // keys of an S buffer: tensor memory holds two a tile
+    static constexpr int U = BLK / SW;             // parts of a block
+    static constexpr int PH = SW / 64;             // halves of P, 4 pages each
+    static constexpr int TILE_COLS = 2 * SW + 128; // tensor memory of a tile: S (and P) twice, then O
     static constexpr int THREADS = 128 + 128 * MT; // warps 0-3: TMA, MMA, two that look V over; then a thread per row
     static constexpr int ROWS = 128 * MT;
     static constexpr int OFF_K = MT * Q_TILE;
     static constexpr int OFF_V = OFF_K + KST * KV_BLK;
     static constexpr int OFF_BAR = OFF_V + VST * KV_BLK;
-    static constexpr int NBAR = 2 * KST + 3 * VST + (2 + 3 * SB) * MT + 2;
+    static constexpr int NBAR = 2 * KST + 3 * VST + (5 + 2 * PH) * MT + 2;
     static constexpr int SMEM = 1024 + OFF_BAR + NBAR * 8 + 32;
     static constexpr uint32_t TMEM_COLS = 512;
 };
@@ -171,7 +177,7 @@ __global__ void __launch_bounds__(Cfg<MT>::THREADS, 1)
 tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
             const __grid_constant__ CUtensorMap tmQ, const Args a) {
     using C = Cfg<MT>;
-    constexpr int KST = C::KST, SB = C::SB, COLS = C::TILE_COLS;
+    constexpr int KST = C::KST, SW = C::SW, U = C::U, PH = C::PH, COLS = C::TILE_COLS;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* sm = align_ptr<1024>(smem_raw);
     uint8_t* qs = sm;
@@ -184,12 +190,14 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
     uint64_t* v_ready = v_empty + VST;       // V looked over, where some row does not see it all
     uint64_t* q_empty = v_ready + VST;       // every S of a segment done: Q may be replaced
     uint64_t* q_full = q_empty + 1;          // [MT] Q of a segment is there
-    uint64_t* s_full = q_full + MT;          // [MT][SB] S written (MMA -> softmax)
-    // [MT][SB][2] P of pages 0-3 / 4-7 written (softmax -> MMA): one per S buffer, since with two the
-    // softmax may end the next block before the MMA warp has seen this one
-    uint64_t* p_full = s_full + MT * SB;
-    uint64_t* o_done = p_full + MT * SB * 2;      // [MT] O holds the block, its P has been read (MMA -> all)
-    uint64_t* done = o_done + MT;            // every issued MMA finished
+    uint64_t* s_full = q_full + MT;          // [MT][2] S written (MMA -> softmax)
+    // [MT][2][PH] P of four pages written (softmax -> MMA): one per S buffer, since the softmax may
+    // end the next part before the MMA warp has seen this one
+    uint64_t* p_full = s_full + MT * 2;
+    // [MT][2] O holds the part, its P has been read (MMA -> all): one per S buffer too, since the last
+    // part's P may be written before O holds the part before it
+    uint64_t* o_done = p_full + MT * 2 * PH;
+    uint64_t* done = o_done + MT * 2;          // every issued MMA finished
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
     volatile int* odd = reinterpret_cast<volatile int*>(tmem_slot + 1);   // unseen V held inf or NaN
     long long* range = reinterpret_cast<long long*>(tmem_slot + 2);       // {left, offset}, sequence
@@ -208,9 +216,11 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
         }
         for (int t = 0; t < MT; t++) {
             mbar_init(&q_full[t], a.q_tma ? 1 : 128);
-            for (int i = 0; i < SB; i++) mbar_init(&s_full[t * SB + i], 1);
-            for (int i = 0; i < 2 * SB; i++) mbar_init(&p_full[t * SB * 2 + i], 128);
-            mbar_init(&o_done[t], 1);
+            for (int i = 0; i < 2; i++) {
+                mbar_init(&s_full[t * 2 + i], 1);
+                mbar_init(&o_done[t * 2 + i], 1);
+            }
+            for (int i = 0; i < 2 * PH; i++) mbar_init(&p_full[t * 2 * PH + i], 128);
         }
         mbar_init(q_empty, 1);
         mbar_init(done, 1);
@@ -271,9 +281,6 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
     int pos_hi;
 
     if (warp < 4) {
-    // 384 threads are launched with 168 registers each, and a thread that holds a row of S needs
-    // more: 128 * 72 + 256 * 216 = 384 * 168
-    if (MT == 2) regs_down<72>();
     if (warp == 0) {
         // ---------------------------------------------------------------- TMA producer
         const uint64_t pol = policy_evict_first();
@@ -357,92 +364,79 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
         }
     } else if (warp == 1) {
         // ---------------------------------------------------------------- MMA issuer
-        // With one S buffer a tile's next S waits for its P V (P lies over the first half of S: the
-        // other half is written meanwhile); with two it runs ahead of the softmax.
-        const uint32_t idesc_s = umma_idesc_f16(128, BLK, false, false);
+        // S runs up to two parts ahead of P V, in the other buffer than the softmax reads: neither waits
+        // for the other
+        const uint32_t idesc_s = umma_idesc_f16(128, SW, false, false);
         const uint32_t idesc_o = umma_idesc_f16(128, D, false, true);
         const uint64_t qd = umma_desc_sw128(smem_u32(qs), 16, 1024);
         const uint64_t kd = umma_desc_sw128(smem_u32(kring), 16, 1024);
         const uint64_t vd = umma_desc_sw128(smem_u32(vring), HALF_TILE, 1024);
         bool ok = true;
         int n = 0;                                      // blocks before this segment
-        int done_blocks[MT], q_seen[MT];                // of each tile, before this segment
+        int done_parts[MT], q_seen[MT];                 // of each tile, before this segment
 #pragma unroll
-        for (int t = 0; t < MT; t++) done_blocks[t] = q_seen[t] = 0;
+        for (int t = 0; t < MT; t++) done_parts[t] = q_seen[t] = 0;
         while (ok && walk.next(a, &g, &s, &w, &pos_hi, lane)) {
-            const int nt = (g.rows + 127) / 128, nb = g.blk1 - g.blk0;
+            const int nt = (g.rows + 127) / 128, nb = g.blk1 - g.blk0, parts = nb * U;
             if (elect_one()) {
                 auto wait = [&](uint64_t* bar, int phase) { return mbar_wait(bar, phase & 1, walk.deadline, a.err); };
-                // S of block j (of this segment), tile t (offsets in descriptors: 16 bytes)
-                auto qk = [&](int j, int t, int buf) {
-                    const uint64_t kb = kd + (uint64_t)((n + j) % KST * (KV_BLK / 16));
+                // S of part x (of this segment), tile t (offsets in descriptors: 16 bytes)
+                auto qk = [&](int x, int t, int buf) {
+                    const int kn = n + x / U;
+                    const uint64_t kb = kd + (uint64_t)(kn % KST * (KV_BLK / 16) + x % U * (SW * 128 / 16));
                     const uint64_t qb = qd + (uint64_t)(t * (Q_TILE / 16));
-                    const uint32_t d = tmem + t * COLS + buf * 128;
+                    const uint32_t d = tmem + t * COLS + buf * SW;
 #pragma unroll
                     for (int kk = 0; kk < 8; kk++)
                         umma_f16(d, qb + ((kk >> 2) * (Q_TILE / 2) + (kk & 3) * 32) / 16,
                                  kb + ((kk >> 2) * (KV_BLK / 2) + (kk & 3) * 32) / 16, idesc_s, kk != 0);
-                };
-                auto qk_done = [&](int j, int t, int buf) {
-                    umma_commit(&s_full[t * SB + buf]);
-                    if (t == nt - 1) {
-                        umma_commit(&k_empty[(n + j) % KST]);
-                        if (j == nb - 1) umma_commit(q_empty);
+                    umma_commit(&s_full[t * 2 + buf]);
+                    if (t == nt - 1 && x % U == U - 1) {
+                        umma_commit(&k_empty[kn % KST]);
+                        if (x == parts - 1) umma_commit(q_empty);
                     }
                 };
-                ok = wait(&k_full[n % KST], n / KST);
-#pragma unroll
-                for (int t = 0; t < MT; t++) {
-                    if (t >= nt || !ok) break;
-                    const int c = done_blocks[t];
-                    ok = wait(&q_full[t], q_seen[t]);
-                    // every P of the earlier segment has been read
-                    if (ok && c > 0) ok = wait(&o_done[t], c - 1);
-                    if (!ok) break;
-                    tc_fence_after_sync();
-                    qk(0, t, c % SB);
-                    qk_done(0, t, c % SB);
-                }
-                for (int j = 0; j < nb && ok; j++) {
-                    const int vs = (n + j) % VST, k1 = n + j + 1;
-                    const uint64_t vb = vd + (uint64_t)(vs * (KV_BLK / 16));
+                // S of part x for every tile; its buffer's P belongs to part x - 2, or to the earlier
+                // segment, all of whose P has been read when its last has
+                auto qk_all = [&](int x) {
+                    if (x >= parts) return;
+                    if (x % U == 0) ok = wait(&k_full[(n + x / U) % KST], (n + x / U) / KST);
 #pragma unroll
                     for (int t = 0; t < MT; t++) {
                         if (t >= nt || !ok) break;
-                        const int c = done_blocks[t] + j, buf = c % SB;
-                        const uint32_t sb = tmem + t * COLS + buf * 128, o = tmem + t * COLS + SB * 128;
-                        if (SB == 2 && j + 1 < nb) {
-                            // S of the next block into the other buffer, whose P belongs to block j - 1
-                            ok = wait(&k_full[k1 % KST], k1 / KST);
-                            if (ok && j > 0) ok = wait(&o_done[t], c - 1);
-                            if (!ok) break;
-                            tc_fence_after_sync();
-                            qk(j + 1, t, buf ^ 1);
-                            qk_done(j + 1, t, buf ^ 1);
-                        }
+                        const int c = done_parts[t] + x, before = x < 2 ? done_parts[t] - 1 : c - 2;
+                        if (x == 0) ok = wait(&q_full[t], q_seen[t]);
+                        if (ok && before >= 0) ok = wait(&o_done[t * 2 + (before & 1)], before >> 1);
+                        if (!ok) break;
+                        tc_fence_after_sync();
+                        qk(x, t, c & 1);
+                    }
+                };
+                qk_all(0);
+                if (ok) qk_all(1);
+                for (int x = 0; x < parts && ok; x++) {
+                    const int vn = n + x / U, vs = vn % VST;
+                    const uint64_t vb = vd + (uint64_t)(vs * (KV_BLK / 16) + x % U * (SW / PAGE * KV_TILE / 16));
 #pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            if (ok) ok = wait(&p_full[(t * SB + buf) * 2 + h], c / SB);
-                            if (ok && t == 0 && h == 0) ok = wait(&v_full[vs], (n + j) / VST) && wait(&v_ready[vs], (n + j) / VST);
+                    for (int t = 0; t < MT; t++) {
+                        if (t >= nt || !ok) break;
+                        const int c = done_parts[t] + x, buf = c & 1;
+                        const uint32_t sb = tmem + t * COLS + buf * SW, o = tmem + t * COLS + 2 * SW;
+#pragma unroll
+                        for (int h = 0; h < PH; h++) {
+                            if (ok) ok = wait(&p_full[(t * 2 + buf) * PH + h], c >> 1);
+                            if (ok && t == 0 && h == 0 && x % U == 0) ok = wait(&v_full[vs], vn / VST) && wait(&v_ready[vs], vn / VST);
                             if (!ok) break;
                             tc_fence_after_sync();
 #pragma unroll
                             for (int pg = 4 * h; pg < 4 * h + 4; pg++)
-                                umma_f16_ts(o, sb + pg * 8, vb + pg * (KV_TILE / 16), idesc_o, pg != 0 || j != 0);
+                                umma_f16_ts(o, sb + pg * 8, vb + pg * (KV_TILE / 16), idesc_o, pg != 0 || x != 0);
                         }
                         if (!ok) break;
-                        umma_commit(&o_done[t]);
-                        if (t == nt - 1) umma_commit(&v_empty[vs]);
-                        if (SB == 1 && j + 1 < nb) {
-                            if (t == 0) ok = wait(&k_full[k1 % KST], k1 / KST);
-                            // P, over S, must have been read
-                            if (ok) ok = wait(&o_done[t], c);
-                            if (!ok) break;
-                            tc_fence_after_sync();
-                            qk(j + 1, t, 0);
-                            qk_done(j + 1, t, 0);
-                        }
+                        umma_commit(&o_done[t * 2 + buf]);
+                        if (t == nt - 1 && x % U == U - 1) umma_commit(&v_empty[vs]);
                     }
+                    if (ok) qk_all(x + 2);
                 }
             }
             ok = __all_sync(0xffffffffu, ok);
@@ -450,7 +444,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
 #pragma unroll
             for (int t = 0; t < MT; t++)
                 if (t < nt) {
-                    done_blocks[t] += nb;
+                    done_parts[t] += parts;
                     q_seen[t]++;
                 }
         }
@@ -505,16 +499,18 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
         }
     }
     } else {
-        if (MT == 2) regs_up<216>();
         // ---------------------------------------------------------------- softmax: a row per thread
         const int t = (warp - 4) >> 2, quarter = warp & 3;
         const int r = quarter * 32 + lane;              // row of the tile
         const uint32_t trow = tmem + t * COLS + ((uint32_t)(quarter * 32) << 16);
-        const uint32_t orow_t = trow + SB * 128;        // this thread's row of O
+        const uint32_t orow_t = trow + 2 * SW;        // this thread's row of O
         bool ok = true;
-        int cnt = 0, n = 0;                             // blocks of this tile; blocks of the CTA
+        int cnt = 0;                                    // parts of this tile
+        auto o_wait = [&](int c) {
+            return __all_sync(0xffffffffu, mbar_wait(&o_done[t * 2 + (c & 1)], (c >> 1) & 1, walk.deadline, a.err));
+        };
         while (walk.next(a, &g, &s, &w, &pos_hi, lane)) {
-            const int nt = (g.rows + 127) / 128, nb = g.blk1 - g.blk0;
+            const int nt = (g.rows + 127) / 128, parts = (g.blk1 - g.blk0) * U;
             if (t < nt) {
                 const int rr = g.row0 + t * 128 + r;
                 Row row;
@@ -535,12 +531,12 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
 
                 const bool idle = t * 128 + quarter * 32 >= g.rows;   // only padding rows: no softmax
                 float m = -INFINITY, l = 0.f;
-                // One block of the row: S from tensor memory, P back. Where every row sees every key S is
+                // One part of the row: S from tensor memory, P back. Where every row sees every key S is
                 // held in registers, with a version each for plain scores (1), capped ones (2), a
                 // distance bias (3) and both (4). Other blocks -- the last one or two, a window's
                 // border, scores beyond the polynomial of the cap -- go through rolled loops (0), scores
                 // back into tensor memory in between: little code to fetch.
-                auto soft = [&](auto kind_, int j, int kbase, uint32_t srow) {
+                auto soft = [&](auto kind_, int x, int kbase, uint32_t srow) {
                     constexpr int KIND = decltype(kind_)::value;
                     constexpr bool HELD = KIND != 0, CAP = KIND == 2 || KIND == 4, BIAS = KIND >= 3;
                     const float2 sc2 = make_float2(a.scale_log2, a.scale_log2);
@@ -553,8 +549,10 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                         };
                         see0 = seen(0);
                         see1 = seen(1);
-                        see2 = seen(2);
-                        see3 = seen(3);
+                        if (SW == 128) {
+                            see2 = seen(2);
+                            see3 = seen(3);
+                        }
                     }
                     auto scored = [&](int q, float (&x)[32]) {
                         score32<EXT>(a, x);
@@ -566,18 +564,18 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
 #pragma unroll
                         for (int c = 0; c < 32; c++) x[c] = (v >> c) & 1u ? x[c] : -INFINITY;
                     };
-                    float row_s[HELD ? 4 : 1][32];
+                    float row_s[HELD ? SW / 32 : 1][32];
                     float mx = -INFINITY;
                     if (HELD) {
 #pragma unroll
-                        for (int q = 0; q < 4; q++)
+                        for (int q = 0; q < SW / 32; q++)
                             tmem_ld32(srow + q * 32, reinterpret_cast<uint32_t(&)[32]>(row_s[HELD ? q : 0]));
                         tmem_ld_wait();
                     }
                     if (CAP) {
                         float lo = INFINITY;
 #pragma unroll
-                        for (int q = 0; q < 4; q++)
+                        for (int q = 0; q < SW / 32; q++)
 #pragma unroll
                             for (int c = 0; c < 32; c += 2) {
                                 const float x0 = row_s[HELD ? q : 0][c], x1 = row_s[HELD ? q : 0][c + 1];
@@ -586,8 +584,8 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                             }
                         if (__any_sync(0xffffffffu, !(fmaxf(mx, -lo) * a.cap_k <= CAP_SMALL))) return false;
                     }
-#pragma unroll(HELD ? 4 : 1)
-                    for (int q = 0; q < 4; q++) {
+#pragma unroll(HELD ? SW / 32 : 1)
+                    for (int q = 0; q < SW / 32; q++) {
                         float (&x)[32] = row_s[HELD ? q : 0];
                         if (!HELD) {
                             tmem_ld32(srow + q * 32, reinterpret_cast<uint32_t(&)[32]>(x));
@@ -621,9 +619,9 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                     if (__any_sync(0xffffffffu, mx > m + RESCALE_THRESHOLD)) {
                         const float mn = fmaxf(m, mx);
                         const float cf = mn == -INFINITY ? 1.f : ex2(m - mn);
-                        if (j > 0 && !(ok = __all_sync(0xffffffffu, mbar_wait(&o_done[t], (cnt - 1) & 1, walk.deadline, a.err))))
+                        if (x > 0 && !(ok = o_wait(cnt - 1)))
                             return true;
-                        if (j > 0) {                    // O holds the blocks before this one now
+                        if (x > 0) {                    // O holds the parts before this one now
                             tc_fence_after_sync();
 #pragma unroll
                             for (int c0 = 0; c0 < D; c0 += 32) {
@@ -645,8 +643,8 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                     float2 l4[4];
 #pragma unroll
                     for (int i = 0; i < 4; i++) l4[i] = make_float2(0.f, 0.f);
-#pragma unroll(HELD ? 2 : 1)
-                    for (int h = 0; h < 2; h++) {        // pages 4h .. 4h + 3
+#pragma unroll(HELD ? PH : 1)
+                    for (int h = 0; h < PH; h++) {        // pages 4h .. 4h + 3
                         uint32_t pk[32];
 #pragma unroll
                         for (int u = 0; u < 2; u++) {
@@ -671,36 +669,35 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                         tmem_st32(srow + h * 32, pk);
                         tmem_st_wait();
                         tc_fence_before_sync();
-                        mbar_arrive(&p_full[(t * SB + cnt % SB) * 2 + h]);
+                        mbar_arrive(&p_full[(t * 2 + (cnt & 1)) * PH + h]);
                     }
                     const float2 l2 = add2(add2(l4[0], l4[1]), add2(l4[2], l4[3]));
                     l += l2.x + l2.y;
                     return true;
                 };
                 const bool capped = EXT && a.cap_log2 > 0.f, biased = EXT && a.slopes;
-                for (int j = 0; j < nb; j++) {
-                    const int kbase = w.first + (g.blk0 + j) * BLK;
-                    const bool whole = kbase + BLK <= s.ctx && (a.window <= 0 || (long long)pos_hi - kbase < a.window);
-                    const uint32_t srow = trow + cnt % SB * 128;
-                    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t * SB + cnt % SB], (cnt / SB) & 1, walk.deadline, a.err));
+                for (int x = 0; x < parts; x++) {
+                    const int kbase = w.first + g.blk0 * BLK + x * SW;
+                    const bool whole = kbase + SW <= s.ctx && (a.window <= 0 || (long long)pos_hi - kbase < a.window);
+                    const uint32_t srow = trow + (cnt & 1) * SW;
+                    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t * 2 + (cnt & 1)], (cnt >> 1) & 1, walk.deadline, a.err));
                     if (!ok) continue;
                     if (idle) {                         // their P is whatever S held: no other row reads it
-                        mbar_arrive(&p_full[(t * SB + cnt % SB) * 2]);
-                        mbar_arrive(&p_full[(t * SB + cnt % SB) * 2 + 1]);
+                        for (int h = 0; h < PH; h++) mbar_arrive(&p_full[(t * 2 + (cnt & 1)) * PH + h]);
                         cnt++;
                         continue;
                     }
                     tc_fence_after_sync();
                     bool did = false;
-                    if (whole && !EXT) did = soft(std::integral_constant<int, 1>{}, j, kbase, srow);
-                    if (EXT && whole && capped && !biased) did = soft(std::integral_constant<int, EXT ? 2 : 1>{}, j, kbase, srow);
-                    if (EXT && whole && !capped && biased) did = soft(std::integral_constant<int, EXT ? 3 : 1>{}, j, kbase, srow);
-                    if (EXT && whole && capped && biased) did = soft(std::integral_constant<int, EXT ? 4 : 1>{}, j, kbase, srow);
-                    if (!did) soft(std::integral_constant<int, 0>{}, j, kbase, srow);
+                    if (whole && !EXT) did = soft(std::integral_constant<int, 1>{}, x, kbase, srow);
+                    if (EXT && whole && capped && !biased) did = soft(std::integral_constant<int, EXT ? 2 : 1>{}, x, kbase, srow);
+                    if (EXT && whole && !capped && biased) did = soft(std::integral_constant<int, EXT ? 3 : 1>{}, x, kbase, srow);
+                    if (EXT && whole && capped && biased) did = soft(std::integral_constant<int, EXT ? 4 : 1>{}, x, kbase, srow);
+                    if (!did) soft(std::integral_constant<int, 0>{}, x, kbase, srow);
                     cnt++;
                 }
                 // epilogue: the last P V has landed
-                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&o_done[t], (cnt - 1) & 1, walk.deadline, a.err));
+                if (ok) ok = o_wait(cnt - 1);
                 if (ok) {
                     tc_fence_after_sync();
                     const bool full = g.blk0 == 0 && g.blk1 == g.nblk;
@@ -759,7 +756,6 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                     tc_fence_before_sync();
                 }
             }
-            n += nb;
         }
     }
     // every MMA must have finished before tensor memory is released

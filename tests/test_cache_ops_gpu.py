@@ -681,3 +681,16 @@ def test_tree_and_weights_calls_longer_than_the_wait_limit(ckl, dev):
     finally:
         ckl.lib().ckl_set_spin_timeout_ns(1000000000)
     assert torch.equal(out, o2) and torch.equal(lse, l2) and torch.equal(acc, a2)
+
+
+@pytest.mark.parametrize("toks,Hq", [(16, 16), (32, 16), (5, 16)])
+def test_tree_short_sequences_many_times(ckl, dev, toks, Hq):
+    """Two to four key blocks a sequence: the softmax ends the last block while the product of the
+    one before it may still wait for its V. The output must hold both, in every call."""
+    bt = ref.Batch([129 + 17 * i for i in range(20)], [toks] * 20, Hq, 2, 43)
+    o, l = check_tree(ckl, dev, bt, force=1)
+    p = run_tree(ckl, dev, bt, force=1)
+    for _ in range(100):
+        out, lse = ckl.tree_attention(p)
+        assert np.array_equal(out.float().cpu().numpy(), o) and np.array_equal(lse.cpu().numpy(), l)
+    finish(ckl)
