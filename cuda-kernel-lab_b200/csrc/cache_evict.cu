@@ -31,7 +31,9 @@ using tree::Seq;
 // staged once and the blocks' K tiles stream past it. Warp 0 loads K (TMA), warp 1 issues the MMAs,
 // warps 2-3 stage Q and the rows' lse, position and slope, and two groups of four warps turn S into
 // weights: for many rows each takes half of the columns of every tile, for few rows, where a tile
-// is mostly waiting, the tiles of every other kv head.
+// is mostly waiting, the tiles of every other kv head. One token of 32 heads over 8 x 8192 keys: 29.4
+// us for 134.8 MB (4.6 TB/s in all, the start and the end of the stream a third of it); 32 tokens over
+// 3 x 7001 keys and 4 kv heads, 256 rows of S a key: 24 us, the exponentials and the start.
 constexpr int W_THREADS = 384;
 constexpr int W_BLK = 128;                     // keys of a tile
 constexpr int W_BLK_PAGES = W_BLK / PAGE;
@@ -748,7 +750,8 @@ struct CArgs {
 // list: every thread loads its pieces of tile t + 1, the CTA meets (tile t has been read), and
 // every thread stores tile t: 64 KB are on their way while 64 KB are written. The places are
 // translated to cache rows ahead of time, so that no load waits for an index. No CTA waits for
-// another. ROWS: list entries translated at a time. The accepted paths of drafts are a few rows a
+// another. 8 x 4096 rows of 8 heads: 55.8 us, 4.8 TB/s of pieces of 256 bytes that lie 2 KB apart.
+// ROWS: list entries translated at a time. The accepted paths of drafts are a few rows a
 // sequence: small CTAs, so that all of them are resident (512 threads: 10.3 us at 32 x 5 rows,
 // 128: 3.3 us). grid = (Hkv * 16 / pieces (+ 1 for acc and the lengths), B, 2).
 template <int C_THREADS, int C_ROWS>
