@@ -33,7 +33,8 @@ using tree::Seq;
 // weights: for many rows each takes half of the columns of every tile, for few rows, where a tile
 // is mostly waiting, the tiles of every other kv head. One token of 32 heads over 8 x 8192 keys: 29.4
 // us for 134.8 MB (4.6 TB/s in all, the start and the end of the stream a third of it); 32 tokens over
-// 3 x 7001 keys and 4 kv heads, 256 rows of S a key: 24 us, the exponentials and the start.
+// 3 x 7001 keys and 4 kv heads, 256 rows of S a key: 22 us, the exponentials and the start (24 with a
+// masked block's columns tested one by one).
 constexpr int W_THREADS = 384;
 constexpr int W_BLK = 128;                     // keys of a tile
 constexpr int W_BLK_PAGES = W_BLK / PAGE;
@@ -114,27 +115,30 @@ __device__ __forceinline__ uint32_t bits32(uint32_t v0, uint32_t v1, uint32_t v2
     return __funnelshift_r(lo, hi, at & 31);
 }
 
+// Of 32 columns, of which the first is `skip` rows into its token, those whose token's bit in `see` (the
+// first column's is bit 0) is set, and only the first `valid`: a token at a time, not a column.
+__device__ __forceinline__ uint32_t columns(uint32_t see, int G, int skip, int valid) {
+    uint32_t v = 0u;
+    for (int lo = -skip; lo < 32 && see; lo += G, see >>= 1) {
+        const uint32_t from = 0xffffffffu << max(lo, 0), upto = lo + G < 32 ? ~(0xffffffffu << (lo + G)) : 0xffffffffu;
+        v |= see & 1u ? from & upto : 0u;
+    }
+    return valid < 32 ? v & ~(0xffffffffu << max(valid, 0)) : v;
+}
+
 // Sum of the weights of M <= 32 columns from `col` on; x holds their scores (bias excluded). Where
-// not every column is a row that sees the key (`whole`), bit i of `see` says whether the token i
-// behind the first column's does.
+// not every column is a row that sees the key (`whole`), bit i of `cols` says whether column col + i
+// does.
 template <bool EXT, int M>
-__device__ __forceinline__ float weigh(const tree::Args& a, const RowInfo& in, bool whole, int kpos, uint32_t see, int col,
+__device__ __forceinline__ float weigh(const tree::Args& a, const RowInfo& in, bool whole, int kpos, uint32_t cols, int col,
                                        float (&x)[M]) {
     if (EXT && a.slopes) {
 #pragma unroll
         for (int i = 0; i < M; i++) x[i] += tree::bias<EXT>(a, *in.slope2(col + i), *in.pos(col + i), kpos);
     }
     if (!whole) {
-        const int t0 = *in.i(col);
 #pragma unroll
-        for (int i = 0; i < M; i += 4) {
-            const int4 t = *reinterpret_cast<const int4*>(in.i(col + i));
-            auto keep = [&](int tok) { return ((see >> ((tok - t0) & 31)) & ~(uint32_t)(tok >> 31) & 1u) != 0u; };
-            x[i] = keep(t.x) ? x[i] : -INFINITY;
-            x[i + 1] = keep(t.y) ? x[i + 1] : -INFINITY;
-            x[i + 2] = keep(t.z) ? x[i + 2] : -INFINITY;
-            x[i + 3] = keep(t.w) ? x[i + 3] : -INFINITY;
-        }
+        for (int i = 0; i < M; i++) x[i] = (cols >> i) & 1u ? x[i] : -INFINITY;
     }
     float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
 #pragma unroll
@@ -422,6 +426,17 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             const int pg0 = max(g.pg0, first), nb = max(0, (g.pg1 - pg0 + W_BLK_PAGES - 1) / W_BLK_PAGES);
             const int rchunks = (nrows + N - 1) / N, chunks = nb > 0 ? a.Hkv * rchunks : 0;
             for (int j = 0; j < nb; j++) sums[(hf * W_SEG + j) * W_BLK + key] = 0.f;
+            // the old weights are on their way while the scores are made
+            const bool keeps = hf == 0 && w.decay != 0.f;
+            auto has = [&](int j) {                              // block j's key of this thread has an entry
+                const int p = (pg0 + j * W_BLK_PAGES) * PAGE + key;
+                return j < nb && p < s.len && p < g.pg1 * PAGE && p < w.acc_stride;
+            };
+            float* acc_row = w.acc + g.b * w.acc_stride + pg0 * PAGE + key;
+            float old[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (keeps && has(j)) old[j] = acc_row[j * W_BLK];
             for (int c = 0; c < chunks; c++, chunk++) {
                 const int ib = chunk % ibufs;
                 walk.renew(a, chunk);
@@ -478,14 +493,18 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                         v3 = seen(3);
                     }
                     float add = 0.f;
-                    auto see_of = [&](int c) { return whole ? 0xffffffffu : bits32(v0, v1, v2, v3, max(*in.i(c), t_lo) - t_lo); };
+                    auto cols_of = [&](int c) {
+                        if (whole && c + 32 <= valid) return 0xffffffffu;
+                        const int i = *in.i(c);
+                        return columns(whole ? 0xffffffffu : bits32(v0, v1, v2, v3, i - t_lo), a.G, r0 + c - i * a.G, valid - c);
+                    };
                     int col = c0;
                     for (; col + 32 <= c1 && col < valid; col += 32) {
                         float x[32];
                         tmem_ld32(trow + d_at + col, reinterpret_cast<uint32_t(&)[32]>(x));
                         tmem_ld_wait();
                         tree::score32<EXT>(a, x);
-                        add += weigh<EXT, 32>(a, in, whole && col + 32 <= valid, kpos, see_of(col), col, x);
+                        add += weigh<EXT, 32>(a, in, whole && col + 32 <= valid, kpos, cols_of(col), col, x);
                     }
                     for (; col < min(c1, valid); col += 8) {
                         float x[8];
@@ -493,7 +512,7 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                         tmem_ld_wait();
 #pragma unroll
                         for (int i = 0; i < 8; i++) x[i] = tree::score<EXT>(a, x[i]);
-                        add += weigh<EXT, 8>(a, in, whole && col + 8 <= valid, kpos, see_of(col), col, x);
+                        add += weigh<EXT, 8>(a, in, whole && col + 8 <= valid, kpos, cols_of(col), col, x);
                     }
                     tc_fence_before_sync();
                     mbar_arrive(&d_empty[d]);
@@ -509,14 +528,15 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                         float* dst = w.acc + g.b * w.acc_stride + p;
                         *dst = w.decay != 0.f ? w.decay * *dst : 0.f;
                     }
-                for (int j = 0; j < nb; j++) {
-                    const int p = (pg0 + j * W_BLK_PAGES) * PAGE + key;
-                    if (p < s.len && p < g.pg1 * PAGE && p < w.acc_stride) {
-                        float* dst = w.acc + g.b * w.acc_stride + p;
-                        const float x = sums[j * W_BLK + key] + sums[(W_SEG + j) * W_BLK + key];
-                        *dst = w.decay != 0.f ? fmaf(w.decay, *dst, x) : x;
-                    }
-                }
+                auto put = [&](int j, float before) {
+                    const float x = sums[j * W_BLK + key] + sums[(W_SEG + j) * W_BLK + key];
+                    acc_row[j * W_BLK] = w.decay != 0.f ? fmaf(w.decay, before, x) : x;
+                };
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (has(j)) put(j, old[j]);
+                for (int j = 4; j < nb; j++)
+                    if (has(j)) put(j, keeps ? acc_row[j * W_BLK] : 0.f);
             }
             asm volatile("bar.sync 1, 256;" ::: "memory");           // before the sums are cleared
         }
