@@ -31,10 +31,10 @@ using tree::Seq;
 // staged once and the blocks' K tiles stream past it. Warp 0 loads K (TMA), warp 1 issues the MMAs,
 // warps 2-3 stage Q and the rows' lse, position and slope, and two groups of four warps turn S into
 // weights: for many rows each takes half of the columns of every tile, for few rows, where a tile
-// is mostly waiting, the tiles of every other kv head. One token of 32 heads over 8 x 8192 keys: 29.4
-// us for 134.8 MB (4.6 TB/s in all, the start and the end of the stream a third of it); 32 tokens over
-// 3 x 7001 keys and 4 kv heads, 256 rows of S a key: 22 us, the exponentials and the start (24 with a
-// masked block's columns tested one by one).
+// is mostly waiting, the tiles of every other kv head. One token of 32 heads over 8 x 8192 keys: 28.7
+// us for 134.8 MB (4.7 TB/s in all, the start and the end of the stream a third of it); 32 tokens over
+// 3 x 7001 keys and 4 kv heads, 256 rows of S a key: 19.6 us, the exponentials and the start (24 with a
+// masked block's columns tested one by one, for every head).
 constexpr int W_THREADS = 384;
 constexpr int W_BLK = 128;                     // keys of a tile
 constexpr int W_BLK_PAGES = W_BLK / PAGE;
@@ -127,16 +127,16 @@ __device__ __forceinline__ uint32_t columns(uint32_t see, int G, int skip, int v
 }
 
 // Sum of the weights of M <= 32 columns from `col` on; x holds their scores (bias excluded). Where
-// not every column is a row that sees the key (`whole`), bit i of `cols` says whether column col + i
+// not every column is a row that sees the key (`full`), bit i of `cols` says whether column col + i
 // does.
 template <bool EXT, int M>
-__device__ __forceinline__ float weigh(const tree::Args& a, const RowInfo& in, bool whole, int kpos, uint32_t cols, int col,
+__device__ __forceinline__ float weigh(const tree::Args& a, const RowInfo& in, bool full, int kpos, uint32_t cols, int col,
                                        float (&x)[M]) {
     if (EXT && a.slopes) {
 #pragma unroll
         for (int i = 0; i < M; i++) x[i] += tree::bias<EXT>(a, *in.slope2(col + i), *in.pos(col + i), kpos);
     }
-    if (!whole) {
+    if (!full) {
 #pragma unroll
         for (int i = 0; i < M; i++) x[i] = (cols >> i) & 1u ? x[i] : -INFINITY;
     }
@@ -437,6 +437,9 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
 #pragma unroll
             for (int j = 0; j < 4; j++)
                 if (keeps && has(j)) old[j] = acc_row[j * W_BLK];
+            // columns of a masked tile that count, 32 a word: the same for every head, kept from one to the next
+            uint32_t m0 = 0u, m1 = 0u, m2 = 0u, m3 = 0u;
+            int masked = -1;                                     // the tile they are of
             for (int c = 0; c < chunks; c++, chunk++) {
                 const int ib = chunk % ibufs;
                 walk.renew(a, chunk);
@@ -456,55 +459,69 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                     tc_fence_after_sync();
                     const int kbase = (pg0 + j * W_BLK_PAGES) * PAGE, p = kbase + key;
                     const bool whole = kbase + W_BLK <= s.ctx && (a.window <= 0 || (long long)pos_hi - kbase < a.window);
+                    const bool full = whole && c1 <= valid;          // every column counts
                     const int kpos = whole ? p : s.pos(a, p);
-                    uint32_t v0 = 0u, v1 = 0u, v2 = 0u, v3 = 0u;     // tokens t_lo .. + 127 that see the key
-                    if (!whole && p < s.len) {
-                        const int k = p - s.ctx;                     // drafted index of the key
-                        const bool bits = k >= 0 && k < 32 * a.mask_words;
-                        const uint32_t* mw = a.mask + (size_t)(s.q0 + t_lo) * a.mask_words + (k >> 5);
-                        // tokens t_lo + 32 q .. that see the key
-                        auto seen = [&](int q) {
-                            const int n32 = min(nt - 32 * q, 32);
-                            if (n32 <= 0) return 0u;
-                            uint32_t v = 0xffffffffu;
-                            if (a.mask) {
-                                if (k >= 0) v = 0u;
-                                if (bits) {
+                    const int id = c % rchunks * W_SEG + j;
+                    if (!whole && id != masked) {
+                        masked = id;
+                        uint32_t v0 = 0u, v1 = 0u, v2 = 0u, v3 = 0u;     // tokens t_lo .. + 127 that see the key
+                        if (p < s.len) {
+                            const int k = p - s.ctx;                     // drafted index of the key
+                            const bool bits = k >= 0 && k < 32 * a.mask_words;
+                            const uint32_t* mw = a.mask + (size_t)(s.q0 + t_lo) * a.mask_words + (k >> 5);
+                            // tokens t_lo + 32 q .. that see the key
+                            auto seen = [&](int q) {
+                                const int n32 = min(nt - 32 * q, 32);
+                                if (n32 <= 0) return 0u;
+                                uint32_t v = 0xffffffffu;
+                                if (a.mask) {
+                                    if (k >= 0) v = 0u;
+                                    if (bits) {
 #pragma unroll 8
-                                    for (int i = 0; i < n32; i++)
-                                        v |= ((__ldg(mw + (size_t)(32 * q + i) * a.mask_words) >> (k & 31)) & 1u) << i;
+                                        for (int i = 0; i < n32; i++)
+                                            v |= ((__ldg(mw + (size_t)(32 * q + i) * a.mask_words) >> (k & 31)) & 1u) << i;
+                                    }
+                                } else {
+                                    const int f = k - t_lo - 32 * q;      // a chain: tokens from k on
+                                    v = f <= 0 ? 0xffffffffu : f >= 32 ? 0u : 0xffffffffu << f;
                                 }
-                            } else {
-                                const int f = k - t_lo - 32 * q;      // a chain: tokens from k on
-                                v = f <= 0 ? 0xffffffffu : f >= 32 ? 0u : 0xffffffffu << f;
-                            }
-                            if (a.window > 0) {
-                                for (int i = 0; i < n32; i++) {
-                                    const int t = t_lo + 32 * q + i;
-                                    const int tp = a.positions ? __ldg(a.positions + s.q0 + t) : s.ctx + t;
-                                    if ((long long)tp - kpos >= a.window) v &= ~(1u << i);
+                                if (a.window > 0) {
+                                    for (int i = 0; i < n32; i++) {
+                                        const int t = t_lo + 32 * q + i;
+                                        const int tp = a.positions ? __ldg(a.positions + s.q0 + t) : s.ctx + t;
+                                        if ((long long)tp - kpos >= a.window) v &= ~(1u << i);
+                                    }
                                 }
-                            }
-                            return v;
+                                return v;
+                            };
+                            v0 = seen(0);
+                            v1 = seen(1);
+                            v2 = seen(2);
+                            v3 = seen(3);
+                        }
+                        auto of = [&](int col) {
+                            if (col >= min(c1, valid)) return 0u;
+                            const int i = *in.i(col);
+                            return columns(bits32(v0, v1, v2, v3, i - t_lo), a.G, r0 + col - i * a.G, valid - col);
                         };
-                        v0 = seen(0);
-                        v1 = seen(1);
-                        v2 = seen(2);
-                        v3 = seen(3);
+                        m0 = of(c0);
+                        m1 = of(c0 + 32);
+                        m2 = of(c0 + 64);
+                        m3 = of(c0 + 96);
                     }
-                    float add = 0.f;
-                    auto cols_of = [&](int c) {
-                        if (whole && c + 32 <= valid) return 0xffffffffu;
-                        const int i = *in.i(c);
-                        return columns(whole ? 0xffffffffu : bits32(v0, v1, v2, v3, i - t_lo), a.G, r0 + c - i * a.G, valid - c);
+                    auto cols_of = [&](int col) {
+                        if (whole) return valid - col < 32 ? ~(0xffffffffu << (valid - col)) : 0xffffffffu;
+                        const int q = (col - c0) >> 5;
+                        return (q == 0 ? m0 : q == 1 ? m1 : q == 2 ? m2 : m3) >> ((col - c0) & 31);
                     };
+                    float add = 0.f;
                     int col = c0;
                     for (; col + 32 <= c1 && col < valid; col += 32) {
                         float x[32];
                         tmem_ld32(trow + d_at + col, reinterpret_cast<uint32_t(&)[32]>(x));
                         tmem_ld_wait();
                         tree::score32<EXT>(a, x);
-                        add += weigh<EXT, 32>(a, in, whole && col + 32 <= valid, kpos, cols_of(col), col, x);
+                        add += weigh<EXT, 32>(a, in, full, kpos, cols_of(col), col, x);
                     }
                     for (; col < min(c1, valid); col += 8) {
                         float x[8];
@@ -512,7 +529,7 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                         tmem_ld_wait();
 #pragma unroll
                         for (int i = 0; i < 8; i++) x[i] = tree::score<EXT>(a, x[i]);
-                        add += weigh<EXT, 8>(a, in, whole && col + 8 <= valid, kpos, cols_of(col), col, x);
+                        add += weigh<EXT, 8>(a, in, full, kpos, cols_of(col), col, x);
                     }
                     tc_fence_before_sync();
                     mbar_arrive(&d_empty[d]);
