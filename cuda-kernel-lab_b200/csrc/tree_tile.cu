@@ -14,8 +14,8 @@
 //
 // Tensor memory is what the parts are cut to: 512 columns hold two tiles' O and twice 64 columns of S
 // each. With one buffer of 128 the softmax waited for P V and the next S in turn (16 x 24 drafts,
-// capped: 118 us, now 109; 8 x 64 drafts, where the SM clock falls to 1.5 GHz under the products:
-// 147 us, now 149, as a product of N = 64 reads Q twice as often: 49 cycles per K = 16 step, of N =
+// capped: 118 us, with two 109; 8 x 64 drafts, where the SM clock falls to 1.5 GHz under the products:
+// 147 us and 149, as a product of N = 64 reads Q twice as often: 49 cycles per K = 16 step, of N =
 // 128 65).
 //
 // V pages arrive as one 4 KB box each, [64-dim half][16 tokens][64 dims]. K pages take a 2 KB box
@@ -690,6 +690,21 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                         continue;
                     }
                     tc_fence_after_sync();
+                    if (kbase >= s.len) {               // a part behind the sequence: weights of 0 (2 us less
+                                                        // than masking it: 16 x 24 drafts 106 us)
+                        uint32_t zero[32];
+#pragma unroll
+                        for (int c = 0; c < 32; c++) zero[c] = 0u;
+#pragma unroll
+                        for (int h = 0; h < PH; h++) {
+                            tmem_st32(srow + h * 32, zero);
+                            tmem_st_wait();
+                            tc_fence_before_sync();
+                            mbar_arrive(&p_full[(t * 2 + (cnt & 1)) * PH + h]);
+                        }
+                        cnt++;
+                        continue;
+                    }
                     bool did = false;
                     if (whole && !EXT) did = soft(std::integral_constant<int, 1>{}, x, kbase, srow);
                     if (EXT && whole && capped && !biased) did = soft(std::integral_constant<int, EXT ? 2 : 1>{}, x, kbase, srow);
