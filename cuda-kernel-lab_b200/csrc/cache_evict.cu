@@ -520,15 +520,14 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                         float x[32];
                         tmem_ld32(trow + d_at + col, reinterpret_cast<uint32_t(&)[32]>(x));
                         tmem_ld_wait();
-                        tree::score32<EXT>(a, x);
+                        tree::score_all<EXT>(a, x);
                         add += weigh<EXT, 32>(a, in, full, kpos, cols_of(col), col, x);
                     }
                     for (; col < min(c1, valid); col += 8) {
                         float x[8];
                         tmem_ld8(trow + d_at + col, reinterpret_cast<uint32_t(&)[8]>(x));
                         tmem_ld_wait();
-#pragma unroll
-                        for (int i = 0; i < 8; i++) x[i] = tree::score<EXT>(a, x[i]);
+                        tree::score_all<EXT>(a, x);
                         add += weigh<EXT, 8>(a, in, full, kpos, cols_of(col), col, x);
                     }
                     tc_fence_before_sync();

@@ -11,7 +11,9 @@
 //   more rows: tcgen05 on 128-row tiles (tree_tile.cu).
 
 #include <algorithm>
+#include <cfloat>
 #include <climits>
+#include <cmath>
 #include <mutex>
 
 #include "tree_tile.cuh"
@@ -42,7 +44,8 @@ struct Keys {
 // ------------------------------------------------------------------ up to 16 rows: mma.sync
 // Online-softmax state of one warp for a tile of 16 rows. Lane (g = lane/4, t = lane%4) holds rows
 // g and g+8, dims 8j + 2t + {0,1} of o[j], and the fragments of Q.
-template <bool EXT>
+// KIND: plain scores (0), a distance bias (1), a cap (2), with or without a bias.
+template <int KIND>
 struct State {
     float o[16][4];
     float m[2], l[2];
@@ -93,14 +96,13 @@ struct State {
             ldmatrix_x4_trans(vb + tile_off(v_key, 2 * i + v_hi), vf[i][0], vf[i][1], vf[i][2], vf[i][3]);
 #pragma unroll
         for (int c = 0; c < 8; c++) sc[c >> 2][c & 3] += sd[c >> 2][c & 3];
-        if (EXT && a.cap_log2 > 0.f) {
-#pragma unroll
-            for (int c = 0; c < 8; c++) sc[c >> 2][c & 3] = score<true>(a, sc[c >> 2][c & 3]);
+        if (KIND == 2) {
+            cap_all(a, reinterpret_cast<float (&)[8]>(sc));
         } else {
 #pragma unroll
             for (int c = 0; c < 8; c++) sc[c >> 2][c & 3] *= a.scale_log2;
         }
-        if (EXT && a.slopes) {
+        if (KIND == 1 || (KIND == 2 && a.slopes)) {
             int kp[4] = {kbase + 2 * t, kbase + 2 * t + 1, kbase + 8 + 2 * t, kbase + 9 + 2 * t};
             if (!whole) {
 #pragma unroll
@@ -219,7 +221,7 @@ struct State {
 // Bound by HBM for many sequences: 64 with a window of 2000 keys over 8 kv heads, one token each, 87-96
 // us by box for 483 MB, the last wave of CTAs not full; by latency for few (1 x 1000 keys: 12.5 us with the
 // merge). grid = (B * Hkv, num_chunks).
-template <bool EXT>
+template <int KIND>
 __global__ void __launch_bounds__(THREADS, 2)
 rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const Args a) {
     extern __shared__ uint8_t smem_raw[];
@@ -258,7 +260,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
     const int p0 = keys.beg / PAGE;
     const int npg = keys.end > keys.beg ? (keys.end - keys.beg + PAGE - 1) / PAGE : 0;
 
-    State<EXT> st;
+    State<KIND> st;
     const int g = lane >> 2, t = lane & 3;
     if (warp == CONSUMERS) {
         const uint64_t pol = policy_evict_first();
@@ -482,7 +484,9 @@ mask_kernel(const int* parents, const int* q_indptr, const int* indptr, const in
 }
 
 // ------------------------------------------------------------------ host
-const void* rows_fn(bool ext) { return ext ? (const void*)rows_kernel<true> : (const void*)rows_kernel<false>; }
+const void* rows_fn(int kind) {
+    return kind == 0 ? (const void*)rows_kernel<0> : kind == 1 ? (const void*)rows_kernel<1> : (const void*)rows_kernel<2>;
+}
 
 struct Setup {
     ckl_status st = CKL_OK;
@@ -493,8 +497,8 @@ const Setup* setup(const DeviceInfo* di) {
     std::call_once(once[di->device], [di] {
         Setup& k = ks[di->device];
         cudaError_t e = cudaSuccess;
-        for (int ext = 0; ext < 2 && e == cudaSuccess; ext++)
-            e = cudaFuncSetAttribute(rows_fn(ext), cudaFuncAttributeMaxDynamicSharedMemorySize, ROWS_SMEM);
+        for (int kind = 0; kind < 3 && e == cudaSuccess; kind++)
+            e = cudaFuncSetAttribute(rows_fn(kind), cudaFuncAttributeMaxDynamicSharedMemorySize, ROWS_SMEM);
         if (e != cudaSuccess) k.st = cuda_status(e, "tree attention setup");
     });
     return &ks[di->device];
@@ -557,11 +561,20 @@ ckl_status fill_args(const ckl_tree_params* p, Args* a) {
     a->num_pages = p->num_pages;
     a->scale_log2 = p->sm_scale * LOG2E;
     if (p->softcap > 0.f) {
+        // finite whatever the cap, so that a product of 0 is a score of 0
+        const double k = (double)p->sm_scale / p->softcap;
+        auto finite = [](double x) { return (float)std::min(x, (double)FLT_MAX); };
         a->cap_log2 = p->softcap * LOG2E;
-        a->cap_in = 2.f * LOG2E * p->sm_scale / p->softcap;
-        a->cap_k = p->sm_scale / p->softcap;
-        double k = a->scale_log2;
-        for (int i = 0; i < 4; i++, k *= (double)a->cap_k * a->cap_k) a->cap_poly[i] = (float)(TANH_POLY[i] * k);
+        a->cap_in = finite(2.0 * LOG2E * k);
+        a->cap_k = finite(k);
+        a->cap_lim = finite(CAP_SMALL / k);
+        const double poly[4] = {TANH_0, TANH_1, TANH_2, TANH_3};
+        double term = a->scale_log2;
+        for (int i = 0; i < 4; i++, term *= k * k) {
+            const double c = poly[i] * term;
+            if (!(std::fabs(c) >= FLT_MIN && std::fabs(c) <= FLT_MAX)) a->cap_lim = -1.f;
+            a->cap_poly[i] = (float)c;
+        }
     }
     return CKL_OK;
 }
@@ -690,12 +703,12 @@ ckl_status ckl_tree_attention(const ckl_tree_params* p, void* out, float* lse, v
     }
     const cudaStream_t s = (cudaStream_t)stream;
     if (use_tiles((long long)p->max_q * (p->Hq / p->Hkv))) return launch_tiles(p, a, workspace, tile_ctas(p, di->sms), s);
-    const bool ext = p->softcap > 0.f || p->slopes;
+    const int kind = p->softcap > 0.f ? 2 : p->slopes ? 1 : 0;
     CUtensorMap tmK, tmV;
     st = encode_page_maps(p->k_cache, p->v_cache, p->Hkv, p->num_pages, &tmK, &tmV);
     if (st != CKL_OK) return st;
     void* args[] = {&tmK, &tmV, &a};
-    CKL_CUDA_TRY(launch(rows_fn(ext), dim3((unsigned)(p->B * p->Hkv), (unsigned)p->num_chunks),
+    CKL_CUDA_TRY(launch(rows_fn(kind), dim3((unsigned)(p->B * p->Hkv), (unsigned)p->num_chunks),
                         dim3(THREADS), ROWS_SMEM, s, args, true));
     if (p->num_chunks == 1) return CKL_OK;
     void* margs[] = {&a};

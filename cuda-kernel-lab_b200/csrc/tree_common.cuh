@@ -30,6 +30,7 @@ struct Args {
     float cap_log2;           // softcap * log2(e), 0: no cap
     float cap_in;             // 2 log2(e) sm_scale / softcap
     float cap_k;              // sm_scale / softcap
+    float cap_lim;            // greatest |q.k| that cap_factor2 is for (-1: none)
     float cap_poly[4];        // of a capped score / q.k in (q.k)^2, see cap_factor2
     int q_tma;                // the tcgen05 kernel reads Q tiles through a tensor map
 };
@@ -126,53 +127,73 @@ struct Row {
     }
 };
 
-// Score in the log2 domain from the raw product q.k. The cap is tanh(x) = 1 - 2/(1 + e^2x):
-// its error is absolute, ~2^-23 of the cap, where tanh.approx would lose 2^-11 of the score.
-template <bool EXT>
-__device__ __forceinline__ float score(const Args& a, float qk) {
-    if (EXT && a.cap_log2 > 0.f)
-        return fmaf(-2.f * a.cap_log2, rcp(1.f + ex2(qk * a.cap_in)), a.cap_log2);
-    return qk * a.scale_log2;
-}
-// tanh(y)/y in y^2 for y <= CAP_SMALL: fitted to it by weighted least squares, off by at most 2^-21.9
-// of it, which is 2^-23 of the cap, as the exact form's own error. The launch scales the terms, so
-// that the polynomial is one in (q.k)^2.
-constexpr float TANH_POLY[4] = {0.99999976f, -0.33329466f, 0.13236369f, -0.04602819f};
+// tanh(y)/y in y^2 for |y| <= CAP_SMALL: fitted to it by weighted least squares, off by at most 2^-21.9
+// of it.
+constexpr float TANH_0 = 0.99999976f, TANH_1 = -0.33329466f, TANH_2 = 0.13236369f, TANH_3 = -0.04602819f;
 constexpr float CAP_SMALL = 0.45f;
-// Capped scores are nearly always far below the cap: up to CAP_SMALL of it a score is q.k times a
-// polynomial of degree 3 in (q.k)^2, five operations on two values each where the exact form takes
-// two of the special-function unit, which the exponentials already fill. A fourth degree would
-// reach to 0.6 of the cap: 16 x 24 drafts 128 us against 118. -> score / q.k, log2 domain
+// A capped score in the log2 domain from the raw product q.k, y = q.k sm_scale / softcap. Up to
+// CAP_SMALL the polynomial, off by 2^-21.9 of the score however loose the cap. Beyond it tanh(y) =
+// 1 - 2/(1 + e^2y), off by ~2^-23 of the cap, which the score is 0.42 of at least (tanh.approx would
+// lose 2^-11). Each value by its own size: what else a warp holds has no part in it.
+__device__ __forceinline__ float2 cap_small2(const Args& a, float2 qk) {
+    const float2 y = mul2(qk, make_float2(a.cap_k, a.cap_k)), t = mul2(y, y);
+    float2 p = fma2(make_float2(TANH_3, TANH_3), t, make_float2(TANH_2, TANH_2));
+    p = fma2(p, t, make_float2(TANH_1, TANH_1));
+    p = fma2(p, t, make_float2(TANH_0, TANH_0));
+    return mul2(mul2(qk, make_float2(a.scale_log2, a.scale_log2)), p);
+}
+__device__ __forceinline__ float cap_exact(const Args& a, float qk) {
+    return fmaf(-2.f * a.cap_log2, rcp(1.f + ex2(qk * a.cap_in)), a.cap_log2);
+}
+// Scores in the log2 domain of the M products that a thread holds. The exponential form is only made
+// in warps that need it.
+template <int M>
+__device__ __forceinline__ void cap_all(const Args& a, float (&x)[M]) {
+    float m4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < M; c++) m4[c & 3] = fmaxf(m4[c & 3], fabsf(x[c]));
+    const float top = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+    if (__any_sync(0xffffffffu, !(top * a.cap_k <= CAP_SMALL))) {
+#pragma unroll
+        for (int c = 0; c < M; c += 2) {
+            const float2 v = make_float2(x[c], x[c + 1]), s = cap_small2(a, v);
+            const float e0 = cap_exact(a, v.x), e1 = cap_exact(a, v.y);
+            x[c] = fabsf(v.x) * a.cap_k <= CAP_SMALL ? s.x : e0;
+            x[c + 1] = fabsf(v.y) * a.cap_k <= CAP_SMALL ? s.y : e1;
+        }
+        return;
+    }
+#pragma unroll
+    for (int c = 0; c < M; c += 2) {
+        const float2 s = cap_small2(a, make_float2(x[c], x[c + 1]));
+        x[c] = s.x;
+        x[c + 1] = s.y;
+    }
+}
+template <bool EXT, int M>
+__device__ __forceinline__ void score_all(const Args& a, float (&x)[M]) {
+    if (EXT && a.cap_log2 > 0.f) {
+        cap_all(a, x);
+        return;
+    }
+#pragma unroll
+    for (int c = 0; c < M; c += 2) {
+        const float2 v = mul2(make_float2(x[c], x[c + 1]), make_float2(a.scale_log2, a.scale_log2));
+        x[c] = v.x;
+        x[c + 1] = v.y;
+    }
+}
+// Capped scores are nearly always far below the cap. In the main loop of the tcgen05 kernel, the terms
+// scaled by the launch so that the polynomial is one in (q.k)^2: five operations on two values each
+// where the exponential form takes two of the special-function unit, which the exponentials already
+// fill. For |q.k| up to cap_lim, that is CAP_SMALL of the cap where the scaled terms are normal numbers.
+// A fourth degree would reach to 0.6 of the cap: 16 x 24 drafts 128 us against 118.
+// -> score / q.k, log2 domain
 __device__ __forceinline__ float2 cap_factor2(const Args& a, float2 qk) {
     const float2 t = mul2(qk, qk);
     float2 p = fma2(make_float2(a.cap_poly[3], a.cap_poly[3]), t, make_float2(a.cap_poly[2], a.cap_poly[2]));
     p = fma2(p, t, make_float2(a.cap_poly[1], a.cap_poly[1]));
     return fma2(p, t, make_float2(a.cap_poly[0], a.cap_poly[0]));
-}
-// The scores of 32 products that one thread holds.
-template <bool EXT>
-__device__ __forceinline__ void score32(const Args& a, float (&x)[32]) {
-    const float2 sc = make_float2(a.scale_log2, a.scale_log2);
-    bool capped = false;
-    if (EXT && a.cap_log2 > 0.f) {
-        float m4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < 32; c++) m4[c & 3] = fmaxf(m4[c & 3], fabsf(x[c]));
-        const float top = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * a.cap_k;
-        if (__any_sync(0xffffffffu, !(top <= CAP_SMALL))) {
-#pragma unroll
-            for (int c = 0; c < 32; c++) x[c] = score<true>(a, x[c]);
-            return;
-        }
-        capped = true;
-    }
-#pragma unroll
-    for (int c = 0; c < 32; c += 2) {
-        float2 v = make_float2(x[c], x[c + 1]);
-        v = mul2(v, EXT && capped ? cap_factor2(a, v) : sc);
-        x[c] = v.x;
-        x[c + 1] = v.y;
-    }
 }
 template <bool EXT>
 __device__ __forceinline__ float bias(const Args& a, float slope2, int pos, int kpos) {

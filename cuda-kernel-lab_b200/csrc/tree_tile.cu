@@ -557,7 +557,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                         }
                     }
                     auto scored = [&](int q, float (&x)[32]) {
-                        score32<EXT>(a, x);
+                        score_all<EXT>(a, x);
                         if (EXT && a.slopes) {
 #pragma unroll
                             for (int c = 0; c < 32; c++) x[c] += bias<true>(a, row.slope2, row.pos, s.pos(a, kbase + 32 * q + c));
@@ -584,7 +584,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                                 mx = fmaxf(mx, fmaxf(x0, x1));
                                 lo = fminf(lo, fminf(x0, x1));
                             }
-                        if (__any_sync(0xffffffffu, !(fmaxf(mx, -lo) * a.cap_k <= CAP_SMALL))) return false;
+                        if (__any_sync(0xffffffffu, !(fmaxf(mx, -lo) <= a.cap_lim))) return false;
                     }
 #pragma unroll(HELD ? SW / 32 : 1)
                     for (int q = 0; q < SW / 32; q++) {
@@ -617,7 +617,8 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                     }
                     if (!HELD) tmem_st_wait();
                     // plain and capped scores grow with the product: the greatest is enough
-                    if (KIND == 1 || KIND == 2) mx = score<CAP>(a, mx);
+                    if (KIND == 1) mx *= a.scale_log2;
+                    if (KIND == 2) mx *= cap_factor2(a, make_float2(mx, mx)).x;
                     if (__any_sync(0xffffffffu, mx > m + RESCALE_THRESHOLD)) {
                         const float mn = fmaxf(m, mx);
                         const float cf = mn == -INFINITY ? 1.f : ex2(m - mn);

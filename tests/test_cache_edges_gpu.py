@@ -1,0 +1,114 @@
+"""GPU tests of the cache operators at the edges of what their header allows."""
+import numpy as np
+import pytest
+
+import cache_ref as ref
+from test_cache_ops_gpu import finish, run_tree, table, up
+
+pytestmark = pytest.mark.gpu
+
+
+def score_error(bt, b, s, big, softcap=0.0, **_):
+    """Bound of a score's error in nats: 128 fp32 additions of exact products and a handful of
+    roundings, and of a cap 2^-21 of the score up to 0.45 of the cap, 2^-21 of the cap beyond (where
+    the score is above 0.42 of it): at most 2^-21 of 2.4 of the greatest score, or of the cap."""
+    fin = s[np.isfinite(s)]
+    top = float(np.abs(fin).max()) if fin.size else 0.0
+    return 2.0 ** -24 * (128 * min(big, 1e30) + 8 * top) + 2.0 ** -21 * min(softcap, 2.4 * top)
+
+
+def attend(bt, **opt):
+    """out, lse and their bounds, as in cache_ref.attention but for the error of a cap (score_error)."""
+    out = np.zeros((bt.T_total, bt.Hq, 128))
+    lse = np.full((bt.T_total, bt.Hq), -np.inf)
+    tol, ltol = np.zeros_like(out), np.zeros_like(lse)
+    for b in range(bt.B):
+        L, T, q0 = bt.lens[b], bt.toks[b], bt.q_indptr[b]
+        if T == 0 or L == 0:
+            continue
+        s, big = ref.scores(bt, b, **opt)
+        ds = score_error(bt, b, s, big, **opt)
+        v = bt.v.reshape(-1, bt.Hkv, 128)[bt.slots(b)].astype(np.float64)
+        for h in range(bt.Hq):
+            vh = np.where(np.isfinite(s[h]).any(0)[:, None], v[:, h // bt.G], 0.0)
+            for i in range(T):
+                m = s[h, i].max()
+                p = np.exp(s[h, i] - m)
+                z = p.sum()
+                o, mag = p @ vh / z, p @ np.abs(vh) / z
+                out[q0 + i, h], lse[q0 + i, h] = o, m + np.log(z)
+                tol[q0 + i, h] = (mag * (2.0 ** -11 + 2 * ds + 2.0 ** -18) + np.abs(o) * 2.0 ** -11
+                                  + 2.0 ** -25 * L * np.abs(vh).max() / z + 2.0 ** -25)
+                ltol[q0 + i, h] = 2 * ds + 2.0 ** -20 * (1 + abs(lse[q0 + i, h]))
+    return out, lse, tol, ltol
+
+
+def check(ckl, bt, p, **opt):
+    out, lse = ckl.tree_attention(p)
+    finish(ckl)
+    want, wl, tol, ltol = attend(bt, **opt)
+    o, l, n = out.float().cpu().numpy(), lse.cpu().numpy(), bt.T_total
+    assert np.isfinite(o[:n]).all() and np.isfinite(l[:n]).all()
+    err, lerr = np.abs(o[:n] - want) - tol, np.abs(l[:n] - wl) - ltol
+    assert np.all(err <= 0) and np.all(lerr <= 0), f"out {err.max():.3e}, lse {lerr.max():.3e} beyond their bounds"
+
+
+def slopes_of(Hq):
+    return np.float32(2.0) ** (-8.0 * (np.arange(Hq, dtype=np.float32) + 1) / Hq)
+
+
+# rows of a kv head: 12 (registers), 28 and 120 (one tile), 160 (two)
+CAPPED = [([300, 290], [3, 2], 8, 2), ([400, 333], [7, 5], 8, 2), ([400, 333], [15, 9], 8, 1), ([600, 280], [40, 33], 4, 1)]
+
+
+# ------------------------------------------------------------------ caps
+@pytest.mark.parametrize("lens,toks,Hq,Hkv", CAPPED)
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("cap", [1e-12, 0.5, 30.0, 1e4, 1e8, 1e30])
+def test_caps_of_every_size(ckl, dev, lens, toks, Hq, Hkv, bias, cap):
+    """From a cap that levels every score to one that leaves them as they are; at 30 every key part
+    that all rows see whole is below 0.45 of the cap."""
+    bt = ref.Batch(lens, toks, Hq, Hkv, 51)
+    _, mask, pos = bt.random_tree(4)
+    opt = dict(mask=mask, positions=pos, softcap=cap)
+    if bias:
+        opt["slopes"] = slopes_of(Hq)
+    check(ckl, bt, run_tree(ckl, dev, bt, force=2, **opt), **opt)
+
+
+@pytest.mark.parametrize("lens,toks,Hq,Hkv", CAPPED)
+def test_cap_below_some_scores(ckl, dev, lens, toks, Hq, Hkv):
+    """One head in four far beyond the cap, the others far below it, in the same warps."""
+    bt = ref.Batch(lens, toks, Hq, Hkv, 52)
+    bt.q[:, ::4] *= 20
+    opt = dict(softcap=30.0)
+    check(ckl, bt, run_tree(ckl, dev, bt, force=2, **opt), **opt)
+
+
+@pytest.mark.parametrize("lens,toks,Hq,Hkv", CAPPED)
+@pytest.mark.parametrize("cap", [1e-30, 1e-12, 1.0, 1e30])
+def test_caps_of_scores_of_zero(ckl, dev, lens, toks, Hq, Hkv, cap):
+    bt = ref.Batch(lens, toks, Hq, Hkv, 53, qscale=0.0)
+    check(ckl, bt, run_tree(ckl, dev, bt, force=1, softcap=cap), softcap=cap)
+
+
+@pytest.mark.parametrize("lens,toks,Hq,Hkv", CAPPED)
+@pytest.mark.parametrize("cap", [1e-12, 0.5, 30.0, 1e4, 1e8, 1e30])
+def test_cache_weights_caps(ckl, dev, lens, toks, Hq, Hkv, cap):
+    import torch
+    bt = ref.Batch(lens, toks, Hq, Hkv, 54)
+    _, mask, pos = bt.random_tree(4)
+    opt = dict(mask=mask, positions=pos, softcap=cap)
+    _, lse, _, _ = attend(bt, **opt)
+    lse = lse.astype(np.float32)
+    acc = ckl.cache_weights(run_tree(ckl, dev, bt, **opt), up(lse, dev), torch.zeros((2, max(lens)), device=dev))
+    finish(ckl)
+    for b in range(2):
+        s, big = ref.scores(bt, b, **opt)
+        l = lse[bt.q_indptr[b]:bt.q_indptr[b + 1]].astype(np.float64).T[:, :, None]
+        want = np.exp(s - l).sum((0, 1))
+        ds = score_error(bt, b, s, big, **opt)
+        # 2^-24 of lse from its own rounding, 2^-23 of each of the score and lse in the exponent
+        ds += 2.0 ** -22 * float(np.abs(lse).max())
+        tol = want * (2 * ds + 2.0 ** -20 + Hq * toks[b] * 2.0 ** -24) + 1e-30
+        assert np.all(np.abs(acc.cpu().numpy()[b, :lens[b]] - want) <= tol)
