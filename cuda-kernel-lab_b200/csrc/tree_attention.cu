@@ -146,6 +146,8 @@ struct State {
         for (int w = 1; w <= 2; w <<= 1)
 #pragma unroll
             for (int r = 0; r < 2; r++) mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], w));
+        mx[0] -= P_LIFT;
+        mx[1] -= P_LIFT;
         if (__any_sync(0xffffffffu, mx[0] > m[0] + RESCALE_THRESHOLD || mx[1] > m[1] + RESCALE_THRESHOLD)) {
 #pragma unroll
             for (int r = 0; r < 2; r++) {
@@ -171,8 +173,7 @@ struct State {
                 p[h][1] = ex2(sc[h][2 * r + 1] - ms);
             }
             l[r] += (p[0][0] + p[0][1]) + (p[1][0] + p[1][1]);
-            // P in fp16 for the product (2^-11 of each weight, as V's own rounding); l sums the
-            // unrounded weights
+            // l sums the unrounded weights
             pa[r] = pack_half2(p[0][0], p[0][1]);
             pa[2 + r] = pack_half2(p[1][0], p[1][1]);
         }

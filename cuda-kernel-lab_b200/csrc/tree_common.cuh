@@ -127,6 +127,12 @@ struct Row {
     }
 };
 
+// P goes to its product in fp16 (2^-11 of each weight, as V's own rounding). The reference that it is
+// taken against stays 2^P_LIFT below the running maximum: weights reach 2^15 with RESCALE_THRESHOLD
+// on top, and one is lost from 2^-32 of the greatest down, where without it a long row of weights
+// below 2^-25 would count in the sum but not in the result.
+constexpr float P_LIFT = 7.f;
+
 // tanh(y)/y in y^2 for |y| <= CAP_SMALL: fitted to it by weighted least squares, off by at most 2^-21.9
 // of it.
 constexpr float TANH_0 = 0.99999976f, TANH_1 = -0.33329466f, TANH_2 = 0.13236369f, TANH_3 = -0.04602819f;

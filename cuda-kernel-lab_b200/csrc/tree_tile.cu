@@ -617,8 +617,8 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                     }
                     if (!HELD) tmem_st_wait();
                     // plain and capped scores grow with the product: the greatest is enough
-                    if (KIND == 1) mx *= a.scale_log2;
-                    if (KIND == 2) mx *= cap_factor2(a, make_float2(mx, mx)).x;
+                    mx = KIND == 1 ? fmaf(mx, a.scale_log2, -P_LIFT)
+                       : KIND == 2 ? fmaf(mx, cap_factor2(a, make_float2(mx, mx)).x, -P_LIFT) : mx - P_LIFT;
                     if (__any_sync(0xffffffffu, mx > m + RESCALE_THRESHOLD)) {
                         const float mn = fmaxf(m, mx);
                         const float cf = mn == -INFINITY ? 1.f : ex2(m - mn);
@@ -641,8 +641,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                     }
                     const float ms = m == -INFINITY ? 0.f : m;   // a row that saw nothing yet
                     const float2 ms2 = make_float2(-ms, -ms);
-                    // P in fp16 for the product (2^-11 of each weight, as V's own rounding); l sums
-                    // the unrounded weights
+                    // l sums the unrounded weights
                     float2 l4[4];
 #pragma unroll
                     for (int i = 0; i < 4; i++) l4[i] = make_float2(0.f, 0.f);

@@ -18,7 +18,9 @@ def score_error(bt, b, s, big, softcap=0.0, **_):
 
 
 def attend(bt, **opt):
-    """out, lse and their bounds, as in cache_ref.attention but for the error of a cap (score_error)."""
+    """out, lse and their bounds, as in cache_ref.attention but for the error of a cap (score_error)
+    and for weights far below the greatest: P is kept 2^7 above fp16's own range, so that at
+    most 2^-32 of the greatest weight is lost of each."""
     out = np.zeros((bt.T_total, bt.Hq, 128))
     lse = np.full((bt.T_total, bt.Hq), -np.inf)
     tol, ltol = np.zeros_like(out), np.zeros_like(lse)
@@ -38,7 +40,7 @@ def attend(bt, **opt):
                 o, mag = p @ vh / z, p @ np.abs(vh) / z
                 out[q0 + i, h], lse[q0 + i, h] = o, m + np.log(z)
                 tol[q0 + i, h] = (mag * (2.0 ** -11 + 2 * ds + 2.0 ** -18) + np.abs(o) * 2.0 ** -11
-                                  + 2.0 ** -25 * L * np.abs(vh).max() / z + 2.0 ** -25)
+                                  + 2.0 ** -32 * L * np.abs(vh).max() / z + 2.0 ** -25)
                 ltol[q0 + i, h] = 2 * ds + 2.0 ** -20 * (1 + abs(lse[q0 + i, h]))
     return out, lse, tol, ltol
 
@@ -112,3 +114,22 @@ def test_cache_weights_caps(ckl, dev, lens, toks, Hq, Hkv, cap):
         ds += 2.0 ** -22 * float(np.abs(lse).max())
         tol = want * (2 * ds + 2.0 ** -20 + Hq * toks[b] * 2.0 ** -24) + 1e-30
         assert np.all(np.abs(acc.cpu().numpy()[b, :lens[b]] - want) <= tol)
+
+
+# ------------------------------------------------------------------ small weights
+@pytest.mark.parametrize("toks,Hq", [(1, 4), (6, 4), (40, 4)])
+def test_many_small_weights(ckl, dev, toks, Hq):
+    """Four keys far above 60,000 others, each of which weighs 2^-25.7 of the greatest: together they
+    are all of the result."""
+    L = 60000
+    bt = ref.Batch([L], [toks], Hq, 1, 61)
+    s = bt.slots(0)
+    bt.q[:] = 0
+    bt.q[:, :, 0] = 14.2
+    k, v = bt.k.reshape(-1, 128), bt.v.reshape(-1, 128)
+    k[s], v[s] = 0, 512
+    k[s, 0] = -14.2
+    # one for each of the four warps that take pages in turn
+    k[s[[0, 16, 32, 48]], 0] = 0
+    v[s[[0, 16, 32, 48]]] = 0
+    check(ckl, bt, run_tree(ckl, dev, bt, force=1))
