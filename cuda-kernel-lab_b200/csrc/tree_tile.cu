@@ -584,7 +584,8 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                                 mx = fmaxf(mx, fmaxf(x0, x1));
                                 lo = fminf(lo, fminf(x0, x1));
                             }
-                        if (__any_sync(0xffffffffu, !(fmaxf(mx, -lo) <= a.cap_lim))) return false;
+                        // padding rows may be another sequence's: they have no vote, here or below
+                        if (__any_sync(0xffffffffu, row.i >= 0 && !(fmaxf(mx, -lo) <= a.cap_lim))) return false;
                     }
 #pragma unroll(HELD ? SW / 32 : 1)
                     for (int q = 0; q < SW / 32; q++) {
@@ -619,7 +620,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                     // plain and capped scores grow with the product: the greatest is enough
                     mx = KIND == 1 ? fmaf(mx, a.scale_log2, -P_LIFT)
                        : KIND == 2 ? fmaf(mx, cap_factor2(a, make_float2(mx, mx)).x, -P_LIFT) : mx - P_LIFT;
-                    if (__any_sync(0xffffffffu, mx > m + RESCALE_THRESHOLD)) {
+                    if (__any_sync(0xffffffffu, row.i >= 0 && mx > m + RESCALE_THRESHOLD)) {
                         const float mn = fmaxf(m, mx);
                         const float cf = mn == -INFINITY ? 1.f : ex2(m - mn);
                         if (x > 0 && !(ok = o_wait(cnt - 1)))

@@ -133,3 +133,29 @@ def test_many_small_weights(ckl, dev, toks, Hq):
     k[s[[0, 16, 32, 48]], 0] = 0
     v[s[[0, 16, 32, 48]]] = 0
     check(ckl, bt, run_tree(ckl, dev, bt, force=1))
+
+
+# ------------------------------------------------------------------ neighbours
+@pytest.mark.parametrize("softcap", [0.0, 30.0])
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("toks,Hq", [([5, 9], 8), ([37, 20], 8), ([3, 30], 8)])
+def test_neighbours_leave_the_same_bits(ckl, dev, toks, Hq, softcap, bias):
+    """What the other sequences of a batch hold -- their q lie in the same tiles, their keys where a
+    last block's are missing -- changes no bit of a sequence's results."""
+    import torch
+    lens = [525, 700]                                        # 33 pages: the last block of 128 keys has one
+    opt = dict(softcap=softcap)
+    if bias:
+        opt["slopes"] = slopes_of(Hq)
+    got = []
+    for scale in (1.0, 60.0):
+        bt = ref.Batch(lens, toks, Hq, 2, 71)
+        bt.q[bt.q_indptr[1]:] *= scale
+        bt.k.reshape(-1, 2, 128)[bt.slots(1)] *= scale
+        p = run_tree(ckl, dev, bt, force=1, **opt)
+        out, lse = ckl.tree_attention(p)
+        acc = ckl.cache_weights(p, lse, torch.zeros((2, 700), device=dev))
+        finish(ckl)
+        got.append([x[:toks[0]].cpu() for x in (out, lse)] + [acc[0].cpu()])
+    for x, y in zip(*got):
+        assert torch.equal(x, y)
