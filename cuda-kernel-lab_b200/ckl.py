@@ -173,6 +173,15 @@ _SIGS = {
                                      C.c_size_t, C.c_void_p]),
     "ckl_cache_weights": (C.c_int, [C.POINTER(TreeParams), C.c_void_p, C.c_void_p, C.c_longlong,
                                     C.c_float, C.c_void_p]),
+    "ckl_cache_weights_ex": (C.c_int, [C.POINTER(TreeParams), C.c_void_p, C.c_void_p, C.c_longlong,
+                                       C.c_longlong, C.c_float, C.c_void_p]),
+    "ckl_cache_select_ex": (C.c_int, [C.c_void_p, C.c_longlong, C.c_longlong, C.c_void_p, C.c_void_p,
+                                      C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p,
+                                      C.c_void_p]),
+    "ckl_cache_compact_ex": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                       C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_void_p,
+                                       C.c_void_p, C.c_void_p, C.c_longlong, C.c_longlong,
+                                       C.c_void_p, C.c_void_p]),
     "ckl_cache_select": (C.c_int, [C.c_void_p, C.c_longlong, C.c_void_p, C.c_void_p, C.c_int,
                                    C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p,
                                    C.c_void_p]),
@@ -634,14 +643,14 @@ def _opt(t, dtype, n, name, who, dev):
 
 
 def _acc_rows(acc, B, who, dev):
-    """(address, row stride) of fp32 rows, one per sequence at least."""
+    """(address, row stride, places of a row) of fp32 rows, one per sequence at least."""
     if not isinstance(acc, _T.Tensor) or acc.dtype is not _F32 or acc.get_device() != dev or acc.dim() != 2 or acc.stride(1) != 1:
         raise CklError(1, who, "acc: expected float32 rows on the current device")
     rows, cols = acc.shape
     stride = acc.stride(0) if rows > 1 else cols
     if rows < B or stride < cols:
         raise CklError(2, who, f"acc: {rows} rows of {cols}, {stride} apart, for {B} sequences")
-    return acc.data_ptr(), stride
+    return acc.data_ptr(), stride, cols
 
 
 def _cache_shape(k_cache, v_cache, who, dev):
@@ -824,14 +833,14 @@ def tree_attention(p: TreeParams, out=None, lse=None, workspace=None, stream=Non
 
 def cache_weights(p: TreeParams, lse, acc, *, decay=1.0, stream=None):
     """acc[b, place] = decay * acc + the attention weight the place received from this call's
-    tokens (ckl_cache_weights), in place; lse from tree_attention, acc fp32 [B, >= max_len]
-    with contiguous rows."""
+    tokens (ckl_cache_weights), in place; lse from tree_attention, acc fp32 [B, places] with
+    contiguous rows (columns of a wider tensor too); places behind a row's are not kept."""
     who, dev = "cache_weights", p._keep[0].get_device()
-    aa, stride = _acc_rows(acc, p.B, who, dev)
-    st = lib().ckl_cache_weights(p, _at(lse, _F32, p.N * p.Hq, "lse", who, dev), aa, stride, decay,
-                                 _stream_of(stream))
+    aa, stride, cols = _acc_rows(acc, p.B, who, dev)
+    st = lib().ckl_cache_weights_ex(p, _at(lse, _F32, p.N * p.Hq, "lse", who, dev), aa, stride, cols,
+                                    decay, _stream_of(stream))
     if st:
-        check(st, "ckl_cache_weights")
+        check(st, "ckl_cache_weights_ex")
     return acc
 
 
@@ -844,16 +853,17 @@ def cache_select(acc, kv_indptr, kv_last_page_len, keep, *, sink=0, recent=0, ke
     who, dev = "cache_select", _device()
     ip = _at(kv_indptr, _I32, 1, "kv_indptr", who, dev)
     B = kv_indptr.numel() - 1
-    aa, stride = _acc_rows(acc, B, who, dev)
+    aa, stride, cols = _acc_rows(acc, B, who, dev)
     if keep_idx is None:
         keep_idx = _empty((B, max(keep, 0)), _I32, acc.device, stream)
     if keep_count is None:
         keep_count = _empty(B, _I32, acc.device, stream)
-    st = lib().ckl_cache_select(aa, stride, ip, _at(kv_last_page_len, _I32, B, "kv_last_page_len", who, dev),
-                                B, keep, sink, recent, _at(keep_idx, _I32, B * keep, "keep_idx", who, dev),
-                                _at(keep_count, _I32, B, "keep_count", who, dev), _stream_of(stream))
+    st = lib().ckl_cache_select_ex(aa, stride, cols, ip,
+                                   _at(kv_last_page_len, _I32, B, "kv_last_page_len", who, dev), B, keep,
+                                   sink, recent, _at(keep_idx, _I32, B * keep, "keep_idx", who, dev),
+                                   _at(keep_count, _I32, B, "keep_count", who, dev), _stream_of(stream))
     if st:
-        check(st, "ckl_cache_select")
+        check(st, "ckl_cache_select_ex")
     return keep_idx, keep_count
 
 
@@ -871,16 +881,16 @@ def cache_compact(k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, kee
     shape = keep_idx.shape
     if len(shape) != 2 or shape[0] < B:
         raise CklError(2, who, f"keep_idx {tuple(shape)} for {B} sequences")
-    aa, stride = (None, 0) if acc is None else _acc_rows(acc, B, who, dev)
+    aa, stride, cols = (None, 0, 0) if acc is None else _acc_rows(acc, B, who, dev)
     if new_len is None:
         new_len = _empty(B, _I32, k_cache.device, stream)
-    st = lib().ckl_cache_compact(kc, vc, ip, _at(kv_indices, _I32, 0, "kv_indices", who, dev),
-                                 _at(kv_last_page_len, _I32, B, "kv_last_page_len", who, dev), B, Hkv, P, ia,
-                                 shape[1], _at(keep_count, _I32, B, "keep_count", who, dev),
-                                 _opt(dst_start, _I32, B, "dst_start", who, dev), aa, stride,
-                                 _at(new_len, _I32, B, "new_len", who, dev), _stream_of(stream))
+    st = lib().ckl_cache_compact_ex(kc, vc, ip, _at(kv_indices, _I32, 0, "kv_indices", who, dev),
+                                    _at(kv_last_page_len, _I32, B, "kv_last_page_len", who, dev), B, Hkv, P,
+                                    ia, shape[1], _at(keep_count, _I32, B, "keep_count", who, dev),
+                                    _opt(dst_start, _I32, B, "dst_start", who, dev), aa, stride, cols,
+                                    _at(new_len, _I32, B, "new_len", who, dev), _stream_of(stream))
     if st:
-        check(st, "ckl_cache_compact")
+        check(st, "ckl_cache_compact_ex")
     return new_len
 
 

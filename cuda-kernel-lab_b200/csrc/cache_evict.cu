@@ -50,7 +50,7 @@ struct WArgs {
     tree::Args t;
     const float* lse_in;
     float* acc;
-    long long acc_stride;
+    long long acc_stride, acc_cols;            // a row's distance and its places
     float decay;
     int rows;                                  // rows per staged Q: a multiple of 16, at most W_ROWS
     int stages;                                // K tiles in flight
@@ -430,7 +430,7 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             const bool keeps = hf == 0 && w.decay != 0.f;
             auto has = [&](int j) {                              // block j's key of this thread has an entry
                 const int p = (pg0 + j * W_BLK_PAGES) * PAGE + key;
-                return j < nb && p < s.len && p < g.pg1 * PAGE && p < w.acc_stride;
+                return j < nb && p < s.len && p < g.pg1 * PAGE && p < w.acc_cols;
             };
             float* acc_row = w.acc + g.b * w.acc_stride + pg0 * PAGE + key;
             float old[4] = {0.f, 0.f, 0.f, 0.f};
@@ -540,7 +540,7 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             if (hf == 0 && ok) {
                 // pages that nobody sees only decay
                 for (int p = g.pg0 * PAGE + key; p < min(s.len, pg0 * PAGE); p += W_BLK)
-                    if (p < w.acc_stride && p < g.pg1 * PAGE) {
+                    if (p < w.acc_cols && p < g.pg1 * PAGE) {
                         float* dst = w.acc + g.b * w.acc_stride + p;
                         *dst = w.decay != 0.f ? w.decay * *dst : 0.f;
                     }
@@ -598,7 +598,7 @@ struct SArgs {
     const int* last;
     int* keep_idx;
     int* keep_count;
-    long long stride;
+    long long stride, cols;
     int keep, sink, recent, cluster;
 };
 struct SShared {
@@ -627,7 +627,7 @@ __device__ __forceinline__ void select_part(const SArgs& a, SShared& sh, const f
     const int per = ((n + S_WARPS - 1) / S_WARPS + 31) & ~31;
     const int w0 = min(n, warp * per), w1 = min(n, w0 + per);
     const float* row = acc_row + beg;
-    const long long have = a.stride - beg;                   // places of the row that exist
+    const long long have = a.cols - beg;                    // places of the row that exist
     auto load = [&](int i) { return i < have ? rank_key(__ldg(row + i)) : 0u; };
     uint32_t held[HELD ? S_KEYS : 1];
     if (HELD) {
@@ -775,7 +775,7 @@ struct CArgs {
     float* acc;
     int* new_len;
     unsigned* err;
-    long long acc_stride;
+    long long acc_stride, acc_cols;
     int Hkv, num_pages, keep_stride;
     int pieces;                  // 16-byte pieces of a row per CTA: a power of two, at most 16
 };
@@ -835,17 +835,17 @@ __global__ void __launch_bounds__(C_THREADS) compact_kernel(const CArgs a) {
             for (int u = 0; u < C_U; u++) {
                 const int i = base + u * C_THREADS + tid;
                 const int src = i < n ? __ldg(idx + i) : 0;
-                x[u] = i < n && src < a.acc_stride ? row[src] : 0.f;
+                x[u] = i < n && src < a.acc_cols ? row[src] : 0.f;
             }
             __syncthreads();
 #pragma unroll
             for (int u = 0; u < C_U; u++) {
                 const int i = base + u * C_THREADS + tid;
-                if (i < n && start + i < a.acc_stride) row[start + i] = x[u];
+                if (i < n && start + i < a.acc_cols) row[start + i] = x[u];
             }
         }
         __syncthreads();
-        for (long long p = (long long)start + n + tid; p < len && p < a.acc_stride; p += C_THREADS) row[p] = 0.f;
+        for (long long p = (long long)start + n + tid; p < len && p < a.acc_cols; p += C_THREADS) row[p] = 0.f;
         return;
     }
     uint4* cache = blockIdx.z ? a.v : a.k;
@@ -918,11 +918,12 @@ using namespace ckl::evict;
 
 extern "C" {
 
-ckl_status ckl_cache_weights(const ckl_tree_params* p, const float* lse, float* acc, long long acc_stride,
-                             float decay, void* stream) {
+ckl_status ckl_cache_weights_ex(const ckl_tree_params* p, const float* lse, float* acc, long long acc_stride,
+                                long long acc_cols, float decay, void* stream) {
     ckl_status st = tree::check_params(p, "cache_weights");
     if (st != CKL_OK) return st;
-    if (acc_stride <= 0) return fail(CKL_INVALID_ARG, "cache_weights: acc_stride=%lld", acc_stride);
+    if (acc_cols <= 0 || acc_cols > acc_stride)
+        return fail(CKL_INVALID_ARG, "cache_weights: acc_stride=%lld acc_cols=%lld", acc_stride, acc_cols);
     if (!(decay >= 0.f && decay <= 1.f)) return fail(CKL_INVALID_ARG, "cache_weights: decay outside [0, 1]");
     if (p->B == 0) return CKL_OK;
     if (p->N == 0) return fail(CKL_INVALID_ARG, "cache_weights: no tokens");
@@ -937,13 +938,14 @@ ckl_status ckl_cache_weights(const ckl_tree_params* p, const float* lse, float* 
     w.lse_in = lse;
     w.acc = acc;
     w.acc_stride = acc_stride;
+    w.acc_cols = acc_cols;
     w.decay = decay;
     // the rows of a kv head in one staged Q where they fit; the rest of shared memory streams K
     const long long rows = (long long)p->max_q * w.t.G;
     w.rows = (int)std::min((rows + 15) / 16 * 16, (long long)W_ROWS);
     w.stages = 2;
     while (w.stages < W_MAX_STAGES && w_smem(w.rows, w.stages + 1) <= (size_t)di->smem_optin - 1024) w.stages++;
-    const long long blocks = (acc_stride + W_BLK - 1) / W_BLK;   // of a sequence, at most (longer ones take longer)
+    const long long blocks = (acc_cols + W_BLK - 1) / W_BLK;    // of a sequence, at most (longer ones take longer)
     const unsigned grid = (unsigned)std::min((long long)di->sms, blocks * p->B);
     CUtensorMap tmK, tmQ;
     st = tree::encode_half_map(p->k_cache, p->Hkv, p->num_pages, 1, &tmK);
@@ -958,12 +960,18 @@ ckl_status ckl_cache_weights(const ckl_tree_params* p, const float* lse, float* 
     return CKL_OK;
 }
 
-ckl_status ckl_cache_select(const float* acc, long long acc_stride, const int* kv_indptr,
-                            const int* kv_last_page_len, int B, int keep, int sink, int recent,
-                            int* keep_idx, int* keep_count, void* stream) {
-    if (B < 0 || keep <= 0 || sink < 0 || recent < 0 || (long long)sink + recent > keep || acc_stride <= 0)
-        return fail(CKL_INVALID_ARG, "cache_select: B=%d keep=%d sink=%d recent=%d acc_stride=%lld", B, keep, sink,
-                    recent, acc_stride);
+ckl_status ckl_cache_weights(const ckl_tree_params* p, const float* lse, float* acc, long long acc_stride,
+                             float decay, void* stream) {
+    return ckl_cache_weights_ex(p, lse, acc, acc_stride, acc_stride, decay, stream);
+}
+
+ckl_status ckl_cache_select_ex(const float* acc, long long acc_stride, long long acc_cols, const int* kv_indptr,
+                               const int* kv_last_page_len, int B, int keep, int sink, int recent,
+                               int* keep_idx, int* keep_count, void* stream) {
+    if (B < 0 || keep <= 0 || sink < 0 || recent < 0 || (long long)sink + recent > keep || acc_cols <= 0 ||
+        acc_cols > acc_stride)
+        return fail(CKL_INVALID_ARG, "cache_select: B=%d keep=%d sink=%d recent=%d acc_stride=%lld acc_cols=%lld", B,
+                    keep, sink, recent, acc_stride, acc_cols);
     if (B == 0) return CKL_OK;
     if (!acc || !kv_indptr || !kv_last_page_len || !keep_idx || !keep_count)
         return fail(CKL_INVALID_ARG, "cache_select: NULL tensor pointer");
@@ -974,8 +982,8 @@ ckl_status ckl_cache_select(const float* acc, long long acc_stride, const int* k
     if (ks->st != CKL_OK) return ks->st;
     // a CTA per S_SLICE places, as long as the clusters of all sequences fit the GPU at once
     int cluster = 1;
-    while (cluster < S_CLUSTER && (long long)cluster * S_SLICE < acc_stride && (long long)B * cluster * 2 <= di->sms) cluster *= 2;
-    SArgs a{acc, kv_indptr, kv_last_page_len, keep_idx, keep_count, acc_stride, keep, sink, recent, cluster};
+    while (cluster < S_CLUSTER && (long long)cluster * S_SLICE < acc_cols && (long long)B * cluster * 2 <= di->sms) cluster *= 2;
+    SArgs a{acc, kv_indptr, kv_last_page_len, keep_idx, keep_count, acc_stride, acc_cols, keep, sink, recent, cluster};
     void* args[] = {&a};
     if (cluster == 1) {
         CKL_CUDA_TRY(launch((const void*)select_kernel<false>, dim3(1, (unsigned)B), dim3(S_THREADS), 0,
@@ -998,14 +1006,21 @@ ckl_status ckl_cache_select(const float* acc, long long acc_stride, const int* k
     return CKL_OK;
 }
 
-ckl_status ckl_cache_compact(void* k_cache, void* v_cache, const int* kv_indptr, const int* kv_indices,
-                             const int* kv_last_page_len, int B, int Hkv, int num_pages,
-                             const int* keep_idx, int keep_stride, const int* keep_count,
-                             const int* dst_start, float* acc, long long acc_stride, int* new_len,
-                             void* stream) {
-    if (B < 0 || Hkv <= 0 || num_pages <= 0 || keep_stride <= 0 || (acc && acc_stride <= 0))
-        return fail(CKL_INVALID_ARG, "cache_compact: B=%d Hkv=%d num_pages=%d keep_stride=%d acc_stride=%lld", B, Hkv,
-                    num_pages, keep_stride, acc_stride);
+ckl_status ckl_cache_select(const float* acc, long long acc_stride, const int* kv_indptr,
+                            const int* kv_last_page_len, int B, int keep, int sink, int recent,
+                            int* keep_idx, int* keep_count, void* stream) {
+    return ckl_cache_select_ex(acc, acc_stride, acc_stride, kv_indptr, kv_last_page_len, B, keep, sink, recent,
+                               keep_idx, keep_count, stream);
+}
+
+ckl_status ckl_cache_compact_ex(void* k_cache, void* v_cache, const int* kv_indptr, const int* kv_indices,
+                                const int* kv_last_page_len, int B, int Hkv, int num_pages,
+                                const int* keep_idx, int keep_stride, const int* keep_count,
+                                const int* dst_start, float* acc, long long acc_stride, long long acc_cols,
+                                int* new_len, void* stream) {
+    if (B < 0 || Hkv <= 0 || num_pages <= 0 || keep_stride <= 0 || (acc && (acc_cols <= 0 || acc_cols > acc_stride)))
+        return fail(CKL_INVALID_ARG, "cache_compact: B=%d Hkv=%d num_pages=%d keep_stride=%d acc_stride=%lld "
+                    "acc_cols=%lld", B, Hkv, num_pages, keep_stride, acc_stride, acc_cols);
     if (B > 65535 || Hkv > 65535) return fail(CKL_UNSUPPORTED_SHAPE, "cache_compact: B=%d Hkv=%d (at most 65535)", B, Hkv);
     if (B == 0) return CKL_OK;
     if (!k_cache || !v_cache || !kv_indptr || !kv_indices || !kv_last_page_len || !keep_idx || !keep_count)
@@ -1036,6 +1051,7 @@ ckl_status ckl_cache_compact(void* k_cache, void* v_cache, const int* kv_indptr,
     a.new_len = new_len;
     a.err = di->err_word;
     a.acc_stride = acc_stride;
+    a.acc_cols = acc_cols;
     a.Hkv = Hkv;
     a.num_pages = num_pages;
     a.keep_stride = keep_stride;
@@ -1049,6 +1065,15 @@ ckl_status ckl_cache_compact(void* k_cache, void* v_cache, const int* kv_indptr,
                         dim3((unsigned)(Hkv * (16 / a.pieces) + 1), (unsigned)B, 2), dim3(few ? 128 : 512), 0,
                         (cudaStream_t)stream, args, true));
     return CKL_OK;
+}
+
+ckl_status ckl_cache_compact(void* k_cache, void* v_cache, const int* kv_indptr, const int* kv_indices,
+                             const int* kv_last_page_len, int B, int Hkv, int num_pages,
+                             const int* keep_idx, int keep_stride, const int* keep_count,
+                             const int* dst_start, float* acc, long long acc_stride, int* new_len,
+                             void* stream) {
+    return ckl_cache_compact_ex(k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, B, Hkv, num_pages, keep_idx,
+                                keep_stride, keep_count, dst_start, acc, acc_stride, acc_stride, new_len, stream);
 }
 
 }  // extern "C"

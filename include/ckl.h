@@ -668,9 +668,27 @@ CKL_API ckl_status ckl_tree_attention(const ckl_tree_params* p, void* out, float
  * with s and the seen keys as in ckl_tree_attention and lse its output (a row with lse = -inf
  * adds nothing). decay in [0, 1]; 0 does not read acc. acc fp32, rows acc_stride elements apart;
  * places p >= acc_stride are not kept, places from L_b on are left. Sums are taken in a fixed
- * order. p->num_chunks and chunk_tokens are not read. */
+ * order. p->num_chunks and chunk_tokens are not read. At least one token (N = 0 with B > 0:
+ * CKL_INVALID_ARG). */
 CKL_API ckl_status ckl_cache_weights(const ckl_tree_params* p, const float* lse, float* acc,
                                      long long acc_stride, float decay, void* stream);
+
+/* ckl_cache_weights, ckl_cache_select and ckl_cache_compact for rows of acc that are columns of
+ * something wider: rows acc_stride elements apart have acc_cols <= acc_stride places, and what
+ * those calls say of places p >= acc_stride holds from acc_cols on. */
+CKL_API ckl_status ckl_cache_weights_ex(const ckl_tree_params* p, const float* lse, float* acc,
+                                        long long acc_stride, long long acc_cols, float decay,
+                                        void* stream);
+CKL_API ckl_status ckl_cache_select_ex(const float* acc, long long acc_stride, long long acc_cols,
+                                       const int* kv_indptr, const int* kv_last_page_len, int B,
+                                       int keep, int sink, int recent, int* keep_idx,
+                                       int* keep_count, void* stream);
+CKL_API ckl_status ckl_cache_compact_ex(void* k_cache, void* v_cache, const int* kv_indptr,
+                                        const int* kv_indices, const int* kv_last_page_len, int B,
+                                        int Hkv, int num_pages, const int* keep_idx,
+                                        int keep_stride, const int* keep_count,
+                                        const int* dst_start, float* acc, long long acc_stride,
+                                        long long acc_cols, int* new_len, void* stream);
 
 /* Chooses the tokens to keep of every sequence: all when L_b <= keep, else `keep` of them --
  * the first `sink`, the last `recent`, and of the rest those with the highest acc[b][p], ties

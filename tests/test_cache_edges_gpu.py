@@ -159,3 +159,37 @@ def test_neighbours_leave_the_same_bits(ckl, dev, toks, Hq, softcap, bias):
         got.append([x[:toks[0]].cpu() for x in (out, lse)] + [acc[0].cpu()])
     for x, y in zip(*got):
         assert torch.equal(x, y)
+
+
+# ------------------------------------------------------------------ rows of weights
+def test_weights_that_are_columns_of_something_wider(ckl, dev):
+    """acc as columns of a wider tensor, sequences longer than its rows: what a contiguous acc of
+    those rows gives, and the columns beside it are neither read nor written."""
+    import torch
+    lens, toks = [300, 70, 390], [3, 5, 1]
+    bt = ref.Batch(lens, toks, 8, 2, 72)
+    p = run_tree(ckl, dev, bt)
+    _, lse = ckl.tree_attention(p)
+    t = table(bt, dev)
+    big = torch.full((3, 500), 1e9, device=dev)
+    view = big[:, 100:250]
+    view.copy_(torch.rand((3, 150), device=dev))
+
+    def both(call):
+        plain = view.clone()
+        a, b = call(view), call(plain)
+        finish(ckl)
+        assert all(torch.equal(x, y) for x, y in zip(a, b)) and torch.equal(view, plain)
+        assert torch.all(big[:, :100] == 1e9) and torch.all(big[:, 250:] == 1e9)
+
+    for decay in (1.0, 0.5, 0.0):
+        both(lambda acc: [ckl.cache_weights(p, lse, acc, decay=decay)])
+    idx = up(np.array([[0, 5, 149, 160, 299], [1, 2, 3, 4, 69], [7, 150, 200, 251, 389]], np.int32), dev)
+    cnt = up(np.full(3, 5, np.int32), dev)
+
+    def compact(acc):
+        k, v = up(bt.k, dev), up(bt.v, dev)
+        return [ckl.cache_compact(k, v, **t, keep_idx=idx, keep_count=cnt, acc=acc), acc]
+
+    both(lambda acc: ckl.cache_select(acc, t["kv_indptr"], t["kv_last_page_len"], 60, sink=2, recent=20))
+    both(compact)
