@@ -882,9 +882,14 @@ def cache_compact(k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, kee
     if len(shape) != 2 or shape[0] < B:
         raise CklError(2, who, f"keep_idx {tuple(shape)} for {B} sequences")
     aa, stride, cols = (None, 0, 0) if acc is None else _acc_rows(acc, B, who, dev)
+    pa = _at(kv_indices, _I32, 0, "kv_indices", who, dev)
     if new_len is None:
         new_len = _empty(B, _I32, k_cache.device, stream)
-    st = lib().ckl_cache_compact_ex(kc, vc, ip, _at(kv_indices, _I32, 0, "kv_indices", who, dev),
+    else:                                          # the library does not know how many entries there are
+        na = _at(new_len, _I32, B, "new_len", who, dev)
+        if na < pa + 4 * kv_indices.numel() and pa < na + 4 * B:
+            raise CklError(1, who, "new_len overlaps kv_indices")
+    st = lib().ckl_cache_compact_ex(kc, vc, ip, pa,
                                     _at(kv_last_page_len, _I32, B, "kv_last_page_len", who, dev), B, Hkv, P,
                                     ia, shape[1], _at(keep_count, _I32, B, "keep_count", who, dev),
                                     _opt(dst_start, _I32, B, "dst_start", who, dev), aa, stride, cols,

@@ -1028,14 +1028,26 @@ ckl_status ckl_cache_compact_ex(void* k_cache, void* v_cache, const int* kv_indp
     if (((uintptr_t)k_cache | (uintptr_t)v_cache) & 15)
         return fail(CKL_INVALID_ARG, "cache_compact: k_cache and v_cache must be 16-byte aligned");
     if (num_pages > INT_MAX / PAGE) return fail(CKL_UNSUPPORTED_SHAPE, "cache_compact: num_pages=%d", num_pages);
-    // what a CTA writes, others still read: the caches and the lengths stand alone
-    auto overlap = [](const void* p, size_t pn, const void* q, size_t qn) {
-        return p && q && (uintptr_t)p < (uintptr_t)q + qn && (uintptr_t)q < (uintptr_t)p + pn;
+    // what a CTA writes, others still read: each output stands alone. (Of kv_indices the host knows
+    // no more than its first entry.)
+    struct Span {
+        const void* at;
+        size_t bytes;
+    };
+    auto overlap = [](Span x, Span y) {
+        return x.at && y.at && (uintptr_t)x.at < (uintptr_t)y.at + y.bytes && (uintptr_t)y.at < (uintptr_t)x.at + x.bytes;
     };
     const size_t cache = (size_t)num_pages * PAGE * Hkv * D * sizeof(__half), ints = (size_t)B * sizeof(int);
-    if (overlap(k_cache, cache, v_cache, cache)) return fail(CKL_INVALID_ARG, "cache_compact: k_cache and v_cache overlap");
-    for (const int* in : {keep_count, dst_start, kv_last_page_len, kv_indptr, kv_indptr + 1})
-        if (overlap(new_len, ints, in, ints)) return fail(CKL_INVALID_ARG, "cache_compact: new_len overlaps an input");
+    const Span out[] = {{k_cache, cache}, {v_cache, cache}, {new_len, ints},
+                        {acc, ((size_t)(B - 1) * acc_stride + acc_cols) * sizeof(float)}};
+    const Span in[] = {{kv_indptr, ints + sizeof(int)}, {kv_indices, sizeof(int)}, {kv_last_page_len, ints},
+                       {keep_idx, ints * keep_stride}, {keep_count, ints}, {dst_start, ints}};
+    for (int i = 0; i < 4; i++) {
+        for (int j = 0; j < i; j++)
+            if (overlap(out[i], out[j])) return fail(CKL_INVALID_ARG, "cache_compact: two of k_cache, v_cache, new_len and acc overlap");
+        for (const Span& x : in)
+            if (overlap(out[i], x)) return fail(CKL_INVALID_ARG, "cache_compact: k_cache, v_cache, new_len or acc overlaps an input");
+    }
     const DeviceInfo* di = device_info();
     if (!di) return CKL_CUDA_ERROR;
     CArgs a{};

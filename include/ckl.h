@@ -706,7 +706,9 @@ CKL_API ckl_status ckl_cache_select(const float* acc, long long acc_stride, cons
  * (ckl_check_device_error). keep_idx rows are keep_stride apart; keep_count is capped at it.
  * acc (optional, as in ckl_cache_weights): its entries move along, and those of places
  * [new length, L_b) become 0. new_len (optional, [B]): dst_start[b] + keep_count[b] (L_b for
- * a refused list), apart from every input. Pages that hold a moved token's new place must belong
+ * a refused list). The caches, acc and new_len must lie apart from one another and from every
+ * input (CKL_INVALID_ARG; of kv_indices, whose length the host does not know, the first entry is
+ * compared). Pages that hold a moved token's new place must belong
  * to that sequence alone; a token whose page id is outside [0, num_pages) moves as zeros, and
  * none moves to such a page. */
 CKL_API ckl_status ckl_cache_compact(void* k_cache, void* v_cache, const int* kv_indptr,

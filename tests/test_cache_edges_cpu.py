@@ -14,3 +14,25 @@ def test_rows_of_weights_hold_their_columns(ckl, stride, cols):
     assert L.ckl_cache_select_ex(P, stride, cols, P, P, 2, 8, 0, 0, P, P, None) == INVALID
     assert L.ckl_cache_compact_ex(P, 0x100000, P, P, P, 2, 2, 4, P, 8, P, None, P, stride, cols, None,
                                   None) == INVALID
+
+
+def test_compact_refuses_what_it_would_write_under_its_readers(ckl):
+    """The parts of one call read the lists and the page table while others write the caches, the
+    weights and the lengths."""
+    L = ckl.lib()
+    # caches of 4 pages x 16 x 2 heads x 256 bytes = 32 KB; five sequences, lists of eight
+    base = dict(k=0x100000, v=0x200000, indptr=0x1000, ind=0x2000, last=0x3000, idx=0x4000, cnt=0x5000, start=0x6000,
+                acc=0x7000, new=0x8000)
+
+    def call(**kw):
+        f = {**base, **kw}
+        return L.ckl_cache_compact_ex(f["k"], f["v"], f["indptr"], f["ind"], f["last"], 5, 2, 4, f["idx"], 8, f["cnt"],
+                                      f["start"], f["acc"], 16, 10, f["new"], None)
+
+    for new in (0x4000 - 16, 0x4000, 0x4000 + 32 * 4, 0x4000 + 39 * 4, 0x2000, 0x1000 + 20, 0x7000 + 72 * 4,
+                0x100000 + 32764, 0x200000):
+        assert call(new=new) == INVALID, hex(new)
+    for acc in (0x4000 - 73 * 4, 0x4000 + 156, 0x2000, 0x1000, 0x3000, 0x5000, 0x6000, 0x100000, 0x200000 + 32764):
+        assert call(acc=acc) == INVALID, hex(acc)
+    for idx in (0x100000, 0x200000 - 156):
+        assert call(idx=idx) == INVALID, hex(idx)

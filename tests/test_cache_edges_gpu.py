@@ -193,3 +193,17 @@ def test_weights_that_are_columns_of_something_wider(ckl, dev):
 
     both(lambda acc: ckl.cache_select(acc, t["kv_indptr"], t["kv_last_page_len"], 60, sink=2, recent=20))
     both(compact)
+
+
+def test_compact_refuses_lengths_over_the_page_table(ckl, dev):
+    import torch
+    bt = ref.Batch([90, 70], [3, 5], 2, 2, 73)
+    t = table(bt, dev)
+    k, v = up(bt.k, dev), up(bt.v, dev)
+    n = t["kv_indices"].numel()
+    idx, cnt = up(np.zeros((2, 1), np.int32), dev), up(np.ones(2, np.int32), dev)
+    for at in (0, n // 2, n - 2):
+        with pytest.raises(ckl.CklError) as e:
+            ckl.cache_compact(k, v, **t, keep_idx=idx, keep_count=cnt, new_len=t["kv_indices"][at:at + 2])
+        assert e.value.status == 1
+    assert torch.equal(t["kv_indices"], up(bt.indices, dev))
