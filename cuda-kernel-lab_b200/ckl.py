@@ -599,9 +599,17 @@ def _bind():
     _T = torch
 
 
-def _stream_of(stream):
-    """The raw handle of `stream`, or of the current device's current stream."""
-    return stream.cuda_stream if stream is not None else _raw_stream(_raw_device())
+def _stream_of(stream, dev, who):
+    """The raw handle of `stream`, or of the current stream. The library launches on the current
+    device: it must be the one that the call's tensors are on."""
+    cur = _raw_device()
+    if cur != dev:
+        raise CklError(1, who, f"the tensors are on cuda:{dev}, the current device is cuda:{cur}")
+    if stream is None:
+        return _raw_stream(dev)
+    if stream.device_index != dev:
+        raise CklError(1, who, f"the stream is on cuda:{stream.device_index}, the tensors on cuda:{dev}")
+    return stream.cuda_stream
 
 
 def _device():
@@ -624,7 +632,7 @@ def _bad(t, dtype, n, name, who, dev):
     if t.dtype is not dtype or not t.is_contiguous():
         raise CklError(1, who, f"{name}: expected contiguous {dtype}, got {t.dtype}")
     if t.get_device() != dev:
-        raise CklError(1, who, f"{name} is on {t.device}, the current device is cuda:{dev}")
+        raise CklError(1, who, f"{name} is on {t.device}, the call on cuda:{dev}")
     raise CklError(2, who, f"{name} has {t.numel()} elements, needs {n}")
 
 
@@ -728,14 +736,14 @@ def make_append_params(q, k, v, k_cache, v_cache, kv_indptr, kv_indices, kv_last
                      0 if q is None else q.shape[1], Hkv, P)
     p._keep = (q, k, v, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, q_indptr,
                positions)
-    p.q_rotated = q_out
+    p._dev, p.q_rotated = dev, q_out
     return p
 
 
 def rope_append(p: AppendParams, rope: Rope = None, stream=None):
     """Rotates and appends (ckl_rope_append) -> the rotated q (p.q_rotated). rope None copies
     q and k unturned."""
-    st = lib().ckl_rope_append(p, rope, _stream_of(stream))
+    st = lib().ckl_rope_append(p, rope, _stream_of(stream, p._dev, "rope_append"))
     if st:
         check(st, "ckl_rope_append")
     return p.q_rotated
@@ -758,8 +766,8 @@ def tree_mask(parents, q_indptr, kv_indptr, kv_last_page_len, max_q, *, mask=Non
     check(lib().ckl_tree_mask(a, _at(q_indptr, _I32, B + 1, "q_indptr", who, dev), ip,
                               _at(kv_last_page_len, _I32, B, "kv_last_page_len", who, dev), B, N, W,
                               _at(mask, _I32, N * W, "mask", who, dev),
-                              _at(positions, _I32, N, "positions", who, dev), _stream_of(stream)),
-          "ckl_tree_mask")
+                              _at(positions, _I32, N, "positions", who, dev),
+                              _stream_of(stream, dev, who)), "ckl_tree_mask")
     return mask, positions
 
 
@@ -799,6 +807,7 @@ def make_tree_params(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_le
                    1.0 / math.sqrt(HEAD_DIM) if sm_scale is None else sm_scale, softcap)
     p._keep = (q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, q_indptr, tree_mask,
                positions, slopes)
+    p._dev = dev
     return p
 
 
@@ -810,13 +819,14 @@ def tree_attention(p: TreeParams, out=None, lse=None, workspace=None, stream=Non
     """Attention of drafted tokens over the cache (ckl_tree_attention) -> (out fp16 [N,Hq,128],
     lse fp32 [N,Hq])."""
     who, L = "tree_attention", lib()
+    d = p._dev
+    handle = _stream_of(stream, d, who)
     dev = p._keep[0].device
     rows = p.N * p.Hq
     if out is None:
         out = _empty((p.N, p.Hq, HEAD_DIM), _F16, dev, stream)
     if lse is None:
         lse = _empty((p.N, p.Hq), _F32, dev, stream)
-    d = dev.index
     oa, la = _at(out, _F16, rows * HEAD_DIM, "out", who, d), _at(lse, _F32, rows, "lse", who, d)
     need = L.ckl_tree_workspace_size(p)
     wa, have = None, 0
@@ -825,7 +835,7 @@ def tree_attention(p: TreeParams, out=None, lse=None, workspace=None, stream=Non
     if have < need:
         workspace = _empty(need, _U8, dev, stream)
         wa, have = workspace.data_ptr(), need
-    st = L.ckl_tree_attention(p, oa, la, wa, have, _stream_of(stream))
+    st = L.ckl_tree_attention(p, oa, la, wa, have, handle)
     if st:
         check(st, "ckl_tree_attention")
     return out, lse
@@ -835,10 +845,11 @@ def cache_weights(p: TreeParams, lse, acc, *, decay=1.0, stream=None):
     """acc[b, place] = decay * acc + the attention weight the place received from this call's
     tokens (ckl_cache_weights), in place; lse from tree_attention, acc fp32 [B, places] with
     contiguous rows (columns of a wider tensor too); places behind a row's are not kept."""
-    who, dev = "cache_weights", p._keep[0].get_device()
+    who, dev = "cache_weights", p._dev
+    handle = _stream_of(stream, dev, who)
     aa, stride, cols = _acc_rows(acc, p.B, who, dev)
     st = lib().ckl_cache_weights_ex(p, _at(lse, _F32, p.N * p.Hq, "lse", who, dev), aa, stride, cols,
-                                    decay, _stream_of(stream))
+                                    decay, handle)
     if st:
         check(st, "ckl_cache_weights_ex")
     return acc
@@ -861,7 +872,8 @@ def cache_select(acc, kv_indptr, kv_last_page_len, keep, *, sink=0, recent=0, ke
     st = lib().ckl_cache_select_ex(aa, stride, cols, ip,
                                    _at(kv_last_page_len, _I32, B, "kv_last_page_len", who, dev), B, keep,
                                    sink, recent, _at(keep_idx, _I32, B * keep, "keep_idx", who, dev),
-                                   _at(keep_count, _I32, B, "keep_count", who, dev), _stream_of(stream))
+                                   _at(keep_count, _I32, B, "keep_count", who, dev),
+                                   _stream_of(stream, dev, who))
     if st:
         check(st, "ckl_cache_select_ex")
     return keep_idx, keep_count
@@ -893,7 +905,8 @@ def cache_compact(k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, kee
                                     _at(kv_last_page_len, _I32, B, "kv_last_page_len", who, dev), B, Hkv, P,
                                     ia, shape[1], _at(keep_count, _I32, B, "keep_count", who, dev),
                                     _opt(dst_start, _I32, B, "dst_start", who, dev), aa, stride, cols,
-                                    _at(new_len, _I32, B, "new_len", who, dev), _stream_of(stream))
+                                    _at(new_len, _I32, B, "new_len", who, dev),
+                                    _stream_of(stream, dev, who))
     if st:
         check(st, "ckl_cache_compact_ex")
     return new_len

@@ -36,3 +36,26 @@ def test_compact_refuses_what_it_would_write_under_its_readers(ckl):
         assert call(acc=acc) == INVALID, hex(acc)
     for idx in (0x100000, 0x200000 - 156):
         assert call(idx=idx) == INVALID, hex(idx)
+
+
+class Stream:
+    cuda_stream = 0
+
+    def __init__(self, dev):
+        self.device_index = dev
+
+
+@pytest.mark.parametrize("current,stream", [(1, None), (1, Stream(0)), (1, Stream(1)), (0, Stream(1))])
+def test_params_of_another_device_are_refused(ckl, monkeypatch, current, stream):
+    """Parameters made on cuda:0 and called while cuda:1 is current, or for a stream of cuda:1:
+    refused before anything is launched or allocated. (Empty batches: nothing would run.)"""
+    monkeypatch.setattr(ckl, "_raw_device", lambda: current)
+    monkeypatch.setattr(ckl, "_raw_stream", lambda dev: 0)
+    ap, tp = ckl.AppendParams(Hkv=1), ckl.TreeParams(Hq=1, Hkv=1)
+    ap._dev = tp._dev = 0
+    ap.q_rotated, tp._keep = None, (None,)
+    for call in (lambda: ckl.rope_append(ap, stream=stream), lambda: ckl.tree_attention(tp, stream=stream),
+                 lambda: ckl.cache_weights(tp, None, None, stream=stream)):
+        with pytest.raises(ckl.CklError, match="cuda:1") as e:
+            call()
+        assert e.value.status == INVALID
