@@ -897,6 +897,7 @@ def cache_compact(k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, kee
     pa = _at(kv_indices, _I32, 0, "kv_indices", who, dev)
     if new_len is None:
         new_len = _empty(B, _I32, k_cache.device, stream)
+        na = new_len.data_ptr()
     else:                                          # the library does not know how many entries there are
         na = _at(new_len, _I32, B, "new_len", who, dev)
         if na < pa + 4 * kv_indices.numel() and pa < na + 4 * B:
@@ -904,8 +905,7 @@ def cache_compact(k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, kee
     st = lib().ckl_cache_compact_ex(kc, vc, ip, pa,
                                     _at(kv_last_page_len, _I32, B, "kv_last_page_len", who, dev), B, Hkv, P,
                                     ia, shape[1], _at(keep_count, _I32, B, "keep_count", who, dev),
-                                    _opt(dst_start, _I32, B, "dst_start", who, dev), aa, stride, cols,
-                                    _at(new_len, _I32, B, "new_len", who, dev),
+                                    _opt(dst_start, _I32, B, "dst_start", who, dev), aa, stride, cols, na,
                                     _stream_of(stream, dev, who))
     if st:
         check(st, "ckl_cache_compact_ex")
