@@ -79,11 +79,6 @@ struct WSeg {
 struct WWalk {
     long long left, off;
     int b;
-    uint64_t deadline;                         // of the waits for eight staged Qs: a call has no limit,
-                                               // however many it takes
-    __device__ __forceinline__ void renew(const tree::Args& a, int chunk) {
-        if (chunk % 8 == 0) deadline = globaltimer() + a.timeout_ns;
-    }
     __device__ __forceinline__ bool next(const tree::Args& a, WSeg* g) {
         while (left > 0 && b < a.B) {
             int page0;
@@ -248,7 +243,7 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     pdl_trigger();
     const uint32_t tmem = *tmem_slot;
     auto d_col = [&](int d) { return (uint32_t)((d / W_BUFS * bufs + d % W_BUFS) * d_cols); };   // of S buffer d
-    WWalk walk{s_left, s_off, s_b, globaltimer() + a.timeout_ns};
+    WWalk walk{s_left, s_off, s_b};
     WSeg g;
     bool ok = true;
     int chunk = 0, n = 0;                        // staged Qs and K tiles so far
@@ -278,7 +273,6 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             }
             for (int h = 0; h < a.Hkv && ok; h++)
                 for (int r0 = 0; r0 < nrows && ok; r0 += N, chunk++) {
-                    walk.renew(a, chunk);
                     for (int pg = pg0; pg < g.pg1 && ok; pg += W_BLK_PAGES, n++) {
                         const int np = min(W_BLK_PAGES, g.pg1 - pg), st = n % KST, j = (pg - pg0) / W_BLK_PAGES;
                         int id = ids[0];
@@ -287,7 +281,7 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                         int page[W_BLK_PAGES];
 #pragma unroll
                         for (int i = 0; i < W_BLK_PAGES; i++) page[i] = __shfl_sync(0xffffffffu, id, (j & 3) * 8 + i);
-                        if (n >= KST) ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[st], (n / KST - 1) & 1, walk.deadline, a.err));
+                        if (n >= KST) ok = __all_sync(0xffffffffu, mbar_wait_for(&k_empty[st], (n / KST - 1) & 1, a.timeout_ns, a.err));
                         if (!ok) break;
                         if (elect_one()) {
                             mbar_arrive_expect_tx(&k_full[st], np * KV_TILE);
@@ -305,7 +299,7 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         // every issued copy must land before the CTA exits
         if (lane == 0)
             for (int i = 0; i < KST && i < n; i++)
-                mbar_wait(&k_full[i], ((i + (n - 1 - i) / KST * KST) / KST) & 1, walk.deadline, a.err);
+                mbar_wait_for(&k_full[i], ((i + (n - 1 - i) / KST * KST) / KST) & 1, DRAIN_NS, a.err);
     } else if (warp == 1) {
         // ---------------------------------------------------------------- MMA issuer
         const uint32_t idesc = umma_idesc_f16(W_BLK, N, false, false);
@@ -321,13 +315,12 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                 int t0 = tiles[0], t1 = tiles[1];
                 for (int c = 0; c < chunks && ok; c++) {
                     const int qb = (chunk + c) % qbufs;
-                    walk.renew(a, chunk + c);
-                    ok = mbar_wait(&q_full[qb], ((chunk + c) / qbufs) & 1, walk.deadline, a.err);
+                    ok = mbar_wait_for(&q_full[qb], ((chunk + c) / qbufs) & 1, a.timeout_ns, a.err);
                     for (int j = 0; j < nb && ok; j++) {
                         const int m = n + c * nb + j, st = m % KST, gr = narrow ? c & 1 : 0;
                         const int t = gr ? t1++ : t0++, d = gr * W_BUFS + t % bufs;
-                        ok = mbar_wait(&k_full[st], (m / KST) & 1, walk.deadline, a.err);
-                        if (ok && t >= bufs) ok = mbar_wait(&d_empty[d], (t / bufs - 1) & 1, walk.deadline, a.err);
+                        ok = mbar_wait_for(&k_full[st], (m / KST) & 1, a.timeout_ns, a.err);
+                        if (ok && t >= bufs) ok = mbar_wait_for(&d_empty[d], (t / bufs - 1) & 1, a.timeout_ns, a.err);
                         if (!ok) break;
                         tc_fence_after_sync();
 #pragma unroll
@@ -360,9 +353,8 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             for (int h = 0; h < a.Hkv && ok; h++)
                 for (int r0 = 0; r0 < nrows && ok; r0 += N, chunk++) {
                     const int qb = chunk % qbufs, ib = chunk % ibufs;
-                    walk.renew(a, chunk);
                     if (chunk >= qbufs)
-                        ok = __all_sync(0xffffffffu, mbar_wait(&q_empty[qb], (chunk / qbufs - 1) & 1, walk.deadline, a.err));
+                        ok = __all_sync(0xffffffffu, mbar_wait_for(&q_empty[qb], (chunk / qbufs - 1) & 1, a.timeout_ns, a.err));
                     if (!ok) break;
                     uint8_t* dst = qs + qb * q_bytes;
                     if (a.q_tma) {
@@ -390,7 +382,7 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                         mbar_arrive(&q_full[qb]);
                     }
                     if (chunk >= ibufs)
-                        ok = __all_sync(0xffffffffu, mbar_wait(&i_empty[ib], (chunk / ibufs - 1) & 1, walk.deadline, a.err));
+                        ok = __all_sync(0xffffffffu, mbar_wait_for(&i_empty[ib], (chunk / ibufs - 1) & 1, a.timeout_ns, a.err));
                     if (!ok) { chunk++; break; }
                     const RowInfo in{infos + ib * 4 * N, N};
                     for (int r = tid; r < N; r += 64) {
@@ -407,10 +399,10 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                     mbar_arrive(&i_full[ib]);
                 }
         }
-        // a staged Q that nobody waited for (after a timeout) must still land
-        if (!ok && tid == 0)
+        // a copied Q that nobody waited for (after a timeout) must still land
+        if (a.q_tma && tid == 0)
             for (int c = max(0, chunk - qbufs); c < chunk; c++)
-                mbar_wait(&q_full[c % qbufs], (c / qbufs) & 1, walk.deadline, a.err);
+                mbar_wait_for(&q_full[c % qbufs], (c / qbufs) & 1, DRAIN_NS, a.err);
     } else {
         // ---------------------------------------------------------------- weights
         const int quarter = warp & 3, hf = (warp - 4) >> 2;
@@ -442,9 +434,8 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             int masked = -1;                                     // the tile they are of
             for (int c = 0; c < chunks; c++, chunk++) {
                 const int ib = chunk % ibufs;
-                walk.renew(a, chunk);
                 const RowInfo in{infos + ib * 4 * N, N};
-                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&i_full[ib], (chunk / ibufs) & 1, walk.deadline, a.err));
+                if (ok) ok = __all_sync(0xffffffffu, mbar_wait_for(&i_full[ib], (chunk / ibufs) & 1, a.timeout_ns, a.err));
                 const int r0 = c % rchunks * N;                      // first row of this chunk
                 const int t_lo = (r0 + c0) / a.G;                    // tokens of this thread's columns
                 const int nt = r0 + c0 < nrows ? (min(nrows, r0 + c1) - 1) / a.G - t_lo + 1 : 0;
@@ -454,7 +445,7 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                 for (int j = 0; mine && j < nb; j++, tile++) {
                     const int d = gr * W_BUFS + tile % bufs;
                     const uint32_t d_at = d_col(d);
-                    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&d_full[d], (tile / bufs) & 1, walk.deadline, a.err));
+                    if (ok) ok = __all_sync(0xffffffffu, mbar_wait_for(&d_full[d], (tile / bufs) & 1, a.timeout_ns, a.err));
                     if (!ok) continue;
                     tc_fence_after_sync();
                     const int kbase = (pg0 + j * W_BLK_PAGES) * PAGE, p = kbase + key;
@@ -558,7 +549,7 @@ weights_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         }
     }
     // every MMA must have finished before tensor memory is released
-    if (threadIdx.x == 0) mbar_wait(done, 0, walk.deadline, a.err);
+    if (threadIdx.x == 0) mbar_wait_for(done, 0, DRAIN_NS, a.err);
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();

@@ -73,6 +73,21 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, uint64
         }
     }
 }
+// The same with a limit on this wait alone (ns), however long the kernel has run.
+__device__ __forceinline__ bool mbar_wait_for(uint64_t* bar, uint32_t parity, uint64_t limit, unsigned* err) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t start = globaltimer();
+    while (true) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (globaltimer() - start > limit) {
+            atomicOr(err, DEVERR_TIMEOUT);
+            return false;
+        }
+    }
+}
+// Limit on a kernel's last waits: for its own copies and products in flight, which must end before
+// its shared and tensor memory goes, whatever limit the caller put on the others.
+constexpr uint64_t DRAIN_NS = 1000000000ull;
 
 // ------------------------------------------------------------------ flags between GPUs
 // Release store / acquire load at system scope (the flag words of peer-mapped windows):

@@ -249,8 +249,6 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
     __syncthreads();
     pdl_wait();
     pdl_trigger();
-    const uint64_t deadline = globaltimer() + a.timeout_ns;
-
     const Seq s(a, b);
     if (s.T > a.max_q && chunk == 0 && threadIdx.x == 0) atomicOr(a.err, DEVERR_BOUND);
     const int nrows = min(s.T, a.max_q) * a.G;
@@ -273,7 +271,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                 const int page = __shfl_sync(0xffffffffu, my_page, j);
                 if (elect_one()) {
                     const int i = base + j, sg = i % STAGES;
-                    if (i >= STAGES) ok = mbar_wait(&empty[sg], ((i / STAGES) - 1) & 1, deadline, a.err);
+                    if (i >= STAGES) ok = mbar_wait_for(&empty[sg], ((i / STAGES) - 1) & 1, a.timeout_ns, a.err);
                     if (ok) {
                         mbar_arrive_expect_tx(&full[sg], STAGE_BYTES);
                         load_page(ring + sg * STAGE_BYTES, &tmK, &tmV, kvh, page, &full[sg], pol);
@@ -288,7 +286,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
         if (lane == 0)
             for (int sg = 0; sg < STAGES && sg < issued; sg++) {
                 const int last = sg + ((issued - 1 - sg) / STAGES) * STAGES;
-                mbar_wait(&full[sg], (last / STAGES) & 1, deadline, a.err);
+                mbar_wait_for(&full[sg], (last / STAGES) & 1, DRAIN_NS, a.err);
             }
     } else {
         // stage the Q rows (zeros behind the rows in use), 16 chunks of 16 bytes each
@@ -307,7 +305,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
         bool ok = true;
         for (int i = warp; i < npg; i += CONSUMERS) {
             const int sg = i % STAGES;
-            const bool got = mbar_wait(&full[sg], (i / STAGES) & 1, deadline, a.err);
+            const bool got = mbar_wait_for(&full[sg], (i / STAGES) & 1, a.timeout_ns, a.err);
             if (!__all_sync(0xffffffffu, got)) { ok = false; break; }
             const int kbase = (p0 + i) * PAGE;
             const bool whole = kbase + PAGE <= s.ctx && (a.window <= 0 || (long long)pos_hi - kbase < a.window);

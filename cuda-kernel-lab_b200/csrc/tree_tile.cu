@@ -112,9 +112,8 @@ struct Walk {
     long long left;              // blocks of this CTA not handed out yet
     long long off;               // next block within sequence b
     int b;
-    uint64_t deadline;           // of a segment's waits: a call has no limit, however many there are
-    __device__ __forceinline__ Walk(const Args& a, long long left_, long long off_, int b_)
-        : left(left_), off(off_), b(b_), deadline(globaltimer() + a.timeout_ns) {}
+    __device__ __forceinline__ Walk(long long left_, long long off_, int b_)
+        : left(left_), off(off_), b(b_) {}
     // The next segment, its sequence and work; false at the end.
     __device__ __forceinline__ bool next(const Args& a, Seg* g, Seq* s, Work* w, int* pos_hi, int lane) {
         while (left > 0 && b < a.B) {
@@ -138,7 +137,6 @@ struct Walk {
             g->blk1 = (int)min((long long)w->nblk, g->blk0 + left);
             off += g->blk1 - g->blk0;
             left -= g->blk1 - g->blk0;
-            deadline = globaltimer() + a.timeout_ns;
             return true;
         }
         return false;
@@ -276,7 +274,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
     tc_fence_after_sync();
     pdl_trigger();
     const uint32_t tmem = *tmem_slot;
-    Walk<C::ROWS> walk(a, range[0], range[1], *range_b);
+    Walk<C::ROWS> walk(range[0], range[1], *range_b);
     Seg g;
     Seq s;
     Work w;
@@ -289,7 +287,8 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
         int qn[MT];                                     // Q loads issued into each tile
 #pragma unroll
         for (int t = 0; t < MT; t++) qn[t] = 0;
-        int ok = 1, n = 0, seg = 0;                     // n: blocks issued
+        int ok = 1, n = 0, seg = 0;
+        int nk = 0, nv = 0;                             // blocks of K and of V issued
         while (ok && walk.next(a, &g, &s, &w, &pos_hi, lane)) {
             const int p0 = w.first / PAGE, npg = (s.len + PAGE - 1) / PAGE;
             int ids_at = 0, my_id = 0;
@@ -307,7 +306,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                 const int ks = n % KST, vs = n % VST;
                 // one elected lane issues: a box per lane would be serialised at ~50 ns each
                 if (elect_one()) {
-                    if (n >= KST) ok = mbar_wait(&k_empty[ks], ((n / KST) - 1) & 1, walk.deadline, a.err);
+                    if (n >= KST) ok = mbar_wait_for(&k_empty[ks], ((n / KST) - 1) & 1, a.timeout_ns, a.err);
                     if (ok) {
                         uint8_t* dst = kring + ks * KV_BLK;
                         mbar_arrive_expect_tx(&k_full[ks], KV_BLK);
@@ -320,8 +319,9 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                 }
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
+                nk = n + 1;
                 if (elect_one()) {
-                    if (n >= VST) ok = mbar_wait(&v_empty[vs], ((n / VST) - 1) & 1, walk.deadline, a.err);
+                    if (n >= VST) ok = mbar_wait_for(&v_empty[vs], ((n / VST) - 1) & 1, a.timeout_ns, a.err);
                     if (ok) {
                         uint8_t* dst = vring + vs * KV_BLK;
                         mbar_arrive_expect_tx(&v_full[vs], KV_BLK);
@@ -331,11 +331,12 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                     }
                 }
                 ok = __all_sync(0xffffffffu, ok);
-                if (!ok) { n++; break; }                // its K is in flight, its V is not
+                if (!ok) break;
+                nv = n + 1;
                 if (j == g.blk0 && a.q_tma) {
                     // the segment's Q, behind its first block: the earlier segment still reads its own
                     if (lane == 0) {
-                        if (seg > 0) ok = mbar_wait(q_empty, (seg - 1) & 1, walk.deadline, a.err);
+                        if (seg > 0) ok = mbar_wait_for(q_empty, (seg - 1) & 1, a.timeout_ns, a.err);
 #pragma unroll
                         for (int t = 0; t < MT; t++) {
                             if (!ok || t * 128 >= g.rows) break;
@@ -348,21 +349,20 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                         }
                     }
                     ok = __shfl_sync(0xffffffffu, ok, 0);
-                    if (!ok) { n++; break; }
+                    if (!ok) break;
                 }
             }
             seg++;
         }
-        // every issued copy must land before the CTA exits (a wait for a phase that was never
-        // armed, after a timeout, ends at the deadline)
+        // every issued copy must land before the CTA exits
         if (lane == 0) {
-            for (int i = 0; i < KST && i < n; i++)
-                mbar_wait(&k_full[i], ((i + (n - 1 - i) / KST * KST) / KST) & 1, walk.deadline, a.err);
-            for (int i = 0; i < VST && i < n; i++)
-                mbar_wait(&v_full[i], ((i + (n - 1 - i) / VST * VST) / VST) & 1, walk.deadline, a.err);
+            for (int i = 0; i < KST && i < nk; i++)
+                mbar_wait_for(&k_full[i], ((i + (nk - 1 - i) / KST * KST) / KST) & 1, DRAIN_NS, a.err);
+            for (int i = 0; i < VST && i < nv; i++)
+                mbar_wait_for(&v_full[i], ((i + (nv - 1 - i) / VST * VST) / VST) & 1, DRAIN_NS, a.err);
 #pragma unroll
             for (int t = 0; t < MT; t++)
-                if (qn[t] > 0) mbar_wait(&q_full[t], (qn[t] - 1) & 1, walk.deadline, a.err);
+                if (qn[t] > 0) mbar_wait_for(&q_full[t], (qn[t] - 1) & 1, DRAIN_NS, a.err);
         }
     } else if (warp == 1) {
         // ---------------------------------------------------------------- MMA issuer
@@ -381,7 +381,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
         while (ok && walk.next(a, &g, &s, &w, &pos_hi, lane)) {
             const int nt = (g.rows + 127) / 128, nb = g.blk1 - g.blk0, parts = nb * U;
             if (elect_one()) {
-                auto wait = [&](uint64_t* bar, int phase) { return mbar_wait(bar, phase & 1, walk.deadline, a.err); };
+                auto wait = [&](uint64_t* bar, int phase) { return mbar_wait_for(bar, phase & 1, a.timeout_ns, a.err); };
                 // S of part x (of this segment), tile t (offsets in descriptors: 16 bytes)
                 auto qk = [&](int x, int t, int buf) {
                     const int kn = n + x / U;
@@ -462,7 +462,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
         while (ok && walk.next(a, &g, &s, &w, &pos_hi, lane)) {
             for (int j = g.blk0; j < g.blk1 && ok; j++, n++) {
                 const int vs = n % VST, kbase = w.first + j * BLK;
-                ok = __all_sync(0xffffffffu, mbar_wait(&v_full[vs], (n / VST) & 1, walk.deadline, a.err));
+                ok = __all_sync(0xffffffffu, mbar_wait_for(&v_full[vs], (n / VST) & 1, a.timeout_ns, a.err));
                 if (!ok) break;
                 if (!(kbase + BLK <= s.ctx && (a.window <= 0 || (long long)pos_hi - kbase < a.window))) {
                     uint8_t* vb = vring + vs * KV_BLK;
@@ -509,7 +509,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
         bool ok = true;
         int cnt = 0;                                    // parts of this tile
         auto o_wait = [&](int c) {
-            return __all_sync(0xffffffffu, mbar_wait(&o_done[t * 2 + (c & 1)], (c >> 1) & 1, walk.deadline, a.err));
+            return __all_sync(0xffffffffu, mbar_wait_for(&o_done[t * 2 + (c & 1)], (c >> 1) & 1, a.timeout_ns, a.err));
         };
         while (walk.next(a, &g, &s, &w, &pos_hi, lane)) {
             const int nt = (g.rows + 127) / 128, parts = (g.blk1 - g.blk0) * U;
@@ -683,7 +683,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                     const int kbase = w.first + g.blk0 * BLK + x * SW;
                     const bool whole = kbase + SW <= s.ctx && (a.window <= 0 || (long long)pos_hi - kbase < a.window);
                     const uint32_t srow = trow + (cnt & 1) * SW;
-                    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t * 2 + (cnt & 1)], (cnt >> 1) & 1, walk.deadline, a.err));
+                    if (ok) ok = __all_sync(0xffffffffu, mbar_wait_for(&s_full[t * 2 + (cnt & 1)], (cnt >> 1) & 1, a.timeout_ns, a.err));
                     if (!ok) continue;
                     if (idle) {                         // their P is whatever S held: no other row reads it
                         for (int h = 0; h < PH; h++) mbar_arrive(&p_full[(t * 2 + (cnt & 1)) * PH + h]);
@@ -777,7 +777,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
         }
     }
     // every MMA must have finished before tensor memory is released
-    if (threadIdx.x == 0) mbar_wait(done, 0, walk.deadline, a.err);
+    if (threadIdx.x == 0) mbar_wait_for(done, 0, DRAIN_NS, a.err);
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();

@@ -207,3 +207,71 @@ def test_compact_refuses_lengths_over_the_page_table(ckl, dev):
             ckl.cache_compact(k, v, **t, keep_idx=idx, keep_count=cnt, new_len=t["kv_indices"][at:at + 2])
         assert e.value.status == 1
     assert torch.equal(t["kv_indices"], up(bt.indices, dev))
+
+
+# ------------------------------------------------------------------ limits on waits
+def long_context(ckl, dev, T, G, L, B=1):
+    """B sequences of L tokens over 64 pages that repeat, one kv head."""
+    import torch
+    g = torch.Generator(device=dev).manual_seed(3)
+    q = torch.randn((B * T, G, 128), device=dev, dtype=torch.float16, generator=g)
+    k, v = (torch.randn((64, 16, 1, 128), device=dev, dtype=torch.float16, generator=g) for _ in range(2))
+    i32 = lambda x: torch.as_tensor(x, dtype=torch.int32, device=dev)
+    ids = torch.randint(0, 64, (B * L // 16,), device=dev, dtype=torch.int32, generator=g)
+    return ckl.make_tree_params(q, k, v, i32([b * L // 16 for b in range(B + 1)]), ids, i32([16] * B), max_len=L, max_q=T,
+                                q_indptr=i32([b * T for b in range(B + 1)]), force_chunks=1)
+
+
+@pytest.fixture
+def wait_limit(ckl):
+    yield ckl.lib().ckl_set_spin_timeout_ns
+    ckl.lib().ckl_set_spin_timeout_ns(1000000000)
+
+
+@pytest.mark.parametrize("T,G", [(1, 4), (6, 4), (64, 4)])
+def test_one_run_of_keys_longer_than_the_wait_limit(ckl, dev, wait_limit, T, G):
+    """The limit is one wait's: a CTA that walks 400,000 keys (several ms) under a limit of 1 ms."""
+    import torch
+    p = long_context(ckl, dev, T, G, 400000)
+    out, lse = ckl.tree_attention(p)
+    finish(ckl)
+    wait_limit(1000000)
+    o2, l2 = ckl.tree_attention(p)
+    finish(ckl)
+    assert torch.equal(out, o2) and torch.equal(lse, l2)
+
+
+@pytest.mark.parametrize("T,G", [(1, 4), (6, 4), (6, 5), (64, 4), (70, 5)])
+def test_waits_that_may_give_up(ckl, dev, wait_limit, T, G):
+    """A limit below what some waits take: the calls return, one that gave up is recorded as
+    CKL_TIMEOUT, and the next calls give what they gave before. (A wait that ends within the
+    hardware's own suspension never looks at the limit, so a call may also be right.)"""
+    import torch
+    p = long_context(ckl, dev, T, G, 4000, B=3)
+    out, lse = ckl.tree_attention(p)
+    acc = ckl.cache_weights(p, lse, torch.zeros((3, 4000), device=dev))
+    finish(ckl)
+
+    def attend():
+        o, l = ckl.tree_attention(p)
+        return torch.equal(o, out) and torch.equal(l, lse)
+
+    def weigh():
+        return torch.equal(ckl.cache_weights(p, lse, torch.zeros((3, 4000), device=dev)), acc)
+
+    for call in [attend, weigh] * 5:
+        wait_limit(1)
+        right = call()
+        torch.cuda.synchronize()
+        if not right:
+            with pytest.raises(ckl.CklError) as e:
+                ckl.check_device_error()
+            assert e.value.status == 5                         # CKL_TIMEOUT
+        else:
+            try:
+                ckl.check_device_error()
+            except ckl.CklError as e:
+                assert e.status == 5
+        wait_limit(1000000000)
+        assert attend() and weigh()
+        finish(ckl)
