@@ -650,6 +650,12 @@ def _opt(t, dtype, n, name, who, dev):
     return None if t is None else _at(t, dtype, n, name, who, dev)
 
 
+def _ids(t, indptr, who, dev):
+    """Address of the page ids; of a batch without pages, where the tensor may have none, another's
+    that is not read."""
+    return _at(t, _I32, 0, "kv_indices", who, dev) or indptr
+
+
 def _acc_rows(acc, B, who, dev):
     """(address, row stride, places of a row) of fp32 rows, one per sequence at least."""
     if not isinstance(acc, _T.Tensor) or acc.dtype is not _F32 or acc.get_device() != dev or acc.dim() != 2 or acc.stride(1) != 1:
@@ -729,7 +735,7 @@ def make_append_params(q, k, v, k_cache, v_cache, kv_indptr, kv_indices, kv_last
     elif tuple(q_out.shape) != tuple(q.shape):
         raise CklError(2, who, f"q_out {tuple(q_out.shape)} for q {tuple(q.shape)}")
     p = AppendParams(*addr, *strides, _opt(q_out, _F16, 0, "q_out", who, dev), kc, vc, ip,
-                     _at(kv_indices, _I32, 0, "kv_indices", who, dev),
+                     _ids(kv_indices, ip, who, dev),
                      _at(kv_last_page_len, _I32, B, "kv_last_page_len", who, dev),
                      _opt(q_indptr, _I32, B + 1, "q_indptr", who, dev),
                      _opt(positions, _I32, N, "positions", who, dev), B, N,
@@ -797,7 +803,7 @@ def make_tree_params(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_le
     if B > 0 and N > 0:
         check(lib().ckl_tree_plan(Hq // Hkv, B, Hkv, max_q, max_len, window, force_chunks,
                                   C.byref(nc), C.byref(ct)), "ckl_tree_plan")
-    p = TreeParams(qa, kc, vc, ip, _at(kv_indices, _I32, 0, "kv_indices", who, dev),
+    p = TreeParams(qa, kc, vc, ip, _ids(kv_indices, ip, who, dev),
                    _at(kv_last_page_len, _I32, B, "kv_last_page_len", who, dev),
                    _opt(q_indptr, _I32, B + 1, "q_indptr", who, dev),
                    None if tree_mask is None else tree_mask.data_ptr(),
@@ -894,7 +900,7 @@ def cache_compact(k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, kee
     if len(shape) != 2 or shape[0] < B:
         raise CklError(2, who, f"keep_idx {tuple(shape)} for {B} sequences")
     aa, stride, cols = (None, 0, 0) if acc is None else _acc_rows(acc, B, who, dev)
-    pa = _at(kv_indices, _I32, 0, "kv_indices", who, dev)
+    pa = _ids(kv_indices, ip, who, dev)
     if new_len is None:
         new_len = _empty(B, _I32, k_cache.device, stream)
         na = new_len.data_ptr()

@@ -275,3 +275,26 @@ def test_waits_that_may_give_up(ckl, dev, wait_limit, T, G):
         wait_limit(1000000000)
         assert attend() and weigh()
         finish(ckl)
+
+
+# ------------------------------------------------------------------ nothing there
+def test_a_batch_without_a_page(ckl, dev):
+    """Every sequence empty, so that there is no page id: tokens see nothing and have no place,
+    lists of nothing move nothing."""
+    import torch
+    bt = ref.Batch([0, 0, 0], [1, 2, 0], 8, 2, 81)
+    t = table(bt, dev)
+    assert t["kv_indices"].numel() == 0
+    k, v = up(bt.k, dev), up(bt.v, dev)
+    q = up(bt.q, dev)
+    p = ckl.make_append_params(q, q[:, :2], q[:, 2:4], k, v, **t, q_indptr=up(bt.q_indptr, dev))
+    assert torch.equal(ckl.rope_append(p), q)
+    tp = ckl.make_tree_params(q, k, v, **t, max_len=0, max_q=2, q_indptr=up(bt.q_indptr, dev))
+    out, lse = ckl.tree_attention(tp)
+    acc = ckl.cache_weights(tp, lse, torch.ones((3, 4), device=dev), decay=0.5)
+    idx, cnt = ckl.cache_select(acc, t["kv_indptr"], t["kv_last_page_len"], 5)
+    new = ckl.cache_compact(k, v, **t, keep_idx=idx, keep_count=cnt, acc=acc)
+    finish(ckl)
+    assert torch.all(out == 0) and torch.all(torch.isneginf(lse)) and torch.all(acc == 1)
+    assert torch.all(idx == -1) and torch.all(cnt == 0) and torch.all(new == 0)
+    assert np.array_equal(k.cpu().numpy(), bt.k, equal_nan=True)
