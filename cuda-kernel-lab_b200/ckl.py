@@ -728,9 +728,10 @@ def make_append_params(q, k, v, k_cache, v_cache, kv_indptr, kv_indices, kv_last
         raise CklError(2, who, f"k {tuple(k.shape)} / v {tuple(v.shape)} for {Hkv} cached heads")
     ip = _at(kv_indptr, _I32, 1, "kv_indptr", who, dev)
     B = kv_indptr.numel() - 1
+    made = q is not None and q_out is None
     if q is None:
         q_out = None
-    elif q_out is None:
+    elif made:
         q_out = _T.empty((N, q.shape[1], HEAD_DIM), dtype=_F16, device=q.device)
     elif tuple(q_out.shape) != tuple(q.shape):
         raise CklError(2, who, f"q_out {tuple(q_out.shape)} for q {tuple(q.shape)}")
@@ -742,7 +743,7 @@ def make_append_params(q, k, v, k_cache, v_cache, kv_indptr, kv_indices, kv_last
                      0 if q is None else q.shape[1], Hkv, P)
     p._keep = (q, k, v, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, q_indptr,
                positions)
-    p._dev, p.q_rotated = dev, q_out
+    p._dev, p.q_rotated, p._made = dev, q_out, made
     return p
 
 
@@ -752,6 +753,8 @@ def rope_append(p: AppendParams, rope: Rope = None, stream=None):
     st = lib().ckl_rope_append(p, rope, _stream_of(stream, p._dev, "rope_append"))
     if st:
         check(st, "ckl_rope_append")
+    if stream is not None and p._made:             # allocated on another stream: kept until this one is done
+        p.q_rotated.record_stream(stream)
     return p.q_rotated
 
 

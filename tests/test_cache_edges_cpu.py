@@ -53,9 +53,27 @@ def test_params_of_another_device_are_refused(ckl, monkeypatch, current, stream)
     monkeypatch.setattr(ckl, "_raw_stream", lambda dev: 0)
     ap, tp = ckl.AppendParams(Hkv=1), ckl.TreeParams(Hq=1, Hkv=1)
     ap._dev = tp._dev = 0
-    ap.q_rotated, tp._keep = None, (None,)
+    ap.q_rotated, ap._made, tp._keep = None, False, (None,)
     for call in (lambda: ckl.rope_append(ap, stream=stream), lambda: ckl.tree_attention(tp, stream=stream),
                  lambda: ckl.cache_weights(tp, None, None, stream=stream)):
         with pytest.raises(ckl.CklError, match="cuda:1") as e:
             call()
         assert e.value.status == INVALID
+
+
+def test_rope_append_keeps_its_own_output_for_the_stream(ckl, monkeypatch):
+    """q_out that make_append_params allocated, on the stream of its time, is written on the call's
+    stream: its memory waits for that one. The caller's own q_out is the caller's."""
+    monkeypatch.setattr(ckl, "_raw_device", lambda: 0)
+    monkeypatch.setattr(ckl, "_raw_stream", lambda dev: 0)
+    seen = []
+
+    class Out:
+        def record_stream(self, stream):
+            seen.append(stream)
+
+    p, s = ckl.AppendParams(Hkv=1), Stream(0)
+    p._dev, p.q_rotated = 0, Out()
+    for made, stream, want in ((False, s, []), (True, None, []), (True, s, [s])):
+        p._made = made
+        assert ckl.rope_append(p, stream=stream) is p.q_rotated and seen == want
