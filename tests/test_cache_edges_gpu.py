@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import cache_ref as ref
-from test_cache_ops_gpu import finish, run_tree, table, up
+from test_cache_ops_gpu import check_tree, finish, run_tree, table, up
 
 pytestmark = pytest.mark.gpu
 
@@ -162,6 +162,22 @@ def test_neighbours_leave_the_same_bits(ckl, dev, toks, Hq, softcap, bias):
 
 
 # ------------------------------------------------------------------ rows of weights
+def test_cache_weights_leaves_the_rest(ckl, dev):
+    """Places from the length on are left for every decay, 0 too."""
+    import torch
+    lens, toks = [40, 300, 1], [3, 5, 1]
+    bt = ref.Batch(lens, toks, 8, 2, 72)
+    p = run_tree(ckl, dev, bt)
+    _, lse = ckl.tree_attention(p)
+    for decay in (0.0, 0.5, 1.0):
+        acc = torch.rand((3, 333), device=dev)
+        was = acc.clone()
+        ckl.cache_weights(p, lse, acc, decay=decay)
+        finish(ckl)
+        for b, L in enumerate(lens):
+            assert torch.equal(acc[b, L:], was[b, L:]) and not torch.equal(acc[b, :L], was[b, :L])
+
+
 def test_weights_that_are_columns_of_something_wider(ckl, dev):
     """acc as columns of a wider tensor, sequences longer than its rows: what a contiguous acc of
     those rows gives, and the columns beside it are neither read nor written."""
@@ -298,3 +314,72 @@ def test_a_batch_without_a_page(ckl, dev):
     assert torch.all(out == 0) and torch.all(torch.isneginf(lse)) and torch.all(acc == 1)
     assert torch.all(idx == -1) and torch.all(cnt == 0) and torch.all(new == 0)
     assert np.array_equal(k.cpu().numpy(), bt.k, equal_nan=True)
+
+
+# ------------------------------------------------------------------ many sequences, graphs
+@pytest.mark.parametrize("toks,Hq,opt", [(1, 4, dict()), (3, 4, dict(window=21)), (9, 4, dict(softcap=20.0)),
+                                         (33, 8, dict(window=40, bias=True))], ids=str)
+def test_many_sequences(ckl, dev, toks, Hq, opt):
+    """More sequences than a warp has lanes, a third of them without tokens or without keys."""
+    r = np.random.default_rng(91)
+    lens = [int(r.choice([0, 1, 40, 300])) for _ in range(75)]
+    bt = ref.Batch(lens, [0 if b % 3 == 1 else min(toks, L) for b, L in enumerate(lens)], Hq, 2, 92, extra_rows=2)
+    _, mask, pos = bt.random_tree(3)
+    opt = dict(opt, mask=mask, positions=pos)
+    if opt.pop("bias", False):
+        opt["slopes"] = slopes_of(Hq)
+    check_tree(ckl, dev, bt, force=1, **opt)
+    p = run_tree(ckl, dev, bt, **opt)
+    import torch
+    _, lse = ckl.tree_attention(p)
+    lse[bt.T_total:] = 0
+    acc = np.random.default_rng(1).random((75, 300)).astype(np.float32)
+    got = ckl.cache_weights(p, lse, up(acc, dev), decay=0.5)
+    finish(ckl)
+    want, tol = ref.weights(bt, acc, lse.cpu().numpy(), 0.5, **opt)
+    assert np.all(np.abs(got.cpu().numpy() - want) <= tol + 2.0 ** -23 * np.abs(want))
+
+
+def test_a_step_captured_on_a_stream_and_replayed(ckl, dev):
+    """Append, masks, attention, weights, selection and compaction in one graph on a stream of its
+    own; each replay does to fresh caches what the calls do one by one."""
+    import torch
+    bt = ref.Batch([200, 61, 333], [12, 20, 7], 8, 2, 77)
+    parents, _, _ = bt.random_tree(5)
+    r = np.random.default_rng(6)
+    q, k, v = (up(r.standard_normal((bt.N, h, 128)).astype(np.float16), dev) for h in (8, 2, 2))
+    t, qi, par = table(bt, dev), up(bt.q_indptr, dev), up(parents, dev)
+    plan = ckl.rope_plan(128)
+    clean = [up(np.nan_to_num(bt.k), dev), up(np.nan_to_num(bt.v), dev)]
+    kc, vc = (x.clone() for x in clean)
+    acc = torch.zeros((3, 400), device=dev)
+
+    def step(stream=None):
+        m, ps = ckl.tree_mask(par, qi, t["kv_indptr"], t["kv_last_page_len"], 20, stream=stream)
+        qr = ckl.rope_append(ckl.make_append_params(q, k, v, kc, vc, **t, q_indptr=qi, positions=ps), plan, stream=stream)
+        tp = ckl.make_tree_params(qr, kc, vc, **t, max_len=333, q_indptr=qi, max_q=20, tree_mask=m, positions=ps)
+        out, lse = ckl.tree_attention(tp, stream=stream)
+        ckl.cache_weights(tp, lse, acc, decay=0.5, stream=stream)
+        ki, kn = ckl.cache_select(acc, t["kv_indptr"], t["kv_last_page_len"], 60, sink=4, recent=16, stream=stream)
+        new = ckl.cache_compact(kc, vc, **t, keep_idx=ki, keep_count=kn, acc=acc, stream=stream)
+        return m, qr, out, lse, ki, kn, new
+
+    def fresh():
+        kc.copy_(clean[0])
+        vc.copy_(clean[1])
+        acc.zero_()
+
+    fresh()
+    side = torch.cuda.Stream()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        got = step(side)
+    for scale in (1.0, -0.5):
+        q.mul_(scale)
+        fresh()
+        want = [x.clone() for x in step()] + [kc.clone(), vc.clone(), acc.clone()]
+        fresh()
+        g.replay()
+        finish(ckl)
+        for x, y in zip(list(got) + [kc, vc, acc], want):
+            assert torch.equal(x, y)
