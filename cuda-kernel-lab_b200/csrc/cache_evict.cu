@@ -31,10 +31,11 @@ using tree::Seq;
 // staged once and the blocks' K tiles stream past it. Warp 0 loads K (TMA), warp 1 issues the MMAs,
 // warps 2-3 stage Q and the rows' lse, position and slope, and two groups of four warps turn S into
 // weights: for many rows each takes half of the columns of every tile, for few rows, where a tile
-// is mostly waiting, the tiles of every other kv head. One token of 32 heads over 8 x 8192 keys: 28.7
-// us for 134.8 MB (4.7 TB/s in all, the start and the end of the stream a third of it); 32 tokens over
-// 3 x 7001 keys and 4 kv heads, 256 rows of S a key: 19.6 us, the exponentials and the start (24 with a
-// masked block's columns tested one by one, for every head).
+// is mostly waiting, the tiles of every other kv head. One token of 32 heads over 8 x 8192 keys: 28.1
+// us for 134.8 MB (4.8 TB/s in all, the start and the end of the stream a third of it; 148 CTAs share 512
+// blocks, so the longest run is 4 against 3.46 on average); 32 tokens over 3 sequences of up to 7001 keys
+// and 4 kv heads, 256 rows of S a key: 19.6 us (24 with a masked block's columns tested one by one, for
+// every head): 104 blocks leave 44 SMs without one, and the others take the kv heads one after another.
 constexpr int W_THREADS = 384;
 constexpr int W_BLK = 128;                     // keys of a tile
 constexpr int W_BLK_PAGES = W_BLK / PAGE;
@@ -777,7 +778,8 @@ struct CArgs {
 // list: every thread loads its pieces of tile t + 1, the CTA meets (tile t has been read), and
 // every thread stores tile t: 64 KB are on their way while 64 KB are written. The places are
 // translated to cache rows ahead of time, so that no load waits for an index. No CTA waits for
-// another. 8 x 4096 rows of 8 heads: 55.8 us, 4.8 TB/s of pieces of 256 bytes that lie 2 KB apart.
+// another. 8 x 4096 rows of 8 heads: 55.8 us, 4.8 TB/s of pieces of 128 bytes that lie 2 KB apart: 256
+// columns, one CTA an SM (512 threads of 101 registers), so some SMs take a second turn.
 // ROWS: list entries translated at a time. The accepted paths of drafts are a few rows a
 // sequence: small CTAs, so that all of them are resident (512 threads: 10.3 us at 32 x 5 rows,
 // 128: 3.3 us). grid = (Hkv * 16 / pieces (+ 1 for acc and the lengths), B, 2).

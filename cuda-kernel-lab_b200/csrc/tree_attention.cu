@@ -219,9 +219,9 @@ struct State {
     }
 };
 
-// Bound by HBM for many sequences: 64 with a window of 2000 keys over 8 kv heads, one token each, 87-96
-// us by box for 483 MB, the last wave of CTAs not full; by latency for few (1 x 1000 keys: 12.5 us with the
-// merge). grid = (B * Hkv, num_chunks).
+// Bound by HBM for many sequences: 64 with a window of 2000 keys over 8 kv heads, one token each, 85-97
+// us by box for 483 MB, the last wave of CTAs not full; by latency for few (one token over 1 x 1000 keys:
+// 10.4 us with the merge). grid = (B * Hkv, num_chunks).
 template <int KIND>
 __global__ void __launch_bounds__(THREADS, 2)
 rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const Args a) {
@@ -587,7 +587,8 @@ ckl_status check_split(const ckl_tree_params* p) {
 
 // More rows than an m16 tile holds go to the tcgen05 kernel, which spends a 128-row tile on any
 // number. At 24 rows a second m16 tile per warp (32 rows) against it, in us: 1 x 1000 keys 17.9 / 14.6,
-// 1 x 4000 17.2 / 20.7, 1 x 30000 45.6 / 41.3, 8 x 4000 54.6 / 40.7, 8 x 16384 167 / 106.
+// 1 x 4000 17.2 / 20.7, 1 x 30000 45.6 / 41.3, 8 x 4000 54.6 / 40.7, 8 x 16384 167 / 106: the tiles lose
+// at one sequence of a few thousand keys, where each CTA has little to do, and gain at the other sizes.
 bool use_tiles(long long rows) { return rows > R; }
 
 // CTAs of the tcgen05 kernel: num_chunks for each unit (sequence, kv head, row group), one wave

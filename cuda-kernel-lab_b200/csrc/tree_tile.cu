@@ -19,9 +19,11 @@
 // 128 65).
 //
 // V pages arrive as one 4 KB box each, [64-dim half][16 tokens][64 dims]. K pages take a 2 KB box
-// per half, so that a part's keys of a half lie together and S is one product. Bound by the tensor
-// cores' clock and the exponentials for 256 rows (8 x 64 drafts over 16,384 keys: 0.92 PFLOP/s), by HBM
-// for up to 128 (8 x 32 drafts: 7 TB/s in the main loop), by start, masked block and join for short ones.
+// per half, so that a part's keys of a half lie together and S is one product. For 256 rows bound by
+// the chain of S, softmax and P V of a part (no unit is busy more than 36 % of the time), at the clock that
+// the power cap leaves: 8 x 64 drafts over 16,384 keys 152-168 us in short runs (0.82-0.90 PFLOP/s), 184 us
+// at 1.52 GHz in a long one. By HBM for up to 128 (8 x 32 drafts: 7 TB/s in the main loop), by start, masked
+// block and join for short ones.
 //
 // Work is divided exactly: the key blocks of all (sequence, row group, kv head) units, end to
 // end, over one wave of CTAs. A unit that lies within one CTA is written out directly; where a
@@ -537,7 +539,8 @@ tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
                 // held in registers, with a version each for plain scores (1), capped ones (2), a
                 // distance bias (3) and both (4). Other blocks -- the last one or two, a window's
                 // border, scores beyond the polynomial of the cap -- go through rolled loops (0), scores
-                // back into tensor memory in between: little code to fetch.
+                // back into tensor memory in between: little code to fetch. (16 x 24 drafts with a cap of 2,
+                // scores beyond 0.45 of it in every part: 210 us, with a cap of 30 111.)
                 auto soft = [&](auto kind_, int x, int kbase, uint32_t srow) {
                     constexpr int KIND = decltype(kind_)::value;
                     constexpr bool HELD = KIND != 0, CAP = KIND == 2 || KIND == 4, BIAS = KIND >= 3;

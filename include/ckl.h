@@ -603,7 +603,8 @@ typedef struct ckl_append_params {
 /* Rotates q into q_out and k into the cache, and copies v into the cache, rounding once from
  * fp32 to fp16; rope NULL copies q and k unturned. All tensors 16-byte aligned; outputs must
  * not overlap the inputs (CKL_INVALID_ARG). A page id outside [0, num_pages) is not written.
- * Two tokens with the same place (a page listed twice) race. */
+ * Two tokens with the same place (a page listed twice) race. An attention call behind it may be told
+ * CKL_DECODE_CACHE_READY only where each sequence's new tokens lie in its last page. */
 CKL_API ckl_status ckl_rope_append(const ckl_append_params* p, const ckl_rope* rope, void* stream);
 
 /* Ancestor masks of draft trees, for ckl_tree_attention. parents[n] is the index, within its
@@ -710,7 +711,7 @@ CKL_API ckl_status ckl_cache_select(const float* acc, long long acc_stride, cons
  * input (CKL_INVALID_ARG; of kv_indices, whose length the host does not know, the first entry is
  * compared). Pages that hold a moved token's new place must belong
  * to that sequence alone; a token whose page id is outside [0, num_pages) moves as zeros, and
- * none moves to such a page. */
+ * none moves to such a page. The attention call behind it must not be told CKL_DECODE_CACHE_READY. */
 CKL_API ckl_status ckl_cache_compact(void* k_cache, void* v_cache, const int* kv_indptr,
                                      const int* kv_indices, const int* kv_last_page_len, int B,
                                      int Hkv, int num_pages, const int* keep_idx, int keep_stride,
