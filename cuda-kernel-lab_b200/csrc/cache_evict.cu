@@ -1023,13 +1023,6 @@ ckl_status ckl_cache_compact_ex(void* k_cache, void* v_cache, const int* kv_indp
     if (num_pages > INT_MAX / PAGE) return fail(CKL_UNSUPPORTED_SHAPE, "cache_compact: num_pages=%d", num_pages);
     // what a CTA writes, others still read: each output stands alone. (Of kv_indices the host knows
     // no more than its first entry.)
-    struct Span {
-        const void* at;
-        size_t bytes;
-    };
-    auto overlap = [](Span x, Span y) {
-        return x.at && y.at && (uintptr_t)x.at < (uintptr_t)y.at + y.bytes && (uintptr_t)y.at < (uintptr_t)x.at + x.bytes;
-    };
     const size_t cache = (size_t)num_pages * PAGE * Hkv * D * sizeof(__half), ints = (size_t)B * sizeof(int);
     const Span out[] = {{k_cache, cache}, {v_cache, cache}, {new_len, ints},
                         {acc, ((size_t)(B - 1) * acc_stride + acc_cols) * sizeof(float)}};

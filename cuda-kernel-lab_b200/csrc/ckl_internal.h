@@ -59,6 +59,16 @@ inline cudaError_t launch(const void* fn, dim3 grid, dim3 block, size_t smem, cu
     return cudaLaunchKernelExC(&cfg, fn, args);
 }
 
+// Do the ranges share a byte? (NULL and empty ones share none.)
+struct Span {
+    const void* at;
+    size_t bytes;
+};
+inline bool overlap(Span x, Span y) {
+    return x.at && y.at && x.bytes && y.bytes && (uintptr_t)x.at < (uintptr_t)y.at + y.bytes &&
+           (uintptr_t)y.at < (uintptr_t)x.at + x.bytes;
+}
+
 inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
 inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 

@@ -194,11 +194,6 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ Arg
     }
 }
 
-bool overlap(const void* p, size_t pn, const void* q, size_t qn) {
-    const uintptr_t a = (uintptr_t)p, b = (uintptr_t)q;
-    return pn && qn && a < b + qn && b < a + pn;
-}
-
 }  // namespace rope
 }  // namespace ckl
 
@@ -287,16 +282,15 @@ ckl_status ckl_rope_append(const ckl_append_params* p, const ckl_rope* rope, voi
     // every output against every input
     const size_t row = D * sizeof(__half), cache = (size_t)p->num_pages * PAGE * p->Hkv * row;
     auto bytes = [&](long long stride, long long heads) { return ((size_t)(p->N - 1) * stride) * sizeof(__half) + heads * row; };
-    const void* in[3] = {p->q, p->k, p->v};
-    const size_t in_n[3] = {p->q ? bytes(p->q_stride, hq) : 0, bytes(p->k_stride, p->Hkv), bytes(p->v_stride, p->Hkv)};
-    const void* out[3] = {p->q_out, p->k_cache, p->v_cache};
-    const size_t out_n[3] = {p->q ? (size_t)p->N * hq * row : 0, cache, cache};
+    const Span in[3] = {{p->q, p->q ? bytes(p->q_stride, hq) : 0}, {p->k, bytes(p->k_stride, p->Hkv)},
+                        {p->v, bytes(p->v_stride, p->Hkv)}};
+    const Span out[3] = {{p->q_out, p->q ? (size_t)p->N * hq * row : 0}, {p->k_cache, cache}, {p->v_cache, cache}};
     for (int i = 0; i < 3; i++)
         for (int o = 0; o < 3; o++)
-            if (overlap(in[i], in_n[i], out[o], out_n[o]))
+            if (overlap(in[i], out[o]))
                 return fail(CKL_INVALID_ARG, "rope_append: an output overlaps an input");
     for (int o = 0; o < 3; o++)
-        if (overlap(out[o], out_n[o], out[(o + 1) % 3], out_n[(o + 1) % 3]))
+        if (overlap(out[o], out[(o + 1) % 3]))
             return fail(CKL_INVALID_ARG, "rope_append: two outputs overlap");
     const DeviceInfo* di = device_info();
     if (!di) return CKL_CUDA_ERROR;

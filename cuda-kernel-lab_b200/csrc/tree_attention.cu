@@ -730,6 +730,14 @@ ckl_status ckl_tree_mask(const int* parents, const int* q_indptr, const int* kv_
     if (B == 0 || N == 0) return CKL_OK;
     if (!parents || !q_indptr || !kv_indptr || !kv_last_page_len || !mask)
         return fail(CKL_INVALID_ARG, "tree_mask: NULL tensor pointer");
+    // a thread walks parents that other threads' results would replace
+    const size_t ints = (size_t)B * sizeof(int), rows = (size_t)N * sizeof(int);
+    const Span out[] = {{mask, rows * mask_words}, {positions, rows}};
+    const Span in[] = {{parents, rows}, {q_indptr, ints + sizeof(int)}, {kv_indptr, ints + sizeof(int)}, {kv_last_page_len, ints}};
+    if (overlap(out[0], out[1])) return fail(CKL_INVALID_ARG, "tree_mask: mask and positions overlap");
+    for (const Span& o : out)
+        for (const Span& i : in)
+            if (overlap(o, i)) return fail(CKL_INVALID_ARG, "tree_mask: an output overlaps an input");
     if (!device_info()) return CKL_CUDA_ERROR;
     void* args[] = {&parents, &q_indptr, &kv_indptr, &kv_last_page_len, &B, &N, &mask_words, &mask, &positions};
     const unsigned gx = (unsigned)std::min(std::max(1, ceil_div(N, 128)), 8);

@@ -611,7 +611,8 @@ CKL_API ckl_status ckl_rope_append(const ckl_append_params* p, const ckl_rope* r
  * own sequence's tokens, of drafted token n's parent, lower than its own; anything else marks
  * a root. Bit j of mask row n (word j/32, bit j%32 of [N][mask_words]) is set when token j of
  * the same sequence is token n or an ancestor of it; tokens from 32*mask_words on have no bit.
- * positions (optional, [N]): L_b - T_b + the token's depth. */
+ * positions (optional, [N]): L_b - T_b + the token's depth. Outputs must not overlap one another or
+ * an input (CKL_INVALID_ARG). */
 CKL_API ckl_status ckl_tree_mask(const int* parents, const int* q_indptr, const int* kv_indptr,
                                  const int* kv_last_page_len, int B, int N, int mask_words,
                                  uint32_t* mask, int* positions, void* stream);

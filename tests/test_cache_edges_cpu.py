@@ -77,3 +77,12 @@ def test_rope_append_keeps_its_own_output_for_the_stream(ckl, monkeypatch):
     for made, stream, want in ((False, s, []), (True, None, []), (True, s, [s])):
         p._made = made
         assert ckl.rope_append(p, stream=stream) is p.q_rotated and seen == want
+
+
+def test_tree_mask_refuses_outputs_over_inputs(ckl):
+    """5 tokens of 2 sequences, 2 words a row: masks of 40 bytes, positions of 20."""
+    call = lambda mask=0x5000, pos=0x6000: ckl.lib().ckl_tree_mask(0x1000, 0x2000, 0x3000, 0x4000, 2, 5, 2, mask, pos, None)
+    for pos in (0x1000 - 16, 0x1000, 0x1000 + 16, 0x2000 + 8, 0x3000, 0x4000 + 4, 0x5000 + 36, 0x5000 - 16):
+        assert call(pos=pos) == INVALID, hex(pos)
+    for mask in (0x1000 - 36, 0x1000 + 16, 0x2000 + 8, 0x3000, 0x4000):
+        assert call(mask=mask) == INVALID, hex(mask)
