@@ -840,7 +840,7 @@ def tree_attention(p: TreeParams, out=None, lse=None, workspace=None, stream=Non
     need = L.ckl_tree_workspace_size(p)
     wa, have = None, 0
     if workspace is not None:
-        wa, have = _at(workspace, workspace.dtype, 0, "workspace", who, d), workspace.nbytes
+        wa, have = _at(workspace, getattr(workspace, "dtype", None), 0, "workspace", who, d), workspace.nbytes
     if have < need:
         workspace = _empty(need, _U8, dev, stream)
         wa, have = workspace.data_ptr(), need

@@ -383,3 +383,11 @@ def test_a_step_captured_on_a_stream_and_replayed(ckl, dev):
         finish(ckl)
         for x, y in zip(list(got) + [kc, vc, acc], want):
             assert torch.equal(x, y)
+
+
+def test_a_workspace_that_is_no_tensor_is_refused(ckl, dev):
+    import torch
+    p = run_tree(ckl, dev, ref.Batch([300], [9], 8, 2, 82))
+    for bad in (3, np.empty(1 << 20, np.uint8), torch.empty(1 << 20, dtype=torch.uint8)):
+        with pytest.raises(ckl.CklError):
+            ckl.tree_attention(p, workspace=bad)
