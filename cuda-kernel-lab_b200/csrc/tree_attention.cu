@@ -220,7 +220,7 @@ struct State {
 };
 
 // Bound by HBM for many sequences: 64 with a window of 2000 keys over 8 kv heads, one token each, 85-97
-// us by box for 483 MB, the last wave of CTAs not full; by latency for few (one token over 1 x 1000 keys:
+// us by run for 483 MB, the last wave of CTAs not full; by latency for few (one token over 1 x 1000 keys:
 // 10.4 us with the merge). grid = (B * Hkv, num_chunks).
 template <int KIND>
 __global__ void __launch_bounds__(THREADS, 2)
